@@ -46,6 +46,8 @@ from .int8_quant import (  # noqa: F401
     stochastic_round_int8_delta,
 )
 
+from .adapters import AdapterBank, forward_adapters  # noqa: F401
+from .block_norms import block_norm, forward_block_norm  # noqa: F401
 from .nodes import NODE_CLASS_MAPPINGS, NODE_DISPLAY_NAME_MAPPINGS  # noqa: E402,F401
 
 

@@ -84,6 +84,16 @@ def lib() -> ctypes.CDLL:
     L.i8f_lora_merge_sr_drawn.argtypes = [vp, vp, f32, i32, vp, i32, f32, ctypes.c_uint64, i64, i64, i64, vp, vp, i64, vp]
     L.i8f_lora_merge_sr_drawn_workspace_bytes.argtypes = [i64, i64, i64, i32]
     L.i8f_lora_merge_sr_drawn_workspace_bytes.restype = i64
+    L.i8f_adapters_down.argtypes = [vp, i32, i64, i64, i64, vp, vp, vp]
+    L.i8f_adapters_up.argtypes = [vp, i32, vp, vp, vp, i32, i64, i64, vp]
+    L.i8f_linear_w8a8_adapters_workspace_bytes.argtypes = [i64, i64, i64]
+    L.i8f_linear_w8a8_adapters_workspace_bytes.restype = i64
+    L.i8f_linear_w8a8_adapters.argtypes = [vp, vp, vp, vp, f32, i32, vp, i32, vp, vp, vp, i32, i64, i64, i64, vp, i64, vp]
+    L.i8f_linear_w8a16_small_m_adapters.argtypes = [vp, i32, i64, i64, i64, vp, vp, f32, i32, vp, i32, vp, vp, vp, i64, vp]
+    L.i8f_block_norm.argtypes = [vp, vp]
+    for name in BLOCK_EXPORTS:
+        if not name.endswith("_bytes"):
+            getattr(L, name).restype = i32
     for name in ("i8f_quant_rowwise_concat_gelu", "i8f_quant_rowwise_rms_norm", "i8f_linear_w8a8_gated", "i8f_quant_rowwise", "i8f_quant_rowwise_grouped", "i8f_quant_rowwise_prologue", "i8f_quant_rowwise_norm_modulate", "i8f_quant_tensorwise", "i8f_quant_tensorwise_static", "i8f_rotate128", "i8f_gemm_i32", "i8f_linear_w8a8", "i8f_linear_w8a8_add", "i8f_linear_w8a8_splitk", "i8f_linear_w8a8_grouped", "i8f_linear_w8a8_lora",
                  "i8f_linear_w8a16_small_m", "i8f_linear_w8a16_small_m_grouped", "i8f_sr_quant_delta", "i8f_lora_merge_sr", "i8f_lora_merge_sr_drawn"):
         getattr(L, name).restype = i32
@@ -119,6 +129,10 @@ EXPORTS = (
 )
 
 
+# the entry points of include/i8f_blocks.h
+BLOCK_EXPORTS = ("i8f_adapters_down", "i8f_adapters_up", "i8f_linear_w8a8_adapters_workspace_bytes", "i8f_linear_w8a8_adapters",
+                 "i8f_linear_w8a16_small_m_adapters", "i8f_block_norm")
+
 ERR_UNSUPPORTED = -2   # I8F_ERR_UNSUPPORTED
 
 
@@ -134,6 +148,14 @@ def _dev(t: torch.Tensor, name: str) -> None:
         raise TypeError(f"{name} must be a torch.Tensor")
     if not t.is_cuda:
         raise RuntimeError(f"{name} is on {t.device}: the INT8 engine runs on a gfx950 GPU only (no CPU path)")
+
+
+def refuse_gradients(**tensors) -> None:
+    """For operators without a backward pass: under grad mode an operand that asks for a gradient would silently get none."""
+    if torch.is_grad_enabled():
+        for name, t in tensors.items():
+            if isinstance(t, torch.Tensor) and t.requires_grad:
+                raise RuntimeError(f"{name} asks for a gradient, which this operator does not have: call it under torch.no_grad()")
 
 
 class _Nop:
@@ -851,6 +873,176 @@ def lora_merge_sr_drawn(w, w_scale, generator, factors, lora_scale=1.0):
         return None
     _check(status, "i8f_lora_merge_sr_drawn")
     return out
+
+
+# --------------------------------------------------------------------------- adapters of many requests, norms between blocks
+class _Adapters(ctypes.Structure):
+    _fields_ = [("down", ctypes.c_void_p), ("up", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("first_rank", ctypes.c_void_p),
+                ("ids", ctypes.c_void_p), ("rows_per_id", ctypes.c_int64), ("count", ctypes.c_int64), ("max_rank", ctypes.c_int64)]
+
+
+def _adapters_arg(bank, ids, rows_per_id):
+    """The C structure of a bank (adapters.AdapterBank) and the adapter numbers of a batch."""
+    return _Adapters(_addr(bank.down), _addr(bank.up), _addr(bank.scale), _addr(bank.first_rank), _addr(ids), rows_per_id, bank.count, bank.max_rank)
+
+
+def adapters_down(x, bank, ids, rows_per_id=1):
+    """t [M, bank.max_rank] of x [M,K]: row m holds scale_a * A_a x[m] for its adapter a = ids[m // rows_per_id] in its first ranks; what lies
+    behind them, and rows without an adapter, are not written.  ids: int32, contiguous, one for each rows_per_id rows."""
+    _dev(x, "x")
+    x = _rows(x, "x")
+    M, K = x.shape
+    if x.dtype != bank.dtype or x.device != bank.device or K != bank.in_features:
+        raise ValueError(f"x must be [M,{bank.in_features}] of {bank.dtype} on {bank.device}")
+    t = torch.empty((M, bank.max_rank), dtype=x.dtype, device=x.device)
+    arg = _adapters_arg(bank, ids, rows_per_id)
+    with _on(x.device):
+        _check(lib().i8f_adapters_down(_ptr(x), dtype_code(x.dtype), M, K, x.stride(0) if M > 1 else K, ctypes.byref(arg), _ptr(t), _stream(x)),
+               "i8f_adapters_down")
+    return t
+
+
+def adapters_up(base, bank, ids, rows_per_id, t):
+    """round(base + B_a t) for base [M,N] of the bank's type or float32."""
+    _dev(base, "base")
+    if base.dim() != 2 or base.shape[1] != bank.out_features or base.device != bank.device or base.dtype not in (bank.dtype, torch.float32):
+        raise ValueError(f"base must be [M,{bank.out_features}] of {bank.dtype} or float32 on {bank.device}")
+    base = base.contiguous()
+    M, N = base.shape
+    out = torch.empty((M, N), dtype=bank.dtype, device=base.device)
+    arg = _adapters_arg(bank, ids, rows_per_id)
+    with _on(base.device):
+        _check(lib().i8f_adapters_up(_ptr(base), dtype_code(base.dtype), ctypes.byref(arg), _ptr(t), _ptr(out), dtype_code(out.dtype), M, N, _stream(base)),
+               "i8f_adapters_up")
+    return out
+
+
+def linear_w8a8_adapters(a, a_scale, w, w_scale, bias, bank, ids, rows_per_id, t):
+    """linear_w8a8 in the order EPI_FUSED with the adapters' share (t of adapters_down) added before its one rounding."""
+    a, w = _i8_matrix(a, "a"), _i8_matrix(w, "w")
+    M, K = a.shape
+    N, K2 = w.shape
+    if K != K2 or N != bank.out_features:
+        raise ValueError(f"a is [{M},{K}], w is [{N},{K2}], the adapters have {bank.out_features} outputs")
+    a_scale = a_scale.reshape(-1).contiguous()
+    if a_scale.numel() != M or a_scale.dtype != torch.float32:
+        raise ValueError("a_scale must be float32 with M elements")
+    ws, ws_host, mode = _scale(w_scale, N, a.device)
+    bias, bcode = _bias_arg(bias, N, a.device)
+    for name, v in (("w", w), ("a_scale", a_scale), ("t", t), ("bank", bank)):
+        if v.device != a.device:
+            raise ValueError(f"{name} is on {v.device}, a is on {a.device}")
+    out = torch.empty((M, N), dtype=bank.dtype, device=a.device)
+    work = torch.empty(lib().i8f_linear_w8a8_adapters_workspace_bytes(M, N, K), dtype=torch.uint8, device=a.device)
+    arg = _adapters_arg(bank, ids, rows_per_id)
+    with _on(a.device):
+        _check(lib().i8f_linear_w8a8_adapters(_ptr(a), _ptr(a_scale), _ptr(w), _ptr(ws), ws_host, mode, _ptr(bias), bcode, ctypes.byref(arg), _ptr(t),
+                                              _ptr(out), dtype_code(out.dtype), M, N, K, _ptr(work), work.numel(), _stream(a)),
+               "i8f_linear_w8a8_adapters")
+    return out
+
+
+def linear_w8a16_small_m_adapters(x, w, w_scale, bias, bank, ids, rows_per_id, t):
+    """linear_w8a16_small_m with the adapters' share (t of adapters_down) added before its one rounding."""
+    _dev(x, "x")
+    x = _rows(x, "x")
+    w = _i8_matrix(w, "w")
+    M, K = x.shape
+    N, K2 = w.shape
+    if K != K2 or N != bank.out_features or x.dtype != bank.dtype:
+        raise ValueError(f"x is [{M},{K}] of {x.dtype}, w is [{N},{K2}], the adapters have {bank.out_features} outputs of {bank.dtype}")
+    ws, ws_host, mode = _scale(w_scale, N, x.device)
+    bias, bcode = _bias_arg(bias, N, x.device)
+    out = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    arg = _adapters_arg(bank, ids, rows_per_id)
+    with _on(x.device):
+        _check(lib().i8f_linear_w8a16_small_m_adapters(_ptr(x), dtype_code(x.dtype), M, K, x.stride(0) if M > 1 else K, _ptr(w), _ptr(ws), ws_host, mode,
+                                                       _ptr(bias), bcode, ctypes.byref(arg), _ptr(t), _ptr(out), N, _stream(x)),
+               "i8f_linear_w8a16_small_m_adapters")
+    return out
+
+
+class _BlockNormArgs(ctypes.Structure):
+    _fields_ = [("y", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("M", ctypes.c_int64), ("K", ctypes.c_int64), ("ldy", ctypes.c_int64),
+                ("ldr", ctypes.c_int64), ("dtype", ctypes.c_int), ("post_norm", ctypes.c_int), ("post_dtype", ctypes.c_int), ("pre_norm", ctypes.c_int),
+                ("pre_dtype", ctypes.c_int), ("post_eps", ctypes.c_float), ("pre_eps", ctypes.c_float), ("post_weight", ctypes.c_void_p),
+                ("post_bias", ctypes.c_void_p), ("pre_weight", ctypes.c_void_p), ("pre_bias", ctypes.c_void_p), ("gate", ctypes.c_void_p),
+                ("rows_per_gate", ctypes.c_int64), ("gate_tanh", ctypes.c_int), ("residual_scale", ctypes.c_float), ("branch_scale", ctypes.c_float),
+                ("mod_scale", ctypes.c_void_p), ("mod_shift", ctypes.c_void_p), ("rows_per_scale", ctypes.c_int64), ("rows_per_shift", ctypes.c_int64),
+                ("x_out", ctypes.c_void_p), ("h", ctypes.c_void_p), ("q", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("rotate_block", ctypes.c_int)]
+
+
+NORMS = {None: 0, "rms": 1, "layer": 2}
+
+
+def _norm_operands(y, kind, weight, bias, eps, name):
+    """Weight, bias and their dtype code of one of block_norm's norms."""
+    if kind not in NORMS:
+        raise ValueError(f"{name}_norm must be 'rms', 'layer' or None, got {kind!r}")
+    if not eps >= 0.0:
+        raise ValueError(f"{name}_eps must not be negative")
+    given = [(n, v) for n, v in ((f"{name}_weight", weight), (f"{name}_bias", bias)) if v is not None]
+    if kind is None and given:
+        raise ValueError(f"{given[0][0]} without a norm")
+    for n, v in given:
+        _dev(v, n)
+        if tuple(v.shape) != (y.shape[-1],) or v.dtype not in (y.dtype, torch.float32) or v.dtype != given[0][1].dtype or v.device != y.device:
+            raise ValueError(f"{n} must be [{y.shape[-1]}] of {y.dtype} or float32 on {y.device}, weight and bias of one type")
+    return (None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous(),
+            dtype_code(given[0][1].dtype if given else y.dtype))
+
+
+def _block_vector(y, v, name):
+    """(contiguous vectors, rows of y to a vector) of an operand that is [K], or has y's dimensions with ones behind some leading ones."""
+    if v is None:
+        return None, 1
+    _dev(v, name)
+    lead, K = tuple(y.shape[:-1]), y.shape[-1]
+    shared = 0   # leading dimensions in which every index has vectors of its own
+    if v.dim() == y.dim():
+        while shared < len(lead) and v.shape[shared] == lead[shared]:
+            shared += 1
+    if (v.dtype != y.dtype or v.device != y.device or v.shape[-1] != K or v.dim() not in (1, y.dim())
+            or (v.dim() == y.dim() and any(n != 1 for n in v.shape[shared:-1]))):
+        raise ValueError(f"{name} must be [{K}] or {list(lead)} with ones from some dimension on, by {K}, of {y.dtype} on {y.device}; it is {list(v.shape)} of {v.dtype}")
+    rows = 1
+    for n in lead[shared:]:
+        rows *= n
+    return v.reshape(-1, K).contiguous(), max(1, rows)
+
+
+def block_norm(y, residual, *, post_norm=None, post_weight=None, post_bias=None, post_eps=1e-6, gate=None, gate_tanh=False, residual_scale=1.0,
+               branch_scale=1.0, pre_norm=None, pre_weight=None, pre_bias=None, pre_eps=1e-6, mod_scale=None, mod_shift=None, quantise=False, rotate=False):
+    """i8f_block_norm on tensors (block_norm.block_norm has the formula and the operands).  -> (x, h), h None without a pre_norm and a
+    modulation; quantise: (x, int8 rows [M,K], their scales [M,1]) with the rotation of `rotate`."""
+    _dev(y, "y")
+    _dev(residual, "residual")
+    if y.shape != residual.shape or y.dtype != residual.dtype or y.device != residual.device or y.dim() < 1:
+        raise ValueError(f"y and residual must be alike: {tuple(y.shape)} of {y.dtype} on {y.device}, {tuple(residual.shape)} of {residual.dtype} on {residual.device}")
+    code, K = dtype_code(y.dtype), y.shape[-1]
+    if K == 0:
+        raise ValueError("rows of no elements have no norm")
+    if rotate and (K % 128 or not quantise):
+        raise ValueError(f"rotation goes with the int8 form and needs K % 128 == 0, got K={K}")
+    pw, pb, pd = _norm_operands(y, post_norm, post_weight, post_bias, post_eps, "post")
+    hw, hb, hd = _norm_operands(y, pre_norm, pre_weight, pre_bias, pre_eps, "pre")
+    g, g_rows = _block_vector(y, gate, "gate")
+    s, s_rows = _block_vector(y, mod_scale, "mod_scale")
+    t, t_rows = _block_vector(y, mod_shift, "mod_shift")
+    y2, r2 = _rows(y.reshape(-1, K), "y"), _rows(residual.reshape(-1, K), "residual")
+    M = y2.shape[0]
+    x = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    h = q = scale = None
+    if quantise:
+        q, scale = torch.empty((M, K), dtype=torch.int8, device=y.device), torch.empty((M, 1), dtype=torch.float32, device=y.device)
+    elif pre_norm is not None or s is not None or t is not None:
+        h = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    arg = _BlockNormArgs(_addr(y2), _addr(r2), M, K, y2.stride(0) if M > 1 else K, r2.stride(0) if M > 1 else K, code, NORMS[post_norm], pd,
+                         NORMS[pre_norm], hd, post_eps, pre_eps, _addr(pw), _addr(pb), _addr(hw), _addr(hb), _addr(g), g_rows, int(bool(gate_tanh)),
+                         residual_scale, branch_scale, _addr(s), _addr(t), s_rows, t_rows, _addr(x), _addr(h), _addr(q), _addr(scale), 128 if rotate else 0)
+    with _on(y.device):
+        _check(lib().i8f_block_norm(ctypes.byref(arg), _stream(y)), "i8f_block_norm")
+    return (x, q, scale) if quantise else (x, h)
 
 
 def version() -> int:

@@ -1,0 +1,155 @@
+"""Low-rank adapters of many requests at once beside quantised projections that all of them share.
+
+`Int8TensorwiseOps.Linear` carries one dynamic LoRA for everything that goes through it (dynamic_lora.py).  A program that
+serves several users from one model has another one for each request of a batch, which changes from call to call: here the
+adapters of a layer lie in an `AdapterBank`, and a call names the adapter of every request.
+"""
+from __future__ import annotations
+
+import torch
+from torch import Tensor, nn
+
+from . import _lib
+from ._comfy_compat import compute_device
+from .dynamic_lora import _factor_pair
+from .int8_quant import SMALL_BATCH_ROWS, _scale_on
+
+
+class AdapterBank:
+    """The adapters of ONE layer on one device, laid out for the kernels.
+
+    adapters: one entry for each adapter number, (down [r, in features], up [out features, r]) or (down, up, scale); None for an
+              adapter that leaves this layer alone.  Ranks may differ.  An adapter adds scale * up @ down to the layer's weight.
+    dtype:    torch.bfloat16 or torch.float16, the activations' (default: the first factor's); factors are rounded to it once.
+    device:   where the layer runs (default: the first factor's device if that is a GPU, else ComfyUI's compute device).
+    in_features / out_features: needed where no entry has factors.
+    """
+
+    def __init__(self, adapters, dtype: torch.dtype | None = None, device=None, in_features: int | None = None, out_features: int | None = None):
+        entries = []
+        for i, entry in enumerate(adapters):
+            if entry is None:
+                entries.append(None)
+                continue
+            if not 2 <= len(entry) <= 3:
+                raise ValueError(f"adapter {i}: expected (down, up) or (down, up, scale)")
+            down, up, scale = (*entry, 1.0)[:3]
+            if down.dim() != 2 or up.dim() != 2 or down.shape[0] != up.shape[1]:
+                raise ValueError(f"adapter {i}: down is {list(down.shape)} and up {list(up.shape)}, expected [r, in features] and [out features, r]")
+            if in_features not in (None, down.shape[1]) or out_features not in (None, up.shape[0]):
+                raise ValueError(f"adapter {i} is for a layer of {down.shape[1]} inputs and {up.shape[0]} outputs, expected {in_features} and {out_features}")
+            in_features, out_features = down.shape[1], up.shape[0]
+            entries.append((down, up, float(scale)))
+        if in_features is None or out_features is None:
+            raise ValueError("a bank without factors needs in_features and out_features")
+        first = next((e for e in entries if e is not None), None)
+        if dtype is None:
+            dtype = torch.bfloat16 if first is None else first[0].dtype
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"adapters are kept in bfloat16 or float16, not {dtype}: give the activations' dtype")
+        if device is None:
+            device = first[0].device if first is not None and first[0].is_cuda else compute_device()
+        self.dtype, self.count, self.in_features, self.out_features = dtype, len(entries), in_features, out_features
+        self.ranks = [0 if e is None else e[0].shape[0] for e in entries]
+        padded = [-(-r // 16) * 16 for r in self.ranks]
+        self.max_rank = max(padded, default=0)
+        offsets = [0]
+        for r in padded:
+            offsets.append(offsets[-1] + r)
+        if offsets[-1] >= 1 << 31 or self.max_rank > 65536:
+            raise ValueError(f"the ranks of a bank add up to less than 2^31 and stay within 65536, got {offsets[-1]} and {self.max_rank}")
+        with torch.no_grad():
+            down_all = torch.zeros((offsets[-1], in_features), dtype=dtype, device=device)
+            up_all = torch.zeros((offsets[-1] * out_features,), dtype=dtype, device=device)
+            for entry, at, r in zip(entries, offsets, padded):
+                if entry is not None and entry[0].shape[0]:
+                    down, up, _ = entry
+                    down_all[at:at + down.shape[0]] = down.detach().to(device=device, dtype=dtype)
+                    up_all[at * out_features:(at + r) * out_features].view(out_features, r)[:, :up.shape[1]] = up.detach().to(device=device, dtype=dtype)
+        self.down, self.up = down_all, up_all
+        self.scale = torch.tensor([0.0 if e is None else e[2] for e in entries], dtype=torch.float32, device=device)
+        self.first_rank = torch.tensor(offsets, dtype=torch.int32, device=device)
+        self.device = down_all.device
+
+    @classmethod
+    def from_patches(cls, patches, **kwargs):
+        """A bank of ComfyUI LoRA patches of one layer: (adapter, strength) for each adapter number or None, as the entries of
+        the dynamic LoRA loaders hold them; alpha, rank and strength make the scale."""
+        return cls([None if p is None else _factor_pair(*p) for p in patches], **kwargs)
+
+
+def _adapter_rows(x: Tensor, ids: Tensor) -> tuple[Tensor, int]:
+    """(ids as the kernels take them, rows of x to each) of adapter numbers shaped like some leading dimensions of x."""
+    _lib._dev(ids, "ids")
+    lead = tuple(x.shape[:-1])
+    if ids.dtype != torch.int32 or ids.device != x.device:
+        raise TypeError(f"ids must be int32 on {x.device}, got {ids.dtype} on {ids.device}")
+    if ids.dim() > len(lead) or tuple(ids.shape) != lead[:ids.dim()]:
+        raise ValueError(f"ids must have the shape of leading dimensions of x, {list(lead)}, got {list(ids.shape)}")
+    rows = 1
+    for n in lead[ids.dim():]:
+        rows *= n
+    return ids.contiguous(), max(1, rows)
+
+
+def _quantised_here(layer, x: Tensor) -> bool:
+    """Whether the layer's own kernels can take the adapters: quantised weights in place, nothing else attached to it."""
+    return bool(getattr(layer, "_is_quantized", False) and layer.lora_A is None and layer.weight.device == x.device
+                and not (layer.comfy_cast_weights or len(layer.weight_function) > 0 or len(layer.bias_function) > 0)
+                and (layer.bias is None or layer.bias.device == x.device))
+
+
+def forward_adapters(layers, x: Tensor, banks, ids: Tensor):
+    """layer(x) + scale_a * up_a @ down_a @ x with the adapter a of each row, for one layer or for several that read the same x.
+
+    layers, banks: an Int8TensorwiseOps.Linear and its AdapterBank, or lists of them (then the result is a list).
+    x:    [..., in features], bfloat16 or float16, the banks' dtype.
+    ids:  int32 tensor on x's device, the adapter number of each request: of the shape of x's leading dimensions, all of them (one number
+          for each token) or fewer ([batch] for x [batch, tokens, features]).  A number that is not one of the bank's (-1, say) is a
+          request without an adapter.  The numbers are read by the kernels, so a captured graph follows what is written into the tensor.
+
+    One rounding at the end: the projection stays in binary32 (in the order of _lib.EPI_FUSED) until the adapter's share has been
+    added; down @ x is rounded to x's dtype for the matrix unit.  x is quantised once for all layers.  The adapter acts on x itself,
+    also where the layer rotates its activations (a dynamic LoRA of the layer gets them rotated).  Layers whose own kernels cannot take
+    the adapters (not quantised, weights that ComfyUI casts or moves for the call, a dynamic LoRA attached) run by themselves, and
+    their rounded result gets the adapters' share.  No gradients: under grad mode an input that asks for one is refused."""
+    single = isinstance(layers, nn.Module)
+    layers, banks = ([layers], [banks]) if single else (list(layers), list(banks))
+    if len(layers) != len(banks):
+        raise ValueError(f"{len(layers)} layers and {len(banks)} banks")
+    _lib._dev(x, "x")
+    if x.dim() < 1:
+        raise ValueError("x must have a feature dimension")
+    _lib.refuse_gradients(x=x)
+    for layer, bank in zip(layers, banks):
+        if x.dtype != bank.dtype or x.device != bank.device:
+            raise TypeError(f"x is {x.dtype} on {x.device}, the adapters are {bank.dtype} on {bank.device}")
+        if x.shape[-1] != bank.in_features or getattr(layer, "out_features", bank.out_features) != bank.out_features:
+            raise ValueError(f"x has {x.shape[-1]} features and the layer {getattr(layer, 'out_features', '?')} outputs, the adapters are for "
+                             f"{bank.in_features} and {bank.out_features}")
+    ids, per = _adapter_rows(x, ids)
+    lead = x.shape[:-1]
+    x2 = x.reshape(-1, x.shape[-1])
+    rows = x2.shape[0]
+    inputs = {}   # what the layers share, by whether they rotate: the rotated rows, or the int8 rows and their scales
+
+    def shared(rotate):
+        if rotate not in inputs:
+            if rows > SMALL_BATCH_ROWS:
+                inputs[rotate] = _lib.quant_rowwise(x2, rotate=rotate)
+            else:
+                inputs[rotate] = _lib.rotate128(x2) if rotate else x2
+        return inputs[rotate]
+
+    outs = []
+    for layer, bank in zip(layers, banks):
+        t = _lib.adapters_down(x2, bank, ids, per)
+        if not _quantised_here(layer, x):
+            y = _lib.adapters_up(layer(x).reshape(-1, bank.out_features), bank, ids, per, t)
+        elif rows > SMALL_BATCH_ROWS:
+            q, s = shared(bool(layer._use_quarot))
+            y = _lib.linear_w8a8_adapters(q, s, layer.weight, _scale_on(layer, x.device), layer.bias, bank, ids, per, t)
+        else:
+            y = _lib.linear_w8a16_small_m_adapters(shared(bool(layer._use_quarot)), layer.weight, _scale_on(layer, x.device), layer.bias, bank, ids, per, t)
+        outs.append(y.reshape(*lead, bank.out_features))
+    return outs[0] if single else outs

@@ -1,0 +1,56 @@
+// What the kernels around a shared projection take of the adapters (include/i8f_blocks.h).
+#pragma once
+
+#include "i8f_common.hpp"
+
+#include "../../include/i8f_blocks.h"
+
+namespace i8f {
+
+// Adapter of row m, or -1: numbers outside [0, count) are rows without one, so that no address is formed from them.
+__device__ __forceinline__ int adapter_of(const i8f_adapters &ad, int64_t m) {
+    const int a = ad.ids[(uint32_t)m / (uint32_t)ad.rows_per_id];   // (M < 2^31)
+    return (uint32_t)a < (uint32_t)ad.count ? a : -1;
+}
+
+// sum_j t[m,j] B_a[n,j] over the adapter's padded ranks, pairs of 16-bit values at a time, in binary32
+template <int DT>
+__device__ __forceinline__ float adapter_term(const i8f_adapters &ad, const void *t, int64_t m, int64_t n, int64_t N, int a) {
+    const int first = ad.first_rank[a], r = ad.first_rank[a + 1] - first;
+    const char *tp = (const char *)t + m * ad.max_rank * 2, *bp = (const char *)ad.up + (N * first + n * r) * 2;
+    float sum = 0.0f;
+    for (int j = 0; j < r; j += 8) {
+        const uint4 tv = *(const uint4 *)(tp + j * 2), bv = *(const uint4 *)(bp + j * 2);
+        const uint32_t tw[4] = {tv.x, tv.y, tv.z, tv.w}, bw[4] = {bv.x, bv.y, bv.z, bv.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (DT == I8F_BF16) {
+                sum = __builtin_fmaf(bf16_bits_to_f32(tw[e] & 0xffffu), bf16_bits_to_f32(bw[e] & 0xffffu), sum);
+                sum = __builtin_fmaf(bf16_bits_to_f32(tw[e] >> 16), bf16_bits_to_f32(bw[e] >> 16), sum);
+            } else {
+                sum = __builtin_fmaf(f16_bits_to_f32(tw[e] & 0xffffu), f16_bits_to_f32(bw[e] & 0xffffu), sum);
+                sum = __builtin_fmaf(f16_bits_to_f32(tw[e] >> 16), f16_bits_to_f32(bw[e] >> 16), sum);
+            }
+        }
+    }
+    return sum;
+}
+
+// Host: whether the structure can be used on M rows of 16-bit type `dtype` at all (I8F_OK), before any pointer in it is.
+inline int validate_adapters(const i8f_adapters *ad, int dtype, int64_t M) {
+    if (!ad || ad->count < 0 || ad->count > 0x7fffffff || ad->max_rank < 0 || ad->max_rank % 16 || ad->rows_per_id <= 0) return I8F_ERR_INVALID;
+    if (dtype != I8F_BF16 && dtype != I8F_F16) return I8F_ERR_INVALID;
+    if (M == 0) return I8F_OK;
+    if (!ad->ids || (ad->count > 0 && (!ad->first_rank || !ad->scale))) return I8F_ERR_INVALID;
+    if (ad->max_rank > 0 && (!ad->down || !ad->up)) return I8F_ERR_INVALID;
+    if (((uintptr_t)ad->down | (uintptr_t)ad->up) % 16) return I8F_ERR_INVALID;
+    return M > 0x7fffffff || ad->max_rank > 65536 ? I8F_ERR_UNSUPPORTED : I8F_OK;
+}
+// A copy whose rows_per_id fits 32 bits (M does)
+inline i8f_adapters for_kernel(const i8f_adapters &ad) {
+    i8f_adapters k = ad;
+    if (k.rows_per_id > 0x7fffffff) k.rows_per_id = 0x7fffffff;
+    return k;
+}
+
+}  // namespace i8f

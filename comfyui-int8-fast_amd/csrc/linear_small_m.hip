@@ -14,7 +14,9 @@
 // butterfly reduction across the wavefront).  The order of the binary32 sums
 // differs between the two; the result is compared with a tolerance of one
 // rounding step of the output type.
-#include "i8f_common.hpp"
+#include <type_traits>
+
+#include "adapters.hpp"
 #include "rotate_run.hpp"
 #include "w8a16_rotated.hpp"
 
@@ -32,6 +34,21 @@ struct SmallMArgs {
     int bias_dtype;
     void *out;
 };
+// What the form with adapters takes besides: out = round(sum + bias + B_a t) (i8f_linear_w8a16_small_m_adapters).
+struct NoAdapters {};
+struct WithAdapters {
+    i8f_adapters ad;
+    const void *t;
+};
+// the adapters' share of out[m,n]
+template <int DT, class AD>
+__device__ __forceinline__ float adapted(float v, const AD &ad, int64_t m, int64_t n, int64_t N) {
+    if constexpr (std::is_same<AD, WithAdapters>::value) {
+        const int a = adapter_of(ad.ad, m);
+        if (a >= 0) v += adapter_term<DT>(ad.ad, ad.t, m, n, N, a);
+    }
+    return v;
+}
 
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
@@ -68,8 +85,8 @@ __device__ __forceinline__ void load16(const void *x, int64_t idx, float (&xf)[1
     }
 }
 
-template <int DT, bool VEC>
-__global__ __launch_bounds__(256) void small_m_kernel(const SmallMArgs a) {
+template <int DT, bool VEC, class AD = NoAdapters>
+__global__ __launch_bounds__(256) void small_m_kernel(const SmallMArgs a, const AD ad = AD{}) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t n = (int64_t)blockIdx.x * 4 + wave;
     if (n >= a.N) return;
@@ -121,7 +138,7 @@ __global__ __launch_bounds__(256) void small_m_kernel(const SmallMArgs a) {
     for (int m = 0; m < 16; ++m) {
         if (m < M) {
             const float s = wave_sum(acc[m]);
-            if (lane == 0) store_from_f32<DT>(a.out, (int64_t)m * a.N + n, s + b);
+            if (lane == 0) store_from_f32<DT>(a.out, (int64_t)m * a.N + n, adapted<DT>(s + b, ad, m, n, a.N));
         }
     }
 }
@@ -173,8 +190,8 @@ __device__ __forceinline__ v4f_t mma8(uint32_t wlo, uint32_t whi, v4u_t xk, floa
 // every row, so the wave rotates what it is about to multiply, 8 lanes of 16 elements to a row's block, and takes it through a
 // tile of its own into the operand layout.  Every workgroup rotates all of x again, mostly while its weights are on their
 // way; what it saves is the rotation's own launch (i8f_internal_w8a16_rotated has the figures).
-template <int DT, int NB, int WAVES, bool ROT>
-__device__ __forceinline__ void small_m_lds_body(const SmallMArgs &a, const int64_t block) {
+template <int DT, int NB, int WAVES, bool ROT, class AD = NoAdapters>
+__device__ __forceinline__ void small_m_lds_body(const SmallMArgs &a, const int64_t block, const AD &ad = AD{}) {
     constexpr int COLS = NB * 16;
     constexpr int PITCH = 144;
     constexpr int XPITCH = 256 + 16;
@@ -309,7 +326,7 @@ __device__ __forceinline__ void small_m_lds_body(const SmallMArgs &a, const int6
                 else bv = f16_bits_to_f32(((const uint16_t *)a.bias)[n]);
                 bv = round_to_dtype<DT>(bv);
             }
-            store_from_f32<DT>(a.out, (int64_t)m * a.N + n, s + bv);
+            store_from_f32<DT>(a.out, (int64_t)m * a.N + n, adapted<DT>(s + bv, ad, m, n, a.N));
         }
     }
 }
@@ -317,6 +334,11 @@ __device__ __forceinline__ void small_m_lds_body(const SmallMArgs &a, const int6
 template <int DT, int NB, int WAVES, bool ROT>
 __global__ __launch_bounds__(WAVES * 64) void small_m_lds_kernel(const SmallMArgs a) {
     small_m_lds_body<DT, NB, WAVES, ROT>(a, (int64_t)blockIdx.x);
+}
+
+template <int DT, int NB, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void small_m_adapters_kernel(const SmallMArgs a, const WithAdapters ad) {
+    small_m_lds_body<DT, NB, WAVES, false>(a, (int64_t)blockIdx.x, ad);
 }
 
 // Several layers in one launch (the modulation projections of the image and of the text stream of a double-stream
@@ -388,6 +410,22 @@ int launch(const SmallMArgs &a, hipStream_t st) {
     dim3 grid((unsigned)((a.N + 3) / 4));
     if (vec) hipLaunchKernelGGL((small_m_kernel<DT, true>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((small_m_kernel<DT, false>), grid, dim3(256), 0, st, a);
+    return check_launch();
+}
+
+template <int DT>
+int launch_adapted(const SmallMArgs &a, const WithAdapters &ad, hipStream_t st) {
+    const bool vec = a.K % 16 == 0 && (uintptr_t)a.w % 16 == 0 && (uintptr_t)a.x % 16 == 0 && a.ldx % 8 == 0;
+    if (vec && a.K < (1ll << 30)) {
+        const int nb = blocks_to_workgroup(&a, 1);
+        const dim3 grid((unsigned)((a.N + 16 * nb - 1) / (16 * nb)));
+        if (nb == 1) hipLaunchKernelGGL((small_m_adapters_kernel<DT, 1, 8>), grid, dim3(512), 0, st, a, ad);
+        else if (nb == 2) hipLaunchKernelGGL((small_m_adapters_kernel<DT, 2, 8>), grid, dim3(512), 0, st, a, ad);
+        else hipLaunchKernelGGL((small_m_adapters_kernel<DT, 3, 8>), grid, dim3(512), 0, st, a, ad);
+        return check_launch();
+    }
+    dim3 grid((unsigned)((a.N + 3) / 4));
+    hipLaunchKernelGGL((small_m_kernel<DT, false, WithAdapters>), grid, dim3(256), 0, st, a, ad);
     return check_launch();
 }
 
@@ -500,4 +538,24 @@ extern "C" int i8f_internal_w8a16_rotated(const void *x, int x_dtype, int64_t M,
     a.x = x, a.M = M, a.K = K, a.ldx = ldx, a.N = N, a.w = w, a.ws = w_scale, a.ws_host = w_scale_host;
     a.row_scale = scale_mode == I8F_SCALE_ROW, a.bias = bias, a.bias_dtype = bias_dtype, a.out = out;
     return x_dtype == I8F_BF16 ? launch_lds<I8F_BF16, 1, 8, true>(a, (hipStream_t)stream) : launch_lds<I8F_F16, 1, 8, true>(a, (hipStream_t)stream);
+}
+
+extern "C" int i8f_linear_w8a16_small_m_adapters(const void *x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const int8_t *w, const float *w_scale,
+                                                 float w_scale_host, int scale_mode, const void *bias, int bias_dtype, const i8f_adapters *adapters,
+                                                 const void *t, void *out, int64_t N, void *stream) {
+    using namespace i8f;
+    if (M < 0 || N < 0 || K < 0 || (bias && !valid_dtype(bias_dtype))) return I8F_ERR_INVALID;
+    if (scale_mode != I8F_SCALE_TENSOR && scale_mode != I8F_SCALE_ROW) return I8F_ERR_INVALID;
+    if (int rc = validate_adapters(adapters, x_dtype, M)) return rc;
+    if (M > 16) return I8F_ERR_UNSUPPORTED;
+    if (M == 0 || N == 0) return I8F_OK;
+    if (!out || ldx < K || (K > 0 && (!x || !w)) || (scale_mode == I8F_SCALE_ROW && !w_scale)) return I8F_ERR_INVALID;
+    if (adapters->max_rank > 0 && (!t || (uintptr_t)t % 16)) return I8F_ERR_INVALID;
+    if (N > 0x7fffffffll * 4) return I8F_ERR_UNSUPPORTED;
+    if (int rc = check_device()) return rc;
+    SmallMArgs a{};
+    a.x = x, a.M = M, a.K = K, a.ldx = ldx, a.N = N, a.w = w, a.ws = w_scale, a.ws_host = w_scale_host;
+    a.row_scale = scale_mode == I8F_SCALE_ROW, a.bias = bias, a.bias_dtype = bias_dtype, a.out = out;
+    const WithAdapters ad{for_kernel(*adapters), t};
+    return x_dtype == I8F_BF16 ? launch_adapted<I8F_BF16>(a, ad, (hipStream_t)stream) : launch_adapted<I8F_F16>(a, ad, (hipStream_t)stream);
 }

@@ -84,5 +84,25 @@ __device__ __forceinline__ void rotate_run16(float (&v)[16], float s0, float s1,
     }
 }
 
+// A wave that holds one 128-block, two elements to a lane (any alignment).
+template <int DT>
+__device__ __forceinline__ void rotate128_wave(float &e0, float &e1, int lane) {
+    // the wave holds one 128-block: lane l has elements l (e0) and l + 64 (e1)
+#pragma unroll
+    for (int b = 1; b < 64; b <<= 1) {
+        const bool upper = (lane & b) != 0;
+        const float o0 = __shfl_xor(e0, b, 64);
+        const float o1 = __shfl_xor(e1, b, 64);
+        e0 = upper ? (o0 - e0) : (e0 + o0);
+        e1 = upper ? (o1 - e1) : (e1 + o1);
+    }
+    const float lo = e0, hi = e1;
+    e0 = lo + hi;
+    e1 = lo - hi;
+    const float h = hadamard_entry<DT>();
+    e0 = round_to_dtype<DT>(e0 * h);
+    e1 = round_to_dtype<DT>(e1 * h);
+}
+
 }  // namespace
 }  // namespace i8f

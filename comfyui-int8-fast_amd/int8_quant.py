@@ -161,6 +161,42 @@ def _fanout_native(layers, x, rotate, prologue, mod_scale, mod_shift, eps, norm_
                               int8_fused_kernel.DEFAULT_EPILOGUE, prologue, mod_scale, mod_shift, eps, norm_weight, bool(fused_add), None, None, work)
 
 
+def _scale_on(lin, device):
+    """A layer's weight scale as the kernels take it: a float, or a tensor on `device`, of which a one-scale layer has element 0."""
+    ws = lin._get_weight_scale()
+    if isinstance(ws, Tensor):
+        if ws.device != device:
+            ws = ws.to(device, non_blocking=True)
+        if not lin._is_per_row and ws.numel() != 1:
+            ws = ws.reshape(-1)[:1]
+    return ws
+
+
+def _project_quantised(layers, q, s, dtype):
+    """The layers' products of the same int8 rows: [M, out features] of `dtype` for each."""
+    problems = []
+    for lin in layers:
+        problems.append((q, s, lin.weight, _scale_on(lin, q.device), lin.bias))
+    # Layers of one form go out in one launch where the library finds that cheaper (8000 x 5120 into three of 5120 columns: 8 rounds of
+    # tiles for 9; 576 and 541 us, 3000 x 3584 into three 121 and 106 us).  Runs of them: a grouped call of several forms, or of more
+    # layers than a launch takes, looks at every operand twice (nine layers of 1536 columns on 300 x 512: 227 us a call, 173 one by one).
+    runs, last = [], None
+    for lin, p in zip(layers, problems):
+        form = (p[2].numel(), lin._is_per_row)   # (one width: as many elements, as many columns)
+        if form == last and len(runs[-1]) < _lib.MAX_LINEAR_GROUPS and len({r[4].dtype for r in (*runs[-1], p) if r[4] is not None}) < 2:
+            runs[-1].append(p)
+        else:
+            runs.append([p])
+            last = form
+    outs = []
+    for run in runs:
+        if len(run) == 1:
+            outs.append(_lib.linear_w8a8(*run[0], dtype, int8_fused_kernel.DEFAULT_EPILOGUE))
+        else:
+            outs += _lib.linear_w8a8_grouped(run, dtype, int8_fused_kernel.DEFAULT_EPILOGUE)
+    return outs
+
+
 def forward_fanout(layers, x, prologue: int = _lib.PRO_NONE, mod_scale=None, mod_shift=None, eps: float = 1e-6, norm_weight=None,
                    fused_add: bool = False):
     """[layer(x) for layer in layers] for quantised layers that read the same activations (separate q, k and v projections,
@@ -241,32 +277,7 @@ def forward_fanout(layers, x, prologue: int = _lib.PRO_NONE, mod_scale=None, mod
     lead = x.shape[:-1]
     q, s = _lib.quant_rowwise(x.reshape(-1, x.shape[-1]), rotate=rot, prologue=prologue, mod_scale=mod_scale, mod_shift=mod_shift,
                               eps=eps, norm_weight=norm_weight, fused_add=fused_add)
-    problems = []
-    for lin in layers:
-        ws = lin._get_weight_scale()
-        if isinstance(ws, Tensor):
-            if ws.device != x.device:
-                ws = ws.to(x.device, non_blocking=True)
-            if not lin._is_per_row and ws.numel() != 1:
-                ws = ws.reshape(-1)[:1]
-        problems.append((q, s, lin.weight, ws, lin.bias))
-    # Layers of one form go out in one launch where the library finds that cheaper (8000 x 5120 into three of 5120 columns: 8 rounds of
-    # tiles for 9; 576 and 541 us, 3000 x 3584 into three 121 and 106 us).  Runs of them: a grouped call of several forms, or of more
-    # layers than a launch takes, looks at every operand twice (nine layers of 1536 columns on 300 x 512: 227 us a call, 173 one by one).
-    runs, last = [], None
-    for lin, p in zip(layers, problems):
-        form = (p[2].numel(), lin._is_per_row)   # (one width: as many elements, as many columns)
-        if form == last and len(runs[-1]) < _lib.MAX_LINEAR_GROUPS and len({r[4].dtype for r in (*runs[-1], p) if r[4] is not None}) < 2:
-            runs[-1].append(p)
-        else:
-            runs.append([p])
-            last = form
-    outs = []
-    for run in runs:
-        if len(run) == 1:
-            outs.append(_lib.linear_w8a8(*run[0], x.dtype, int8_fused_kernel.DEFAULT_EPILOGUE))
-        else:
-            outs += _lib.linear_w8a8_grouped(run, x.dtype, int8_fused_kernel.DEFAULT_EPILOGUE)
+    outs = _project_quantised(layers, q, s, x.dtype)
     return [y.reshape(*lead, y.shape[-1]) for y in outs]
 
 
