@@ -933,12 +933,15 @@ def linear_w8a8_adapters(a, a_scale, w, w_scale, bias, bank, ids, rows_per_id, t
         if v.device != a.device:
             raise ValueError(f"{name} is on {v.device}, a is on {a.device}")
     out = torch.empty((M, N), dtype=bank.dtype, device=a.device)
-    work = torch.empty(lib().i8f_linear_w8a8_adapters_workspace_bytes(M, N, K), dtype=torch.uint8, device=a.device)
+    nbytes = lib().i8f_linear_w8a8_adapters_workspace_bytes(M, N, K)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=a.device) if nbytes else None
     arg = _adapters_arg(bank, ids, rows_per_id)
     with _on(a.device):
-        _check(lib().i8f_linear_w8a8_adapters(_ptr(a), _ptr(a_scale), _ptr(w), _ptr(ws), ws_host, mode, _ptr(bias), bcode, ctypes.byref(arg), _ptr(t),
-                                              _ptr(out), dtype_code(out.dtype), M, N, K, _ptr(work), work.numel(), _stream(a)),
-               "i8f_linear_w8a8_adapters")
+        status = lib().i8f_linear_w8a8_adapters(_ptr(a), _ptr(a_scale), _ptr(w), _ptr(ws), ws_host, mode, _ptr(bias), bcode, ctypes.byref(arg), _ptr(t),
+                                                _ptr(out), dtype_code(out.dtype), M, N, K, _ptr(work), nbytes, _stream(a))
+    if status == ERR_UNSUPPORTED:   # (operands that are not 16-byte aligned)
+        return adapters_up(linear_w8a8(a, a_scale, w, w_scale, bias, torch.float32, EPI_FUSED), bank, ids, rows_per_id, t)
+    _check(status, "i8f_linear_w8a8_adapters")
     return out
 
 

@@ -2,6 +2,8 @@
 // output types are instantiated in gemm_i8_f16.hip and gemm_i8_wide.hip.
 #include "gemm_i8_impl.hpp"
 
+#include "adapters.hpp"
+
 namespace i8f {
 namespace gemm {
 template int launch<OUT_BF16>(GemmArgs &, hipStream_t);
@@ -98,6 +100,47 @@ extern "C" int i8f_linear_w8a8_lora(const int8_t *a, const float *a_scale, const
     g.bias = bias, g.bias_dtype = bias_dtype, g.order = order, g.addend = nullptr;
     g.side_t = side_t, g.side_b = side_b, g.side_rank = (int)rank, g.side_has_alpha = has_alpha != 0, g.side_alpha = alpha;
     hipStream_t st = (hipStream_t)stream;
+    return out_dtype == I8F_BF16 ? launch<OUT_BF16>(g, st) : launch<OUT_F16>(g, st);
+}
+
+// Shapes that the tiled kernels take (others: the projection in binary32 in the workspace, then i8f_adapters_up)
+static bool adapters_fused(int64_t M, int64_t N, int64_t K) {
+    return K > 0 && K % 16 == 0 && N % 8 == 0 && N * K < (1ll << 31) && (M * K < (1ll << 31) || 256 * K < (1ll << 31));
+}
+extern "C" int64_t i8f_linear_w8a8_adapters_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    return M <= 0 || N <= 0 || adapters_fused(M, N, K) ? 0 : M * N * 4;
+}
+
+extern "C" int i8f_linear_w8a8_adapters(const int8_t *a, const float *a_scale, const int8_t *w, const float *w_scale, float w_scale_host, int scale_mode,
+                                        const void *bias, int bias_dtype, const i8f_adapters *adapters, const void *t, void *out, int out_dtype,
+                                        int64_t M, int64_t N, int64_t K, void *workspace, int64_t workspace_bytes, void *stream) {
+    using namespace i8f;
+    using namespace i8f::gemm;
+    if (int rc = validate_adapters(adapters, out_dtype, M)) return rc;
+    if (int rc = validate(a, w, M, N, K, out)) return rc;
+    if (bias && !valid_dtype(bias_dtype)) return I8F_ERR_INVALID;
+    if (scale_mode != I8F_SCALE_TENSOR && scale_mode != I8F_SCALE_ROW) return I8F_ERR_INVALID;
+    if (M == 0 || N == 0) return I8F_OK;
+    if (!a_scale || (scale_mode == I8F_SCALE_ROW && !w_scale)) return I8F_ERR_INVALID;
+    if (adapters->max_rank > 0 && (!t || (uintptr_t)t % 16)) return I8F_ERR_INVALID;
+    if (workspace && (uintptr_t)workspace % 16) return I8F_ERR_INVALID;
+    hipStream_t st = (hipStream_t)stream;
+    if (!adapters_fused(M, N, K)) {
+        if (!workspace || workspace_bytes < M * N * 4) return I8F_ERR_INVALID;
+        if (int rc = i8f_linear_w8a8(a, a_scale, w, w_scale, w_scale_host, scale_mode, bias, bias_dtype, workspace, I8F_F32, M, N, K, I8F_EPI_FUSED, stream))
+            return rc;
+        return i8f_adapters_up(workspace, I8F_F32, adapters, t, out, out_dtype, M, N, stream);
+    }
+    // 16-byte pieces of the operands, which any torch allocation has
+    if (((uintptr_t)a | (uintptr_t)w | (uintptr_t)out | (uintptr_t)bias) % 16 || (scale_mode == I8F_SCALE_ROW && (uintptr_t)w_scale % 16)) return I8F_ERR_UNSUPPORTED;
+    if (int rc = check_device()) return rc;
+    const i8f_adapters ad = for_kernel(*adapters);
+    GemmArgs g{};
+    g.x = a, g.w = w, g.M = (int)M, g.N = (int)N, g.K = (int)K, g.out = out;
+    g.xs = a_scale, g.ws = w_scale, g.ws_host = w_scale_host, g.row_scale = scale_mode == I8F_SCALE_ROW;
+    g.bias = bias, g.bias_dtype = bias_dtype, g.order = I8F_EPI_FUSED;
+    g.side_t = t, g.side_b = ad.up, g.side_rank = (int)ad.max_rank;
+    g.ids = ad.ids, g.first_rank = ad.first_rank, g.rows_per_id = (int)ad.rows_per_id, g.adapters = ad.max_rank > 0 ? (int)ad.count : 0;
     return out_dtype == I8F_BF16 ? launch<OUT_BF16>(g, st) : launch<OUT_F16>(g, st);
 }
 

@@ -90,6 +90,10 @@ struct GemmArgs {
     const void *side_t, *side_b;
     int side_rank, side_has_alpha;
     float side_alpha;
+    // adapters of the rows (i8f_linear_w8a8_adapters): row m takes adapter ids[(row0 + m) / rows_per_id], side_t [M, side_rank] holds its first
+    // product, side_b the adapters' second factors, from element N * first_rank[a] on
+    const int *ids, *first_rank;
+    int rows_per_id, adapters, row0;
     void *out;
     int tiles_m, tiles_n;
     // K split over `splits` workgroups per tile (1: none): partial sums and per-tile arrival counters in caller memory
@@ -302,13 +306,189 @@ __device__ __forceinline__ uint4 mul_rounded(uint4 y, uint4 s) {
     }
 }
 
+// 16 x 16 x 32 product of two 16-bit fragments (8 values per lane each) into a binary32 block
+template <int OUT>
+__device__ __forceinline__ v4f side_mfma32(v4i a, v4i b, v4f c) {
+    if constexpr (OUT == OUT_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf_t, a), __builtin_bit_cast(v8bf_t, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h_t, a), __builtin_bit_cast(v8h_t, b), c, 0, 0, 0);
+}
+
+// The epilogue with an adapter for every row: out = round(acc * (xs * ws) + bias + sum_j t[m,j] B_a[n,j]).
+// A block of CB columns after the other, its accumulators become the projection's binary32 values and the matrix unit adds the adapters'
+// products to them, with the operand roles of the main product (rows n from B_a, columns m from t): no second set of accumulators, any
+// number of adapters and ranks, one rounding at the end.  A wave goes through the adapters that occur in its rows.  A product's column
+// depends on its own row of t alone, so rows of other adapters are left out by keeping what they had (a select per lane: a lane's values
+// belong to one row); zeros in t instead would let an adapter that is not finite into every row of the tile.
+// Where all rows of the wave have one adapter of up to 64 ranks, as in a batch of long requests, their t is fetched once and
+// nothing is selected.  (Blocks of columns innermost, with all accumulators converted first, took 40 to 200 spilled registers.)
+template <class C, int OUT, class ACC, class ACC16>
+__device__ __forceinline__ void adapters_epilogue(const GemmArgs &g, const int gM, const int gN, const int m0, const int n0, const int wm, const int wn,
+                                                  const int lane, const float *s_xs, const float *s_ws, const float *s_bias, char *ebuf, ACC &acc,
+                                                  ACC16 &acc16, void *gout) {
+    static_assert(OUT == OUT_BF16 || OUT == OUT_F16, "16-bit factors");
+    constexpr bool M16 = C::MF == 16;
+    constexpr int MI = C::MI, NJ = C::NJ, CB = C::CB, GR = M16 ? 16 : 32, GROUPS = C::WTM / GR;   // groups of rows, of which a lane has one row each
+    constexpr int STEP = M16 ? 32 : 16, QPG = M16 ? 1 : 4;                                       // ranks of a product; quads of a group and column block
+    typedef typename std::conditional<M16, v4f, v16f>::type block_t;
+    const int l16 = lane & 15, lq = lane >> 4, l32 = lane & 31, lhalf = lane >> 5;
+    const int mw = m0 + wm * C::WTM, nw = n0 + wn * C::WTN;
+    const int lrow = M16 ? l16 : l32, lk = (M16 ? lq : lhalf) * 8;
+    auto mma = [](v4i b, v4i t, block_t c) -> block_t {
+        if constexpr (M16) return side_mfma32<OUT>(b, t, c);
+        else return side_mfma<OUT>(b, t, c);
+    };
+    // the adapter of the lane's row in each group
+    int id[GROUPS];
+    uint64_t todo[GROUPS];
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) {
+        const int m = mw + i * GR + lrow;
+        const int a = g.ids[(uint32_t)(g.row0 + min(m, gM - 1)) / (uint32_t)g.rows_per_id];
+        id[i] = m < gM && (uint32_t)a < (uint32_t)g.adapters ? a : -1;
+        todo[i] = __builtin_amdgcn_ballot_w64(id[i] >= 0);
+    }
+    // the first of the adapters that are left, taken out of todo; -1: none
+    auto next_adapter = [&](uint64_t (&left)[GROUPS]) {
+        int a = -1;
+#pragma unroll
+        for (int i = GROUPS - 1; i >= 0; --i)
+            if (left[i]) a = __builtin_amdgcn_readlane(id[i], __builtin_ctzll(left[i]));
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) left[i] &= ~__builtin_amdgcn_ballot_w64(id[i] == a);
+        return a;
+    };
+    // rows of t and of a factor as buffers (rows and columns past the matrices load zeros)
+    const auto tr = buffer_at(g.side_t, (int64_t)mw * g.side_rank * 2, (int64_t)min(gM - mw, C::WTM) * g.side_rank * 2);
+    auto factor = [&](int first, int rank) {
+        return buffer_at(g.side_b, ((int64_t)gN * first + (int64_t)nw * rank) * 2, (int64_t)min(gN - nw, C::WTN) * rank * 2);
+    };
+    // (the lane's eight ranks from k0 on; past the adapter's last one, which may be half a step of 32, an offset that loads zeros)
+    auto rank_at = [&](int k0, int rank) { return k0 + lk < rank ? (uint32_t)(k0 + lk) * 2u : 0x80000000u; };
+    auto load_t = [&](int i, uint32_t kb) { return __builtin_bit_cast(v4i, buffer_load16(tr, (uint32_t)((i * GR + lrow) * g.side_rank * 2) + kb)); };
+    auto load_b = [&](__amdgpu_buffer_rsrc_t b, int j, int rank, uint32_t kb) {
+        return __builtin_bit_cast(v4i, buffer_load16(b, (uint32_t)((j * CB + lrow) * rank * 2) + kb));
+    };
+    constexpr int ROW_BYTES = C::WTN * 2, PITCH = ROW_BYTES + 8, CPO = ROW_BYTES / 16;
+    // a block's projection in the operation order of I8F_EPI_FUSED, and its way to LDS
+    auto project = [&](int j, block_t (&f)[GROUPS]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int qd = 0; qd < QPG; ++qd) {
+            const int nl = wn * C::WTN + j * CB + (M16 ? lq * 4 : qd * 8 + lhalf * 4);
+            const float4 w4 = *(const float4 *)&s_ws[nl], b4 = *(const float4 *)&s_bias[nl];
+#pragma unroll
+            for (int i = 0; i < GROUPS; ++i) {
+                const float xs = s_xs[wm * C::WTM + i * GR + lrow];
+                int a4[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (M16) a4[e] = acc16[i >> 1][j][i & 1][e];
+                    else a4[e] = acc[i][j][4 * qd + e];
+                }
+                f[i][4 * qd] = (float)a4[0] * (xs * w4.x) + b4.x, f[i][4 * qd + 1] = (float)a4[1] * (xs * w4.y) + b4.y;
+                f[i][4 * qd + 2] = (float)a4[2] * (xs * w4.z) + b4.z, f[i][4 * qd + 3] = (float)a4[3] * (xs * w4.w) + b4.w;
+            }
+        }
+    };
+    auto stage = [&](int j, const block_t (&f)[GROUPS]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i)
+#pragma unroll
+            for (int qd = 0; qd < QPG; ++qd) {
+                const float v[4] = {f[i][4 * qd], f[i][4 * qd + 1], f[i][4 * qd + 2], f[i][4 * qd + 3]};
+                char *dst = ebuf + (i * GR + lrow) * PITCH + (j * CB + (M16 ? lq * 4 : qd * 8 + lhalf * 4)) * 2;
+                if constexpr (OUT == OUT_BF16) *(uint2 *)dst = make_uint2(f32x2_to_bf16x2_bits(v[0], v[1]), f32x2_to_bf16x2_bits(v[2], v[3]));
+                else *(uint2 *)dst = make_uint2(f32x2_to_f16x2_bits(v[0], v[1]), f32x2_to_f16x2_bits(v[2], v[3]));
+            }
+    };
+    const int a0 = next_adapter(todo);
+    bool one = a0 < 0;   // no adapter, or one for all rows, of up to 64 ranks
+    int first0 = 0, rank0 = 0;
+    if (a0 >= 0) {
+        first0 = __builtin_amdgcn_readfirstlane(g.first_rank[a0]), rank0 = __builtin_amdgcn_readfirstlane(g.first_rank[a0 + 1]) - first0;
+        one = rank0 <= 64;
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) one = one && __builtin_amdgcn_ballot_w64(id[i] == a0 || mw + i * GR + lrow >= gM) == ~0ull;
+    }
+    if (one) {
+        constexpr int KS = 64 / STEP;
+        const auto up = factor(first0, rank0);
+        v4i tf[KS][GROUPS];
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int i = 0; i < GROUPS; ++i) tf[s][i] = load_t(i, rank_at(s * STEP, rank0));
+        constexpr int AHEAD = C::NT <= 512 ? 1 : 0;   // (twelve waves have no registers for the next block's factors)
+        v4i bf[AHEAD + 1][KS];
+        auto fetch = [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) bf[j & AHEAD][s] = load_b(up, j, rank0, rank_at(s * STEP, rank0));
+        };
+        if (AHEAD) fetch(0);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            if (j + AHEAD < NJ) fetch(j + AHEAD);
+            block_t f[GROUPS];
+            project(j, f);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                if (s * STEP < rank0) {
+#pragma unroll
+                    for (int i = 0; i < GROUPS; ++i) f[i] = mma(bf[j & AHEAD][s], tf[s][i], f[i]);
+                }
+            }
+            stage(j, f);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            block_t f[GROUPS];
+            project(j, f);
+            uint64_t left[GROUPS];
+#pragma unroll
+            for (int i = 0; i < GROUPS; ++i) left[i] = __builtin_amdgcn_ballot_w64(id[i] >= 0);
+            for (int a = next_adapter(left); a >= 0; a = next_adapter(left)) {
+                const int first = __builtin_amdgcn_readfirstlane(g.first_rank[a]), rank = __builtin_amdgcn_readfirstlane(g.first_rank[a + 1]) - first;
+                const auto up = factor(first, rank);
+                for (int k0 = 0; k0 < rank; k0 += STEP) {
+                    const uint32_t kb = rank_at(k0, rank);
+                    const v4i bf = load_b(up, j, rank, kb);
+                    v4i tf[GROUPS];
+#pragma unroll
+                    for (int i = 0; i < GROUPS; ++i) tf[i] = load_t(i, kb);
+#pragma unroll
+                    for (int i = 0; i < GROUPS; ++i) {
+                        const block_t sum = mma(bf, tf[i], f[i]);
+#pragma unroll
+                        for (int e = 0; e < 4 * QPG; ++e) f[i][e] = id[i] == a ? sum[e] : f[i][e];
+                    }
+                }
+            }
+            stage(j, f);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    // rows from LDS, 16 bytes to a lane
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int p = 0; p < C::WTM * CPO / 64; ++p) {
+        const int at = p * 64 + lane, row = at / CPO, cc = at % CPO;
+        const int mm = mw + row, nn = nw + cc * 8;
+        if (mm < gM && nn < gN) stream_store16((char *)gout + ((int64_t)mm * gN + nn) * 2, *(const uint4 *)(ebuf + row * PITCH + cc * 16));
+    }
+}
+
 // KTAIL: K is not a multiple of BK (the last tile is ragged); the common case is the other kernel.
 // What the prologue needs (operand pointers, sizes, tile counts) comes first in the argument list: the
 // first 16 dwords of the kernel arguments are preloaded into SGPRs at wave launch, the rest (epilogue
 // operands) is fetched by scalar loads that have the whole main loop to land.
 // (The body is shared by the kernel of one problem and the kernel of a group of problems: wg_id is the workgroup's
 // number within its problem, gout / gaddend / ggate / ws_host that problem's output, addend, gate and host-side weight scale.)
-template <class C, int OUT, bool KTAIL, bool SIDE = false, bool SPLITK = false>
+template <class C, int OUT, bool KTAIL, bool SIDE = false, bool SPLITK = false, bool ADAPT = false>
 __device__ __forceinline__ void gemm_i8_body(const int8_t *gx, const int8_t *gw, int gM, int gN, int gK, int tiles_m, int tiles_n,
                                              const float *gxs, const float *gws, const void *gbias, int flags, const GemmArgs &g,
                                              const int wg_id, void *gout, const void *gaddend, const float ws_host,
@@ -1128,6 +1308,8 @@ __device__ __forceinline__ void gemm_i8_body(const int8_t *gx, const int8_t *gw,
     using S0 = std::integral_constant<int, 0>;
     if constexpr (OUT == OUT_I32) {
         run_epilogue(O0{}, F_{}, F_{}, S0{}, F_{});  // (the raw product: no gate and no addend)
+    } else if constexpr (ADAPT) {
+        adapters_epilogue<C, OUT>(g, gM, gN, m0, n0, wm, wn, lane, s_xs, s_ws, s_bias, ebuf, acc, acc16, gout);
     } else if constexpr (SIDE) {  // (no gate and no addend beside a side branch)
         if (g.side_rank > 32) choose(std::integral_constant<int, 4>{});
         else choose(std::integral_constant<int, 2>{});
@@ -1142,6 +1324,14 @@ __global__ __launch_bounds__(C::NT) void gemm_i8_kernel(const int8_t *gx, const 
                                                         const GemmArgs g) {
     gemm_i8_body<C, OUT, KTAIL, SIDE, SPLITK>(gx, gw, gM, gN, gK, tiles_m, tiles_n, gxs, gws, gbias, flags, g, (int)blockIdx.x, g.out,
                                               g.addend, g.ws_host, g.gate, g.gate_rows);
+}
+
+// the same with an adapter for every row
+template <class C, int OUT, bool KTAIL>
+__global__ __launch_bounds__(C::NT) void gemm_i8_adapters_kernel(const int8_t *gx, const int8_t *gw, int gM, int gN, int gK, int tiles_m, int tiles_n,
+                                                                 const float *gxs, const float *gws, const void *gbias, int flags, const GemmArgs g) {
+    gemm_i8_body<C, OUT, KTAIL, false, false, true>(gx, gw, gM, gN, gK, tiles_m, tiles_n, gxs, gws, gbias, flags, g, (int)blockIdx.x, g.out, nullptr,
+                                                    g.ws_host, nullptr, 1);
 }
 
 // Several problems of one layer shape (N, K, scale mode, dtypes) with their own activations, weights and outputs in
@@ -1216,6 +1406,17 @@ int launch_cfg(GemmArgs &g, hipStream_t st) {
     g.tiles_n = (g.N + C::BN - 1) / C::BN;
     const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n;
     const int flags = (g.row_scale ? 1 : 0) | (g.bias_dtype << 1);  // what the prologue wants to know of the epilogue
+    if (g.ids) {
+        if constexpr (OUT == OUT_BF16 || OUT == OUT_F16) {
+            auto go = [&](auto kernel) {
+                hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(C::NT), 0, st, g.x, g.w, g.M, g.N, g.K, g.tiles_m, g.tiles_n, g.xs, g.ws, g.bias, flags, g);
+                return check_launch();
+            };
+            return g.K % C::BK ? go(gemm_i8_adapters_kernel<C, OUT, true>) : go(gemm_i8_adapters_kernel<C, OUT, false>);
+        } else {
+            return I8F_ERR_UNSUPPORTED;
+        }
+    }
     if (g.side_t) {  // validated by the entry point: K % BK == 0 here
         if constexpr (OUT == OUT_BF16 || OUT == OUT_F16) {
             hipLaunchKernelGGL((gemm_i8_kernel<C, OUT, false, true>), dim3((unsigned)tiles), dim3(C::NT), 0, st, g.x, g.w, g.M, g.N,
@@ -1402,18 +1603,20 @@ int launch(GemmArgs &g, hipStream_t st) {
                 sub.gate = (const char *)g.gate + (m0 / g.gate_rows) * g.N * ob;
             }
             if (g.side_t) sub.side_t = (const char *)g.side_t + m0 * g.side_rank * 2;
+            sub.row0 = g.row0 + (int)m0;
             if (int rc = launch<OUT>(sub, st)) return rc;
         }
         return I8F_OK;
     }
     const bool fast = aligned && ((int64_t)g.M * g.K < (1ll << 31));
-    if (g.side_t && (!fast || g.K % 128 || (uintptr_t)g.side_t % 16 || (uintptr_t)g.side_b % 16)) return I8F_ERR_UNSUPPORTED;
+    if (g.ids && !fast) return I8F_ERR_UNSUPPORTED;
+    if (g.side_t && !g.ids && (!fast || g.K % 128 || (uintptr_t)g.side_t % 16 || (uintptr_t)g.side_b % 16)) return I8F_ERR_UNSUPPORTED;
     if (!fast) {
         return launch_ragged<OUT>(g, st);
     }
     Tile t = choose_tile(g.M, g.N);
     int splits = 1;
-    if (g.partials && !g.side_t) choose_split(g.M, g.N, g.K, t, splits);
+    if (g.partials && !g.side_t && !g.ids) choose_split(g.M, g.N, g.K, t, splits);
     g.splits = splits;
     if (splits > 1) {
         static std::atomic<uint32_t> launches{0};
