@@ -1,5 +1,7 @@
 // Between two blocks: the norm behind a block, its gate and the scales of branch and residual stream, and the norm and modulation in
 // front of the next block, in one pass over the two rows that it takes (include/i8f_blocks.h has the formula).
+#include <type_traits>
+
 #include "i8f_common.hpp"
 #include "quant_run.hpp"
 #include "rotate_run.hpp"
@@ -106,8 +108,264 @@ __global__ __launch_bounds__(256) void block_norm_generic_kernel(const i8f_block
     }
 }
 
+// ---- rows that stay in registers --------------------------------------------------------------------------------------------
+// Both rows are read once, the sums are taken over registers: 7 or 8 bytes an element in 16 bits, which is what bounds it.
+// WPR waves share a row, a lane holds NCH runs of RUN consecutive elements (32 bytes of a 16-bit row, 16 of a binary32 one).  How many waves
+// a row gets depends on its width alone, so that a row's bits depend neither on the rows beside it nor on what becomes of h.
+template <int DT>
+struct Run {
+    static constexpr int N = DT == I8F_F32 ? 4 : 16;
+};
+
+// a lane's sum over the wave, in a fixed order: within quads, halves of rows and rows of 16 lanes, then across rows (as wave_max)
+__device__ __forceinline__ float wave_sum_dpp(float v) {
+    auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+        const int moved = __builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+        v += __int_as_float(moved);
+    };
+    using std::integral_constant;
+    add(integral_constant<int, 0xb1>{}, integral_constant<int, 0xf>{});    // quad_perm [1,0,3,2]
+    add(integral_constant<int, 0x4e>{}, integral_constant<int, 0xf>{});    // quad_perm [2,3,0,1]
+    add(integral_constant<int, 0x141>{}, integral_constant<int, 0xf>{});   // row_half_mirror
+    add(integral_constant<int, 0x140>{}, integral_constant<int, 0xf>{});   // row_mirror
+    add(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});   // row_bcast 15 into rows 1 and 3
+    add(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});   // row_bcast 31 into rows 2 and 3
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
+template <int DT>
+struct Raw {
+    uint4 v[DT == I8F_F32 ? 1 : 2];
+};
+template <int DT>
+__device__ __forceinline__ Raw<DT> load_run(const char *p) {
+    Raw<DT> r;
+    r.v[0] = *(const uint4 *)p;
+    if constexpr (DT != I8F_F32) r.v[1] = *(const uint4 *)(p + 16);
+    return r;
+}
+template <int DT>
+__device__ __forceinline__ void expand(const Raw<DT> &r, float (&v)[Run<DT>::N]) {
+    if constexpr (DT == I8F_F32) v[0] = __uint_as_float(r.v[0].x), v[1] = __uint_as_float(r.v[0].y), v[2] = __uint_as_float(r.v[0].z), v[3] = __uint_as_float(r.v[0].w);
+    else expand16<DT>(r.v[0], r.v[1], v);
+}
+template <int DT>
+__device__ __forceinline__ void store_run(char *p, const float (&v)[Run<DT>::N]) {
+    if constexpr (DT == I8F_F32) {
+        stream_store16(p, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
+    } else {
+        uint32_t o[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = DT == I8F_BF16 ? f32x2_to_bf16x2_bits(v[2 * e], v[2 * e + 1]) : f32x2_to_f16x2_bits(v[2 * e], v[2 * e + 1]);
+        stream_store16(p, make_uint4(o[0], o[1], o[2], o[3]));
+        stream_store16(p + 16, make_uint4(o[4], o[5], o[6], o[7]));
+    }
+}
+// the run of a weight or bias that starts at element k
+template <int DT>
+__device__ __forceinline__ void operand_run(const void *p, int dtype, int64_t k, float (&v)[Run<DT>::N]) {
+    if (DT != I8F_F32 && dtype == I8F_F32) {
+#pragma unroll
+        for (int e = 0; e < Run<DT>::N; e += 4) {
+            const float4 f = *(const float4 *)((const float *)p + k + e);
+            v[e] = f.x, v[e + 1] = f.y, v[e + 2] = f.z, v[e + 3] = f.w;
+        }
+    } else {
+        expand<DT>(load_run<DT>((const char *)p + k * (DT == I8F_F32 ? 4 : 2)), v);
+    }
+}
+
+template <int DT, int H, int WPR, int NCH>
+__global__ __launch_bounds__(256) void block_norm_kernel(const i8f_block_norm_args a) {
+    constexpr int N = Run<DT>::N, TPR = 64 * WPR, ROWS = 4 / WPR, SIZE = DT == I8F_F32 ? 4 : 2;
+    __shared__ float red[5][ROWS][WPR];
+    const int t = threadIdx.x % TPR, rb = threadIdx.x / TPR, lane = threadIdx.x & 63;
+    const int64_t K = a.K;
+    const int runs = (int)(K / N);
+    const int64_t own = (int64_t)blockIdx.x * ROWS + rb;
+    const bool ok = own < a.M;
+    const int64_t m = ok ? own : a.M - 1;   // (a wave past the last row computes it again and stores nothing)
+    // which of its runs a lane holds: its own, or where the rotation pairs lanes by DPP the one that it wants there (rotate_run16,
+    // rotate_chunk_f32); the sums pair the same runs either way
+    const int p = H != H_INT8_ROTATED ? t : DT == I8F_F32 ? (t & ~15) | chunk_of_lane16(t & 15) : t ^ (((t >> 2) & 1) * 3);
+    auto sum_over_row = [&](float part, int slot) {
+        part = wave_sum_dpp(part);
+        if constexpr (WPR > 1) {   // (a slot for each sum: nobody waits for its readers)
+            if (lane == 0) red[slot][rb][t / 64] = part;
+            __syncthreads();
+            part = red[slot][rb][0];
+#pragma unroll
+            for (int w = 1; w < WPR; ++w) part += red[slot][rb][w];
+        }
+        return part;
+    };
+    int64_t at[NCH];   // first element of each run; a lane without one takes the row's first and leaves it out of the sums
+    bool in[NCH];
+    Raw<DT> yr[NCH], rr[NCH];
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        in[i] = i * TPR + p < runs;
+        at[i] = in[i] ? (int64_t)(i * TPR + p) * N : 0;
+        yr[i] = load_run<DT>((const char *)a.y + (m * a.ldy + at[i]) * SIZE);
+        rr[i] = load_run<DT>((const char *)a.residual + (m * a.ldr + at[i]) * SIZE);
+    }
+    float x[NCH][N];
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) expand<DT>(yr[i], x[i]);
+    // (x - mean) * rstd * weight + bias of the rows in x, in place
+    auto normalise = [&](int norm, float eps, const void *w, const void *b, int dtype, int slot) __attribute__((always_inline)) {
+        if (norm == I8F_NORM_NONE) return;
+        if (norm == I8F_NORM_LAYER) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NCH; ++i)
+#pragma unroll
+                for (int e = 0; e < N; ++e) sum += in[i] ? x[i][e] : 0.0f;
+            const float mean = sum_over_row(sum, slot) / (float)K;
+#pragma unroll
+            for (int i = 0; i < NCH; ++i)
+#pragma unroll
+                for (int e = 0; e < N; ++e) x[i][e] -= mean;
+        }
+        float squares = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            float s = 0.0f;
+#pragma unroll
+            for (int e = 0; e < N; ++e) s = __builtin_fmaf(x[i][e], x[i][e], s);
+            squares += in[i] ? s : 0.0f;
+        }
+        const float rstd = 1.0f / sqrtf(sum_over_row(squares, slot + 1) / (float)K + eps);
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            float v[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[i][e] *= rstd;
+            if (w) {
+                operand_run<DT>(w, dtype, at[i], v);
+#pragma unroll
+                for (int e = 0; e < N; ++e) x[i][e] *= v[e];
+            }
+            if (b) {
+                operand_run<DT>(b, dtype, at[i], v);
+#pragma unroll
+                for (int e = 0; e < N; ++e) x[i][e] += v[e];
+            }
+        }
+    };
+    auto vector_of = [&](const void *v, int64_t rows_per) { return (const char *)v + (int64_t)((uint32_t)m / (uint32_t)rows_per) * K * SIZE; };
+    normalise(a.post_norm, a.post_eps, a.post_weight, a.post_bias, a.post_dtype, 0);
+    const char *gate = a.gate ? vector_of(a.gate, a.rows_per_gate) : nullptr;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        float r[N], g[N];
+        expand<DT>(rr[i], r);
+        if (gate) {
+            expand<DT>(load_run<DT>(gate + at[i] * SIZE), g);
+            if (a.gate_tanh) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) g[e] = gate_tanh<DT>(g[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[i][e] = __builtin_fmaf(x[i][e], g[e] * a.branch_scale, a.residual_scale * r[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[i][e] = __builtin_fmaf(x[i][e], a.branch_scale, a.residual_scale * r[e]);
+        }
+        if (ok && in[i]) store_run<DT>((char *)a.x_out + (m * K + at[i]) * SIZE, x[i]);
+    }
+    if constexpr (H == H_NONE) return;
+    normalise(a.pre_norm, a.pre_eps, a.pre_weight, a.pre_bias, a.pre_dtype, 2);
+    const char *ms = a.mod_scale ? vector_of(a.mod_scale, a.rows_per_scale) : nullptr, *mt = a.mod_shift ? vector_of(a.mod_shift, a.rows_per_shift) : nullptr;
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        float v[N];
+        if (ms) {
+            expand<DT>(load_run<DT>(ms + at[i] * SIZE), v);
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[i][e] *= 1.0f + v[e];
+        }
+        if (mt) {
+            expand<DT>(load_run<DT>(mt + at[i] * SIZE), v);
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[i][e] += v[e];
+        }
+        if constexpr (H == H_STORED) {
+            if (ok && in[i]) store_run<DT>((char *)a.h + (m * K + at[i]) * SIZE, x[i]);
+        } else {   // i8f_quant_rowwise's arithmetic on the rounded h
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[i][e] = in[i] ? round_to_dtype<DT>(x[i][e]) : 0.0f;
+            if constexpr (H == H_INT8_ROTATED) {
+                if constexpr (DT == I8F_F32) rotate_chunk_f32(x[i], t);
+                else rotate_run16<DT>(x[i], (p & 1) ? -1.0f : 1.0f, (p & 2) ? -1.0f : 1.0f, (p & 4) ? -1.0f : 1.0f);
+            }
+#pragma unroll
+            for (int e = 0; e < N; e += 2) amax = max3_abs(amax, x[i][e], x[i][e + 1]);
+        }
+    }
+    if constexpr (H == H_INT8 || H == H_INT8_ROTATED) {
+        amax = wave_max(amax);
+        if constexpr (WPR > 1) {
+            if (lane == 0) red[4][rb][t / 64] = amax;
+            __syncthreads();
+            amax = red[4][rb][0];
+#pragma unroll
+            for (int w = 1; w < WPR; ++w) amax = fmaxf(amax, red[4][rb][w]);
+        }
+        float s, inv;
+        if constexpr (DT == I8F_F32) {
+            s = amax / 127.0f;
+            s = s < 1e-30f ? 1e-30f : s;
+            inv = 1.0f / s;
+        } else {
+            scale_and_inverse16(amax, s, inv);
+        }
+        if (!ok) return;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            if (!in[i]) continue;
+            int8_t *dst = a.q + m * K + at[i];
+            if constexpr (DT == I8F_F32) {
+                uint32_t w = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w |= ((uint32_t)quant_i8(x[i][e] * inv) & 0xffu) << (8 * e);
+                *(uint32_t *)dst = w;
+            } else {
+                stream_store16(dst, quant16_magic(x[i], inv));
+            }
+        }
+        if (t == 0) a.scale[m] = s;
+    }
+}
+
+template <int DT, int H, int WPR, int NCH>
+int launch_rows(const i8f_block_norm_args &a, hipStream_t st) {
+    constexpr int ROWS = 4 / WPR;
+    hipLaunchKernelGGL((block_norm_kernel<DT, H, WPR, NCH>), dim3((unsigned)((a.M + ROWS - 1) / ROWS)), dim3(256), 0, st, a);
+    return check_launch();
+}
+
+// Aligned rows of whole runs; 16-byte pieces of every operand
+bool in_registers(const i8f_block_norm_args &a, int run) {
+    const uintptr_t all = (uintptr_t)a.y | (uintptr_t)a.residual | (uintptr_t)a.post_weight | (uintptr_t)a.post_bias | (uintptr_t)a.pre_weight |
+                          (uintptr_t)a.pre_bias | (uintptr_t)a.gate | (uintptr_t)a.mod_scale | (uintptr_t)a.mod_shift | (uintptr_t)a.x_out |
+                          (uintptr_t)a.h | (uintptr_t)a.q;
+    const int64_t per16 = 16 / (int64_t)dtype_size(a.dtype);
+    return all % 16 == 0 && a.K % run == 0 && a.K / run <= 1024 && a.ldy % per16 == 0 && a.ldr % per16 == 0;
+}
+
 template <int DT, int H>
 int launch(const i8f_block_norm_args &a, hipStream_t st) {
+    if (in_registers(a, Run<DT>::N)) {
+        const int runs = (int)(a.K / Run<DT>::N);
+        if (runs <= 64) return launch_rows<DT, H, 1, 1>(a, st);
+        if (runs <= 128) return launch_rows<DT, H, 1, 2>(a, st);
+        if (runs <= 256) return launch_rows<DT, H, 4, 1>(a, st);
+        if (runs <= 512) return launch_rows<DT, H, 4, 2>(a, st);
+        if (runs <= 768) return launch_rows<DT, H, 4, 3>(a, st);
+        return launch_rows<DT, H, 4, 4>(a, st);
+    }
     hipLaunchKernelGGL((block_norm_generic_kernel<DT, H>), dim3((unsigned)a.M), dim3(256), 0, st, a);
     return check_launch();
 }
@@ -149,9 +407,11 @@ extern "C" int i8f_block_norm(const i8f_block_norm_args *args, void *stream) {
     if (a.M == 0 || a.K == 0) return I8F_OK;
     if (int rc = check_device()) return rc;
     hipStream_t st = (hipStream_t)stream;
-    switch (a.dtype) {
-    case I8F_BF16: return dispatch<I8F_BF16>(a, st);
-    case I8F_F16: return dispatch<I8F_F16>(a, st);
-    default: return dispatch<I8F_F32>(a, st);
+    i8f_block_norm_args k = a;   // (M is below 2^31, and so are the rows of a vector then)
+    for (int64_t *rows : {&k.rows_per_gate, &k.rows_per_scale, &k.rows_per_shift}) *rows = *rows < 1 ? 1 : *rows > 0x7fffffff ? 0x7fffffff : *rows;
+    switch (k.dtype) {
+    case I8F_BF16: return dispatch<I8F_BF16>(k, st);
+    case I8F_F16: return dispatch<I8F_F16>(k, st);
+    default: return dispatch<I8F_F32>(k, st);
     }
 }
