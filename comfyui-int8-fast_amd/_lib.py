@@ -84,12 +84,12 @@ def lib() -> ctypes.CDLL:
     L.i8f_lora_merge_sr_drawn.argtypes = [vp, vp, f32, i32, vp, i32, f32, ctypes.c_uint64, i64, i64, i64, vp, vp, i64, vp]
     L.i8f_lora_merge_sr_drawn_workspace_bytes.argtypes = [i64, i64, i64, i32]
     L.i8f_lora_merge_sr_drawn_workspace_bytes.restype = i64
-    L.i8f_adapters_down.argtypes = [vp, i32, i64, i64, i64, vp, vp, vp]
+    L.i8f_adapters_down.argtypes = [vp, i32, i64, i64, i64, vp, i32, i32, vp, vp, vp]
     L.i8f_adapters_up.argtypes = [vp, i32, vp, vp, vp, i32, i64, i64, vp]
     L.i8f_linear_w8a8_adapters_workspace_bytes.argtypes = [i64, i64, i64]
     L.i8f_linear_w8a8_adapters_workspace_bytes.restype = i64
-    L.i8f_linear_w8a8_adapters.argtypes = [vp, vp, vp, vp, f32, i32, vp, i32, vp, vp, vp, i32, i64, i64, i64, vp, i64, vp]
-    L.i8f_linear_w8a16_small_m_adapters.argtypes = [vp, i32, i64, i64, i64, vp, vp, f32, i32, vp, i32, vp, vp, vp, i64, vp]
+    L.i8f_linear_w8a8_adapters.argtypes = [vp, vp, vp, i32, i32, i64, i64, vp, i64, vp]
+    L.i8f_linear_w8a16_small_m_adapters.argtypes = [vp, i32, i64, i64, i64, vp, i32, vp]
     L.i8f_block_norm.argtypes = [vp, vp]
     for name in BLOCK_EXPORTS:
         if not name.endswith("_bytes"):
@@ -881,25 +881,41 @@ class _Adapters(ctypes.Structure):
                 ("ids", ctypes.c_void_p), ("rows_per_id", ctypes.c_int64), ("count", ctypes.c_int64), ("max_rank", ctypes.c_int64)]
 
 
+class _AdaptedLayer(ctypes.Structure):
+    _fields_ = [("w", ctypes.c_void_p), ("w_scale", ctypes.c_void_p), ("w_scale_host", ctypes.c_float), ("scale_mode", ctypes.c_int), ("bias", ctypes.c_void_p),
+                ("bias_dtype", ctypes.c_int), ("N", ctypes.c_int64), ("adapters", _Adapters), ("t", ctypes.c_void_p), ("out", ctypes.c_void_p)]
+
+
+MAX_ADAPTED_LAYERS = 4
+
+
 def _adapters_arg(bank, ids, rows_per_id):
     """The C structure of a bank (adapters.AdapterBank) and the adapter numbers of a batch."""
     return _Adapters(_addr(bank.down), _addr(bank.up), _addr(bank.scale), _addr(bank.first_rank), _addr(ids), rows_per_id, bank.count, bank.max_rank)
 
 
-def adapters_down(x, bank, ids, rows_per_id=1):
-    """t [M, bank.max_rank] of x [M,K]: row m holds scale_a * A_a x[m] for its adapter a = ids[m // rows_per_id] in its first ranks; what lies
-    behind them, and rows without an adapter, are not written.  ids: int32, contiguous, one for each rows_per_id rows."""
+def adapters_down(x, banks, ids, rows_per_id=1, quantise=False, rotate=False):
+    """The first product of every bank's adapters, [t [M, bank.max_rank], ...] of x [M,K]: row m holds scale_a * A_a x[m] for its adapter
+    a = ids[m // rows_per_id] in its first ranks; what lies behind them, and rows without an adapter, are not written.  ids: int32,
+    contiguous, one for each rows_per_id rows.  quantise: (ts, int8 rows, their scales) as quant_rowwise(x, rotate) besides."""
     _dev(x, "x")
     x = _rows(x, "x")
     M, K = x.shape
-    if x.dtype != bank.dtype or x.device != bank.device or K != bank.in_features:
-        raise ValueError(f"x must be [M,{bank.in_features}] of {bank.dtype} on {bank.device}")
-    t = torch.empty((M, bank.max_rank), dtype=x.dtype, device=x.device)
-    arg = _adapters_arg(bank, ids, rows_per_id)
+    for bank in banks:
+        if x.dtype != bank.dtype or x.device != bank.device or K != bank.in_features:
+            raise ValueError(f"x must be [M,{bank.in_features}] of {bank.dtype} on {bank.device}")
+    if len(banks) > MAX_ADAPTED_LAYERS:
+        raise ValueError(f"at most {MAX_ADAPTED_LAYERS} layers go together")
+    ts = [torch.empty((M, bank.max_rank), dtype=x.dtype, device=x.device) for bank in banks]
+    q = torch.empty((M, K), dtype=torch.int8, device=x.device) if quantise else None
+    s = torch.empty((M, 1), dtype=torch.float32, device=x.device) if quantise else None
+    layers = (_AdaptedLayer * max(1, len(banks)))()
+    for e, bank, t in zip(layers, banks, ts):
+        e.adapters, e.t = _adapters_arg(bank, ids, rows_per_id), _addr(t)
     with _on(x.device):
-        _check(lib().i8f_adapters_down(_ptr(x), dtype_code(x.dtype), M, K, x.stride(0) if M > 1 else K, ctypes.byref(arg), _ptr(t), _stream(x)),
-               "i8f_adapters_down")
-    return t
+        _check(lib().i8f_adapters_down(_ptr(x), dtype_code(x.dtype), M, K, x.stride(0) if M > 1 else K, layers, len(banks), 128 if rotate else 0,
+                                       _ptr(q), _ptr(s), _stream(x)), "i8f_adapters_down")
+    return (ts, q, s) if quantise else ts
 
 
 def adapters_up(base, bank, ids, rows_per_id, t):
@@ -917,52 +933,63 @@ def adapters_up(base, bank, ids, rows_per_id, t):
     return out
 
 
-def linear_w8a8_adapters(a, a_scale, w, w_scale, bias, bank, ids, rows_per_id, t):
-    """linear_w8a8 in the order EPI_FUSED with the adapters' share (t of adapters_down) added before its one rounding."""
-    a, w = _i8_matrix(a, "a"), _i8_matrix(w, "w")
+def _adapted_layers(M, K, device, layers, ids, rows_per_id):
+    """(C array, outputs, tensors to keep until the launch) of layers (w, w_scale, bias, bank, t)."""
+    arr, outs, keep = (_AdaptedLayer * max(1, len(layers)))(), [], []
+    if len(layers) > MAX_ADAPTED_LAYERS:
+        raise ValueError(f"at most {MAX_ADAPTED_LAYERS} layers go together")
+    for e, (w, w_scale, bias, bank, t) in zip(arr, layers):
+        w = _i8_matrix(w, "w")
+        N, K2 = w.shape
+        if K != K2 or N != bank.out_features:
+            raise ValueError(f"the rows have {K} features, w is [{N},{K2}], the adapters have {bank.out_features} outputs")
+        for name, v in (("w", w), ("t", t), ("bank", bank)):
+            if v.device != device:
+                raise ValueError(f"{name} is on {v.device}, the rows are on {device}")
+        ws, ws_host, mode = _scale(w_scale, N, device)
+        bias, bcode = _bias_arg(bias, N, device)
+        out = torch.empty((M, N), dtype=bank.dtype, device=device)
+        e.w, e.w_scale, e.w_scale_host, e.scale_mode, e.bias, e.bias_dtype, e.N = _addr(w), _addr(ws), ws_host, mode, _addr(bias), bcode, N
+        e.adapters, e.t, e.out = _adapters_arg(bank, ids, rows_per_id), _addr(t), _addr(out)
+        outs.append(out)
+        keep.append((w, ws, bias))
+    return arr, outs, keep
+
+
+def linear_w8a8_adapters(a, a_scale, layers, ids, rows_per_id=1):
+    """linear_w8a8 of the int8 rows a for layers (w, w_scale, bias, bank, t), in the order EPI_FUSED, with each one's adapters' share (t of
+    adapters_down) added before the one rounding.  -> list of outputs of the banks' type."""
+    a = _i8_matrix(a, "a")
     M, K = a.shape
-    N, K2 = w.shape
-    if K != K2 or N != bank.out_features:
-        raise ValueError(f"a is [{M},{K}], w is [{N},{K2}], the adapters have {bank.out_features} outputs")
     a_scale = a_scale.reshape(-1).contiguous()
-    if a_scale.numel() != M or a_scale.dtype != torch.float32:
-        raise ValueError("a_scale must be float32 with M elements")
-    ws, ws_host, mode = _scale(w_scale, N, a.device)
-    bias, bcode = _bias_arg(bias, N, a.device)
-    for name, v in (("w", w), ("a_scale", a_scale), ("t", t), ("bank", bank)):
-        if v.device != a.device:
-            raise ValueError(f"{name} is on {v.device}, a is on {a.device}")
-    out = torch.empty((M, N), dtype=bank.dtype, device=a.device)
-    nbytes = lib().i8f_linear_w8a8_adapters_workspace_bytes(M, N, K)
+    if a_scale.numel() != M or a_scale.dtype != torch.float32 or a_scale.device != a.device:
+        raise ValueError(f"a_scale must be float32 with M elements on {a.device}")
+    arr, outs, keep = _adapted_layers(M, K, a.device, layers, ids, rows_per_id)
+    if not layers:
+        return outs
+    nbytes = max(lib().i8f_linear_w8a8_adapters_workspace_bytes(M, o.shape[1], K) for o in outs)
     work = torch.empty(nbytes, dtype=torch.uint8, device=a.device) if nbytes else None
-    arg = _adapters_arg(bank, ids, rows_per_id)
     with _on(a.device):
-        status = lib().i8f_linear_w8a8_adapters(_ptr(a), _ptr(a_scale), _ptr(w), _ptr(ws), ws_host, mode, _ptr(bias), bcode, ctypes.byref(arg), _ptr(t),
-                                                _ptr(out), dtype_code(out.dtype), M, N, K, _ptr(work), nbytes, _stream(a))
+        status = lib().i8f_linear_w8a8_adapters(_ptr(a), _ptr(a_scale), arr, len(layers), dtype_code(outs[0].dtype), M, K, _ptr(work), nbytes, _stream(a))
     if status == ERR_UNSUPPORTED:   # (operands that are not 16-byte aligned)
-        return adapters_up(linear_w8a8(a, a_scale, w, w_scale, bias, torch.float32, EPI_FUSED), bank, ids, rows_per_id, t)
+        return [adapters_up(linear_w8a8(a, a_scale, w, w_scale, bias, torch.float32, EPI_FUSED), bank, ids, rows_per_id, t)
+                for w, w_scale, bias, bank, t in layers]
     _check(status, "i8f_linear_w8a8_adapters")
-    return out
+    return outs
 
 
-def linear_w8a16_small_m_adapters(x, w, w_scale, bias, bank, ids, rows_per_id, t):
-    """linear_w8a16_small_m with the adapters' share (t of adapters_down) added before its one rounding."""
+def linear_w8a16_small_m_adapters(x, layers, ids, rows_per_id=1):
+    """linear_w8a16_small_m of x for layers (w, w_scale, bias, bank, t), with each one's adapters' share added before the one rounding."""
     _dev(x, "x")
     x = _rows(x, "x")
-    w = _i8_matrix(w, "w")
     M, K = x.shape
-    N, K2 = w.shape
-    if K != K2 or N != bank.out_features or x.dtype != bank.dtype:
-        raise ValueError(f"x is [{M},{K}] of {x.dtype}, w is [{N},{K2}], the adapters have {bank.out_features} outputs of {bank.dtype}")
-    ws, ws_host, mode = _scale(w_scale, N, x.device)
-    bias, bcode = _bias_arg(bias, N, x.device)
-    out = torch.empty((M, N), dtype=x.dtype, device=x.device)
-    arg = _adapters_arg(bank, ids, rows_per_id)
+    if any(bank.dtype != x.dtype for _, _, _, bank, _ in layers):
+        raise ValueError(f"x is {x.dtype}, the adapters are not")
+    arr, outs, keep = _adapted_layers(M, K, x.device, layers, ids, rows_per_id)
     with _on(x.device):
-        _check(lib().i8f_linear_w8a16_small_m_adapters(_ptr(x), dtype_code(x.dtype), M, K, x.stride(0) if M > 1 else K, _ptr(w), _ptr(ws), ws_host, mode,
-                                                       _ptr(bias), bcode, ctypes.byref(arg), _ptr(t), _ptr(out), N, _stream(x)),
+        _check(lib().i8f_linear_w8a16_small_m_adapters(_ptr(x), dtype_code(x.dtype), M, K, x.stride(0) if M > 1 else K, arr, len(layers), _stream(x)),
                "i8f_linear_w8a16_small_m_adapters")
-    return out
+    return outs
 
 
 class _BlockNormArgs(ctypes.Structure):

@@ -131,25 +131,33 @@ def forward_adapters(layers, x: Tensor, banks, ids: Tensor):
     lead = x.shape[:-1]
     x2 = x.reshape(-1, x.shape[-1])
     rows = x2.shape[0]
-    inputs = {}   # what the layers share, by whether they rotate: the rotated rows, or the int8 rows and their scales
-
-    def shared(rotate):
-        if rotate not in inputs:
-            if rows > SMALL_BATCH_ROWS:
-                inputs[rotate] = _lib.quant_rowwise(x2, rotate=rotate)
+    outs = [None] * len(layers)
+    # layers of one rotation flag go together, as many as a launch takes: x quantised (or rotated) once, the adapters' first products in
+    # one launch, the layers in another
+    together = {}
+    for i, layer in enumerate(layers):
+        together.setdefault(bool(layer._use_quarot) if _quantised_here(layer, x) else None, []).append(i)
+    for rotate, members in together.items():
+        q = s = rows_in = None
+        for at in range(0, len(members), _lib.MAX_ADAPTED_LAYERS):
+            part = members[at:at + _lib.MAX_ADAPTED_LAYERS]
+            some = [banks[i] for i in part]
+            if rotate is not None and rows > SMALL_BATCH_ROWS and q is None:
+                ts, q, s = _lib.adapters_down(x2, some, ids, per, quantise=True, rotate=rotate)
             else:
-                inputs[rotate] = _lib.rotate128(x2) if rotate else x2
-        return inputs[rotate]
-
-    outs = []
-    for layer, bank in zip(layers, banks):
-        t = _lib.adapters_down(x2, bank, ids, per)
-        if not _quantised_here(layer, x):
-            y = _lib.adapters_up(layer(x).reshape(-1, bank.out_features), bank, ids, per, t)
-        elif rows > SMALL_BATCH_ROWS:
-            q, s = shared(bool(layer._use_quarot))
-            y = _lib.linear_w8a8_adapters(q, s, layer.weight, _scale_on(layer, x.device), layer.bias, bank, ids, per, t)
-        else:
-            y = _lib.linear_w8a16_small_m_adapters(shared(bool(layer._use_quarot)), layer.weight, _scale_on(layer, x.device), layer.bias, bank, ids, per, t)
-        outs.append(y.reshape(*lead, bank.out_features))
+                ts = _lib.adapters_down(x2, some, ids, per)
+            if rotate is None:   # layers that go alone
+                for i, bank, t in zip(part, some, ts):
+                    outs[i] = _lib.adapters_up(layers[i](x).reshape(-1, bank.out_features), bank, ids, per, t)
+                continue
+            problems = [(layers[i].weight, _scale_on(layers[i], x.device), layers[i].bias, bank, t) for i, bank, t in zip(part, some, ts)]
+            if rows > SMALL_BATCH_ROWS:
+                got = _lib.linear_w8a8_adapters(q, s, problems, ids, per)
+            else:
+                if rows_in is None:
+                    rows_in = _lib.rotate128(x2) if rotate else x2
+                got = _lib.linear_w8a16_small_m_adapters(rows_in, problems, ids, per)
+            for i, y in zip(part, got):
+                outs[i] = y
+    outs = [y.reshape(*lead, y.shape[-1]) for y in outs]
     return outs[0] if single else outs

@@ -63,7 +63,8 @@ def units() -> list[tuple[str, str, list[str]]]:
     for cfg in GEMM_CFGS:
         for o in GEMM_OUTS:
             grouped = int(cfg in GEMM_GROUPED and o != "OUT_I32")
-            out.append((tiles, f"gemm_i8_tiles_{cfg}_{o}.o", [f"-DI8F_TU_CFG={cfg}", f"-DI8F_TU_OUT={o}", f"-DI8F_TU_GROUPED={grouped}"]))
+            adapted = int(o in ("OUT_BF16", "OUT_F16"))
+            out.append((tiles, f"gemm_i8_tiles_{cfg}_{o}.o", [f"-DI8F_TU_CFG={cfg}", f"-DI8F_TU_OUT={o}", f"-DI8F_TU_GROUPED={grouped}", f"-DI8F_TU_ADAPTED={adapted}"]))
     for src in sorted(glob.glob(os.path.join(CSRC, "*.hip"))):
         if src != tiles:
             out.append((src, os.path.basename(src)[:-4] + ".o", []))

@@ -46,6 +46,19 @@ inline int validate_adapters(const i8f_adapters *ad, int dtype, int64_t M) {
     if (((uintptr_t)ad->down | (uintptr_t)ad->up) % 16) return I8F_ERR_INVALID;
     return M > 0x7fffffff || ad->max_rank > 65536 ? I8F_ERR_UNSUPPORTED : I8F_OK;
 }
+// The same of the layers of a call, and of what else they name
+inline int validate_layers(const i8f_adapted_layer *layers, int n, int dtype, int64_t M) {
+    if (M < 0 || n < 0 || (n > 0 && !layers)) return I8F_ERR_INVALID;
+    if (n > I8F_MAX_ADAPTED_LAYERS) return I8F_ERR_UNSUPPORTED;
+    for (int i = 0; i < n; ++i) {
+        const i8f_adapted_layer &l = layers[i];
+        if (int rc = validate_adapters(&l.adapters, dtype, M)) return rc;
+        if (l.N < 0 || (l.bias && !valid_dtype(l.bias_dtype)) || (l.scale_mode != I8F_SCALE_TENSOR && l.scale_mode != I8F_SCALE_ROW)) return I8F_ERR_INVALID;
+        if (l.adapters.ids != layers[0].adapters.ids || l.adapters.rows_per_id != layers[0].adapters.rows_per_id) return I8F_ERR_INVALID;
+        if (M > 0 && l.adapters.max_rank > 0 && l.adapters.count > 0 && (!l.t || (uintptr_t)l.t % 16)) return I8F_ERR_INVALID;
+    }
+    return I8F_OK;
+}
 // A copy whose rows_per_id fits 32 bits (M does)
 inline i8f_adapters for_kernel(const i8f_adapters &ad) {
     i8f_adapters k = ad;

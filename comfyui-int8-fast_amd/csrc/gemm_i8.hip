@@ -105,43 +105,52 @@ extern "C" int i8f_linear_w8a8_lora(const int8_t *a, const float *a_scale, const
 
 // Shapes that the tiled kernels take (others: the projection in binary32 in the workspace, then i8f_adapters_up)
 static bool adapters_fused(int64_t M, int64_t N, int64_t K) {
-    return K > 0 && K % 16 == 0 && N % 8 == 0 && N * K < (1ll << 31) && (M * K < (1ll << 31) || 256 * K < (1ll << 31));
+    return K > 0 && K % 16 == 0 && N % 8 == 0 && N * K < (1ll << 31) && M * K < (1ll << 31);
 }
 extern "C" int64_t i8f_linear_w8a8_adapters_workspace_bytes(int64_t M, int64_t N, int64_t K) {
     return M <= 0 || N <= 0 || adapters_fused(M, N, K) ? 0 : M * N * 4;
 }
 
-extern "C" int i8f_linear_w8a8_adapters(const int8_t *a, const float *a_scale, const int8_t *w, const float *w_scale, float w_scale_host, int scale_mode,
-                                        const void *bias, int bias_dtype, const i8f_adapters *adapters, const void *t, void *out, int out_dtype,
-                                        int64_t M, int64_t N, int64_t K, void *workspace, int64_t workspace_bytes, void *stream) {
+extern "C" int i8f_linear_w8a8_adapters(const int8_t *a, const float *a_scale, const i8f_adapted_layer *layers, int n_layers, int out_dtype, int64_t M,
+                                        int64_t K, void *workspace, int64_t workspace_bytes, void *stream) {
     using namespace i8f;
     using namespace i8f::gemm;
-    if (int rc = validate_adapters(adapters, out_dtype, M)) return rc;
-    if (int rc = validate(a, w, M, N, K, out)) return rc;
-    if (bias && !valid_dtype(bias_dtype)) return I8F_ERR_INVALID;
-    if (scale_mode != I8F_SCALE_TENSOR && scale_mode != I8F_SCALE_ROW) return I8F_ERR_INVALID;
-    if (M == 0 || N == 0) return I8F_OK;
-    if (!a_scale || (scale_mode == I8F_SCALE_ROW && !w_scale)) return I8F_ERR_INVALID;
-    if (adapters->max_rank > 0 && (!t || (uintptr_t)t % 16)) return I8F_ERR_INVALID;
+    if (int rc = validate_layers(layers, n_layers, out_dtype, M)) return rc;
     if (workspace && (uintptr_t)workspace % 16) return I8F_ERR_INVALID;
-    hipStream_t st = (hipStream_t)stream;
-    if (!adapters_fused(M, N, K)) {
-        if (!workspace || workspace_bytes < M * N * 4) return I8F_ERR_INVALID;
-        if (int rc = i8f_linear_w8a8(a, a_scale, w, w_scale, w_scale_host, scale_mode, bias, bias_dtype, workspace, I8F_F32, M, N, K, I8F_EPI_FUSED, stream))
-            return rc;
-        return i8f_adapters_up(workspace, I8F_F32, adapters, t, out, out_dtype, M, N, stream);
+    bool aligned = (uintptr_t)a % 16 == 0;
+    for (int i = 0; i < n_layers; ++i) {
+        const i8f_adapted_layer &y = layers[i];
+        if (int rc = validate(a, y.w, M, y.N, K, y.out)) return rc;
+        if (M == 0 || y.N == 0) continue;
+        if (!a_scale || (y.scale_mode == I8F_SCALE_ROW && !y.w_scale)) return I8F_ERR_INVALID;
+        if (!adapters_fused(M, y.N, K)) {
+            if (!workspace || workspace_bytes < M * y.N * 4) return I8F_ERR_INVALID;
+        } else {   // 16-byte pieces of the operands, which any torch allocation has
+            aligned = aligned && ((uintptr_t)y.w | (uintptr_t)y.out | (uintptr_t)y.bias) % 16 == 0 && (y.scale_mode != I8F_SCALE_ROW || (uintptr_t)y.w_scale % 16 == 0);
+        }
     }
-    // 16-byte pieces of the operands, which any torch allocation has
-    if (((uintptr_t)a | (uintptr_t)w | (uintptr_t)out | (uintptr_t)bias) % 16 || (scale_mode == I8F_SCALE_ROW && (uintptr_t)w_scale % 16)) return I8F_ERR_UNSUPPORTED;
+    if (M == 0 || n_layers == 0) return I8F_OK;
+    if (!aligned) return I8F_ERR_UNSUPPORTED;
     if (int rc = check_device()) return rc;
-    const i8f_adapters ad = for_kernel(*adapters);
-    GemmArgs g{};
-    g.x = a, g.w = w, g.M = (int)M, g.N = (int)N, g.K = (int)K, g.out = out;
-    g.xs = a_scale, g.ws = w_scale, g.ws_host = w_scale_host, g.row_scale = scale_mode == I8F_SCALE_ROW;
-    g.bias = bias, g.bias_dtype = bias_dtype, g.order = I8F_EPI_FUSED;
-    g.side_t = t, g.side_b = ad.up, g.side_rank = (int)ad.max_rank;
-    g.ids = ad.ids, g.first_rank = ad.first_rank, g.rows_per_id = (int)ad.rows_per_id, g.adapters = ad.max_rank > 0 ? (int)ad.count : 0;
-    return out_dtype == I8F_BF16 ? launch<OUT_BF16>(g, st) : launch<OUT_F16>(g, st);
+    hipStream_t st = (hipStream_t)stream;
+    AdaptedLayers l{};
+    for (int i = 0; i < n_layers; ++i) {
+        const i8f_adapted_layer &y = layers[i];
+        if (y.N == 0) continue;
+        if (!adapters_fused(M, y.N, K)) {
+            if (int rc = i8f_linear_w8a8(a, a_scale, y.w, y.w_scale, y.w_scale_host, y.scale_mode, y.bias, y.bias_dtype, workspace, I8F_F32, M, y.N, K, I8F_EPI_FUSED, stream))
+                return rc;
+            if (int rc = i8f_adapters_up(workspace, I8F_F32, &y.adapters, y.t, y.out, out_dtype, M, y.N, stream)) return rc;
+            continue;
+        }
+        const i8f_adapters ad = for_kernel(y.adapters);
+        const int k = l.n++;
+        l.w[k] = y.w, l.ws[k] = y.w_scale, l.ws_host[k] = y.w_scale_host, l.bias[k] = y.bias, l.out[k] = y.out, l.N[k] = (int)y.N;
+        l.flags[k] = (y.scale_mode == I8F_SCALE_ROW ? 1 : 0) | (y.bias_dtype << 1);
+        l.adapters[k] = {ad.ids, ad.first_rank, y.t, ad.up, (int)ad.rows_per_id, ad.max_rank > 0 ? (int)ad.count : 0, (int)ad.max_rank};
+    }
+    if (l.n == 0) return I8F_OK;
+    return out_dtype == I8F_BF16 ? launch_adapted<OUT_BF16>(l, a, a_scale, (int)M, (int)K, st) : launch_adapted<OUT_F16>(l, a, a_scale, (int)M, (int)K, st);
 }
 
 extern "C" int i8f_linear_w8a8(const int8_t *a, const float *a_scale, const int8_t *w, const float *w_scale,

@@ -28,6 +28,7 @@
 
 #pragma once
 
+#include "../../include/i8f_blocks.h"
 #include "i8f_common.hpp"
 #include "splitk_protocol.h"
 #include <algorithm>
@@ -90,10 +91,6 @@ struct GemmArgs {
     const void *side_t, *side_b;
     int side_rank, side_has_alpha;
     float side_alpha;
-    // adapters of the rows (i8f_linear_w8a8_adapters): row m takes adapter ids[(row0 + m) / rows_per_id], side_t [M, side_rank] holds its first
-    // product, side_b the adapters' second factors, from element N * first_rank[a] on
-    const int *ids, *first_rank;
-    int rows_per_id, adapters, row0;
     void *out;
     int tiles_m, tiles_n;
     // K split over `splits` workgroups per tile (1: none): partial sums and per-tile arrival counters in caller memory
@@ -315,22 +312,31 @@ __device__ __forceinline__ v4f side_mfma32(v4i a, v4i b, v4f c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h_t, a), __builtin_bit_cast(v8h_t, b), c, 0, 0, 0);
 }
 
+// The adapters of a problem's rows: row m takes adapter ids[m / rows_per_id], t [M, max_rank] holds its first product, up the adapters'
+// second factors, from element N * first_rank[a] on.
+struct AdapterArgs {
+    const int *ids, *first_rank;
+    const void *t, *up;
+    int rows_per_id, count, max_rank;
+};
+
 // The epilogue with an adapter for every row: out = round(acc * (xs * ws) + bias + sum_j t[m,j] B_a[n,j]).
-// A block of CB columns after the other, its accumulators become the projection's binary32 values and the matrix unit adds the adapters'
-// products to them, with the operand roles of the main product (rows n from B_a, columns m from t): no second set of accumulators, any
-// number of adapters and ranks, one rounding at the end.  A wave goes through the adapters that occur in its rows.  A product's column
-// depends on its own row of t alone, so rows of other adapters are left out by keeping what they had (a select per lane: a lane's values
-// belong to one row); zeros in t instead would let an adapter that is not finite into every row of the tile.
-// Where all rows of the wave have one adapter of up to 64 ranks, as in a batch of long requests, their t is fetched once and
-// nothing is selected.  (Blocks of columns innermost, with all accumulators converted first, took 40 to 200 spilled registers.)
+// Blocks of accumulators become the projection's binary32 values and the matrix unit adds B_a t to them, with the operand roles of the
+// main product (rows n from B_a, columns m from t): no second set of accumulators and one rounding at the end.
+// Where all rows of a wave have one adapter, as in a batch of long requests, one block of CB columns follows the other; up to 128 ranks (32
+// with twelve waves, which have fewer registers) the rows' t are fetched once.
+// A wave with several adapters goes by groups of 16 (32) rows: a product for every adapter that occurs in the group and STEP of its ranks,
+// over all the wave's columns, and the rows of other adapters keep what they had (a select per lane: a lane's values belong to one row, and
+// a column of the product depends on its own row of t alone; zeros in t instead would let an adapter that is not finite into every
+// row).  What counts there is the trip to memory for each adapter's factor, so the loads run RING products ahead.
 template <class C, int OUT, class ACC, class ACC16>
-__device__ __forceinline__ void adapters_epilogue(const GemmArgs &g, const int gM, const int gN, const int m0, const int n0, const int wm, const int wn,
+__device__ __forceinline__ void adapters_epilogue(const AdapterArgs &g, const int gM, const int gN, const int m0, const int n0, const int wm, const int wn,
                                                   const int lane, const float *s_xs, const float *s_ws, const float *s_bias, char *ebuf, ACC &acc,
                                                   ACC16 &acc16, void *gout) {
     static_assert(OUT == OUT_BF16 || OUT == OUT_F16, "16-bit factors");
     constexpr bool M16 = C::MF == 16;
-    constexpr int MI = C::MI, NJ = C::NJ, CB = C::CB, GR = M16 ? 16 : 32, GROUPS = C::WTM / GR;   // groups of rows, of which a lane has one row each
-    constexpr int STEP = M16 ? 32 : 16, QPG = M16 ? 1 : 4;                                       // ranks of a product; quads of a group and column block
+    constexpr int NJ = C::NJ, CB = C::CB, GR = M16 ? 16 : 32, GROUPS = C::WTM / GR;   // groups of rows, of which a lane has one row each
+    constexpr int STEP = M16 ? 32 : 16, QPG = M16 ? 1 : 4;                           // ranks of a product; quads of a group and column block
     typedef typename std::conditional<M16, v4f, v16f>::type block_t;
     const int l16 = lane & 15, lq = lane >> 4, l32 = lane & 31, lhalf = lane >> 5;
     const int mw = m0 + wm * C::WTM, nw = n0 + wn * C::WTN;
@@ -339,141 +345,183 @@ __device__ __forceinline__ void adapters_epilogue(const GemmArgs &g, const int g
         if constexpr (M16) return side_mfma32<OUT>(b, t, c);
         else return side_mfma<OUT>(b, t, c);
     };
-    // the adapter of the lane's row in each group
-    int id[GROUPS];
-    uint64_t todo[GROUPS];
+    // the adapter of the lane's row in each group, and its ranks
+    int id[GROUPS], first[GROUPS], rank[GROUPS];
+    uint64_t with[GROUPS];
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i) {
         const int m = mw + i * GR + lrow;
-        const int a = g.ids[(uint32_t)(g.row0 + min(m, gM - 1)) / (uint32_t)g.rows_per_id];
-        id[i] = m < gM && (uint32_t)a < (uint32_t)g.adapters ? a : -1;
-        todo[i] = __builtin_amdgcn_ballot_w64(id[i] >= 0);
+        const int a = g.ids[(uint32_t)min(m, gM - 1) / (uint32_t)g.rows_per_id];
+        id[i] = m < gM && (uint32_t)a < (uint32_t)g.count ? a : -1;
     }
-    // the first of the adapters that are left, taken out of todo; -1: none
-    auto next_adapter = [&](uint64_t (&left)[GROUPS]) {
-        int a = -1;
 #pragma unroll
-        for (int i = GROUPS - 1; i >= 0; --i)
-            if (left[i]) a = __builtin_amdgcn_readlane(id[i], __builtin_ctzll(left[i]));
+    for (int i = 0; i < GROUPS; ++i) {
+        with[i] = __builtin_amdgcn_ballot_w64(id[i] >= 0);
+        first[i] = rank[i] = 0;
+        if (id[i] >= 0) first[i] = g.first_rank[id[i]], rank[i] = g.first_rank[id[i] + 1] - first[i];
+    }
+    int a0 = -1, first0 = 0, rank0 = 0;   // the first of them
 #pragma unroll
-        for (int i = 0; i < GROUPS; ++i) left[i] &= ~__builtin_amdgcn_ballot_w64(id[i] == a);
-        return a;
-    };
-    // rows of t and of a factor as buffers (rows and columns past the matrices load zeros)
-    const auto tr = buffer_at(g.side_t, (int64_t)mw * g.side_rank * 2, (int64_t)min(gM - mw, C::WTM) * g.side_rank * 2);
-    auto factor = [&](int first, int rank) {
-        return buffer_at(g.side_b, ((int64_t)gN * first + (int64_t)nw * rank) * 2, (int64_t)min(gN - nw, C::WTN) * rank * 2);
-    };
-    // (the lane's eight ranks from k0 on; past the adapter's last one, which may be half a step of 32, an offset that loads zeros)
-    auto rank_at = [&](int k0, int rank) { return k0 + lk < rank ? (uint32_t)(k0 + lk) * 2u : 0x80000000u; };
-    auto load_t = [&](int i, uint32_t kb) { return __builtin_bit_cast(v4i, buffer_load16(tr, (uint32_t)((i * GR + lrow) * g.side_rank * 2) + kb)); };
-    auto load_b = [&](__amdgpu_buffer_rsrc_t b, int j, int rank, uint32_t kb) {
-        return __builtin_bit_cast(v4i, buffer_load16(b, (uint32_t)((j * CB + lrow) * rank * 2) + kb));
-    };
-    constexpr int ROW_BYTES = C::WTN * 2, PITCH = ROW_BYTES + 8, CPO = ROW_BYTES / 16;
-    // a block's projection in the operation order of I8F_EPI_FUSED, and its way to LDS
-    auto project = [&](int j, block_t (&f)[GROUPS]) __attribute__((always_inline)) {
+    for (int i = GROUPS - 1; i >= 0; --i)
+        if (with[i]) {
+            const int l = __builtin_ctzll(with[i]);
+            a0 = __builtin_amdgcn_readlane(id[i], l), first0 = __builtin_amdgcn_readlane(first[i], l), rank0 = __builtin_amdgcn_readlane(rank[i], l);
+        }
+    bool one = true;   // of all rows, or none
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) one = one && __builtin_amdgcn_ballot_w64(id[i] == a0 || mw + i * GR + lrow >= gM) == ~0ull;
+
+    // a block's projection in the operation order of I8F_EPI_FUSED
+    auto project = [&](int i, int j, block_t &f) __attribute__((always_inline)) {
+        const float xs = s_xs[wm * C::WTM + i * GR + lrow];
 #pragma unroll
         for (int qd = 0; qd < QPG; ++qd) {
             const int nl = wn * C::WTN + j * CB + (M16 ? lq * 4 : qd * 8 + lhalf * 4);
             const float4 w4 = *(const float4 *)&s_ws[nl], b4 = *(const float4 *)&s_bias[nl];
+            int a4[4];
 #pragma unroll
-            for (int i = 0; i < GROUPS; ++i) {
-                const float xs = s_xs[wm * C::WTM + i * GR + lrow];
-                int a4[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if constexpr (M16) a4[e] = acc16[i >> 1][j][i & 1][e];
-                    else a4[e] = acc[i][j][4 * qd + e];
-                }
-                f[i][4 * qd] = (float)a4[0] * (xs * w4.x) + b4.x, f[i][4 * qd + 1] = (float)a4[1] * (xs * w4.y) + b4.y;
-                f[i][4 * qd + 2] = (float)a4[2] * (xs * w4.z) + b4.z, f[i][4 * qd + 3] = (float)a4[3] * (xs * w4.w) + b4.w;
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (M16) a4[e] = acc16[i >> 1][j][i & 1][e];
+                else a4[e] = acc[i][j][4 * qd + e];
             }
+            f[4 * qd] = (float)a4[0] * (xs * w4.x) + b4.x, f[4 * qd + 1] = (float)a4[1] * (xs * w4.y) + b4.y;
+            f[4 * qd + 2] = (float)a4[2] * (xs * w4.z) + b4.z, f[4 * qd + 3] = (float)a4[3] * (xs * w4.w) + b4.w;
         }
     };
-    auto stage = [&](int j, const block_t (&f)[GROUPS]) __attribute__((always_inline)) {
+
+    // rows of t as a buffer (rows past the matrix load zeros)
+    const auto tr = buffer_at(g.t, (int64_t)mw * g.max_rank * 2, (int64_t)min(gM - mw, C::WTM) * g.max_rank * 2);
+    constexpr int ROW_BYTES = C::WTN * 2, PITCH = ROW_BYTES + 8, CPO = ROW_BYTES / 16;
+    auto stage = [&](int i, int j, const block_t &f) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < GROUPS; ++i)
-#pragma unroll
-            for (int qd = 0; qd < QPG; ++qd) {
-                const float v[4] = {f[i][4 * qd], f[i][4 * qd + 1], f[i][4 * qd + 2], f[i][4 * qd + 3]};
-                char *dst = ebuf + (i * GR + lrow) * PITCH + (j * CB + (M16 ? lq * 4 : qd * 8 + lhalf * 4)) * 2;
-                if constexpr (OUT == OUT_BF16) *(uint2 *)dst = make_uint2(f32x2_to_bf16x2_bits(v[0], v[1]), f32x2_to_bf16x2_bits(v[2], v[3]));
-                else *(uint2 *)dst = make_uint2(f32x2_to_f16x2_bits(v[0], v[1]), f32x2_to_f16x2_bits(v[2], v[3]));
-            }
+        for (int qd = 0; qd < QPG; ++qd) {
+            const float v[4] = {f[4 * qd], f[4 * qd + 1], f[4 * qd + 2], f[4 * qd + 3]};
+            char *dst = ebuf + (i * GR + lrow) * PITCH + (j * CB + (M16 ? lq * 4 : qd * 8 + lhalf * 4)) * 2;
+            if constexpr (OUT == OUT_BF16) *(uint2 *)dst = make_uint2(f32x2_to_bf16x2_bits(v[0], v[1]), f32x2_to_bf16x2_bits(v[2], v[3]));
+            else *(uint2 *)dst = make_uint2(f32x2_to_f16x2_bits(v[0], v[1]), f32x2_to_f16x2_bits(v[2], v[3]));
+        }
     };
-    const int a0 = next_adapter(todo);
-    bool one = a0 < 0;   // no adapter, or one for all rows, of up to 64 ranks
-    int first0 = 0, rank0 = 0;
-    if (a0 >= 0) {
-        first0 = __builtin_amdgcn_readfirstlane(g.first_rank[a0]), rank0 = __builtin_amdgcn_readfirstlane(g.first_rank[a0 + 1]) - first0;
-        one = rank0 <= 64;
+    if (!one) {
+        constexpr int RING = C::STAGES == 4 ? 8 : C::NT > 512 ? 1 : C::STAGES == 3 ? 4 : 2;
 #pragma unroll
-        for (int i = 0; i < GROUPS; ++i) one = one && __builtin_amdgcn_ballot_w64(id[i] == a0 || mw + i * GR + lrow >= gM) == ~0ull;
-    }
-    if (one) {
-        constexpr int KS = 64 / STEP;
-        const auto up = factor(first0, rank0);
-        v4i tf[KS][GROUPS];
+        for (int i = 0; i < GROUPS; ++i) {
+            block_t f[NJ];
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
+            for (int j = 0; j < NJ; ++j) project(i, j, f[j]);
+            // the products one after the other: an adapter of the group that is left and STEP of its ranks; -1 when there is none
+            uint64_t left = with[i];
+            int a = -1, a_first = 0, a_rank = 0, k0 = 0;
+            auto next = [&]() __attribute__((always_inline)) {
+                k0 += STEP;
+                while (k0 >= a_rank && a != -2) {
+                    if (!left) a = -2;   // (that no row has)
+                    else {
+                        const int l = __builtin_ctzll(left);
+                        a = __builtin_amdgcn_readlane(id[i], l), a_first = __builtin_amdgcn_readlane(first[i], l), a_rank = __builtin_amdgcn_readlane(rank[i], l);
+                        left &= ~__builtin_amdgcn_ballot_w64(id[i] == a);
+                        k0 = 0;
+                    }
+                }
+            };
+            v4i tf[RING], bf[RING][NJ];
+            int whose[RING];
+            auto fetch = [&](int s) __attribute__((always_inline)) {   // (past the last product everything is out of range and loads zeros)
+                next();
+                whose[s] = a;
+                const auto up = buffer_at(g.up, ((int64_t)gN * a_first + (int64_t)nw * a_rank) * 2, a < 0 ? 0 : (int64_t)min(gN - nw, C::WTN) * a_rank * 2);
+                const uint32_t kb = a >= 0 && k0 + lk < a_rank ? (uint32_t)(k0 + lk) * 2u : 0x80000000u;
+                tf[s] = __builtin_bit_cast(v4i, buffer_load16(tr, (uint32_t)((i * GR + lrow) * g.max_rank * 2) + kb));
 #pragma unroll
-            for (int i = 0; i < GROUPS; ++i) tf[s][i] = load_t(i, rank_at(s * STEP, rank0));
-        constexpr int AHEAD = C::NT <= 512 ? 1 : 0;   // (twelve waves have no registers for the next block's factors)
-        v4i bf[AHEAD + 1][KS];
-        auto fetch = [&](int j) __attribute__((always_inline)) {
+                for (int j = 0; j < NJ; ++j) bf[s][j] = __builtin_bit_cast(v4i, buffer_load16(up, (uint32_t)((j * CB + lrow) * a_rank * 2) + kb));
+            };
 #pragma unroll
-            for (int s = 0; s < KS; ++s) bf[j & AHEAD][s] = load_b(up, j, rank0, rank_at(s * STEP, rank0));
-        };
-        if (AHEAD) fetch(0);
+            for (int s = 0; s < RING; ++s) fetch(s);
+            while (whose[0] >= 0) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            if (j + AHEAD < NJ) fetch(j + AHEAD);
-            block_t f[GROUPS];
-            project(j, f);
+                for (int s = 0; s < RING; ++s) {
+                    const bool mine = id[i] == whose[s];
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                if (s * STEP < rank0) {
+                    for (int j = 0; j < NJ; ++j) {
+                        const block_t sum = mma(bf[s][j], tf[s], f[j]);
 #pragma unroll
-                    for (int i = 0; i < GROUPS; ++i) f[i] = mma(bf[j & AHEAD][s], tf[s][i], f[i]);
+                        for (int e = 0; e < 4 * QPG; ++e) f[j][e] = mine ? sum[e] : f[j][e];
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                    fetch(s);
                 }
             }
-            stage(j, f);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) stage(i, j, f[j]);
             __builtin_amdgcn_sched_barrier(0);
         }
     } else {
+    const auto up = buffer_at(g.up, ((int64_t)gN * first0 + (int64_t)nw * rank0) * 2, (int64_t)min(gN - nw, C::WTN) * rank0 * 2);
+    // (the lane's eight ranks from k0 on; past the adapter's last one, which may be half a step of 32, an offset that loads zeros)
+    auto rank_at = [&](int k0) { return k0 + lk < rank0 ? (uint32_t)(k0 + lk) * 2u : 0x80000000u; };
+    auto load_t = [&](int i, uint32_t kb) { return __builtin_bit_cast(v4i, buffer_load16(tr, (uint32_t)((i * GR + lrow) * g.max_rank * 2) + kb)); };
+    auto load_b = [&](int j, uint32_t kb) { return __builtin_bit_cast(v4i, buffer_load16(up, (uint32_t)((j * CB + lrow) * rank0 * 2) + kb)); };
+    // up to STEPS products of STEP ranks with the rows' t in registers
+    auto resident = [&](auto STEPS) __attribute__((always_inline)) {
+        constexpr int KS = decltype(STEPS)::value, AHEAD = KS && C::NT <= 512 ? 1 : 0;   // (twelve waves have no registers for the next block's factors)
+        v4i tf[KS ? KS : 1][GROUPS], bf[AHEAD + 1][KS ? KS : 1];
+        auto fetch = [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) bf[j & AHEAD][s] = load_b(j, rank_at(s * STEP));
+        };
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int i = 0; i < GROUPS; ++i) tf[s][i] = load_t(i, rank_at(s * STEP));
+        if (AHEAD) fetch(0);
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             block_t f[GROUPS];
-            project(j, f);
-            uint64_t left[GROUPS];
 #pragma unroll
-            for (int i = 0; i < GROUPS; ++i) left[i] = __builtin_amdgcn_ballot_w64(id[i] >= 0);
-            for (int a = next_adapter(left); a >= 0; a = next_adapter(left)) {
-                const int first = __builtin_amdgcn_readfirstlane(g.first_rank[a]), rank = __builtin_amdgcn_readfirstlane(g.first_rank[a + 1]) - first;
-                const auto up = factor(first, rank);
-                for (int k0 = 0; k0 < rank; k0 += STEP) {
-                    const uint32_t kb = rank_at(k0, rank);
-                    const v4i bf = load_b(up, j, rank, kb);
-                    v4i tf[GROUPS];
+            for (int i = 0; i < GROUPS; ++i) project(i, j, f[i]);
+            if (j + AHEAD < NJ) fetch(j + AHEAD);
 #pragma unroll
-                    for (int i = 0; i < GROUPS; ++i) tf[i] = load_t(i, kb);
+            for (int s = 0; s < KS; ++s)
 #pragma unroll
-                    for (int i = 0; i < GROUPS; ++i) {
-                        const block_t sum = mma(bf, tf[i], f[i]);
+                for (int i = 0; i < GROUPS; ++i) f[i] = mma(bf[j & AHEAD][s], tf[s][i], f[i]);
 #pragma unroll
-                        for (int e = 0; e < 4 * QPG; ++e) f[i][e] = id[i] == a ? sum[e] : f[i][e];
-                    }
+            for (int i = 0; i < GROUPS; ++i) stage(i, j, f[i]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    constexpr int MOST = C::NT <= 512 ? 128 : 32, PART = C::NT <= 512 ? 64 : 32;
+    if (rank0 == 0) resident(std::integral_constant<int, 0>{});
+    else if (rank0 <= 32) resident(std::integral_constant<int, 32 / STEP>{});
+    else if (MOST > 32 && rank0 <= 64) resident(std::integral_constant<int, (MOST > 32 ? 64 / STEP : 0)>{});
+    else if (MOST > 32 && rank0 <= MOST) resident(std::integral_constant<int, (MOST > 32 ? MOST / STEP : 0)>{});
+    else {   // PART ranks at a time, t from cache for every block
+        constexpr int KS = PART / STEP;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            block_t f[GROUPS];
+#pragma unroll
+            for (int i = 0; i < GROUPS; ++i) project(i, j, f[i]);
+            for (int k0 = 0; k0 < rank0; k0 += PART) {
+                v4i tf[KS][GROUPS], bf[KS];
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    bf[s] = load_b(j, rank_at(k0 + s * STEP));
+#pragma unroll
+                    for (int i = 0; i < GROUPS; ++i) tf[s][i] = load_t(i, rank_at(k0 + s * STEP));
                 }
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+#pragma unroll
+                    for (int i = 0; i < GROUPS; ++i) f[i] = mma(bf[s], tf[s][i], f[i]);
             }
-            stage(j, f);
+#pragma unroll
+            for (int i = 0; i < GROUPS; ++i) stage(i, j, f[i]);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
+    }
     // rows from LDS, 16 bytes to a lane
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
     for (int p = 0; p < C::WTM * CPO / 64; ++p) {
         const int at = p * 64 + lane, row = at / CPO, cc = at % CPO;
@@ -492,7 +540,7 @@ template <class C, int OUT, bool KTAIL, bool SIDE = false, bool SPLITK = false, 
 __device__ __forceinline__ void gemm_i8_body(const int8_t *gx, const int8_t *gw, int gM, int gN, int gK, int tiles_m, int tiles_n,
                                              const float *gxs, const float *gws, const void *gbias, int flags, const GemmArgs &g,
                                              const int wg_id, void *gout, const void *gaddend, const float ws_host,
-                                             const void *ggate, const int ggate_rows) {
+                                             const void *ggate, const int ggate_rows, const AdapterArgs *adapters = nullptr) {
     constexpr int BM = C::BM, BN = C::BN, BK = C::BK, NW = C::NW, MI = C::MI, NJ = C::NJ, CB = C::CB, CPR = C::CPR;
     constexpr int S = C::STAGES, WS = C::WSTAGES;
     constexpr bool ASYM = WS != S;  // the W tile one stage deeper than the X tile
@@ -1309,7 +1357,7 @@ __device__ __forceinline__ void gemm_i8_body(const int8_t *gx, const int8_t *gw,
     if constexpr (OUT == OUT_I32) {
         run_epilogue(O0{}, F_{}, F_{}, S0{}, F_{});  // (the raw product: no gate and no addend)
     } else if constexpr (ADAPT) {
-        adapters_epilogue<C, OUT>(g, gM, gN, m0, n0, wm, wn, lane, s_xs, s_ws, s_bias, ebuf, acc, acc16, gout);
+        adapters_epilogue<C, OUT>(*adapters, gM, gN, m0, n0, wm, wn, lane, s_xs, s_ws, s_bias, ebuf, acc, acc16, gout);
     } else if constexpr (SIDE) {  // (no gate and no addend beside a side branch)
         if (g.side_rank > 32) choose(std::integral_constant<int, 4>{});
         else choose(std::integral_constant<int, 2>{});
@@ -1324,14 +1372,6 @@ __global__ __launch_bounds__(C::NT) void gemm_i8_kernel(const int8_t *gx, const 
                                                         const GemmArgs g) {
     gemm_i8_body<C, OUT, KTAIL, SIDE, SPLITK>(gx, gw, gM, gN, gK, tiles_m, tiles_n, gxs, gws, gbias, flags, g, (int)blockIdx.x, g.out,
                                               g.addend, g.ws_host, g.gate, g.gate_rows);
-}
-
-// the same with an adapter for every row
-template <class C, int OUT, bool KTAIL>
-__global__ __launch_bounds__(C::NT) void gemm_i8_adapters_kernel(const int8_t *gx, const int8_t *gw, int gM, int gN, int gK, int tiles_m, int tiles_n,
-                                                                 const float *gxs, const float *gws, const void *gbias, int flags, const GemmArgs g) {
-    gemm_i8_body<C, OUT, KTAIL, false, false, true>(gx, gw, gM, gN, gK, tiles_m, tiles_n, gxs, gws, gbias, flags, g, (int)blockIdx.x, g.out, nullptr,
-                                                    g.ws_host, nullptr, 1);
 }
 
 // Several problems of one layer shape (N, K, scale mode, dtypes) with their own activations, weights and outputs in
@@ -1361,6 +1401,33 @@ __global__ __launch_bounds__(C::NT) void gemm_i8_grouped_kernel(int gN, int gK, 
     gemm_i8_body<C, OUT, false>(gg.x[grp], gg.w[grp], gg.M[grp], gN, gK, gg.tiles_m[grp], tiles_n, gg.xs[grp], gg.ws[grp], gg.bias[grp],
                                 flags, g, (int)blockIdx.x - gg.first_tile[grp], gg.out[grp], gg.addend[grp], gg.ws_host[grp], gg.gate[grp],
                                 gg.gate_rows[grp]);
+}
+
+// Layers that read the same int8 rows, each with its width, weights, output and adapters, in one launch: the q, k and v projections of a few
+// dozen tokens are 16 to 64 tiles each, on 256 CUs.  (Two waves to a SIMD where two workgroups fit into a CU's LDS.)
+constexpr int MAX_ADAPTED = I8F_MAX_ADAPTED_LAYERS;
+struct AdaptedLayers {
+    const int8_t *w[MAX_ADAPTED];
+    const float *ws[MAX_ADAPTED];
+    const void *bias[MAX_ADAPTED];
+    void *out[MAX_ADAPTED];
+    float ws_host[MAX_ADAPTED];
+    int N[MAX_ADAPTED], tiles_n[MAX_ADAPTED], flags[MAX_ADAPTED];
+    AdapterArgs adapters[MAX_ADAPTED];
+    int first_tile[MAX_ADAPTED + 1];  // [n] = all tiles
+    int n;
+};
+
+template <class C, int OUT, bool KTAIL>
+__global__ __launch_bounds__(C::NT, (C::NT == 256 && C::LDS_BYTES <= 80 * 1024 ? 2 : 1)) void gemm_i8_adapters_kernel(
+    const int8_t *gx, const float *gxs, int gM, int gK, int tiles_m, const AdaptedLayers l, const GemmArgs g) {
+    int k = 0;
+#pragma unroll
+    for (int i = 1; i < MAX_ADAPTED; ++i)
+        if (i < l.n && (int)blockIdx.x >= l.first_tile[i]) k = i;
+    k = __builtin_amdgcn_readfirstlane(k);
+    gemm_i8_body<C, OUT, KTAIL, false, false, true>(gx, l.w[k], gM, l.N[k], gK, tiles_m, l.tiles_n[k], gxs, l.ws[k], l.bias[k], l.flags[k], g,
+                                                    (int)blockIdx.x - l.first_tile[k], l.out[k], nullptr, l.ws_host[k], nullptr, 1, &l.adapters[k]);
 }
 
 }  // namespace gemm
@@ -1406,17 +1473,6 @@ int launch_cfg(GemmArgs &g, hipStream_t st) {
     g.tiles_n = (g.N + C::BN - 1) / C::BN;
     const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n;
     const int flags = (g.row_scale ? 1 : 0) | (g.bias_dtype << 1);  // what the prologue wants to know of the epilogue
-    if (g.ids) {
-        if constexpr (OUT == OUT_BF16 || OUT == OUT_F16) {
-            auto go = [&](auto kernel) {
-                hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(C::NT), 0, st, g.x, g.w, g.M, g.N, g.K, g.tiles_m, g.tiles_n, g.xs, g.ws, g.bias, flags, g);
-                return check_launch();
-            };
-            return g.K % C::BK ? go(gemm_i8_adapters_kernel<C, OUT, true>) : go(gemm_i8_adapters_kernel<C, OUT, false>);
-        } else {
-            return I8F_ERR_UNSUPPORTED;
-        }
-    }
     if (g.side_t) {  // validated by the entry point: K % BK == 0 here
         if constexpr (OUT == OUT_BF16 || OUT == OUT_F16) {
             hipLaunchKernelGGL((gemm_i8_kernel<C, OUT, false, true>), dim3((unsigned)tiles), dim3(C::NT), 0, st, g.x, g.w, g.M, g.N,
@@ -1447,6 +1503,25 @@ int launch_cfg(GemmArgs &g, hipStream_t st) {
     return check_launch();
 }
 
+// layers with adapters: l has everything but the tiles
+template <class C, int OUT>
+int launch_cfg_adapted(AdaptedLayers &l, const int8_t *x, const float *xs, int M, int K, hipStream_t st) {
+    const int tiles_m = (M + C::BM - 1) / C::BM;
+    int64_t first = 0;
+    for (int i = 0; i < l.n; ++i) {
+        l.tiles_n[i] = (l.N[i] + C::BN - 1) / C::BN;
+        l.first_tile[i] = (int)first;
+        first += (int64_t)tiles_m * l.tiles_n[i];
+    }
+    if (first > 0x7fffffff) return I8F_ERR_UNSUPPORTED;
+    for (int i = l.n; i <= MAX_ADAPTED; ++i) l.first_tile[i] = (int)first;
+    GemmArgs g{};
+    g.order = I8F_EPI_FUSED;
+    if (K % C::BK) hipLaunchKernelGGL((gemm_i8_adapters_kernel<C, OUT, true>), dim3((unsigned)first), dim3(C::NT), 0, st, x, xs, M, K, tiles_m, l, g);
+    else hipLaunchKernelGGL((gemm_i8_adapters_kernel<C, OUT, false>), dim3((unsigned)first), dim3(C::NT), 0, st, x, xs, M, K, tiles_m, l, g);
+    return check_launch();
+}
+
 // Every tile configuration is compiled once per output type in a translation unit of its own (gemm_i8_tiles.hip, built
 // once for each pair), so that they compile side by side.
 #define I8F_GEMM_CFGS(X) X(CfgBig) X(CfgB192) X(CfgMid) X(CfgTall) X(CfgWide) X(CfgW96) X(CfgMidDeep) X(CfgM96Deep) X(CfgS64Deep) X(CfgT64Deep)
@@ -1454,7 +1529,9 @@ int launch_cfg(GemmArgs &g, hipStream_t st) {
     extern template int launch_cfg<C, OUT_BF16>(GemmArgs &, hipStream_t);                                        \
     extern template int launch_cfg<C, OUT_F16>(GemmArgs &, hipStream_t);                                         \
     extern template int launch_cfg<C, OUT_F32>(GemmArgs &, hipStream_t);                                         \
-    extern template int launch_cfg<C, OUT_I32>(GemmArgs &, hipStream_t);
+    extern template int launch_cfg<C, OUT_I32>(GemmArgs &, hipStream_t);                                         \
+    extern template int launch_cfg_adapted<C, OUT_BF16>(AdaptedLayers &, const int8_t *, const float *, int, int, hipStream_t); \
+    extern template int launch_cfg_adapted<C, OUT_F16>(AdaptedLayers &, const int8_t *, const float *, int, int, hipStream_t);
 I8F_GEMM_CFGS(I8F_EXTERN_CFG)
 #undef I8F_EXTERN_CFG
 
@@ -1575,6 +1652,25 @@ int launch_tile(Tile t, GemmArgs &g, hipStream_t st) {
     }
 }
 
+// (the layers' tiles run side by side: what counts is how many they are together)
+template <int OUT>
+int launch_adapted(AdaptedLayers &l, const int8_t *x, const float *xs, int M, int K, hipStream_t st) {
+    int64_t N = 0;
+    for (int i = 0; i < l.n; ++i) N += l.N[i];
+    switch (choose_tile(M, N)) {
+    case TILE_BIG: return launch_cfg_adapted<CfgBig, OUT>(l, x, xs, M, K, st);
+    case TILE_B192: return launch_cfg_adapted<CfgB192, OUT>(l, x, xs, M, K, st);
+    case TILE_MID: return launch_cfg_adapted<CfgMid, OUT>(l, x, xs, M, K, st);
+    case TILE_TALL: return launch_cfg_adapted<CfgTall, OUT>(l, x, xs, M, K, st);
+    case TILE_WIDE: return launch_cfg_adapted<CfgWide, OUT>(l, x, xs, M, K, st);
+    case TILE_W96: return launch_cfg_adapted<CfgW96, OUT>(l, x, xs, M, K, st);
+    case TILE_MID_DEEP: return launch_cfg_adapted<CfgMidDeep, OUT>(l, x, xs, M, K, st);
+    case TILE_M96_DEEP: return launch_cfg_adapted<CfgM96Deep, OUT>(l, x, xs, M, K, st);
+    case TILE_S64_DEEP: return launch_cfg_adapted<CfgS64Deep, OUT>(l, x, xs, M, K, st);
+    default: return launch_cfg_adapted<CfgT64Deep, OUT>(l, x, xs, M, K, st);
+    }
+}
+
 template <class C>
 void tile_dims(int *bm, int *bn, int *stages) {
     *bm = C::BM, *bn = C::BN, *stages = C::STAGES;
@@ -1603,20 +1699,18 @@ int launch(GemmArgs &g, hipStream_t st) {
                 sub.gate = (const char *)g.gate + (m0 / g.gate_rows) * g.N * ob;
             }
             if (g.side_t) sub.side_t = (const char *)g.side_t + m0 * g.side_rank * 2;
-            sub.row0 = g.row0 + (int)m0;
             if (int rc = launch<OUT>(sub, st)) return rc;
         }
         return I8F_OK;
     }
     const bool fast = aligned && ((int64_t)g.M * g.K < (1ll << 31));
-    if (g.ids && !fast) return I8F_ERR_UNSUPPORTED;
-    if (g.side_t && !g.ids && (!fast || g.K % 128 || (uintptr_t)g.side_t % 16 || (uintptr_t)g.side_b % 16)) return I8F_ERR_UNSUPPORTED;
+    if (g.side_t && (!fast || g.K % 128 || (uintptr_t)g.side_t % 16 || (uintptr_t)g.side_b % 16)) return I8F_ERR_UNSUPPORTED;
     if (!fast) {
         return launch_ragged<OUT>(g, st);
     }
     Tile t = choose_tile(g.M, g.N);
     int splits = 1;
-    if (g.partials && !g.side_t && !g.ids) choose_split(g.M, g.N, g.K, t, splits);
+    if (g.partials && !g.side_t) choose_split(g.M, g.N, g.K, t, splits);
     g.splits = splits;
     if (splits > 1) {
         static std::atomic<uint32_t> launches{0};

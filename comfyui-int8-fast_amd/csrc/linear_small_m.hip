@@ -298,6 +298,17 @@ __device__ __forceinline__ void small_m_lds_body(const SmallMArgs &a, const int6
 
     int t = wave;
     if (t < nsteps) fetch(t, 0);
+    // (the adapters' share of this thread's outputs, a chain of four dependent loads, while the first weights are on their way)
+    constexpr bool ADAPTED = std::is_same<AD, WithAdapters>::value;
+    [[maybe_unused]] float side[(COLS * 16 + WAVES * 64 - 1) / (WAVES * 64)];
+    if constexpr (ADAPTED) {
+#pragma unroll
+        for (int i = 0; i < (COLS * 16 + WAVES * 64 - 1) / (WAVES * 64); ++i) {
+            const int o = threadIdx.x + i * WAVES * 64, m = o / COLS;
+            const int64_t n = n0 + o % COLS;
+            side[i] = o < COLS * 16 && m < (int)a.M && n < a.N ? adapted<DT>(0.0f, ad, m, n, a.N) : 0.0f;
+        }
+    }
     for (; t < nsteps; t += 2 * WAVES) {
         if (t + WAVES < nsteps) fetch(t + WAVES, 1);
         compute(0);
@@ -312,10 +323,12 @@ __device__ __forceinline__ void small_m_lds_body(const SmallMArgs &a, const int6
 #pragma unroll
         for (int i = 0; i < 4; ++i) red[wave][b * 16 + 4 * g + i][r] = acc[b][i];
     __syncthreads();
-    for (int o = threadIdx.x; o < COLS * 16; o += WAVES * 64) {
+#pragma unroll
+    for (int i = 0; i < (COLS * 16 + WAVES * 64 - 1) / (WAVES * 64); ++i) {
+        const int o = threadIdx.x + i * WAVES * 64;
         const int m = o / COLS, c = o % COLS;
         const int64_t n = n0 + c;
-        if (m < (int)a.M && n < a.N) {
+        if (o < COLS * 16 && m < (int)a.M && n < a.N) {
             float s = red[0][c][m];
 #pragma unroll
             for (int w = 1; w < WAVES; ++w) s += red[w][c][m];
@@ -326,7 +339,9 @@ __device__ __forceinline__ void small_m_lds_body(const SmallMArgs &a, const int6
                 else bv = f16_bits_to_f32(((const uint16_t *)a.bias)[n]);
                 bv = round_to_dtype<DT>(bv);
             }
-            store_from_f32<DT>(a.out, (int64_t)m * a.N + n, adapted<DT>(s + bv, ad, m, n, a.N));
+            s = s + bv;
+            if constexpr (ADAPTED) s = s + side[i];
+            store_from_f32<DT>(a.out, (int64_t)m * a.N + n, s);
         }
     }
 }
@@ -334,11 +349,6 @@ __device__ __forceinline__ void small_m_lds_body(const SmallMArgs &a, const int6
 template <int DT, int NB, int WAVES, bool ROT>
 __global__ __launch_bounds__(WAVES * 64) void small_m_lds_kernel(const SmallMArgs a) {
     small_m_lds_body<DT, NB, WAVES, ROT>(a, (int64_t)blockIdx.x);
-}
-
-template <int DT, int NB, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void small_m_adapters_kernel(const SmallMArgs a, const WithAdapters ad) {
-    small_m_lds_body<DT, NB, WAVES, false>(a, (int64_t)blockIdx.x, ad);
 }
 
 // Several layers in one launch (the modulation projections of the image and of the text stream of a double-stream
@@ -413,19 +423,45 @@ int launch(const SmallMArgs &a, hipStream_t st) {
     return check_launch();
 }
 
+// Layers with adapters (one or several, of one input): a launch for those on the fast path, as above, one each for the others
+struct AdaptedSmallM {
+    SmallMArgs a[I8F_MAX_ADAPTED_LAYERS];
+    WithAdapters ad[I8F_MAX_ADAPTED_LAYERS];
+    int first_block[I8F_MAX_ADAPTED_LAYERS + 1];
+    int n;
+};
+
+template <int DT, int NB, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void small_m_adapters_kernel(const AdaptedSmallM l) {
+    int k = 0;
+#pragma unroll
+    for (int i = 1; i < I8F_MAX_ADAPTED_LAYERS; ++i)
+        if (i < l.n && (int)blockIdx.x >= l.first_block[i]) k = i;
+    k = __builtin_amdgcn_readfirstlane(k);
+    small_m_lds_body<DT, NB, WAVES, false>(l.a[k], (int64_t)((int)blockIdx.x - l.first_block[k]), l.ad[k]);
+}
+
 template <int DT>
-int launch_adapted(const SmallMArgs &a, const WithAdapters &ad, hipStream_t st) {
-    const bool vec = a.K % 16 == 0 && (uintptr_t)a.w % 16 == 0 && (uintptr_t)a.x % 16 == 0 && a.ldx % 8 == 0;
-    if (vec && a.K < (1ll << 30)) {
-        const int nb = blocks_to_workgroup(&a, 1);
-        const dim3 grid((unsigned)((a.N + 16 * nb - 1) / (16 * nb)));
-        if (nb == 1) hipLaunchKernelGGL((small_m_adapters_kernel<DT, 1, 8>), grid, dim3(512), 0, st, a, ad);
-        else if (nb == 2) hipLaunchKernelGGL((small_m_adapters_kernel<DT, 2, 8>), grid, dim3(512), 0, st, a, ad);
-        else hipLaunchKernelGGL((small_m_adapters_kernel<DT, 3, 8>), grid, dim3(512), 0, st, a, ad);
-        return check_launch();
+int launch_adapted(const SmallMArgs *as, const WithAdapters *ads, int n, hipStream_t st) {
+    AdaptedSmallM l{};
+    for (int i = 0; i < n; ++i) {
+        const SmallMArgs &a = as[i];
+        if (a.K % 16 == 0 && (uintptr_t)a.w % 16 == 0 && (uintptr_t)a.x % 16 == 0 && a.ldx % 8 == 0 && a.K > 0 && a.K < (1ll << 30)) {
+            l.a[l.n] = a, l.ad[l.n++] = ads[i];
+            continue;
+        }
+        hipLaunchKernelGGL((small_m_kernel<DT, false, WithAdapters>), dim3((unsigned)((a.N + 3) / 4)), dim3(256), 0, st, a, ads[i]);
+        if (int rc = check_launch()) return rc;
     }
-    dim3 grid((unsigned)((a.N + 3) / 4));
-    hipLaunchKernelGGL((small_m_kernel<DT, false, WithAdapters>), grid, dim3(256), 0, st, a, ad);
+    if (l.n == 0) return I8F_OK;
+    const int together = blocks_to_workgroup(l.a, l.n);
+    int64_t first = 0;
+    for (int i = 0; i < l.n; ++i) l.first_block[i] = (int)first, first += (l.a[i].N + 16 * together - 1) / (16 * together);
+    if (first > 0x7fffffff) return I8F_ERR_UNSUPPORTED;
+    for (int i = l.n; i <= I8F_MAX_ADAPTED_LAYERS; ++i) l.first_block[i] = (int)first;
+    if (together == 3) hipLaunchKernelGGL((small_m_adapters_kernel<DT, 3, 8>), dim3((unsigned)first), dim3(512), 0, st, l);
+    else if (together == 2) hipLaunchKernelGGL((small_m_adapters_kernel<DT, 2, 8>), dim3((unsigned)first), dim3(512), 0, st, l);
+    else hipLaunchKernelGGL((small_m_adapters_kernel<DT, 1, 8>), dim3((unsigned)first), dim3(512), 0, st, l);
     return check_launch();
 }
 
@@ -540,22 +576,30 @@ extern "C" int i8f_internal_w8a16_rotated(const void *x, int x_dtype, int64_t M,
     return x_dtype == I8F_BF16 ? launch_lds<I8F_BF16, 1, 8, true>(a, (hipStream_t)stream) : launch_lds<I8F_F16, 1, 8, true>(a, (hipStream_t)stream);
 }
 
-extern "C" int i8f_linear_w8a16_small_m_adapters(const void *x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const int8_t *w, const float *w_scale,
-                                                 float w_scale_host, int scale_mode, const void *bias, int bias_dtype, const i8f_adapters *adapters,
-                                                 const void *t, void *out, int64_t N, void *stream) {
+extern "C" int i8f_linear_w8a16_small_m_adapters(const void *x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const i8f_adapted_layer *layers,
+                                                 int n_layers, void *stream) {
     using namespace i8f;
-    if (M < 0 || N < 0 || K < 0 || (bias && !valid_dtype(bias_dtype))) return I8F_ERR_INVALID;
-    if (scale_mode != I8F_SCALE_TENSOR && scale_mode != I8F_SCALE_ROW) return I8F_ERR_INVALID;
-    if (int rc = validate_adapters(adapters, x_dtype, M)) return rc;
+    if (K < 0) return I8F_ERR_INVALID;
+    if (int rc = validate_layers(layers, n_layers, x_dtype, M)) return rc;
     if (M > 16) return I8F_ERR_UNSUPPORTED;
-    if (M == 0 || N == 0) return I8F_OK;
-    if (!out || ldx < K || (K > 0 && (!x || !w)) || (scale_mode == I8F_SCALE_ROW && !w_scale)) return I8F_ERR_INVALID;
-    if (adapters->max_rank > 0 && (!t || (uintptr_t)t % 16)) return I8F_ERR_INVALID;
-    if (N > 0x7fffffffll * 4) return I8F_ERR_UNSUPPORTED;
+    if (M == 0 || n_layers == 0) return I8F_OK;
+    if (ldx < K || (K > 0 && !x)) return I8F_ERR_INVALID;
+    SmallMArgs as[I8F_MAX_ADAPTED_LAYERS];
+    WithAdapters ads[I8F_MAX_ADAPTED_LAYERS];
+    int n = 0;
+    for (int i = 0; i < n_layers; ++i) {
+        const i8f_adapted_layer &y = layers[i];
+        if (y.N == 0) continue;
+        if (!y.out || (K > 0 && !y.w) || (y.scale_mode == I8F_SCALE_ROW && !y.w_scale)) return I8F_ERR_INVALID;
+        if (y.N > 0x7fffffff) return I8F_ERR_UNSUPPORTED;
+        SmallMArgs a{};
+        a.x = x, a.M = M, a.K = K, a.ldx = ldx, a.N = y.N, a.w = y.w, a.ws = y.w_scale, a.ws_host = y.w_scale_host;
+        a.row_scale = y.scale_mode == I8F_SCALE_ROW, a.bias = y.bias, a.bias_dtype = y.bias_dtype, a.out = y.out;
+        as[n] = a, ads[n] = WithAdapters{for_kernel(y.adapters), y.t};
+        if (ads[n].ad.max_rank == 0) ads[n].ad.count = 0;
+        ++n;
+    }
+    if (n == 0) return I8F_OK;
     if (int rc = check_device()) return rc;
-    SmallMArgs a{};
-    a.x = x, a.M = M, a.K = K, a.ldx = ldx, a.N = N, a.w = w, a.ws = w_scale, a.ws_host = w_scale_host;
-    a.row_scale = scale_mode == I8F_SCALE_ROW, a.bias = bias, a.bias_dtype = bias_dtype, a.out = out;
-    const WithAdapters ad{for_kernel(*adapters), t};
-    return x_dtype == I8F_BF16 ? launch_adapted<I8F_BF16>(a, ad, (hipStream_t)stream) : launch_adapted<I8F_F16>(a, ad, (hipStream_t)stream);
+    return x_dtype == I8F_BF16 ? launch_adapted<I8F_BF16>(as, ads, n, (hipStream_t)stream) : launch_adapted<I8F_F16>(as, ads, n, (hipStream_t)stream);
 }

@@ -20,6 +20,7 @@
 // registers, the rest across lanes; the order of operations does not depend on
 // how the block is spread over lanes.
 #include <cstdlib>
+#include <type_traits>
 
 #include "i8f_common.hpp"
 #include "quant_run.hpp"
@@ -1085,3 +1086,4 @@ extern "C" int i8f_rotate128(const void *x, int dtype, int64_t M, int64_t K, int
 }
 
 #include "quant_lora.hpp"
+#include "quant_adapters.hpp"

@@ -26,15 +26,35 @@ typedef struct i8f_adapters {
     const int32_t *ids;        /* [ceil(M / rows_per_id)] */
     int64_t rows_per_id;
     int64_t count;
-    int64_t max_rank;          /* the largest padded rank: a multiple of 16, the row stride of t below */
+    int64_t max_rank;          /* the largest padded rank: a multiple of 16, the row stride of t */
 } i8f_adapters;
 
 /*
- * t[m, 0 ... r) = scale_a * A_a x[m] for the adapter a of row m and its padded rank r: sums in binary32, one rounding to x's type (what the
- * matrix unit multiplies with in the second product).  t [M, max_rank]; ranks beyond r and rows without an adapter are left as they are.
- * x_dtype I8F_BF16 or I8F_F16.
+ * A layer and its adapters.  Layers of one call read the same rows, and their adapters have the same ids and rows_per_id.
  */
-int i8f_adapters_down(const void *x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const i8f_adapters *adapters, void *t, void *stream);
+#define I8F_MAX_ADAPTED_LAYERS 4
+typedef struct i8f_adapted_layer {
+    const int8_t *w;           /* [N,K] int8, with w_scale [N] float (I8F_SCALE_ROW) or one scale: w_scale[0], or w_scale_host where it is NULL */
+    const float *w_scale;
+    float w_scale_host;
+    int scale_mode;
+    const void *bias;          /* [N] of bias_dtype or NULL */
+    int bias_dtype;
+    int64_t N;
+    i8f_adapters adapters;
+    void *t;                   /* [M, max_rank] of the activations' type: the adapters' first product */
+    void *out;                 /* [M,N] of the activations' type */
+} i8f_adapted_layer;
+
+/*
+ * t[m, 0 ... r) = scale_a * A_a x[m] of every layer, for the adapter a of row m and its padded rank r: sums in binary32, one rounding to
+ * x's type (what the matrix unit multiplies with in the second product); ranks beyond r and rows without an adapter are left as they
+ * are.  Of the layers only adapters and t are looked at.  x_dtype I8F_BF16 or I8F_F16, n_layers up to I8F_MAX_ADAPTED_LAYERS.
+ * q, scale: NULL, or the int8 rows of x and their scales besides, as i8f_quant_rowwise with rotate_block leaves them (the adapters take
+ * x as it is).
+ */
+int i8f_adapters_down(const void *x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const i8f_adapted_layer *layers, int n_layers,
+                      int rotate_block, int8_t *q, float *scale, void *stream);
 
 /*
  * out[m,n] = round(base[m,n] + sum_j t[m,j] B_a[n,j]); base [M,N] of base_dtype, which is I8F_F32 or out_dtype; out may be base then.
@@ -43,22 +63,23 @@ int i8f_adapters_up(const void *base, int base_dtype, const i8f_adapters *adapte
                     int64_t N, void *stream);
 
 /*
- * i8f_linear_w8a8 with the adapters' second product in its epilogue, in the operation order I8F_EPI_FUSED and rounded once:
+ * i8f_linear_w8a8 of every layer with its adapters' second product in the epilogue, in the operation order I8F_EPI_FUSED and rounded once:
  *   out[m,n] = round(acc * (a_scale[m] * w_scale[n]) + bias[n] + sum_j t[m,j] B_a[n,j])
- * t as i8f_adapters_down leaves it; out_dtype is the factors'.  workspace: any contents, workspace_bytes at least
- * i8f_linear_w8a8_adapters_workspace_bytes(M, N, K).  Rows without an adapter get i8f_linear_w8a8's result in that order, bit for bit.
+ * t as i8f_adapters_down leaves it; out_dtype is the factors'.  Rows without an adapter get i8f_linear_w8a8's result in that order, bit
+ * for bit.  workspace: any contents, at least i8f_linear_w8a8_adapters_workspace_bytes(M, N, K) for the layer that needs most (shapes
+ * that the tiled kernels do not take; 0 else).  I8F_ERR_UNSUPPORTED for operands of the other shapes that are not 16-byte aligned: the
+ * caller then takes i8f_linear_w8a8 in binary32 and i8f_adapters_up.
  */
 int64_t i8f_linear_w8a8_adapters_workspace_bytes(int64_t M, int64_t N, int64_t K);
-int i8f_linear_w8a8_adapters(const int8_t *a, const float *a_scale, const int8_t *w, const float *w_scale, float w_scale_host,
-                             int scale_mode, const void *bias, int bias_dtype, const i8f_adapters *adapters, const void *t, void *out,
-                             int out_dtype, int64_t M, int64_t N, int64_t K, void *workspace, int64_t workspace_bytes, void *stream);
+int i8f_linear_w8a8_adapters(const int8_t *a, const float *a_scale, const i8f_adapted_layer *layers, int n_layers, int out_dtype, int64_t M,
+                             int64_t K, void *workspace, int64_t workspace_bytes, void *stream);
 
 /*
- * i8f_linear_w8a16_small_m (M <= 16) with the adapters' second product added before its one rounding.  x_dtype is the factors' type.
+ * i8f_linear_w8a16_small_m (M <= 16) of every layer with its adapters' second product added before its one rounding.  x_dtype is the
+ * factors' type.
  */
-int i8f_linear_w8a16_small_m_adapters(const void *x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const int8_t *w, const float *w_scale,
-                                      float w_scale_host, int scale_mode, const void *bias, int bias_dtype, const i8f_adapters *adapters,
-                                      const void *t, void *out, int64_t N, void *stream);
+int i8f_linear_w8a16_small_m_adapters(const void *x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const i8f_adapted_layer *layers,
+                                      int n_layers, void *stream);
 
 /*
  * From a block's output y and the residual stream r to the residual stream x behind the block and the input h of the next one:

@@ -18,47 +18,71 @@ def test_the_header_declares_what_the_binding_names(L):
         assert getattr(L.lib(), name) is not None
 
 
+BANK = {"down": 16, "up": 16, "scale": 16, "first_rank": 16, "ids": 16, "rows_per_id": 1, "count": 2, "max_rank": 32}
+LAYER = {"w": 16, "w_scale": 16, "w_scale_host": 1.0, "scale_mode": 0, "N": 8, "t": 16, "out": 16}
+
+
 def _bank(L, **over):
-    fields = {"down": 16, "up": 16, "scale": 16, "first_rank": 16, "ids": 16, "rows_per_id": 1, "count": 2, "max_rank": 32, **over}
-    return ctypes.byref(L._Adapters(*(fields[n] for n, _ in L._Adapters._fields_)))
+    return ctypes.byref(L._Adapters(*({**BANK, **over}[n] for n, _ in L._Adapters._fields_)))
+
+
+def _layers(L, *overs):
+    """An array of layers, each with the fields of its dict (of the layer or of its adapters) instead of the usual ones."""
+    arr = (L._AdaptedLayer * max(1, len(overs)))()
+    for e, over in zip(arr, overs):
+        e.adapters = L._Adapters(*({**BANK, **over}[n] for n, _ in L._Adapters._fields_))
+        for k, v in {**LAYER, **over}.items():
+            if k not in BANK:
+                setattr(e, k, v)
+    return arr
 
 
 def test_adapters_arguments_are_checked_before_any_launch(L):
     lib, null, one = L.lib(), ctypes.c_void_p(None), ctypes.c_void_p(16)
-    down = lambda b, dt=L.BF16, M=4, K=64, ld=64, x=one, t=one: lib.i8f_adapters_down(x, dt, M, K, ld, b, t, null)  # noqa: E731
-    assert down(None) == INVALID
+
+    def down(*overs, dt=L.BF16, M=4, K=64, ld=64, x=one, n=None, rb=0, q=null, s=null):
+        return lib.i8f_adapters_down(x, dt, M, K, ld, _layers(L, *overs), len(overs) if n is None else n, rb, q, s, null)
+
     for bad in ({"count": -1}, {"max_rank": 24}, {"max_rank": -16}, {"rows_per_id": 0}, {"ids": None}, {"first_rank": None}, {"scale": None}, {"down": None},
-                {"up": None}, {"up": 8}):
-        assert down(_bank(L, **bad)) == INVALID, bad
-    assert down(_bank(L, max_rank=1 << 20)) == UNSUPPORTED
-    assert down(_bank(L), dt=L.F32) == INVALID and down(_bank(L), dt=9) == INVALID
-    assert down(_bank(L), M=-1) == INVALID and down(_bank(L), ld=32) == INVALID and down(_bank(L), x=null) == INVALID and down(_bank(L), t=null) == INVALID
-    assert down(_bank(L), t=ctypes.c_void_p(24)) == INVALID
-    assert down(_bank(L), M=1 << 31) == UNSUPPORTED
-    assert down(_bank(L, ids=None), M=0) == 0 and down(_bank(L, count=0), t=null) == 0 and down(_bank(L, max_rank=0, down=None, up=None), t=null) == 0
-    up = lambda b, base=one, bd=L.F32, dt=L.BF16, out=ctypes.c_void_p(32), M=4, N=8, t=one: lib.i8f_adapters_up(base, bd, b, t, out, dt, M, N, null)  # noqa: E731
-    assert up(_bank(L), bd=L.F16) == INVALID and up(_bank(L), dt=L.F32) == INVALID and up(_bank(L), base=null) == INVALID and up(_bank(L), t=null) == INVALID
-    assert up(_bank(L), out=one) == INVALID           # binary32 read where 16 bits are written
-    assert up(_bank(L), N=-1) == INVALID and up(_bank(L), M=0) == 0 and up(_bank(L), N=0) == 0
-    need = lib.i8f_linear_w8a8_adapters_workspace_bytes(20, 8, 64)
-    assert need >= 0 and lib.i8f_linear_w8a8_adapters_workspace_bytes(0, 8, 64) == 0
+                {"up": None}, {"up": 8}, {"t": None}, {"t": 24}):
+        assert down(bad) == INVALID, bad
+        assert down({}, bad) == INVALID, bad
+    assert down({"max_rank": 1 << 20}) == UNSUPPORTED and down(*[{}] * 5) == UNSUPPORTED and down({}, n=-1) == INVALID
+    assert lib.i8f_adapters_down(one, L.BF16, 4, 64, 64, None, 1, 0, null, null, null) == INVALID
+    assert down({}, {"ids": 32}) == INVALID and down({}, {"rows_per_id": 2}) == INVALID     # layers of one call have the same requests
+    assert down({}, dt=L.F32) == INVALID and down({}, dt=9) == INVALID
+    assert down({}, M=-1) == INVALID and down({}, ld=32) == INVALID and down({}, x=null) == INVALID
+    assert down({}, q=one) == INVALID and down({}, s=one) == INVALID and down({}, rb=64) == UNSUPPORTED and down({}, rb=128) == INVALID
+    assert down({}, M=1 << 31) == UNSUPPORTED
+    assert down({"ids": None, "t": None}, M=0) == 0
 
-    def linear(b, M=20, N=8, K=64, t=one, work=one, nbytes=None, dt=L.BF16, mode=0, ws=one):
-        return lib.i8f_linear_w8a8_adapters(one, one, one, ws, 1.0, mode, null, 0, b, t, one, dt, M, N, K, work, 1 << 40 if nbytes is None else nbytes, null)
+    def up(base=one, bd=L.F32, dt=L.BF16, out=ctypes.c_void_p(32), M=4, N=8, t=one):
+        return lib.i8f_adapters_up(base, bd, _bank(L), t, out, dt, M, N, null)
 
-    assert linear(_bank(L), dt=L.F32) == INVALID and linear(_bank(L), t=null) == INVALID and linear(_bank(L), K=-1) == INVALID
-    assert linear(_bank(L), mode=7) == INVALID and linear(_bank(L), mode=1, ws=null) == INVALID
-    assert linear(_bank(L), work=ctypes.c_void_p(24)) == INVALID
-    if need:
-        assert linear(_bank(L), nbytes=need - 1) == INVALID and linear(_bank(L), work=null) == INVALID
-    assert linear(_bank(L), M=0) == 0 and linear(_bank(L), N=0) == 0
+    assert up(bd=L.F16) == INVALID and up(dt=L.F32) == INVALID and up(base=null) == INVALID and up(t=null) == INVALID
+    assert up(out=one) == INVALID           # binary32 read where 16 bits are written
+    assert up(N=-1) == INVALID and up(M=0) == 0 and up(N=0) == 0
+    assert lib.i8f_linear_w8a8_adapters_workspace_bytes(20, 8, 64) == 0 and lib.i8f_linear_w8a8_adapters_workspace_bytes(0, 9, 63) == 0
+    assert lib.i8f_linear_w8a8_adapters_workspace_bytes(20, 9, 64) == 20 * 9 * 4
 
-    def small(b, M=4, N=8, K=64, ld=64, t=one, dt=L.BF16, mode=0, ws=one):
-        return lib.i8f_linear_w8a16_small_m_adapters(one, dt, M, K, ld, one, ws, 1.0, mode, null, 0, b, t, one, N, null)
+    def linear(*overs, M=20, K=64, work=null, nbytes=0, dt=L.BF16, a=one, s=one):
+        return lib.i8f_linear_w8a8_adapters(a, s, _layers(L, *overs), len(overs), dt, M, K, work, nbytes, null)
 
-    assert small(_bank(L), M=17) == UNSUPPORTED and small(_bank(L), ld=32) == INVALID and small(_bank(L), t=null) == INVALID
-    assert small(_bank(L), dt=L.F32) == INVALID and small(_bank(L), mode=3) == INVALID and small(_bank(L), mode=1, ws=null) == INVALID
-    assert small(_bank(L), M=0) == 0
+    for bad in ({"t": None}, {"scale_mode": 7}, {"scale_mode": 1, "w_scale": None}, {"N": -1}, {"w": None}, {"out": None}, {"bias": 16, "bias_dtype": 9}, {"ids": None}):
+        assert linear(bad) == INVALID, bad
+    assert linear({}, dt=L.F32) == INVALID and linear({}, K=-1) == INVALID and linear({}, s=null) == INVALID and linear({}, a=null) == INVALID
+    assert linear({}, work=ctypes.c_void_p(24)) == INVALID
+    assert linear({"N": 9}) == INVALID and linear({"N": 9}, work=one, nbytes=20 * 9 * 4 - 1) == INVALID     # needs a workspace
+    assert linear({"w": 24}) == UNSUPPORTED and linear({"out": 18}) == UNSUPPORTED and linear({}, a=ctypes.c_void_p(20)) == UNSUPPORTED
+    assert linear({}, M=0) == 0 and linear() == 0
+
+    def small(*overs, M=4, K=64, ld=64, dt=L.BF16, x=one):
+        return lib.i8f_linear_w8a16_small_m_adapters(x, dt, M, K, ld, _layers(L, *overs), len(overs), null)
+
+    for bad in ({"t": None}, {"scale_mode": 3}, {"scale_mode": 1, "w_scale": None}, {"w": None}, {"out": None}, {"N": -1}):
+        assert small(bad) == INVALID, bad
+    assert small({}, M=17) == UNSUPPORTED and small({}, ld=32) == INVALID and small({}, dt=L.F32) == INVALID and small({}, x=null) == INVALID
+    assert small({}, M=0) == 0 and small() == 0
 
 
 def _norm(L, **over):
