@@ -10,9 +10,9 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from . import _lib
+from . import _lib, int8_fused_kernel
 from .adapters import _quantised_here
-from .int8_quant import SMALL_BATCH_ROWS, _project_quantised, forward_fanout
+from .int8_quant import SMALL_BATCH_ROWS, _layers_in_place, _project_quantised, forward_fanout
 
 
 def block_norm(y: Tensor, residual: Tensor, *, post_norm: str | None = None, post_weight: Tensor | None = None, post_bias: Tensor | None = None,
@@ -28,6 +28,11 @@ def block_norm(y: Tensor, residual: Tensor, *, post_norm: str | None = None, pos
     y, residual: tensors alike, bfloat16, float16 or float32.  gate, mod_scale, mod_shift: of y's dtype, [K] or y's shape with ones from
     some leading dimension on ([batch, 1, K] for one vector to an image).  Everything is computed in binary32, h from x before its
     rounding; x and h are rounded once.  No gradients: under grad mode an input that asks for one is refused."""
+    if type(y) is Tensor and y.is_cuda and not torch.compiler.is_compiling():
+        out = _lib.host().block_norm(y, residual, post_norm, post_weight, post_bias, post_eps, gate, gate_tanh, residual_scale, branch_scale, pre_norm,
+                                     pre_weight, pre_bias, pre_eps, mod_scale, mod_shift, None, None, None, None, False, 0, None)
+        if out is not None:
+            return out
     operands = dict(post_norm=post_norm, post_weight=post_weight, post_bias=post_bias, post_eps=post_eps, gate=gate, gate_tanh=gate_tanh,
                     residual_scale=residual_scale, branch_scale=branch_scale, pre_norm=pre_norm, pre_weight=pre_weight, pre_bias=pre_bias,
                     pre_eps=pre_eps, mod_scale=mod_scale, mod_shift=mod_shift)
@@ -35,11 +40,27 @@ def block_norm(y: Tensor, residual: Tensor, *, post_norm: str | None = None, pos
     return _lib.block_norm(y, residual, **operands)
 
 
+def _forward_native(layers, y, residual, post_norm=None, post_weight=None, post_bias=None, post_eps=1e-6, gate=None, gate_tanh=False, residual_scale=1.0,
+                    branch_scale=1.0, pre_norm=None, pre_weight=None, pre_bias=None, pre_eps=1e-6, mod_scale=None, mod_shift=None):
+    """forward_block_norm() without the interpreter's part of it, for layers of one rotation flag on the W8A8 path with everything in place;
+    None for everything else."""
+    parts = _layers_in_place(layers)
+    if parts is None:
+        return None
+    work = _lib._splitk_workspace if y.shape[-1] >= _lib.SPLITK_MIN_K else None
+    return _lib.host().block_norm(y, residual, post_norm, post_weight, post_bias, post_eps, gate, gate_tanh, residual_scale, branch_scale, pre_norm, pre_weight,
+                                  pre_bias, pre_eps, mod_scale, mod_shift, *parts, int8_fused_kernel.DEFAULT_EPILOGUE, work)
+
+
 def forward_block_norm(layers, y: Tensor, residual: Tensor, **operands):
     """(x, [layer(h) for layer in layers]) of block_norm(y, residual, **operands), which has to have an h: the next block's first projections
     along with the step in front of them.  Where the layers are on the W8A8 path (as for forward_fanout) h is quantised where it is computed
     and never stored; the results are those of block_norm and the layers' own forward bit for bit."""
     layers = list(layers)
+    if type(y) is Tensor and y.is_cuda and 0 < len(layers) <= 8 and y.numel() // max(1, y.shape[-1]) > SMALL_BATCH_ROWS and not torch.compiler.is_compiling():
+        out = _forward_native(layers, y, residual, **operands)
+        if out is not None:
+            return out
     _refuse_gradients(y, residual, operands)
     if operands.get("pre_norm") is None and operands.get("mod_scale") is None and operands.get("mod_shift") is None:
         raise ValueError("the layers need an h: give pre_norm, mod_scale or mod_shift")

@@ -7,6 +7,8 @@
 //   linear(...)                 one layer: Linear.forward with its optional prologue, gate and residual
 //   fanout(...)                 several layers that read the same tokens, quantised once
 //   vector_fanout(...)          several small-batch layers that read the same rows, in one launch
+//   adapters(...)               layers that read the same rows, with a low-rank adapter for each of them
+//   block_norm(...)             what lies between two blocks, and the next one's projections where they are given
 //
 // Every function takes the cases it can decide on cheaply and returns None for all others (tensors of other types,
 // devices or layouts, operands that need a cast or a copy, errors): the caller then goes the general way in Python, which
@@ -21,12 +23,14 @@
 #include <ATen/autocast_mode.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../../include/i8f.h"
+#include "../../../include/i8f_blocks.h"
 #include "../quant_lora_entry.hpp"
 #include "../w8a16_rotated.hpp"
 
@@ -36,7 +40,8 @@ namespace {
 #define I8F_ENTRY_POINTS(X)                                                                                              \
     X(i8f_quant_rowwise) X(i8f_quant_rowwise_prologue) X(i8f_quant_rowwise_norm_modulate) X(i8f_quant_rowwise_rms_norm)  \
     X(i8f_quant_rowwise_concat_gelu) X(i8f_rotate128) X(i8f_linear_w8a8_gated) X(i8f_linear_w8a8_grouped) X(i8f_linear_w8a16_small_m) \
-    X(i8f_linear_w8a16_small_m_grouped) X(i8f_internal_w8a16_rotated) X(i8f_linear_w8a8_lora) X(i8f_internal_quant_lora)
+    X(i8f_linear_w8a16_small_m_grouped) X(i8f_internal_w8a16_rotated) X(i8f_linear_w8a8_lora) X(i8f_internal_quant_lora)    \
+    X(i8f_adapters_down) X(i8f_linear_w8a8_adapters) X(i8f_linear_w8a8_adapters_workspace_bytes) X(i8f_linear_w8a16_small_m_adapters) X(i8f_block_norm)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
     I8F_ENTRY_POINTS(X)
@@ -265,6 +270,27 @@ PyObject *list_of(at::Tensor *y, Py_ssize_t count) {
     return out;
 }
 
+// The layers' products of the same int8 rows: layers of one form, a launch for as many as the library puts together.
+int project(const Layer *l, int count, int8_t *q, float *qs, int64_t M, int64_t K, int dt, int order, at::Tensor *y, void *work, int64_t work_bytes,
+            void *stream) {
+    int rc = 0;
+    for (int first = 0, next; !rc && first < count; first = next) {
+        i8f_linear_group g[I8F_MAX_LINEAR_GROUPS] = {};
+        int bias_code = -1;
+        for (next = first; next < count && next - first < I8F_MAX_LINEAR_GROUPS; ++next) {
+            const Layer &o = l[next];
+            if (o.N != l[first].N || o.mode != l[first].mode || (o.bias && bias_code >= 0 && o.bias_code != bias_code)) break;
+            if (o.bias) bias_code = o.bias_code;
+            i8f_linear_group &e = g[next - first];
+            e.a = q, e.a_scale = qs, e.w = o.w, e.w_scale = o.ws, e.w_scale_host = o.ws_host, e.bias = o.bias, e.out = y[next].data_ptr(), e.M = M;
+            e.rows_per_gate = 1;
+        }
+        rc = lib.i8f_linear_w8a8_grouped(g, next - first, l[first].mode, bias_code < 0 ? (int)I8F_BF16 : bias_code, dt, l[first].N, K, order, work,
+                                         work_bytes, stream);
+    }
+    return rc;
+}
+
 // The W8A8 form of linear and fanout, whose arguments these are; a gate or a residual for one layer only.
 PyObject *w8a8(PyObject *const *a, const at::Tensor &x, int64_t M, int64_t K, int64_t ld, const Layer *l, int count, const Stream &st) {
     const int dt = code_of(x.scalar_type()), order = (int)PyLong_AsLong(a[7]), kind = (int)PyLong_AsLong(a[8]);
@@ -375,20 +401,7 @@ PyObject *w8a8(PyObject *const *a, const at::Tensor &x, int64_t M, int64_t K, in
         if (!rc && count == 1)
             rc = lib.i8f_linear_w8a8_gated(q, qs, l[0].w, l[0].ws, l[0].ws_host, l[0].mode, l[0].bias, l[0].bias_code, gate_p, gate_rows, res_p,
                                            y[0].data_ptr(), dt, M, l[0].N, l[0].K, order, work_p, work_bytes, st.handle);
-        for (int first = 0, next; count > 1 && !rc && first < count; first = next) {  // layers of one form, a launch for as many as the library puts together
-            i8f_linear_group g[I8F_MAX_LINEAR_GROUPS] = {};
-            int bias_code = -1;
-            for (next = first; next < count && next - first < I8F_MAX_LINEAR_GROUPS; ++next) {
-                const Layer &o = l[next];
-                if (o.N != l[first].N || o.mode != l[first].mode || (o.bias && bias_code >= 0 && o.bias_code != bias_code)) break;
-                if (o.bias) bias_code = o.bias_code;
-                i8f_linear_group &e = g[next - first];
-                e.a = q, e.a_scale = qs, e.w = o.w, e.w_scale = o.ws, e.w_scale_host = o.ws_host, e.bias = o.bias, e.out = y[next].data_ptr(), e.M = M;
-                e.rows_per_gate = 1;
-            }
-            rc = lib.i8f_linear_w8a8_grouped(g, next - first, l[first].mode, bias_code < 0 ? (int)I8F_BF16 : bias_code, dt, l[first].N, Kall, order, work_p,
-                                             work_bytes, st.handle);
-        }
+        if (!rc && count > 1) rc = project(l, count, q, qs, M, Kall, dt, order, y, work_p, work_bytes, st.handle);
     }
     if (rc) Py_RETURN_NONE;
     return count == 1 ? THPVariable_Wrap(std::move(y[0])) : list_of(y, count);
@@ -494,6 +507,230 @@ PyObject *vector_fanout(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return list_of(y, count);
 }
 
+// Whether an operand asks for a gradient that these operators do not have: the general path words the refusal.
+bool wants_gradient(const at::Tensor *t) { return t && t->requires_grad() && c10::GradMode::is_enabled(); }
+
+// v has the shape of t's leading dimensions, all of them but the last or fewer: the rows of t to an element of v, 0 if it has not.
+int64_t rows_to_element(const at::Tensor &t, const at::Tensor &v) {
+    const int64_t lead = t.dim() - 1;
+    if (v.dim() > lead) return 0;
+    for (int64_t i = 0; i < v.dim(); ++i)
+        if (v.size(i) != t.size(i)) return 0;
+    int64_t rows = 1;
+    for (int64_t i = v.dim(); i < lead; ++i) rows *= t.size(i);
+    return rows;
+}
+
+// adapters(x, ids, weights, scales, biases, per_row, rotate, small_rows, banks): tuples with an entry for each layer, a bank being (down,
+// up, scale, first_rank, count, max_rank) -> list of outputs.
+PyObject *adapters(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 9) return PyErr_Format(PyExc_TypeError, "adapters takes 9 arguments, got %zd", n);
+    const at::Tensor *xt = tensor(a[0]), *ids = tensor(a[1]);
+    if (!lib.bound || !xt || !ids || !xt->is_cuda()) Py_RETURN_NONE;
+    const at::Tensor &x = *xt;
+    const int dt = code_of(x.scalar_type());
+    const Py_ssize_t count = PyTuple_Check(a[2]) ? PyTuple_GET_SIZE(a[2]) : 0;
+    const bool rotate = a[6] == Py_True;
+    int64_t M, K, ld;
+    const Stream st(x.device());
+    if (!st.ok || (dt != I8F_BF16 && dt != I8F_F16) || wants_gradient(xt) || !rows_of(x, M, K, ld) || count < 1 || count > I8F_MAX_ADAPTED_LAYERS ||
+        (rotate && K % 128))
+        Py_RETURN_NONE;
+    if (ids->scalar_type() != at::kInt || ids->device() != x.device() || !ids->is_contiguous()) Py_RETURN_NONE;
+    const int64_t per = rows_to_element(x, *ids);
+    if (per < 1) Py_RETURN_NONE;
+    for (int i : {3, 4, 5, 8})
+        if (!PyTuple_Check(a[i]) || PyTuple_GET_SIZE(a[i]) != count) Py_RETURN_NONE;
+    const bool few = M <= PyLong_AsLongLong(a[7]);
+    i8f_adapted_layer l[I8F_MAX_ADAPTED_LAYERS] = {};
+    Size size[I8F_MAX_ADAPTED_LAYERS];
+    int64_t bytes = 0, t_at[I8F_MAX_ADAPTED_LAYERS], work_bytes = 0;
+    const auto take = [&](int64_t b) {   // a piece of the scratch memory
+        const int64_t at = bytes;
+        bytes += (b + 255) / 256 * 256;
+        return at;
+    };
+    const int64_t q_at = few ? (rotate ? take(2 * M * K) : 0) : take(M * K), qs_at = few ? 0 : take(4 * M);
+    for (Py_ssize_t i = 0; i < count; ++i) {
+        Layer o;
+        if (!layer_of(PyTuple_GET_ITEM(a[2], i), PyTuple_GET_ITEM(a[3], i), PyTuple_GET_ITEM(a[4], i), PyTuple_GET_ITEM(a[5], i) == Py_True, x.device(), o) || o.K != K)
+            Py_RETURN_NONE;
+        PyObject *bank = PyTuple_GET_ITEM(a[8], i);
+        if (!PyTuple_Check(bank) || PyTuple_GET_SIZE(bank) != 6) Py_RETURN_NONE;
+        const at::Tensor *down = tensor(PyTuple_GET_ITEM(bank, 0)), *up = tensor(PyTuple_GET_ITEM(bank, 1)), *scale = tensor(PyTuple_GET_ITEM(bank, 2)),
+                         *first = tensor(PyTuple_GET_ITEM(bank, 3));
+        i8f_adapters &ad = l[i].adapters;
+        ad.count = PyLong_AsLongLong(PyTuple_GET_ITEM(bank, 4)), ad.max_rank = PyLong_AsLongLong(PyTuple_GET_ITEM(bank, 5));
+        if (!down || !up || !scale || !first || down->scalar_type() != x.scalar_type() || down->device() != x.device() || down->dim() != 2 || down->size(1) != K ||
+            up->scalar_type() != x.scalar_type() || up->device() != x.device() || up->numel() != down->size(0) * o.N || scale->numel() != ad.count ||
+            first->numel() != ad.count + 1)
+            Py_RETURN_NONE;
+        ad.down = down->const_data_ptr(), ad.up = up->const_data_ptr(), ad.scale = (const float *)scale->const_data_ptr();
+        ad.first_rank = (const int32_t *)first->const_data_ptr(), ad.ids = (const int32_t *)ids->const_data_ptr(), ad.rows_per_id = per;
+        l[i].w = o.w, l[i].w_scale = o.ws, l[i].w_scale_host = o.ws_host, l[i].scale_mode = o.mode, l[i].bias = o.bias, l[i].bias_dtype = o.bias_code, l[i].N = o.N;
+        size[i] = output_size(x, o.N);
+        t_at[i] = take(2 * M * ad.max_rank);
+        const int64_t need = few ? 0 : lib.i8f_linear_w8a8_adapters_workspace_bytes(M, o.N, K);
+        work_bytes = need > work_bytes ? need : work_bytes;
+    }
+    const int64_t work_at = work_bytes ? take(work_bytes) : 0;
+    const at::ScalarType type = x.scalar_type();
+    const at::Device dev = x.device();
+    const void *xp = x.const_data_ptr();
+    at::Tensor scratch, y[I8F_MAX_ADAPTED_LAYERS];
+    int rc;
+    {
+        const WithoutGil released;
+        scratch = empty({bytes + 256}, at::kByte, dev);
+        char *base = (char *)scratch.data_ptr();
+        for (Py_ssize_t i = 0; i < count; ++i) {
+            y[i] = empty(size[i], type, dev);
+            l[i].t = base + t_at[i], l[i].out = y[i].data_ptr();
+        }
+        if (few) {
+            rc = lib.i8f_adapters_down(xp, dt, M, K, ld, l, (int)count, 0, nullptr, nullptr, st.handle);
+            if (!rc && rotate) {
+                rc = lib.i8f_rotate128(xp, dt, M, K, ld, base + q_at, st.handle);
+                xp = base + q_at, ld = K;
+            }
+            if (!rc) rc = lib.i8f_linear_w8a16_small_m_adapters(xp, dt, M, K, ld, l, (int)count, st.handle);
+        } else {
+            int8_t *q = (int8_t *)base + q_at;
+            float *qs = (float *)(base + qs_at);
+            rc = lib.i8f_adapters_down(xp, dt, M, K, ld, l, (int)count, rotate ? 128 : 0, q, qs, st.handle);
+            if (!rc) rc = lib.i8f_linear_w8a8_adapters(q, qs, l, (int)count, dt, M, K, work_bytes ? base + work_at : nullptr, work_bytes, st.handle);
+        }
+    }
+    if (rc) Py_RETURN_NONE;
+    return list_of(y, count);
+}
+
+// An operand of block_norm's vectors: [K], or y's dimensions with ones from some dimension on; *rows of y to a vector.
+bool block_vector(const at::Tensor &y, PyObject *o, const void **p, int64_t *rows) {
+    if (o == Py_None) return true;
+    const at::Tensor *v = tensor(o);
+    const int64_t lead = y.dim() - 1, K = y.size(lead);
+    if (!v || wants_gradient(v) || v->scalar_type() != y.scalar_type() || v->device() != y.device() || !v->is_contiguous() || v->dim() < 1 || v->size(-1) != K) return false;
+    int64_t shared = 0;
+    if (v->dim() != 1) {
+        if (v->dim() != y.dim()) return false;
+        while (shared < lead && v->size(shared) == y.size(shared)) ++shared;
+        for (int64_t i = shared; i < lead; ++i)
+            if (v->size(i) != 1) return false;
+    }
+    *rows = 1;
+    for (int64_t i = shared; i < lead; ++i) *rows *= y.size(i);
+    *p = v->const_data_ptr();
+    return true;
+}
+
+// One of block_norm's norms: kind, weight, bias, eps at a[0..3]
+bool block_norm_of(const at::Tensor &y, PyObject *const *a, int *kind, const void **weight, const void **bias, int *dtype, float *eps) {
+    *dtype = code_of(y.scalar_type());
+    if (a[0] == Py_None) *kind = I8F_NORM_NONE;
+    else if (PyUnicode_Check(a[0]) && PyUnicode_CompareWithASCIIString(a[0], "rms") == 0) *kind = I8F_NORM_RMS;
+    else if (PyUnicode_Check(a[0]) && PyUnicode_CompareWithASCIIString(a[0], "layer") == 0) *kind = I8F_NORM_LAYER;
+    else return false;
+    *eps = (float)PyFloat_AsDouble(a[3]);
+    if (PyErr_Occurred() || !(*eps >= 0.0f)) return false;
+    int found = -1;
+    for (int i = 1; i <= 2; ++i) {
+        if (a[i] == Py_None) continue;
+        const at::Tensor *v = tensor(a[i]);
+        if (!v || *kind == I8F_NORM_NONE || wants_gradient(v) || v->dim() != 1 || v->size(0) != y.size(-1) || v->device() != y.device() || !v->is_contiguous()) return false;
+        const int code = code_of(v->scalar_type());
+        if ((code != *dtype && code != I8F_F32) || (found >= 0 && code != found)) return false;
+        found = code;
+        *(i == 1 ? weight : bias) = v->const_data_ptr();
+    }
+    if (found >= 0) *dtype = found;
+    return true;
+}
+
+// block_norm(y, residual, post_norm, post_weight, post_bias, post_eps, gate, gate_tanh, residual_scale, branch_scale, pre_norm, pre_weight,
+//            pre_bias, pre_eps, mod_scale, mod_shift, weights, scales, biases, per_row, rotate, order, workspace): weights is None -> (x,
+// h); tuples with an entry for each layer -> (x, list of the layers' outputs), not for 16 rows or fewer
+PyObject *block_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 23) return PyErr_Format(PyExc_TypeError, "block_norm takes 23 arguments, got %zd", n);
+    const at::Tensor *yt = tensor(a[0]), *rt = tensor(a[1]);
+    if (!lib.bound || !yt || !rt || !yt->is_cuda()) Py_RETURN_NONE;
+    const at::Tensor &y = *yt, &r = *rt;
+    const int dt = code_of(y.scalar_type());
+    int64_t M, K, Mr, Kr;
+    i8f_block_norm_args g = {};
+    const Stream st(y.device());
+    if (!st.ok || dt < 0 || wants_gradient(yt) || wants_gradient(rt) || r.scalar_type() != y.scalar_type() || r.device() != y.device() || r.sizes() != y.sizes() ||
+        !rows_of(y, M, K, g.ldy) || !rows_of(r, Mr, Kr, g.ldr))
+        Py_RETURN_NONE;
+    g.rows_per_gate = g.rows_per_scale = g.rows_per_shift = 1;
+    if (!block_norm_of(y, a + 2, &g.post_norm, &g.post_weight, &g.post_bias, &g.post_dtype, &g.post_eps) ||
+        !block_norm_of(y, a + 10, &g.pre_norm, &g.pre_weight, &g.pre_bias, &g.pre_dtype, &g.pre_eps) || !block_vector(y, a[6], &g.gate, &g.rows_per_gate) ||
+        !block_vector(y, a[14], &g.mod_scale, &g.rows_per_scale) || !block_vector(y, a[15], &g.mod_shift, &g.rows_per_shift))
+        Py_RETURN_NONE;
+    g.gate_tanh = PyObject_IsTrue(a[7]) == 1;
+    g.residual_scale = (float)PyFloat_AsDouble(a[8]), g.branch_scale = (float)PyFloat_AsDouble(a[9]);
+    if (PyErr_Occurred()) return nullptr;
+    g.y = y.const_data_ptr(), g.residual = r.const_data_ptr(), g.M = M, g.K = K, g.dtype = dt;
+    const bool with_h = g.pre_norm != I8F_NORM_NONE || g.mod_scale || g.mod_shift;
+    const Py_ssize_t count = PyTuple_Check(a[16]) ? PyTuple_GET_SIZE(a[16]) : 0;
+    Layer l[MAX_FANOUT];
+    Size size[MAX_FANOUT];
+    Owned work_object;
+    const at::Tensor *work = nullptr;
+    if (a[16] != Py_None) {
+        if (count < 1 || count > MAX_FANOUT || !with_h || dt == I8F_F32 || y.dim() < 2 || M <= 16) Py_RETURN_NONE;
+        g.rotate_block = a[20] == Py_True ? 128 : 0;
+        if (g.rotate_block && K % 128) Py_RETURN_NONE;
+        int64_t narrowest = -1;
+        for (int i = 17; i <= 19; ++i)
+            if (!PyTuple_Check(a[i]) || PyTuple_GET_SIZE(a[i]) != count) Py_RETURN_NONE;
+        for (Py_ssize_t i = 0; i < count; ++i) {
+            if (!layer_of(PyTuple_GET_ITEM(a[16], i), PyTuple_GET_ITEM(a[17], i), PyTuple_GET_ITEM(a[18], i), PyTuple_GET_ITEM(a[19], i) == Py_True, y.device(), l[i]) ||
+                l[i].K != K)
+                Py_RETURN_NONE;
+            size[i] = output_size(y, l[i].N);
+            narrowest = narrowest < 0 || l[i].N < narrowest ? l[i].N : narrowest;
+        }
+        if (a[22] != Py_None) {
+            work_object.p = PyObject_CallFunction(a[22], "OLLL", a[0], (long long)M, (long long)narrowest, (long long)K);
+            if (!work_object.p) return nullptr;
+            if (work_object.p != Py_None && !(work = tensor(work_object.p))) Py_RETURN_NONE;
+        }
+    }
+    const int order = (int)PyLong_AsLong(a[21]);
+    const at::ScalarType type = y.scalar_type();
+    const at::Device dev = y.device();
+    const Size shape(y.sizes().begin(), y.sizes().end());
+    void *work_p = work ? work->data_ptr() : nullptr;
+    const int64_t work_bytes = work ? work->numel() : 0;
+    at::Tensor x, h, scratch, outs[MAX_FANOUT];
+    int rc;
+    {
+        const WithoutGil released;
+        x = empty(shape, type, dev);
+        g.x_out = x.data_ptr();
+        if (count) {
+            const int64_t q_bytes = (M * K + 255) / 256 * 256;
+            scratch = empty({q_bytes + 4 * M}, at::kByte, dev);
+            g.q = (int8_t *)scratch.data_ptr(), g.scale = (float *)(g.q + q_bytes);
+            for (Py_ssize_t i = 0; i < count; ++i) outs[i] = empty(size[i], type, dev);
+        } else if (with_h) {
+            h = empty(shape, type, dev);
+            g.h = h.data_ptr();
+        }
+        rc = lib.i8f_block_norm(&g, st.handle);
+        if (!rc && count) rc = project(l, (int)count, g.q, g.scale, M, K, dt, order, outs, work_p, work_bytes, st.handle);
+    }
+    if (rc) Py_RETURN_NONE;
+    Owned first, second;
+    first.p = THPVariable_Wrap(std::move(x));
+    if (count) second.p = list_of(outs, count);
+    else if (with_h) second.p = THPVariable_Wrap(std::move(h));
+    else Py_INCREF(Py_None), second.p = Py_None;
+    if (!first.p || !second.p) return nullptr;
+    return PyTuple_Pack(2, first.p, second.p);
+}
+
 // No C++ exception leaves an entry point: an allocator that has nothing left, say, becomes the general path's to report.
 template <PyObject *(*F)(PyObject *, PyObject *const *, Py_ssize_t)>
 PyObject *guarded(PyObject *self, PyObject *const *a, Py_ssize_t n) {
@@ -516,6 +753,8 @@ PyMethodDef methods[] = {
     {"fanout", (PyCFunction)(void (*)(void))guarded<fanout>, METH_FASTCALL, "several quantised layers of the same tokens, or None"},
     {"linear_lora", (PyCFunction)(void (*)(void))guarded<linear_lora>, METH_FASTCALL, "one quantised layer with a dynamic LoRA, or None"},
     {"vector_fanout", (PyCFunction)(void (*)(void))guarded<vector_fanout>, METH_FASTCALL, "several small-batch layers, or None"},
+    {"adapters", (PyCFunction)(void (*)(void))guarded<adapters>, METH_FASTCALL, "quantised layers with an adapter for each row, or None"},
+    {"block_norm", (PyCFunction)(void (*)(void))guarded<block_norm>, METH_FASTCALL, "what lies between two blocks, or None"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_i8f_host", "Native host path of the INT8 linear layers.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -172,6 +172,29 @@ def _scale_on(lin, device):
     return ws
 
 
+def _layers_in_place(layers):
+    """(weights, scales, biases, per-row flags, rotation flag) of quantised layers as the host path takes them, or None where a layer has
+    something that is not in place: managed casting, a dynamic LoRA, a weight or bias that is no parameter, another rotation flag."""
+    weights, scales, biases, per_row = [], [], [], []
+    rotate = bool(getattr(layers[0], "_use_quarot", False))
+    for lin in layers:
+        scale = getattr(lin, "_weight_scale_scalar", None)
+        if not getattr(lin, "_is_quantized", False) or bool(lin._use_quarot) != rotate:
+            return None
+        params = lin._parameters
+        weight = params.get("weight")
+        if scale is None:
+            scale = lin._buffers.get("weight_scale")
+        if (lin.comfy_cast_weights or lin.lora_A is not None or weight is None or scale is None or "bias" not in params
+                or len(lin.weight_function) > 0 or len(lin.bias_function) > 0):
+            return None
+        weights.append(weight)
+        scales.append(scale)
+        biases.append(params["bias"])
+        per_row.append(bool(lin._is_per_row))
+    return tuple(weights), tuple(scales), tuple(biases), tuple(per_row), rotate
+
+
 def _project_quantised(layers, q, s, dtype):
     """The layers' products of the same int8 rows: [M, out features] of `dtype` for each."""
     problems = []
