@@ -84,7 +84,9 @@ def lib() -> ctypes.CDLL:
     L.i8f_lora_merge_sr_drawn.argtypes = [vp, vp, f32, i32, vp, i32, f32, ctypes.c_uint64, i64, i64, i64, vp, vp, i64, vp]
     L.i8f_lora_merge_sr_drawn_workspace_bytes.argtypes = [i64, i64, i64, i32]
     L.i8f_lora_merge_sr_drawn_workspace_bytes.restype = i64
-    L.i8f_adapters_down.argtypes = [vp, i32, i64, i64, i64, vp, i32, i32, vp, vp, vp]
+    L.i8f_adapters_down.argtypes = [vp, i32, i64, i64, i64, vp, i32, i32, vp, vp, vp, i64, vp]
+    L.i8f_adapters_down_workspace_bytes.argtypes = [i64, i64, i64]
+    L.i8f_adapters_down_workspace_bytes.restype = i64
     L.i8f_adapters_up.argtypes = [vp, i32, vp, vp, vp, i32, i64, i64, vp]
     L.i8f_linear_w8a8_adapters_workspace_bytes.argtypes = [i64, i64, i64]
     L.i8f_linear_w8a8_adapters_workspace_bytes.restype = i64
@@ -130,7 +132,7 @@ EXPORTS = (
 
 
 # the entry points of include/i8f_blocks.h
-BLOCK_EXPORTS = ("i8f_adapters_down", "i8f_adapters_up", "i8f_linear_w8a8_adapters_workspace_bytes", "i8f_linear_w8a8_adapters",
+BLOCK_EXPORTS = ("i8f_adapters_down_workspace_bytes", "i8f_adapters_down", "i8f_adapters_up", "i8f_linear_w8a8_adapters_workspace_bytes", "i8f_linear_w8a8_adapters",
                  "i8f_linear_w8a16_small_m_adapters", "i8f_block_norm")
 
 ERR_UNSUPPORTED = -2   # I8F_ERR_UNSUPPORTED
@@ -912,9 +914,11 @@ def adapters_down(x, banks, ids, rows_per_id=1, quantise=False, rotate=False):
     layers = (_AdaptedLayer * max(1, len(banks)))()
     for e, bank, t in zip(layers, banks, ts):
         e.adapters, e.t = _adapters_arg(bank, ids, rows_per_id), _addr(t)
+    nbytes = lib().i8f_adapters_down_workspace_bytes(M, K, sum(bank.max_rank for bank in banks))
+    work = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
     with _on(x.device):
         _check(lib().i8f_adapters_down(_ptr(x), dtype_code(x.dtype), M, K, x.stride(0) if M > 1 else K, layers, len(banks), 128 if rotate else 0,
-                                       _ptr(q), _ptr(s), _stream(x)), "i8f_adapters_down")
+                                       _ptr(q), _ptr(s), _ptr(work), nbytes, _stream(x)), "i8f_adapters_down")
     return (ts, q, s) if quantise else ts
 
 

@@ -36,6 +36,19 @@ __device__ __forceinline__ float adapter_term(const i8f_adapters &ad, const void
     return sum;
 }
 
+// The adapters of up to four layers, of one ids and rows_per_id, and where their first products go
+struct DownLayers {
+    i8f_adapters ad[I8F_MAX_ADAPTED_LAYERS];
+    char *t[I8F_MAX_ADAPTED_LAYERS];
+    int first_block[I8F_MAX_ADAPTED_LAYERS + 1];   // (rows form: first workgroup of each layer behind the quantiser's; [n] = all)
+    int first_column[I8F_MAX_ADAPTED_LAYERS + 1];  // (partial sums: first column of each layer, max_rank of them; [n] = all)
+    int n;
+};
+// Many rows (adapters_down.hip): slices of the columns that a launch for M rows is split into, and the launch; partial: [slices, M,
+// first_column[n]] float where slices > 1.
+int adapters_down_slices(int64_t M, int64_t K);
+int adapters_down_partial(const void *x, int dtype, int64_t M, int64_t K, int64_t ldx, const DownLayers &g, float *partial, int slices, hipStream_t st);
+
 // Host: whether the structure can be used on M rows of 16-bit type `dtype` at all (I8F_OK), before any pointer in it is.
 inline int validate_adapters(const i8f_adapters *ad, int dtype, int64_t M) {
     if (!ad || ad->count < 0 || ad->count > 0x7fffffff || ad->max_rank < 0 || ad->max_rank % 16 || ad->rows_per_id <= 0) return I8F_ERR_INVALID;

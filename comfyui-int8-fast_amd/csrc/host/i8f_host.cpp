@@ -41,7 +41,7 @@ namespace {
     X(i8f_quant_rowwise) X(i8f_quant_rowwise_prologue) X(i8f_quant_rowwise_norm_modulate) X(i8f_quant_rowwise_rms_norm)  \
     X(i8f_quant_rowwise_concat_gelu) X(i8f_rotate128) X(i8f_linear_w8a8_gated) X(i8f_linear_w8a8_grouped) X(i8f_linear_w8a16_small_m) \
     X(i8f_linear_w8a16_small_m_grouped) X(i8f_internal_w8a16_rotated) X(i8f_linear_w8a8_lora) X(i8f_internal_quant_lora)    \
-    X(i8f_adapters_down) X(i8f_linear_w8a8_adapters) X(i8f_linear_w8a8_adapters_workspace_bytes) X(i8f_linear_w8a16_small_m_adapters) X(i8f_block_norm)
+    X(i8f_adapters_down) X(i8f_adapters_down_workspace_bytes) X(i8f_linear_w8a8_adapters) X(i8f_linear_w8a8_adapters_workspace_bytes) X(i8f_linear_w8a16_small_m_adapters) X(i8f_block_norm)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
     I8F_ENTRY_POINTS(X)
@@ -573,7 +573,11 @@ PyObject *adapters(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const int64_t need = few ? 0 : lib.i8f_linear_w8a8_adapters_workspace_bytes(M, o.N, K);
         work_bytes = need > work_bytes ? need : work_bytes;
     }
-    const int64_t work_at = work_bytes ? take(work_bytes) : 0;
+    // (the memory of the first products is free when the projections start)
+    int64_t ranks = 0;
+    for (Py_ssize_t i = 0; i < count; ++i) ranks += l[i].adapters.max_rank;
+    const int64_t down_bytes = lib.i8f_adapters_down_workspace_bytes(M, K, ranks), more = down_bytes > work_bytes ? down_bytes : work_bytes;
+    const int64_t work_at = more ? take(more) : 0;
     const at::ScalarType type = x.scalar_type();
     const at::Device dev = x.device();
     const void *xp = x.const_data_ptr();
@@ -588,7 +592,7 @@ PyObject *adapters(PyObject *, PyObject *const *a, Py_ssize_t n) {
             l[i].t = base + t_at[i], l[i].out = y[i].data_ptr();
         }
         if (few) {
-            rc = lib.i8f_adapters_down(xp, dt, M, K, ld, l, (int)count, 0, nullptr, nullptr, st.handle);
+            rc = lib.i8f_adapters_down(xp, dt, M, K, ld, l, (int)count, 0, nullptr, nullptr, nullptr, 0, st.handle);
             if (!rc && rotate) {
                 rc = lib.i8f_rotate128(xp, dt, M, K, ld, base + q_at, st.handle);
                 xp = base + q_at, ld = K;
@@ -597,7 +601,7 @@ PyObject *adapters(PyObject *, PyObject *const *a, Py_ssize_t n) {
         } else {
             int8_t *q = (int8_t *)base + q_at;
             float *qs = (float *)(base + qs_at);
-            rc = lib.i8f_adapters_down(xp, dt, M, K, ld, l, (int)count, rotate ? 128 : 0, q, qs, st.handle);
+            rc = lib.i8f_adapters_down(xp, dt, M, K, ld, l, (int)count, rotate ? 128 : 0, q, qs, down_bytes ? base + work_at : nullptr, down_bytes, st.handle);
             if (!rc) rc = lib.i8f_linear_w8a8_adapters(q, qs, l, (int)count, dt, M, K, work_bytes ? base + work_at : nullptr, work_bytes, st.handle);
         }
     }

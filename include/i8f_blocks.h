@@ -52,9 +52,12 @@ typedef struct i8f_adapted_layer {
  * are.  Of the layers only adapters and t are looked at.  x_dtype I8F_BF16 or I8F_F16, n_layers up to I8F_MAX_ADAPTED_LAYERS.
  * q, scale: NULL, or the int8 rows of x and their scales besides, as i8f_quant_rowwise with rotate_block leaves them (the adapters take
  * x as it is).
+ * workspace: any contents; i8f_adapters_down_workspace_bytes(M, K, the sum of the layers' max_rank) bytes let many rows' columns be dealt over
+ * more workgroups; less, or NULL, is slower there and rounds otherwise in the last place of the binary32 sums.
  */
+int64_t i8f_adapters_down_workspace_bytes(int64_t M, int64_t K, int64_t ranks);
 int i8f_adapters_down(const void *x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const i8f_adapted_layer *layers, int n_layers,
-                      int rotate_block, int8_t *q, float *scale, void *stream);
+                      int rotate_block, int8_t *q, float *scale, void *workspace, int64_t workspace_bytes, void *stream);
 
 /*
  * out[m,n] = round(base[m,n] + sum_j t[m,j] B_a[n,j]); base [M,N] of base_dtype, which is I8F_F32 or out_dtype; out may be base then.

@@ -40,19 +40,23 @@ def _layers(L, *overs):
 def test_adapters_arguments_are_checked_before_any_launch(L):
     lib, null, one = L.lib(), ctypes.c_void_p(None), ctypes.c_void_p(16)
 
-    def down(*overs, dt=L.BF16, M=4, K=64, ld=64, x=one, n=None, rb=0, q=null, s=null):
-        return lib.i8f_adapters_down(x, dt, M, K, ld, _layers(L, *overs), len(overs) if n is None else n, rb, q, s, null)
+    def down(*overs, dt=L.BF16, M=4, K=64, ld=64, x=one, n=None, rb=0, q=null, s=null, work=null):
+        return lib.i8f_adapters_down(x, dt, M, K, ld, _layers(L, *overs), len(overs) if n is None else n, rb, q, s, work, 0, null)
 
     for bad in ({"count": -1}, {"max_rank": 24}, {"max_rank": -16}, {"rows_per_id": 0}, {"ids": None}, {"first_rank": None}, {"scale": None}, {"down": None},
                 {"up": None}, {"up": 8}, {"t": None}, {"t": 24}):
         assert down(bad) == INVALID, bad
         assert down({}, bad) == INVALID, bad
     assert down({"max_rank": 1 << 20}) == UNSUPPORTED and down(*[{}] * 5) == UNSUPPORTED and down({}, n=-1) == INVALID
-    assert lib.i8f_adapters_down(one, L.BF16, 4, 64, 64, None, 1, 0, null, null, null) == INVALID
+    assert lib.i8f_adapters_down(one, L.BF16, 4, 64, 64, None, 1, 0, null, null, null, 0, null) == INVALID
     assert down({}, {"ids": 32}) == INVALID and down({}, {"rows_per_id": 2}) == INVALID     # layers of one call have the same requests
     assert down({}, dt=L.F32) == INVALID and down({}, dt=9) == INVALID
     assert down({}, M=-1) == INVALID and down({}, ld=32) == INVALID and down({}, x=null) == INVALID
     assert down({}, q=one) == INVALID and down({}, s=one) == INVALID and down({}, rb=64) == UNSUPPORTED and down({}, rb=128) == INVALID
+    assert down({}, work=ctypes.c_void_p(8)) == INVALID
+    size = lib.i8f_adapters_down_workspace_bytes
+    assert size(16, 4096, 32) == size(0, 64, 16) == size(4096, 0, 16) == size(4096, 64, 0) == size(1 << 31, 64, 16) == 0
+    assert size(4096, 4096, 32) % (4096 * 32 * 4) == 0 and size(4096, 4096, 32) > 0
     assert down({}, M=1 << 31) == UNSUPPORTED
     assert down({"ids": None, "t": None}, M=0) == 0
 
