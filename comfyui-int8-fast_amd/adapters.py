@@ -119,7 +119,8 @@ def forward_adapters(layers, x: Tensor, banks, ids: Tensor):
           request without an adapter.  The numbers are read by the kernels, so a captured graph follows what is written into the tensor.
 
     One rounding at the end: the projection stays in binary32 (in the order of _lib.EPI_FUSED) until the adapter's share has been
-    added; down @ x is rounded to x's dtype for the matrix unit.  x is quantised once for all layers.  The adapter acts on x itself,
+    added; down @ x is rounded to x's dtype for the matrix unit.  x is quantised once for all layers; which layers go together may change the
+    order of binary32 sums.  The adapter acts on x itself,
     also where the layer rotates its activations (a dynamic LoRA of the layer gets them rotated).  Layers whose own kernels cannot take
     the adapters (not quantised, weights that ComfyUI casts or moves for the call, a dynamic LoRA attached) run by themselves, and
     their rounded result gets the adapters' share.  No gradients: under grad mode an input that asks for one is refused."""

@@ -58,15 +58,15 @@ GEMM_OUTS = ("OUT_BF16", "OUT_F16", "OUT_F32", "OUT_I32")
 
 def units() -> list[tuple[str, str, list[str]]]:
     """(source, name of the object file, extra flags) of every compilation, the longest first."""
-    out = []
-    tiles = os.path.join(CSRC, "gemm_i8_tiles.hip")
+    tiles, norms = os.path.join(CSRC, "gemm_i8_tiles.hip"), os.path.join(CSRC, "block_norm.hip")
+    out = [(norms, "block_norm.o", [])]
     for cfg in GEMM_CFGS:
         for o in GEMM_OUTS:
             grouped = int(cfg in GEMM_GROUPED and o != "OUT_I32")
             adapted = int(o in ("OUT_BF16", "OUT_F16"))
             out.append((tiles, f"gemm_i8_tiles_{cfg}_{o}.o", [f"-DI8F_TU_CFG={cfg}", f"-DI8F_TU_OUT={o}", f"-DI8F_TU_GROUPED={grouped}", f"-DI8F_TU_ADAPTED={adapted}"]))
     for src in sorted(glob.glob(os.path.join(CSRC, "*.hip"))):
-        if src != tiles:
+        if src not in (tiles, norms):
             out.append((src, os.path.basename(src)[:-4] + ".o", []))
     return out
 

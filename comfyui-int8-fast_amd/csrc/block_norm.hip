@@ -27,7 +27,7 @@ __device__ __forceinline__ float norm_operand(const void *p, int dtype, int64_t 
     return DT == I8F_F32 || dtype == I8F_F32 ? ((const float *)p)[k] : load_as_f32<DT>(p, k);
 }
 
-// ---- any width, any alignment: 256 threads to a row, which is read again for every statistic (from cache) ------------------
+// ---- rows of less than a run, or too wide for registers: 256 threads to a row, which is read again for every statistic (from cache) ----------------
 template <int DT, int H>
 __global__ __launch_bounds__(256) void block_norm_generic_kernel(const i8f_block_norm_args a) {
     __shared__ float red[4];
@@ -137,11 +137,16 @@ template <int DT>
 struct Raw {
     uint4 v[DT == I8F_F32 ? 1 : 2];
 };
-template <int DT>
+// ANY: from whatever address it has
+template <int DT, bool ANY>
 __device__ __forceinline__ Raw<DT> load_run(const char *p) {
     Raw<DT> r;
-    r.v[0] = *(const uint4 *)p;
-    if constexpr (DT != I8F_F32) r.v[1] = *(const uint4 *)(p + 16);
+    if constexpr (ANY) {
+        __builtin_memcpy(&r, p, sizeof(r));
+    } else {
+        r.v[0] = *(const uint4 *)p;
+        if constexpr (DT != I8F_F32) r.v[1] = *(const uint4 *)(p + 16);
+    }
     return r;
 }
 template <int DT>
@@ -149,39 +154,44 @@ __device__ __forceinline__ void expand(const Raw<DT> &r, float (&v)[Run<DT>::N])
     if constexpr (DT == I8F_F32) v[0] = __uint_as_float(r.v[0].x), v[1] = __uint_as_float(r.v[0].y), v[2] = __uint_as_float(r.v[0].z), v[3] = __uint_as_float(r.v[0].w);
     else expand16<DT>(r.v[0], r.v[1], v);
 }
-template <int DT>
+template <int DT, bool ANY>
 __device__ __forceinline__ void store_run(char *p, const float (&v)[Run<DT>::N]) {
-    if constexpr (DT == I8F_F32) {
-        stream_store16(p, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
-    } else {
-        uint32_t o[8];
+    constexpr int N = Run<DT>::N;
+    uint32_t o[DT == I8F_F32 ? 4 : 8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = DT == I8F_BF16 ? f32x2_to_bf16x2_bits(v[2 * e], v[2 * e + 1]) : f32x2_to_f16x2_bits(v[2 * e], v[2 * e + 1]);
+    for (int e = 0; e < (DT == I8F_F32 ? 4 : 8); ++e)
+        o[e] = DT == I8F_F32 ? __float_as_uint(v[e % N]) : DT == I8F_BF16 ? f32x2_to_bf16x2_bits(v[2 * e % N], v[(2 * e + 1) % N]) : f32x2_to_f16x2_bits(v[2 * e % N], v[(2 * e + 1) % N]);
+    if constexpr (ANY) {
+        __builtin_memcpy(p, o, sizeof(o));
+    } else {
         stream_store16(p, make_uint4(o[0], o[1], o[2], o[3]));
-        stream_store16(p + 16, make_uint4(o[4], o[5], o[6], o[7]));
+        if constexpr (DT != I8F_F32) stream_store16(p + 16, make_uint4(o[4], o[5], o[6], o[7]));
     }
 }
 // the run of a weight or bias that starts at element k
-template <int DT>
+template <int DT, bool ANY>
 __device__ __forceinline__ void operand_run(const void *p, int dtype, int64_t k, float (&v)[Run<DT>::N]) {
     if (DT != I8F_F32 && dtype == I8F_F32) {
 #pragma unroll
         for (int e = 0; e < Run<DT>::N; e += 4) {
-            const float4 f = *(const float4 *)((const float *)p + k + e);
-            v[e] = f.x, v[e + 1] = f.y, v[e + 2] = f.z, v[e + 3] = f.w;
+            float f[4];
+            expand<I8F_F32>(load_run<I8F_F32, ANY>((const char *)((const float *)p + k + e)), f);
+            v[e] = f[0], v[e + 1] = f[1], v[e + 2] = f[2], v[e + 3] = f[3];
         }
     } else {
-        expand<DT>(load_run<DT>((const char *)p + k * (DT == I8F_F32 ? 4 : 2)), v);
+        expand<DT>(load_run<DT, ANY>((const char *)p + k * (DT == I8F_F32 ? 4 : 2)), v);
     }
 }
 
-template <int DT, int H, int WPR, int NCH>
+// ANY: rows of any width (a run at least) and alignment.  A row's last run then ends with it and begins in the run before, whose elements it
+// computes again and leaves out of the sums, which are the same ones in the same order.
+template <int DT, int H, int WPR, int NCH, bool ANY>
 __global__ __launch_bounds__(256) void block_norm_kernel(const i8f_block_norm_args a) {
     constexpr int N = Run<DT>::N, TPR = 64 * WPR, ROWS = 4 / WPR, SIZE = DT == I8F_F32 ? 4 : 2;
     __shared__ float red[5][ROWS][WPR];
     const int t = threadIdx.x % TPR, rb = threadIdx.x / TPR, lane = threadIdx.x & 63;
     const int64_t K = a.K;
-    const int runs = (int)(K / N);
+    const int runs = (int)((K + N - 1) / N);
     const int64_t own = (int64_t)blockIdx.x * ROWS + rb;
     const bool ok = own < a.M;
     const int64_t m = ok ? own : a.M - 1;   // (a wave past the last row computes it again and stores nothing)
@@ -201,13 +211,16 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const i8f_block_norm_ar
     };
     int64_t at[NCH];   // first element of each run; a lane without one takes the row's first and leaves it out of the sums
     bool in[NCH];
+    int skip[NCH];     // ANY: elements that belong to the run before
     Raw<DT> yr[NCH], rr[NCH];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
         in[i] = i * TPR + p < runs;
         at[i] = in[i] ? (int64_t)(i * TPR + p) * N : 0;
-        yr[i] = load_run<DT>((const char *)a.y + (m * a.ldy + at[i]) * SIZE);
-        rr[i] = load_run<DT>((const char *)a.residual + (m * a.ldr + at[i]) * SIZE);
+        skip[i] = 0;
+        if (ANY && at[i] > K - N) skip[i] = (int)(at[i] - (K - N)), at[i] = K - N;
+        yr[i] = load_run<DT, ANY>((const char *)a.y + (m * a.ldy + at[i]) * SIZE);
+        rr[i] = load_run<DT, ANY>((const char *)a.residual + (m * a.ldr + at[i]) * SIZE);
     }
     float x[NCH][N];
 #pragma unroll
@@ -220,7 +233,7 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const i8f_block_norm_ar
 #pragma unroll
             for (int i = 0; i < NCH; ++i)
 #pragma unroll
-                for (int e = 0; e < N; ++e) sum += in[i] ? x[i][e] : 0.0f;
+                for (int e = 0; e < N; ++e) sum += in[i] && (!ANY || e >= skip[i]) ? x[i][e] : 0.0f;
             const float mean = sum_over_row(sum, slot) / (float)K;
 #pragma unroll
             for (int i = 0; i < NCH; ++i)
@@ -232,7 +245,7 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const i8f_block_norm_ar
         for (int i = 0; i < NCH; ++i) {
             float s = 0.0f;
 #pragma unroll
-            for (int e = 0; e < N; ++e) s = __builtin_fmaf(x[i][e], x[i][e], s);
+            for (int e = 0; e < N; ++e) s = ANY && e < skip[i] ? s : __builtin_fmaf(x[i][e], x[i][e], s);
             squares += in[i] ? s : 0.0f;
         }
         const float rstd = 1.0f / sqrtf(sum_over_row(squares, slot + 1) / (float)K + eps);
@@ -242,12 +255,12 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const i8f_block_norm_ar
 #pragma unroll
             for (int e = 0; e < N; ++e) x[i][e] *= rstd;
             if (w) {
-                operand_run<DT>(w, dtype, at[i], v);
+                operand_run<DT, ANY>(w, dtype, at[i], v);
 #pragma unroll
                 for (int e = 0; e < N; ++e) x[i][e] *= v[e];
             }
             if (b) {
-                operand_run<DT>(b, dtype, at[i], v);
+                operand_run<DT, ANY>(b, dtype, at[i], v);
 #pragma unroll
                 for (int e = 0; e < N; ++e) x[i][e] += v[e];
             }
@@ -261,7 +274,7 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const i8f_block_norm_ar
         float r[N], g[N];
         expand<DT>(rr[i], r);
         if (gate) {
-            expand<DT>(load_run<DT>(gate + at[i] * SIZE), g);
+            expand<DT>(load_run<DT, ANY>(gate + at[i] * SIZE), g);
             if (a.gate_tanh) {
 #pragma unroll
                 for (int e = 0; e < N; ++e) g[e] = gate_tanh<DT>(g[e]);
@@ -272,7 +285,7 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const i8f_block_norm_ar
 #pragma unroll
             for (int e = 0; e < N; ++e) x[i][e] = __builtin_fmaf(x[i][e], a.branch_scale, a.residual_scale * r[e]);
         }
-        if (ok && in[i]) store_run<DT>((char *)a.x_out + (m * K + at[i]) * SIZE, x[i]);
+        if (ok && in[i]) store_run<DT, ANY>((char *)a.x_out + (m * K + at[i]) * SIZE, x[i]);
     }
     if constexpr (H == H_NONE) return;
     normalise(a.pre_norm, a.pre_eps, a.pre_weight, a.pre_bias, a.pre_dtype, 2);
@@ -282,17 +295,17 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const i8f_block_norm_ar
     for (int i = 0; i < NCH; ++i) {
         float v[N];
         if (ms) {
-            expand<DT>(load_run<DT>(ms + at[i] * SIZE), v);
+            expand<DT>(load_run<DT, ANY>(ms + at[i] * SIZE), v);
 #pragma unroll
             for (int e = 0; e < N; ++e) x[i][e] *= 1.0f + v[e];
         }
         if (mt) {
-            expand<DT>(load_run<DT>(mt + at[i] * SIZE), v);
+            expand<DT>(load_run<DT, ANY>(mt + at[i] * SIZE), v);
 #pragma unroll
             for (int e = 0; e < N; ++e) x[i][e] += v[e];
         }
         if constexpr (H == H_STORED) {
-            if (ok && in[i]) store_run<DT>((char *)a.h + (m * K + at[i]) * SIZE, x[i]);
+            if (ok && in[i]) store_run<DT, ANY>((char *)a.h + (m * K + at[i]) * SIZE, x[i]);
         } else {   // i8f_quant_rowwise's arithmetic on the rounded h
 #pragma unroll
             for (int e = 0; e < N; ++e) x[i][e] = in[i] ? round_to_dtype<DT>(x[i][e]) : 0.0f;
@@ -330,42 +343,48 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const i8f_block_norm_ar
                 uint32_t w = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w |= ((uint32_t)quant_i8(x[i][e] * inv) & 0xffu) << (8 * e);
-                *(uint32_t *)dst = w;
+                __builtin_memcpy(dst, &w, 4);
             } else {
-                stream_store16(dst, quant16_magic(x[i], inv));
+                const uint4 o = quant16_magic(x[i], inv);
+                if constexpr (ANY) __builtin_memcpy(dst, &o, 16);
+                else stream_store16(dst, o);
             }
         }
         if (t == 0) a.scale[m] = s;
     }
 }
 
-template <int DT, int H, int WPR, int NCH>
+template <int DT, int H, int WPR, int NCH, bool ANY>
 int launch_rows(const i8f_block_norm_args &a, hipStream_t st) {
     constexpr int ROWS = 4 / WPR;
-    hipLaunchKernelGGL((block_norm_kernel<DT, H, WPR, NCH>), dim3((unsigned)((a.M + ROWS - 1) / ROWS)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((block_norm_kernel<DT, H, WPR, NCH, ANY>), dim3((unsigned)((a.M + ROWS - 1) / ROWS)), dim3(256), 0, st, a);
     return check_launch();
 }
 
 // Aligned rows of whole runs; 16-byte pieces of every operand
-bool in_registers(const i8f_block_norm_args &a, int run) {
+bool whole_runs(const i8f_block_norm_args &a, int run) {
     const uintptr_t all = (uintptr_t)a.y | (uintptr_t)a.residual | (uintptr_t)a.post_weight | (uintptr_t)a.post_bias | (uintptr_t)a.pre_weight |
                           (uintptr_t)a.pre_bias | (uintptr_t)a.gate | (uintptr_t)a.mod_scale | (uintptr_t)a.mod_shift | (uintptr_t)a.x_out |
                           (uintptr_t)a.h | (uintptr_t)a.q;
     const int64_t per16 = 16 / (int64_t)dtype_size(a.dtype);
-    return all % 16 == 0 && a.K % run == 0 && a.K / run <= 1024 && a.ldy % per16 == 0 && a.ldr % per16 == 0;
+    return all % 16 == 0 && a.K % run == 0 && a.ldy % per16 == 0 && a.ldr % per16 == 0;
+}
+
+template <int DT, int H, bool ANY>
+int launch_width(const i8f_block_norm_args &a, int64_t runs, hipStream_t st) {
+    if (runs <= 64) return launch_rows<DT, H, 1, 1, ANY>(a, st);
+    if (runs <= 128) return launch_rows<DT, H, 1, 2, ANY>(a, st);
+    if (runs <= 256) return launch_rows<DT, H, 4, 1, ANY>(a, st);
+    if (runs <= 512) return launch_rows<DT, H, 4, 2, ANY>(a, st);
+    if (runs <= 768) return launch_rows<DT, H, 4, 3, ANY>(a, st);
+    return launch_rows<DT, H, 4, 4, ANY>(a, st);
 }
 
 template <int DT, int H>
 int launch(const i8f_block_norm_args &a, hipStream_t st) {
-    if (in_registers(a, Run<DT>::N)) {
-        const int runs = (int)(a.K / Run<DT>::N);
-        if (runs <= 64) return launch_rows<DT, H, 1, 1>(a, st);
-        if (runs <= 128) return launch_rows<DT, H, 1, 2>(a, st);
-        if (runs <= 256) return launch_rows<DT, H, 4, 1>(a, st);
-        if (runs <= 512) return launch_rows<DT, H, 4, 2>(a, st);
-        if (runs <= 768) return launch_rows<DT, H, 4, 3>(a, st);
-        return launch_rows<DT, H, 4, 4>(a, st);
-    }
+    constexpr int N = Run<DT>::N;
+    const int64_t runs = (a.K + N - 1) / N;
+    if (runs <= 1024 && a.K >= N) return whole_runs(a, N) ? launch_width<DT, H, false>(a, runs, st) : launch_width<DT, H, true>(a, runs, st);
     hipLaunchKernelGGL((block_norm_generic_kernel<DT, H>), dim3((unsigned)a.M), dim3(256), 0, st, a);
     return check_launch();
 }

@@ -83,9 +83,10 @@ __global__ __launch_bounds__(256) void adapters_rows_kernel(const char *__restri
     if (lane == 0) store_from_f32<DT>(g.t[l], m * ad.max_rank + j, sum * ad.scale[a]);
 }
 
-// Rows up to which a rank of a row is a wave of its own: whatever adapters the rows have, x and a factor's row are fetched again for
-// each, so that there is a limit of bytes too; beyond, rows share the factors (adapters_down.hip).
-constexpr int64_t DOWN_ROWS = 256, DOWN_BYTES = 64ll << 20;
+// Where a rank of a row is a wave of its own: few rows, whatever adapters they have, or a small x; x and a factor's row are fetched again
+// for each, so that beyond it rows share the factors (adapters_down.hip).  Not by the number of ranks: a layer's sums do not depend on the
+// layers beside it.
+constexpr int64_t DOWN_ROWS = 256, DOWN_ELEMENTS = 1 << 19;
 
 template <int DT, bool ROT, int RUNS>
 int launch_rows_form(const void *x, int64_t M, int64_t K, int64_t ldx, int8_t *q, float *scale, DownLayers &g, hipStream_t st) {
@@ -102,7 +103,7 @@ int launch_rows_form(const void *x, int64_t M, int64_t K, int64_t ldx, int8_t *q
 enum DownForm { DOWN_ANY, DOWN_ROW_WAVES, DOWN_PARTIAL };
 inline DownForm down_form(const void *x, int64_t M, int64_t K, int64_t ldx, int64_t ranks) {
     if (K % 8 || (uintptr_t)x % 16 || ldx % 8 || K < 1 || ldx >= (1ll << 23)) return DOWN_ANY;   // (32-bit offsets within 64 rows)
-    return M * ranks < (1ll << 30) && (M <= DOWN_ROWS || M * ranks * K * 4 <= DOWN_BYTES) ? DOWN_ROW_WAVES : DOWN_PARTIAL;
+    return M * ranks < (1ll << 30) && (M <= DOWN_ROWS || M * K <= DOWN_ELEMENTS) ? DOWN_ROW_WAVES : DOWN_PARTIAL;
 }
 
 template <int DT>
@@ -165,5 +166,5 @@ extern "C" int i8f_adapters_down(const void *x, int x_dtype, int64_t M, int64_t 
 extern "C" int64_t i8f_adapters_down_workspace_bytes(int64_t M, int64_t K, int64_t ranks) {
     if (M <= 0 || K <= 0 || ranks <= 0 || M > 0x7fffffff || K > 0x7fffffff) return 0;
     const int slices = i8f::adapters_down_slices(M, K);
-    return M <= i8f::DOWN_ROWS || slices < 2 ? 0 : slices * M * ranks * 4;
+    return M <= i8f::DOWN_ROWS || M * K <= i8f::DOWN_ELEMENTS || slices < 2 ? 0 : slices * M * ranks * 4;
 }

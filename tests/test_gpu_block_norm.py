@@ -294,19 +294,21 @@ def test_refusals(pkg, L, dev):
 
 def test_a_run_of_blocks(pkg, L, dev):
     """The two operators as a model uses them: adapted projections, what lies between the blocks, and the feed-forward's projections."""
-    from test_gpu_adapters import factors_of
+    from test_gpu_adapters import check as check_adapted, expected as expected_adapted, factors_of
 
     dtype, batch, tokens, K, hidden = torch.bfloat16, 3, 40, 256, 512
     qkv, proj, up, down = layers_of(pkg, K, (K, K, K), dtype), layers_of(pkg, K, (K,), dtype)[0], layers_of(pkg, K, (hidden, hidden), dtype), layers_of(pkg, hidden, (K,), dtype)[0]
-    banks = [pkg.AdapterBank(factors_of(K, K, (8, None, 32), dtype, i)) for i in range(3)]
+    adapters = [factors_of(K, K, (8, None, 32), dtype, i) for i in range(3)]
+    banks = [pkg.AdapterBank(a) for a in adapters]
     ids = torch.tensor([2, -1, 0], dtype=torch.int32, device=dev)
     x, ops = inputs((batch, tokens, K), dtype)[0], operands((batch, tokens, K), dtype, "rms", "rms", "tanh")[0]
     branch = torch.zeros_like(x)
     for _ in range(2):
         x, h = pkg.block_norm(branch, x, **ops)
         q, k, v = pkg.forward_adapters(qkv, h, banks, ids)
-        for lin, bank, o in zip(qkv, banks, (q, k, v)):
-            assert torch.equal(o, pkg.forward_adapters(lin, h, bank, ids))
+        for lin, some, o in zip(qkv, adapters, (q, k, v)):
+            want, bound = expected_adapted(pkg, lin, h.view(-1, K), some, ids.repeat_interleave(tokens))
+            check_adapted(o.view(-1, K), want, bound)
         mixed = torch.softmax(q.float() @ k.float().transpose(1, 2) / K ** 0.5, -1) @ v.float()
         x_before = x
         x, (a, b) = pkg.forward_block_norm(up, proj(mixed.to(dtype)), x, **ops)
