@@ -85,7 +85,7 @@ def lib() -> ctypes.CDLL:
     L.i8f_lora_merge_sr_drawn_workspace_bytes.argtypes = [i64, i64, i64, i32]
     L.i8f_lora_merge_sr_drawn_workspace_bytes.restype = i64
     L.i8f_adapters_down.argtypes = [vp, i32, i64, i64, i64, vp, i32, i32, vp, vp, vp, i64, vp]
-    L.i8f_adapters_down_workspace_bytes.argtypes = [i64, i64, i64]
+    L.i8f_adapters_down_workspace_bytes.argtypes = [i64, i64, i64, i32]
     L.i8f_adapters_down_workspace_bytes.restype = i64
     L.i8f_adapters_up.argtypes = [vp, i32, vp, vp, vp, i32, i64, i64, vp]
     L.i8f_linear_w8a8_adapters_workspace_bytes.argtypes = [i64, i64, i64]
@@ -914,7 +914,8 @@ def adapters_down(x, banks, ids, rows_per_id=1, quantise=False, rotate=False):
     layers = (_AdaptedLayer * max(1, len(banks)))()
     for e, bank, t in zip(layers, banks, ts):
         e.adapters, e.t = _adapters_arg(bank, ids, rows_per_id), _addr(t)
-    nbytes = lib().i8f_adapters_down_workspace_bytes(M, K, sum(bank.max_rank for bank in banks))
+    aligned = x.data_ptr() % 16 == 0 and (M <= 1 or x.stride(0) % 8 == 0)
+    nbytes = lib().i8f_adapters_down_workspace_bytes(M, K, sum(bank.max_rank for bank in banks), int(aligned))
     work = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
     with _on(x.device):
         _check(lib().i8f_adapters_down(_ptr(x), dtype_code(x.dtype), M, K, x.stride(0) if M > 1 else K, layers, len(banks), 128 if rotate else 0,

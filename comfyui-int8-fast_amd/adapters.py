@@ -59,12 +59,12 @@ class AdapterBank:
         if offsets[-1] >= 1 << 31 or self.max_rank > 65536:
             raise ValueError(f"the ranks of a bank add up to less than 2^31 and stay within 65536, got {offsets[-1]} and {self.max_rank}")
         with torch.no_grad():
-            down_all = torch.zeros((offsets[-1], in_features), dtype=dtype, device=device)
+            down_all = torch.zeros((offsets[-1], -(-in_features // 8) * 8), dtype=dtype, device=device)   # (whole 16-byte pieces)
             up_all = torch.zeros((offsets[-1] * out_features,), dtype=dtype, device=device)
             for entry, at, r in zip(entries, offsets, padded):
                 if entry is not None and entry[0].shape[0]:
                     down, up, _ = entry
-                    down_all[at:at + down.shape[0]] = down.detach().to(device=device, dtype=dtype)
+                    down_all[at:at + down.shape[0], :in_features] = down.detach().to(device=device, dtype=dtype)
                     up_all[at * out_features:(at + r) * out_features].view(out_features, r)[:, :up.shape[1]] = up.detach().to(device=device, dtype=dtype)
         self.down, self.up = down_all, up_all
         self.scale = torch.tensor([0.0 if e is None else e[2] for e in entries], dtype=torch.float32, device=device)

@@ -202,6 +202,26 @@ __global__ __launch_bounds__(256) void adapters_combine_kernel(const float *__re
     *(uint2 *)(g.t[l] + (m * g.ad[l].max_rank + j) * 2) = o;
 }
 
+// rows of 16-bit values to rows of a multiple of eight of them, zeros behind: eight to a thread
+__global__ __launch_bounds__(256) void copy_rows_kernel(const uint16_t *__restrict__ x, int64_t pieces, int K, int64_t ldx, int per_row, char *__restrict__ to) {
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at >= pieces) return;
+    const int64_t m = at / per_row;
+    const int k = (int)(at % per_row) * 8;
+    const uint16_t *p = x + m * ldx + k;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (k + 8 <= K) {
+        __builtin_memcpy(&v, p, 16);
+    } else {
+        uint16_t e[8] = {};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (k + i < K) e[i] = p[i];
+        __builtin_memcpy(&v, e, 16);
+    }
+    *(uint4 *)(to + at * 16) = v;
+}
+
 template <int DT>
 int launch(const char *x, int M, int K, int ldx_bytes, const DownLayers &g, float *partial, int slices, hipStream_t st) {
     const int per = ((K + BK - 1) / BK + slices - 1) / slices;
@@ -223,13 +243,20 @@ int launch(const char *x, int M, int K, int ldx_bytes, const DownLayers &g, floa
 
 // Two workgroups to a CU, slices of at least four K-tiles, none of them empty
 int adapters_down_slices(int64_t M, int64_t K) {
-    const int64_t blocks = (M + ROWS - 1) / ROWS, tiles = (K + BK - 1) / BK;
+    const int64_t blocks = (M + ROWS - 1) / ROWS, tiles = (factor_width(K) + BK - 1) / BK;
     int64_t s = 512 / blocks;
     if (s > tiles / 4) s = tiles / 4;
     if (s > 16) s = 16;
     if (s < 2) return 1;
     const int64_t per = (tiles + s - 1) / s;
     return (int)((tiles + per - 1) / per);
+}
+
+int adapters_copy_rows(const void *x, int64_t M, int64_t K, int64_t ldx, void *to, hipStream_t st) {
+    const int64_t per_row = factor_width(K) / 8, pieces = M * per_row;
+    if ((pieces + 255) / 256 > 0x7fffffff) return I8F_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL(copy_rows_kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, st, (const uint16_t *)x, pieces, (int)K, ldx, (int)per_row, (char *)to);
+    return check_launch();
 }
 
 int adapters_down_partial(const void *x, int dtype, int64_t M, int64_t K, int64_t ldx, const DownLayers &g, float *partial, int slices, hipStream_t st) {

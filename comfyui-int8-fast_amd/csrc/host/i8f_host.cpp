@@ -561,7 +561,7 @@ PyObject *adapters(PyObject *, PyObject *const *a, Py_ssize_t n) {
                          *first = tensor(PyTuple_GET_ITEM(bank, 3));
         i8f_adapters &ad = l[i].adapters;
         ad.count = PyLong_AsLongLong(PyTuple_GET_ITEM(bank, 4)), ad.max_rank = PyLong_AsLongLong(PyTuple_GET_ITEM(bank, 5));
-        if (!down || !up || !scale || !first || down->scalar_type() != x.scalar_type() || down->device() != x.device() || down->dim() != 2 || down->size(1) != K ||
+        if (!down || !up || !scale || !first || down->scalar_type() != x.scalar_type() || down->device() != x.device() || down->dim() != 2 || down->size(1) != (K + 7) / 8 * 8 ||
             up->scalar_type() != x.scalar_type() || up->device() != x.device() || up->numel() != down->size(0) * o.N || scale->numel() != ad.count ||
             first->numel() != ad.count + 1)
             Py_RETURN_NONE;
@@ -576,7 +576,7 @@ PyObject *adapters(PyObject *, PyObject *const *a, Py_ssize_t n) {
     // (the memory of the first products is free when the projections start)
     int64_t ranks = 0;
     for (Py_ssize_t i = 0; i < count; ++i) ranks += l[i].adapters.max_rank;
-    const int64_t down_bytes = lib.i8f_adapters_down_workspace_bytes(M, K, ranks), more = down_bytes > work_bytes ? down_bytes : work_bytes;
+    const int64_t down_bytes = lib.i8f_adapters_down_workspace_bytes(M, K, ranks, aligned16(x) && (M <= 1 || ld % 8 == 0)), more = down_bytes > work_bytes ? down_bytes : work_bytes;
     const int64_t work_at = more ? take(more) : 0;
     const at::ScalarType type = x.scalar_type();
     const at::Device dev = x.device();

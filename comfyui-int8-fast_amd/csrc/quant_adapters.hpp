@@ -5,26 +5,6 @@
 namespace i8f {
 namespace {
 
-// ---- any width and alignment: one wave to a rank of a row --------------------------------------------------------------------
-template <int DT>
-__global__ __launch_bounds__(256) void adapters_down_kernel(const char *__restrict__ x, int64_t K, int64_t ldx, const DownLayers g) {
-    const int64_t m = blockIdx.x;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int l = 0; l < g.n; ++l) {
-        const i8f_adapters &ad = g.ad[l];
-        const int a = adapter_of(ad, m);
-        if (a < 0) continue;
-        const int first = ad.first_rank[a], r = ad.first_rank[a + 1] - first;
-        const float s = ad.scale[a];
-        for (int j = wave; j < r; j += 4) {
-            float sum = 0.0f;
-            for (int64_t k = lane; k < K; k += 64) sum = __builtin_fmaf(load_as_f32<DT>(x, m * ldx + k), load_as_f32<DT>(ad.down, (first + j) * K + k), sum);
-            sum = wave_sum_all(sum);
-            if (lane == 0) store_from_f32<DT>(g.t[l], m * ad.max_rank + j, sum * s);
-        }
-    }
-}
-
 template <int DT>
 __device__ __forceinline__ float dot8(v4u a, v4u b, float sum) {
 #pragma unroll
@@ -40,9 +20,11 @@ __device__ __forceinline__ float dot8(v4u a, v4u b, float sum) {
     return sum;
 }
 
-// ---- few rows (K % 8 == 0, aligned): every rank of every row is a wave of its own, with 16-byte loads, eight of each operand under way at
-// once; what counts is the one trip to memory.  The first quant_blocks workgroups quantise a row of x each (RUNS > 0).
-template <int DT, bool ROT, int RUNS>
+// ---- few rows: every rank of every row is a wave of its own, with 16-byte loads, eight of each operand under way at once; what counts is
+// the one trip to memory.  The first quant_blocks workgroups quantise a row of x each (RUNS > 0).
+// ANY: x of any width and alignment (a row's last eight elements, where it has fewer of them, are fetched one by one; the factors' rows
+// are padded).
+template <int DT, bool ROT, int RUNS, bool ANY>
 __global__ __launch_bounds__(256) void adapters_rows_kernel(const char *__restrict__ x, int64_t M, int K, int64_t ldx, int8_t *__restrict__ q,
                                                             float *__restrict__ scale, int quant_blocks, const DownLayers g) {
     if constexpr (RUNS > 0) {
@@ -66,15 +48,30 @@ __global__ __launch_bounds__(256) void adapters_rows_kernel(const char *__restri
     if (a < 0) return;
     const int first = ad.first_rank[a];
     if (j >= ad.first_rank[a + 1] - first) return;
-    const char *xp = x + m * ldx * 2, *ap = (const char *)ad.down + (int64_t)(first + j) * K * 2;
+    const char *xp = x + m * ldx * 2, *ap = (const char *)ad.down + (int64_t)(first + j) * factor_width(K) * 2;
     float sum = 0.0f;
     for (int k0 = lane * 8; k0 < K; k0 += 8 * 512) {
         v4u xv[8], av[8];
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
             const int k = k0 + c * 512;
-            xv[c] = k < K ? *(const v4u *)(xp + (int64_t)k * 2) : (v4u)0u;
+            if constexpr (ANY) {
+                xv[c] = (v4u)0u;
+                if (k + 8 <= K) __builtin_memcpy(&xv[c], xp + (int64_t)k * 2, 16);
+            } else {
+                xv[c] = k < K ? *(const v4u *)(xp + (int64_t)k * 2) : (v4u)0u;
+            }
             av[c] = k < K ? *(const v4u *)(ap + (int64_t)k * 2) : (v4u)0u;
+        }
+        if constexpr (ANY) {
+            const int c = (K - k0) / 512, k = k0 + c * 512;   // the piece that holds the row's end, if it is this lane's
+            if (K % 8 && c < 8 && K - k < 8) {
+                v4u end = (v4u)0u;
+                for (int e = 0; e < K - k; ++e) end[e / 2] |= (uint32_t)((const uint16_t *)xp)[k + e] << (16 * (e % 2));
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i == c) xv[i] = end;
+            }
         }
 #pragma unroll
         for (int c = 0; c < 8; ++c) sum = dot8<DT>(xv[c], av[c], sum);
@@ -88,30 +85,28 @@ __global__ __launch_bounds__(256) void adapters_rows_kernel(const char *__restri
 // layers beside it.
 constexpr int64_t DOWN_ROWS = 256, DOWN_ELEMENTS = 1 << 19;
 
-template <int DT, bool ROT, int RUNS>
+template <int DT, bool ROT, int RUNS, bool ANY = false>
 int launch_rows_form(const void *x, int64_t M, int64_t K, int64_t ldx, int8_t *q, float *scale, DownLayers &g, hipStream_t st) {
     const int64_t quant_blocks = RUNS > 0 ? M : 0;
     int64_t first = 0;
     for (int i = 0; i < g.n; ++i) g.first_block[i] = (int)first, first += M * (g.ad[i].max_rank / 4);
     for (int i = g.n; i <= I8F_MAX_ADAPTED_LAYERS; ++i) g.first_block[i] = (int)first;
     if (quant_blocks + first == 0) return I8F_OK;
-    hipLaunchKernelGGL((adapters_rows_kernel<DT, ROT, RUNS>), dim3((unsigned)(quant_blocks + first)), dim3(256), 0, st, (const char *)x, M, (int)K, ldx, q, scale,
+    hipLaunchKernelGGL((adapters_rows_kernel<DT, ROT, RUNS, ANY>), dim3((unsigned)(quant_blocks + first)), dim3(256), 0, st, (const char *)x, M, (int)K, ldx, q, scale,
                        (int)quant_blocks, g);
     return check_launch();
 }
 
-enum DownForm { DOWN_ANY, DOWN_ROW_WAVES, DOWN_PARTIAL };
-inline DownForm down_form(const void *x, int64_t M, int64_t K, int64_t ldx, int64_t ranks) {
-    if (K % 8 || (uintptr_t)x % 16 || ldx % 8 || K < 1 || ldx >= (1ll << 23)) return DOWN_ANY;   // (32-bit offsets within 64 rows)
-    return M * ranks < (1ll << 30) && (M <= DOWN_ROWS || M * K <= DOWN_ELEMENTS) ? DOWN_ROW_WAVES : DOWN_PARTIAL;
-}
+inline bool down_by_rows(int64_t M, int64_t K) { return M <= DOWN_ROWS || M * K <= DOWN_ELEMENTS; }
+inline bool down_in_place(const void *x, int64_t K, int64_t ldx) { return K % 8 == 0 && (uintptr_t)x % 16 == 0 && ldx % 8 == 0 && ldx < (1ll << 23); }   // (32-bit offsets within 64 rows)
 
 template <int DT>
 int launch_down(const void *x, int64_t M, int64_t K, int64_t ldx, DownLayers &g, int rotate_block, int8_t *q, float *scale, void *workspace,
                 int64_t workspace_bytes, hipStream_t st) {
     const int64_t ranks = g.first_column[g.n];
-    const DownForm form = down_form(x, M, K, ldx, ranks);
-    if (form == DOWN_ROW_WAVES && q && M <= DOWN_ROWS && K % 16 == 0 && K <= 16384 && (uintptr_t)q % 16 == 0) {   // the quantiser in the same launch
+    const bool in_place = down_in_place(x, K, ldx), by_rows = down_by_rows(M, K);
+    if (M * ranks >= (1ll << 30)) return I8F_ERR_UNSUPPORTED;
+    if (by_rows && in_place && q && M <= DOWN_ROWS && K % 16 == 0 && K <= 16384 && (uintptr_t)q % 16 == 0) {   // the quantiser in the same launch
         const int64_t runs = (K / 16 + 255) / 256;
         auto go = [&](auto ROT) {
             switch (runs) {
@@ -126,14 +121,18 @@ int launch_down(const void *x, int64_t M, int64_t K, int64_t ldx, DownLayers &g,
     if (q)
         if (int rc = i8f_quant_rowwise(x, DT, M, K, ldx, rotate_block, q, scale, st)) return rc;
     if (ranks == 0) return I8F_OK;
-    if (form == DOWN_ROW_WAVES) return launch_rows_form<DT, false, 0>(x, M, K, ldx, q, scale, g, st);
-    if (form == DOWN_PARTIAL) {
-        int slices = adapters_down_slices(M, K);
-        if (!workspace || workspace_bytes < slices * M * ranks * 4) slices = 1;
-        return adapters_down_partial(x, DT, M, K, ldx, g, (float *)workspace, slices, st);
+    if (by_rows)
+        return in_place ? launch_rows_form<DT, false, 0>(x, M, K, ldx, q, scale, g, st) : launch_rows_form<DT, false, 0, true>(x, M, K, ldx, q, scale, g, st);
+    // rows that the direct loads do not take are copied first, padded like the factors
+    const int64_t copy = in_place ? 0 : adapters_copy_bytes(M, K);
+    int slices = adapters_down_slices(M, K);
+    if (!workspace || workspace_bytes < copy + slices * M * ranks * 4) slices = 1;
+    if (copy) {
+        if (!workspace || workspace_bytes < copy) return launch_rows_form<DT, false, 0, true>(x, M, K, ldx, q, scale, g, st);
+        if (int rc = adapters_copy_rows(x, M, K, ldx, workspace, st)) return rc;
+        x = workspace, K = ldx = factor_width(K);
     }
-    hipLaunchKernelGGL((adapters_down_kernel<DT>), dim3((unsigned)M), dim3(256), 0, st, (const char *)x, K, ldx, g);
-    return check_launch();
+    return adapters_down_partial(x, DT, M, K, ldx, g, (float *)((char *)workspace + copy), slices, st);
 }
 
 }  // namespace
@@ -163,8 +162,9 @@ extern "C" int i8f_adapters_down(const void *x, int x_dtype, int64_t M, int64_t 
                                : launch_down<I8F_F16>(x, M, K, ldx, g, rotate_block, q, scale, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
-extern "C" int64_t i8f_adapters_down_workspace_bytes(int64_t M, int64_t K, int64_t ranks) {
-    if (M <= 0 || K <= 0 || ranks <= 0 || M > 0x7fffffff || K > 0x7fffffff) return 0;
-    const int slices = i8f::adapters_down_slices(M, K);
-    return M <= i8f::DOWN_ROWS || M * K <= i8f::DOWN_ELEMENTS || slices < 2 ? 0 : slices * M * ranks * 4;
+extern "C" int64_t i8f_adapters_down_workspace_bytes(int64_t M, int64_t K, int64_t ranks, int x_aligned) {
+    using namespace i8f;
+    if (M <= 0 || K <= 0 || ranks <= 0 || M > 0x7fffffff || K > 0x7fffffff || down_by_rows(M, K)) return 0;
+    const int slices = adapters_down_slices(M, K);
+    return (x_aligned && K % 8 == 0 ? 0 : adapters_copy_bytes(M, K)) + (slices < 2 ? 0 : slices * M * ranks * 4);
 }

@@ -19,7 +19,8 @@ extern "C" {
  * not one of 0 ... count - 1.  All pointers are device pointers; the factors have the type of the activations (bfloat16 or binary16).
  */
 typedef struct i8f_adapters {
-    const void *down;          /* [first_rank[count], K]: the adapters' A one below the other */
+    const void *down;          /* [first_rank[count], K]: the adapters' A one below the other, each row padded with zeros to a multiple of
+                                  eight elements in memory */
     const void *up;            /* adapter a: B as [N, padded r_a] from element N * first_rank[a] on */
     const float *scale;        /* [count] multiplies A x */
     const int32_t *first_rank; /* [count + 1], multiples of 16, first_rank[0] = 0 */
@@ -52,10 +53,11 @@ typedef struct i8f_adapted_layer {
  * are.  Of the layers only adapters and t are looked at.  x_dtype I8F_BF16 or I8F_F16, n_layers up to I8F_MAX_ADAPTED_LAYERS.
  * q, scale: NULL, or the int8 rows of x and their scales besides, as i8f_quant_rowwise with rotate_block leaves them (the adapters take
  * x as it is).
- * workspace: any contents; i8f_adapters_down_workspace_bytes(M, K, the sum of the layers' max_rank) bytes let many rows' columns be dealt over
- * more workgroups; less, or NULL, is slower there and rounds otherwise in the last place of the binary32 sums.
+ * workspace: any contents; i8f_adapters_down_workspace_bytes(M, K, the sum of the layers' max_rank, x_aligned) bytes let many rows' columns
+ * be dealt over more workgroups, and rows that are not 16-byte aligned (x_aligned 0: x, or ldx in elements, is no multiple of 16 bytes) be
+ * copied; less, or NULL, is slower there and rounds otherwise in the last place of the binary32 sums.
  */
-int64_t i8f_adapters_down_workspace_bytes(int64_t M, int64_t K, int64_t ranks);
+int64_t i8f_adapters_down_workspace_bytes(int64_t M, int64_t K, int64_t ranks, int x_aligned);
 int i8f_adapters_down(const void *x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const i8f_adapted_layer *layers, int n_layers,
                       int rotate_block, int8_t *q, float *scale, void *workspace, int64_t workspace_bytes, void *stream);
 

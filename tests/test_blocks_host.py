@@ -55,8 +55,9 @@ def test_adapters_arguments_are_checked_before_any_launch(L):
     assert down({}, q=one) == INVALID and down({}, s=one) == INVALID and down({}, rb=64) == UNSUPPORTED and down({}, rb=128) == INVALID
     assert down({}, work=ctypes.c_void_p(8)) == INVALID
     size = lib.i8f_adapters_down_workspace_bytes
-    assert size(16, 4096, 32) == size(0, 64, 16) == size(4096, 0, 16) == size(4096, 64, 0) == size(1 << 31, 64, 16) == 0
-    assert size(4096, 4096, 32) % (4096 * 32 * 4) == 0 and size(4096, 4096, 32) > 0
+    assert size(16, 4096, 32, 1) == size(0, 64, 16, 1) == size(4096, 0, 16, 1) == size(4096, 64, 0, 1) == size(1 << 31, 64, 16, 1) == 0
+    assert size(4096, 4096, 32, 1) % (4096 * 32 * 4) == 0 and size(4096, 4096, 32, 1) > 0
+    assert size(4096, 4096, 32, 0) == size(4096, 4096, 32, 1) + 4096 * 4096 * 2 and size(4096, 4089, 32, 1) == size(4096, 4089, 32, 0)
     assert down({}, M=1 << 31) == UNSUPPORTED
     assert down({"ids": None, "t": None}, M=0) == 0
 
@@ -127,8 +128,8 @@ def test_a_bank_keeps_its_factors_padded_to_sixteen_ranks(pkg):
             assert r == 0
             continue
         n = f[0].shape[0]
-        assert torch.equal(down[:n], f[0].bfloat16()) and torch.equal(up[:, :n], f[1].bfloat16())
-        assert not down[n:].any() and not up[:, n:].any()
+        assert torch.equal(down[:n, :10], f[0].bfloat16()) and torch.equal(up[:, :n], f[1].bfloat16())
+        assert down.shape[1] == 16 and not down[:, 10:].any() and not down[n:].any() and not up[:, n:].any()
 
 
 def test_banks_refuse_what_is_no_adapter(pkg):

@@ -100,6 +100,10 @@ CASES = [
     (1100, 512, 2304, (32, 16), torch.bfloat16, {}),
     (4200, 256, 3840, (32, 160, 16), torch.float16, {}),             # several rounds of large tiles
     (2100, 384, 4608, (20, 64), torch.bfloat16, {"bias": False}),
+    (700, 1003, 96, (9, 33, 16), torch.bfloat16, {}),                # odd rows: copied for the first product
+    (900, 700, 1001, (130,), torch.float16, {"bias": False}),        # K % 8 of them
+    (1500, 2048, 264, (40, 16, 256), torch.bfloat16, {"rotate": True}),
+    (8300, 264, 512, (16, 100), torch.float16, {}),
 ]
 
 
@@ -181,7 +185,7 @@ def test_strides_and_offsets(pkg, dev):
     lin = layer_of(pkg, K, N, torch.float16)
     adapters = factors_of(K, N, (16, 20), torch.float16)
     bank = pkg.AdapterBank(adapters)
-    for rows in (6, 90):
+    for rows in (6, 90, 1200):
         ids = torch.arange(rows, device=dev, dtype=torch.int32) % 3 - 1
         wide = torch.randn(rows, K + 24, device=dev).half()
         flat = torch.randn(rows * K + 1, device=dev).half()
