@@ -52,6 +52,7 @@ def hipcc() -> str:
 
 # gemm_i8_tiles.hip is compiled once per tile configuration and output type (names of csrc/gemm_i8_impl.hpp)
 GEMM_CFGS = ("CfgBig", "CfgB192", "CfgTall", "CfgWide", "CfgMid", "CfgW96", "CfgMidDeep", "CfgM96Deep", "CfgS64Deep", "CfgT64Deep")
+GEMM_ADAPTED = ("CfgMidAd", "CfgM96Ad", "CfgS64Ad", "CfgT64Ad")   # for layers with adapters only, in place of the last four
 GEMM_GROUPED = ("CfgBig", "CfgB192", "CfgTall", "CfgWide")
 GEMM_OUTS = ("OUT_BF16", "OUT_F16", "OUT_F32", "OUT_I32")
 
@@ -60,11 +61,15 @@ def units() -> list[tuple[str, str, list[str]]]:
     """(source, name of the object file, extra flags) of every compilation, the longest first."""
     tiles, norms = os.path.join(CSRC, "gemm_i8_tiles.hip"), os.path.join(CSRC, "block_norm.hip")
     out = [(norms, "block_norm.o", [])]
-    for cfg in GEMM_CFGS:
+    for cfg in (*GEMM_CFGS, *GEMM_ADAPTED):
         for o in GEMM_OUTS:
+            only = cfg in GEMM_ADAPTED
             grouped = int(cfg in GEMM_GROUPED and o != "OUT_I32")
-            adapted = int(o in ("OUT_BF16", "OUT_F16"))
-            out.append((tiles, f"gemm_i8_tiles_{cfg}_{o}.o", [f"-DI8F_TU_CFG={cfg}", f"-DI8F_TU_OUT={o}", f"-DI8F_TU_GROUPED={grouped}", f"-DI8F_TU_ADAPTED={adapted}"]))
+            adapted = int(o in ("OUT_BF16", "OUT_F16") and not cfg.endswith("Deep"))
+            if only and not adapted:
+                continue
+            out.append((tiles, f"gemm_i8_tiles_{cfg}_{o}.o", [f"-DI8F_TU_CFG={cfg}", f"-DI8F_TU_OUT={o}", f"-DI8F_TU_GROUPED={grouped}",
+                                                             f"-DI8F_TU_ADAPTED={adapted}", f"-DI8F_TU_ADAPTED_ONLY={int(only)}"]))
     for src in sorted(glob.glob(os.path.join(CSRC, "*.hip"))):
         if src not in (tiles, norms):
             out.append((src, os.path.basename(src)[:-4] + ".o", []))

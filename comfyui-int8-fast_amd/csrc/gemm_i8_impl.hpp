@@ -294,8 +294,9 @@ struct AdapterArgs {
 // main product (rows n from B_a, columns m from t): no second set of accumulators and one rounding at the end.
 // Where all rows of a wave have one adapter, as in a batch of long requests, one block of CB columns follows the other; up to 128 ranks (32
 // with twelve waves, which have fewer registers) the rows' t are fetched once.
-// A wave with several adapters goes by groups of 16 (32) rows: a product for every adapter that occurs in the group and STEP of its ranks,
-// over all the wave's columns, and the rows of other adapters keep what they had (a select per lane: a lane's values belong to one row, and
+// Two adapters in a wave, or one and rows without, as where a request ends, go the same way with both factors' blocks.
+// A wave with more of them goes by groups of 16 (32) rows: a product for every run of rows with one adapter and STEP of its ranks,
+// over all the wave's columns, and the other rows keep what they had (a select per lane: a lane's values belong to one row, and
 // a column of the product depends on its own row of t alone; zeros in t instead would let an adapter that is not finite into every
 // row).  What counts there is the trip to memory for each adapter's factor, so the loads run RING products ahead.
 template <class C, int OUT, class ACC, class ACC16>
@@ -336,9 +337,23 @@ __device__ __forceinline__ void adapters_epilogue(const AdapterArgs &g, const in
             const int l = __builtin_ctzll(with[i]);
             a0 = __builtin_amdgcn_readlane(id[i], l), first0 = __builtin_amdgcn_readlane(first[i], l), rank0 = __builtin_amdgcn_readlane(rank[i], l);
         }
-    bool one = true;   // of all rows, or none
+    // all rows have the first one (or none has any); two adapters, of up to MOST ranks, and rows without
+    constexpr int MOST = C::NT <= 512 ? 128 : 32, PART = C::NT <= 512 ? 64 : 32;
+    bool one = true, two = true;
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i) one = one && __builtin_amdgcn_ballot_w64(id[i] == a0 || mw + i * GR + lrow >= gM) == ~0ull;
+    int a1 = -1, first1 = 0, rank1 = 0;
+#pragma unroll
+    for (int i = GROUPS - 1; i >= 0; --i) {
+        const uint64_t others = __builtin_amdgcn_ballot_w64(id[i] >= 0 && id[i] != a0);
+        if (others) {
+            const int l = __builtin_ctzll(others);
+            a1 = __builtin_amdgcn_readlane(id[i], l), first1 = __builtin_amdgcn_readlane(first[i], l), rank1 = __builtin_amdgcn_readlane(rank[i], l);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) two = two && __builtin_amdgcn_ballot_w64(id[i] >= 0 && id[i] != a0 && id[i] != a1) == 0;
+    two = two && rank0 <= MOST && rank1 <= MOST;
 
     // a block's projection in the operation order of I8F_EPI_FUSED
     auto project = [&](int i, int j, block_t &f) __attribute__((always_inline)) {
@@ -370,45 +385,97 @@ __device__ __forceinline__ void adapters_epilogue(const AdapterArgs &g, const in
             else *(uint2 *)dst = make_uint2(f32x2_to_f16x2_bits(v[0], v[1]), f32x2_to_f16x2_bits(v[2], v[3]));
         }
     };
-    if (!one) {
-        constexpr int RING = C::STAGES == 4 ? 8 : C::NT > 512 ? 1 : C::STAGES == 3 ? 4 : 2;
+    // (columns past the output load zeros; the lane's eight ranks from k0 on, past the adapter's last one, which may be half a step of 32, too)
+    auto factor_of = [&](int f, int r) { return buffer_at(g.up, ((int64_t)gN * f + (int64_t)nw * r) * 2, (int64_t)min(gN - nw, C::WTN) * r * 2); };
+    auto rank_at = [&](int k0, int r) { return k0 + lk < r ? (uint32_t)(k0 + lk) * 2u : 0x80000000u; };
+    auto load_t = [&](int i, uint32_t kb) { return __builtin_bit_cast(v4i, buffer_load16(tr, (uint32_t)((i * GR + lrow) * g.max_rank * 2) + kb)); };
+    auto load_b = [&](__amdgpu_buffer_rsrc_t f, int r, int j, uint32_t kb) {
+        return __builtin_bit_cast(v4i, buffer_load16(f, (uint32_t)((j * CB + lrow) * r * 2) + kb));
+    };
+    if (!one && two) {   // up to KS products of STEP ranks for each of the two
+        const auto up0 = factor_of(first0, rank0), up1 = factor_of(first1, rank1);
+        auto paired = [&](auto STEPS) __attribute__((always_inline)) {
+            constexpr int KS = decltype(STEPS)::value;
+            v4i tf[KS][GROUPS];
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int i = 0; i < GROUPS; ++i) tf[s][i] = load_t(i, rank_at(s * STEP, rank[i]));
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                v4i b0[KS], b1[KS];
+#pragma unroll
+                for (int s = 0; s < KS; ++s) b0[s] = load_b(up0, rank0, j, rank_at(s * STEP, rank0));
+#pragma unroll
+                for (int s = 0; s < KS; ++s) b1[s] = load_b(up1, rank1, j, rank_at(s * STEP, rank1));
+#pragma unroll
+                for (int i = 0; i < GROUPS; ++i) {
+                    block_t f, sum;
+                    project(i, j, f);
+                    sum = f;
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) sum = mma(b0[s], tf[s][i], sum);
+#pragma unroll
+                    for (int e = 0; e < 4 * QPG; ++e) sum[e] = id[i] == a0 ? sum[e] : f[e];
+                    f = sum;
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) sum = mma(b1[s], tf[s][i], sum);
+#pragma unroll
+                    for (int e = 0; e < 4 * QPG; ++e) sum[e] = id[i] == a1 && a1 >= 0 ? sum[e] : f[e];
+                    stage(i, j, sum);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        const int most = max(rank0, rank1);
+        if (most <= 32) paired(std::integral_constant<int, 32 / STEP>{});
+        else if (MOST > 32 && most <= 64) paired(std::integral_constant<int, (MOST > 32 ? 64 : 32) / STEP>{});
+        else paired(std::integral_constant<int, MOST / STEP>{});
+    } else if (!one) {
+        constexpr int RING = C::STAGES == 4 ? 8 : C::STAGES == 3 ? 4 : 1;   // (two stages: the accumulators leave no registers)
+        const int nc = min(nw, gN - 1);   // (columns past the output repeat its last one and are not stored)
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) {
-            block_t f[NJ];
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) project(i, j, f[j]);
-            // the products one after the other: an adapter of the group that is left and STEP of its ranks; -1 when there is none
-            uint64_t left = with[i];
-            int a = -1, a_first = 0, a_rank = 0, k0 = 0;
-            auto next = [&]() __attribute__((always_inline)) {
-                k0 += STEP;
-                while (k0 >= a_rank && a != -2) {
-                    if (!left) a = -2;   // (that no row has)
-                    else {
-                        const int l = __builtin_ctzll(left);
-                        a = __builtin_amdgcn_readlane(id[i], l), a_first = __builtin_amdgcn_readlane(first[i], l), a_rank = __builtin_amdgcn_readlane(rank[i], l);
-                        left &= ~__builtin_amdgcn_ballot_w64(id[i] == a);
-                        k0 = 0;
-                    }
-                }
-            };
+            // runs of rows with one adapter, numbered from 1 (0: a row without); the first row of each, in the first GR lanes, leads it
+            const int before = __shfl(id[i], max(lrow - 1, 0));
+            const bool leads = lane < GR && rank[i] > 0 && (lrow == 0 || before != id[i]);
+            const uint32_t leaders = (uint32_t)__builtin_amdgcn_ballot_w64(leads);
+            const int run = rank[i] > 0 ? __builtin_popcount(leaders & ((2u << lrow) - 1u)) : 0;
+            const uint64_t factor = (uint64_t)g.up + ((uint64_t)gN * (uint32_t)first[i] + (uint64_t)nc * (uint32_t)rank[i]) * 2u;
+            const uint32_t t_at = (uint32_t)((i * GR + lrow) * g.max_rank) * 2u;
+            // the products one after the other: STEP ranks of every run that has them, then the next STEP
+            uint32_t left = leaders;
+            int k0 = 0;
             v4i tf[RING], bf[RING][NJ];
-            int whose[RING];
-            auto fetch = [&](int s) __attribute__((always_inline)) {   // (past the last product everything is out of range and loads zeros)
-                next();
-                whose[s] = a;
-                const auto up = buffer_at(g.up, ((int64_t)gN * a_first + (int64_t)nw * a_rank) * 2, a < 0 ? 0 : (int64_t)min(gN - nw, C::WTN) * a_rank * 2);
-                const uint32_t kb = a >= 0 && k0 + lk < a_rank ? (uint32_t)(k0 + lk) * 2u : 0x80000000u;
-                tf[s] = __builtin_bit_cast(v4i, buffer_load16(tr, (uint32_t)((i * GR + lrow) * g.max_rank * 2) + kb));
+            int whose[RING], ends[RING];   // the run, and the adapter's ranks from k0 on
+            auto fetch = [&](int s) __attribute__((always_inline)) {   // (past the last product: run -1, and the factors' first bytes)
+                if (!left) k0 += STEP, left = (uint32_t)__builtin_amdgcn_ballot_w64(leads && rank[i] > k0);
+                const bool some = left != 0;
+                const int l = some ? __builtin_ctz(left) : 0;
+                const int r = some ? __builtin_amdgcn_readlane(rank[i], l) : 0;
+                const uint64_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)factor, l), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(factor >> 32), l);
+                const char *up = some ? (const char *)(hi << 32 | lo) : (const char *)g.up;
+                whose[s] = some ? __builtin_amdgcn_readlane(run, l) : -1;
+                ends[s] = r - k0;
+                left &= left - 1;
+                tf[s] = __builtin_bit_cast(v4i, buffer_load16(tr, k0 + lk < rank[i] ? t_at + (uint32_t)(k0 + lk) * 2u : 0x80000000u));
+                const uint32_t kb = (uint32_t)max(min(k0 + lk, r - 8), 0) * 2u;
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) bf[s][j] = __builtin_bit_cast(v4i, buffer_load16(up, (uint32_t)((j * CB + lrow) * a_rank * 2) + kb));
+                for (int j = 0; j < NJ; ++j) bf[s][j] = *(const v4i *)(up + ((uint32_t)min(j * CB + lrow, gN - 1 - nc) * (uint32_t)(r * 2) + kb));
             };
 #pragma unroll
             for (int s = 0; s < RING; ++s) fetch(s);
+            block_t f[NJ];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) project(i, j, f[j]);
             while (whose[0] >= 0) {
 #pragma unroll
                 for (int s = 0; s < RING; ++s) {
-                    const bool mine = id[i] == whose[s];
+                    const bool mine = run == whose[s];
+                    if (M16 && ends[s] < STEP) {   // (ranks come in sixteens: half a step of 32)
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j) bf[s][j] = lk < ends[s] ? bf[s][j] : (v4i)0;
+                    }
 #pragma unroll
                     for (int j = 0; j < NJ; ++j) {
                         const block_t sum = mma(bf[s][j], tf[s], f[j]);
@@ -424,23 +491,19 @@ __device__ __forceinline__ void adapters_epilogue(const AdapterArgs &g, const in
             __builtin_amdgcn_sched_barrier(0);
         }
     } else {
-    const auto up = buffer_at(g.up, ((int64_t)gN * first0 + (int64_t)nw * rank0) * 2, (int64_t)min(gN - nw, C::WTN) * rank0 * 2);
-    // (the lane's eight ranks from k0 on; past the adapter's last one, which may be half a step of 32, an offset that loads zeros)
-    auto rank_at = [&](int k0) { return k0 + lk < rank0 ? (uint32_t)(k0 + lk) * 2u : 0x80000000u; };
-    auto load_t = [&](int i, uint32_t kb) { return __builtin_bit_cast(v4i, buffer_load16(tr, (uint32_t)((i * GR + lrow) * g.max_rank * 2) + kb)); };
-    auto load_b = [&](int j, uint32_t kb) { return __builtin_bit_cast(v4i, buffer_load16(up, (uint32_t)((j * CB + lrow) * rank0 * 2) + kb)); };
+    const auto up = factor_of(first0, rank0);
     // up to STEPS products of STEP ranks with the rows' t in registers
     auto resident = [&](auto STEPS) __attribute__((always_inline)) {
         constexpr int KS = decltype(STEPS)::value, AHEAD = KS && C::NT <= 512 ? 1 : 0;   // (twelve waves have no registers for the next block's factors)
         v4i tf[KS ? KS : 1][GROUPS], bf[AHEAD + 1][KS ? KS : 1];
         auto fetch = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
-            for (int s = 0; s < KS; ++s) bf[j & AHEAD][s] = load_b(j, rank_at(s * STEP));
+            for (int s = 0; s < KS; ++s) bf[j & AHEAD][s] = load_b(up, rank0, j, rank_at(s * STEP, rank0));
         };
 #pragma unroll
         for (int s = 0; s < KS; ++s)
 #pragma unroll
-            for (int i = 0; i < GROUPS; ++i) tf[s][i] = load_t(i, rank_at(s * STEP));
+            for (int i = 0; i < GROUPS; ++i) tf[s][i] = load_t(i, rank_at(s * STEP, rank0));
         if (AHEAD) fetch(0);
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
@@ -457,7 +520,6 @@ __device__ __forceinline__ void adapters_epilogue(const AdapterArgs &g, const in
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    constexpr int MOST = C::NT <= 512 ? 128 : 32, PART = C::NT <= 512 ? 64 : 32;
     if (rank0 == 0) resident(std::integral_constant<int, 0>{});
     else if (rank0 <= 32) resident(std::integral_constant<int, 32 / STEP>{});
     else if (MOST > 32 && rank0 <= 64) resident(std::integral_constant<int, (MOST > 32 ? 64 / STEP : 0)>{});
@@ -473,9 +535,9 @@ __device__ __forceinline__ void adapters_epilogue(const AdapterArgs &g, const in
                 v4i tf[KS][GROUPS], bf[KS];
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
-                    bf[s] = load_b(j, rank_at(k0 + s * STEP));
+                    bf[s] = load_b(up, rank0, j, rank_at(k0 + s * STEP, rank0));
 #pragma unroll
-                    for (int i = 0; i < GROUPS; ++i) tf[s][i] = load_t(i, rank_at(k0 + s * STEP));
+                    for (int i = 0; i < GROUPS; ++i) tf[s][i] = load_t(i, rank_at(k0 + s * STEP, rank0));
                 }
 #pragma unroll
                 for (int s = 0; s < KS; ++s)
@@ -1436,6 +1498,12 @@ using CfgMidDeep = Cfg<128, 128, 128, 2, 2, 4, 8>;
 using CfgM96Deep = Cfg<128, 96, 128, 4, 1, 4, 8>;
 using CfgS64Deep = Cfg<128, 64, 128, 2, 2, 4, 8>;
 using CfgT64Deep = Cfg<64, 64, 128, 2, 2, 4, 8>;
+// The few-tile configurations of layers with adapters: the 16x16x64 form, in whose epilogue a request of one token costs a product of 16 rows
+// instead of 32 and a quarter of the selections.
+using CfgMidAd = Cfg<128, 128, 128, 2, 2, 4, 8, 0, 16>;
+using CfgM96Ad = Cfg<128, 96, 128, 4, 1, 4, 8, 0, 16>;
+using CfgS64Ad = Cfg<128, 64, 128, 2, 2, 4, 8, 0, 16>;
+using CfgT64Ad = Cfg<64, 64, 128, 2, 2, 4, 8, 0, 16>;
 template <class C, int OUT>
 int launch_cfg(GemmArgs &g, hipStream_t st) {
     g.tiles_m = (g.M + C::BM - 1) / C::BM;
@@ -1498,10 +1566,14 @@ int launch_cfg_adapted(AdaptedLayers &l, const int8_t *x, const float *xs, int M
     extern template int launch_cfg<C, OUT_BF16>(GemmArgs &, hipStream_t);                                        \
     extern template int launch_cfg<C, OUT_F16>(GemmArgs &, hipStream_t);                                         \
     extern template int launch_cfg<C, OUT_F32>(GemmArgs &, hipStream_t);                                         \
-    extern template int launch_cfg<C, OUT_I32>(GemmArgs &, hipStream_t);                                         \
+    extern template int launch_cfg<C, OUT_I32>(GemmArgs &, hipStream_t);
+I8F_GEMM_CFGS(I8F_EXTERN_CFG)
+#undef I8F_EXTERN_CFG
+#define I8F_EXTERN_CFG(C)                                                                                                       \
     extern template int launch_cfg_adapted<C, OUT_BF16>(AdaptedLayers &, const int8_t *, const float *, int, int, hipStream_t); \
     extern template int launch_cfg_adapted<C, OUT_F16>(AdaptedLayers &, const int8_t *, const float *, int, int, hipStream_t);
-I8F_GEMM_CFGS(I8F_EXTERN_CFG)
+I8F_EXTERN_CFG(CfgBig) I8F_EXTERN_CFG(CfgB192) I8F_EXTERN_CFG(CfgMid) I8F_EXTERN_CFG(CfgTall) I8F_EXTERN_CFG(CfgWide) I8F_EXTERN_CFG(CfgW96)
+I8F_EXTERN_CFG(CfgMidAd) I8F_EXTERN_CFG(CfgM96Ad) I8F_EXTERN_CFG(CfgS64Ad) I8F_EXTERN_CFG(CfgT64Ad)
 #undef I8F_EXTERN_CFG
 
 enum Tile { TILE_BIG, TILE_B192, TILE_MID, TILE_TALL, TILE_WIDE, TILE_W96, TILE_MID_DEEP, TILE_M96_DEEP, TILE_S64_DEEP, TILE_T64_DEEP };
@@ -1633,10 +1705,10 @@ int launch_adapted(AdaptedLayers &l, const int8_t *x, const float *xs, int M, in
     case TILE_TALL: return launch_cfg_adapted<CfgTall, OUT>(l, x, xs, M, K, st);
     case TILE_WIDE: return launch_cfg_adapted<CfgWide, OUT>(l, x, xs, M, K, st);
     case TILE_W96: return launch_cfg_adapted<CfgW96, OUT>(l, x, xs, M, K, st);
-    case TILE_MID_DEEP: return launch_cfg_adapted<CfgMidDeep, OUT>(l, x, xs, M, K, st);
-    case TILE_M96_DEEP: return launch_cfg_adapted<CfgM96Deep, OUT>(l, x, xs, M, K, st);
-    case TILE_S64_DEEP: return launch_cfg_adapted<CfgS64Deep, OUT>(l, x, xs, M, K, st);
-    default: return launch_cfg_adapted<CfgT64Deep, OUT>(l, x, xs, M, K, st);
+    case TILE_MID_DEEP: return launch_cfg_adapted<CfgMidAd, OUT>(l, x, xs, M, K, st);
+    case TILE_M96_DEEP: return launch_cfg_adapted<CfgM96Ad, OUT>(l, x, xs, M, K, st);
+    case TILE_S64_DEEP: return launch_cfg_adapted<CfgS64Ad, OUT>(l, x, xs, M, K, st);
+    default: return launch_cfg_adapted<CfgT64Ad, OUT>(l, x, xs, M, K, st);
     }
 }
 

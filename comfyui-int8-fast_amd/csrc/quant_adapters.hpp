@@ -105,7 +105,7 @@ int launch_down(const void *x, int64_t M, int64_t K, int64_t ldx, DownLayers &g,
                 int64_t workspace_bytes, hipStream_t st) {
     const int64_t ranks = g.first_column[g.n];
     const bool in_place = down_in_place(x, K, ldx), by_rows = down_by_rows(M, K);
-    if (M * ranks >= (1ll << 30)) return I8F_ERR_UNSUPPORTED;
+    if (by_rows && M * ranks >= (1ll << 30)) return I8F_ERR_UNSUPPORTED;
     if (by_rows && in_place && q && M <= DOWN_ROWS && K % 16 == 0 && K <= 16384 && (uintptr_t)q % 16 == 0) {   // the quantiser in the same launch
         const int64_t runs = (K / 16 + 255) / 256;
         auto go = [&](auto ROT) {
