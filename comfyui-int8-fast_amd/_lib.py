@@ -92,6 +92,7 @@ def lib() -> ctypes.CDLL:
     L.i8f_linear_w8a8_adapters_workspace_bytes.restype = i64
     L.i8f_linear_w8a8_adapters.argtypes = [vp, vp, vp, i32, i32, i64, i64, vp, i64, vp]
     L.i8f_linear_w8a16_small_m_adapters.argtypes = [vp, i32, i64, i64, i64, vp, i32, vp]
+    L.i8f_adapters_by_side.argtypes = [i64, i64, i64, i64]
     L.i8f_block_norm.argtypes = [vp, vp]
     for name in BLOCK_EXPORTS:
         if not name.endswith("_bytes"):
@@ -132,7 +133,7 @@ EXPORTS = (
 
 
 # the entry points of include/i8f_blocks.h
-BLOCK_EXPORTS = ("i8f_adapters_down_workspace_bytes", "i8f_adapters_down", "i8f_adapters_up", "i8f_linear_w8a8_adapters_workspace_bytes", "i8f_linear_w8a8_adapters",
+BLOCK_EXPORTS = ("i8f_adapters_by_side", "i8f_adapters_down_workspace_bytes", "i8f_adapters_down", "i8f_adapters_up", "i8f_linear_w8a8_adapters_workspace_bytes", "i8f_linear_w8a8_adapters",
                  "i8f_linear_w8a16_small_m_adapters", "i8f_block_norm")
 
 ERR_UNSUPPORTED = -2   # I8F_ERR_UNSUPPORTED
@@ -885,7 +886,7 @@ class _Adapters(ctypes.Structure):
 
 class _AdaptedLayer(ctypes.Structure):
     _fields_ = [("w", ctypes.c_void_p), ("w_scale", ctypes.c_void_p), ("w_scale_host", ctypes.c_float), ("scale_mode", ctypes.c_int), ("bias", ctypes.c_void_p),
-                ("bias_dtype", ctypes.c_int), ("N", ctypes.c_int64), ("adapters", _Adapters), ("t", ctypes.c_void_p), ("out", ctypes.c_void_p)]
+                ("bias_dtype", ctypes.c_int), ("N", ctypes.c_int64), ("adapters", _Adapters), ("t", ctypes.c_void_p), ("side", ctypes.c_void_p), ("out", ctypes.c_void_p)]
 
 
 MAX_ADAPTED_LAYERS = 4

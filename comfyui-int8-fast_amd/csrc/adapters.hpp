@@ -40,6 +40,8 @@ __device__ __forceinline__ float adapter_term(const i8f_adapters &ad, const void
 struct DownLayers {
     i8f_adapters ad[I8F_MAX_ADAPTED_LAYERS];
     char *t[I8F_MAX_ADAPTED_LAYERS];
+    float *side[I8F_MAX_ADAPTED_LAYERS];
+    int64_t N[I8F_MAX_ADAPTED_LAYERS];
     int first_block[I8F_MAX_ADAPTED_LAYERS + 1];   // (rows form: first workgroup of each layer behind the quantiser's; [n] = all)
     int first_column[I8F_MAX_ADAPTED_LAYERS + 1];  // (partial sums: first column of each layer, max_rank of them; [n] = all)
     int n;
@@ -74,6 +76,7 @@ inline int validate_layers(const i8f_adapted_layer *layers, int n, int dtype, in
         if (l.N < 0 || (l.bias && !valid_dtype(l.bias_dtype)) || (l.scale_mode != I8F_SCALE_TENSOR && l.scale_mode != I8F_SCALE_ROW)) return I8F_ERR_INVALID;
         if (l.adapters.ids != layers[0].adapters.ids || l.adapters.rows_per_id != layers[0].adapters.rows_per_id) return I8F_ERR_INVALID;
         if (M > 0 && l.adapters.max_rank > 0 && l.adapters.count > 0 && (!l.t || (uintptr_t)l.t % 16)) return I8F_ERR_INVALID;
+        if ((l.side != nullptr) != (layers[0].side != nullptr) || (uintptr_t)l.side % 16) return I8F_ERR_INVALID;
     }
     return I8F_OK;
 }

@@ -124,6 +124,7 @@ extern "C" int i8f_linear_w8a8_adapters(const int8_t *a, const float *a_scale, c
         if (M == 0 || y.N == 0) continue;
         if (!a_scale || (y.scale_mode == I8F_SCALE_ROW && !y.w_scale)) return I8F_ERR_INVALID;
         if (!adapters_fused(M, y.N, K)) {
+            if (y.side) return I8F_ERR_UNSUPPORTED;
             if (!workspace || workspace_bytes < M * y.N * 4) return I8F_ERR_INVALID;
         } else {   // 16-byte pieces of the operands, which any torch allocation has
             aligned = aligned && ((uintptr_t)y.w | (uintptr_t)y.out | (uintptr_t)y.bias) % 16 == 0 && (y.scale_mode != I8F_SCALE_ROW || (uintptr_t)y.w_scale % 16 == 0);
@@ -147,7 +148,7 @@ extern "C" int i8f_linear_w8a8_adapters(const int8_t *a, const float *a_scale, c
         const int k = l.n++;
         l.w[k] = y.w, l.ws[k] = y.w_scale, l.ws_host[k] = y.w_scale_host, l.bias[k] = y.bias, l.out[k] = y.out, l.N[k] = (int)y.N;
         l.flags[k] = (y.scale_mode == I8F_SCALE_ROW ? 1 : 0) | (y.bias_dtype << 1);
-        l.adapters[k] = {ad.ids, ad.first_rank, y.t, ad.up, (int)ad.rows_per_id, ad.max_rank > 0 ? (int)ad.count : 0, (int)ad.max_rank};
+        l.adapters[k] = {ad.ids, ad.first_rank, y.t, ad.up, y.side, (int)ad.rows_per_id, ad.max_rank > 0 ? (int)ad.count : 0, (int)ad.max_rank};
     }
     if (l.n == 0) return I8F_OK;
     return out_dtype == I8F_BF16 ? launch_adapted<OUT_BF16>(l, a, a_scale, (int)M, (int)K, st) : launch_adapted<OUT_F16>(l, a, a_scale, (int)M, (int)K, st);

@@ -286,6 +286,7 @@ __device__ __forceinline__ v4f side_mfma32(v4i a, v4i b, v4f c) {
 struct AdapterArgs {
     const int *ids, *first_rank;
     const void *t, *up;
+    const float *side;   // nullptr, or [M,N]: the adapters' whole share
     int rows_per_id, count, max_rank;
 };
 
@@ -315,6 +316,65 @@ __device__ __forceinline__ void adapters_epilogue(const AdapterArgs &g, const in
         if constexpr (M16) return side_mfma32<OUT>(b, t, c);
         else return side_mfma<OUT>(b, t, c);
     };
+    // a block's projection in the operation order of I8F_EPI_FUSED
+    auto project = [&](int i, int j, block_t &f) __attribute__((always_inline)) {
+        const float xs = s_xs[wm * C::WTM + i * GR + lrow];
+#pragma unroll
+        for (int qd = 0; qd < QPG; ++qd) {
+            const int nl = wn * C::WTN + j * CB + (M16 ? lq * 4 : qd * 8 + lhalf * 4);
+            const float4 w4 = *(const float4 *)&s_ws[nl], b4 = *(const float4 *)&s_bias[nl];
+            int a4[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (M16) a4[e] = acc16[i >> 1][j][i & 1][e];
+                else a4[e] = acc[i][j][4 * qd + e];
+            }
+            f[4 * qd] = (float)a4[0] * (xs * w4.x) + b4.x, f[4 * qd + 1] = (float)a4[1] * (xs * w4.y) + b4.y;
+            f[4 * qd + 2] = (float)a4[2] * (xs * w4.z) + b4.z, f[4 * qd + 3] = (float)a4[3] * (xs * w4.w) + b4.w;
+        }
+    };
+    constexpr int ROW_BYTES = C::WTN * 2, PITCH = ROW_BYTES + 8, CPO = ROW_BYTES / 16;
+    auto stage = [&](int i, int j, const block_t &f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int qd = 0; qd < QPG; ++qd) {
+            const float v[4] = {f[4 * qd], f[4 * qd + 1], f[4 * qd + 2], f[4 * qd + 3]};
+            char *dst = ebuf + (i * GR + lrow) * PITCH + (j * CB + (M16 ? lq * 4 : qd * 8 + lhalf * 4)) * 2;
+            if constexpr (OUT == OUT_BF16) *(uint2 *)dst = make_uint2(f32x2_to_bf16x2_bits(v[0], v[1]), f32x2_to_bf16x2_bits(v[2], v[3]));
+            else *(uint2 *)dst = make_uint2(f32x2_to_f16x2_bits(v[0], v[1]), f32x2_to_f16x2_bits(v[2], v[3]));
+        }
+    };
+    auto store = [&]() __attribute__((always_inline)) {   // rows from LDS, 16 bytes to a lane
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int p = 0; p < C::WTM * CPO / 64; ++p) {
+            const int at = p * 64 + lane, row = at / CPO, cc = at % CPO;
+            const int mm = mw + row, nn = nw + cc * 8;
+            if (mm < gM && nn < gN) stream_store16((char *)gout + ((int64_t)mm * gN + nn) * 2, *(const uint4 *)(ebuf + row * PITCH + cc * 16));
+        }
+    };
+    if (g.side) {   // (rows and columns past the output repeat the last ones and are not stored)
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            const float *side = g.side + (int64_t)min(mw + i * GR + lrow, gM - 1) * gN;
+            float4 add[NJ][QPG];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int qd = 0; qd < QPG; ++qd) add[j][qd] = *(const float4 *)(side + min(nw + j * CB + (M16 ? lq * 4 : qd * 8 + lhalf * 4), gN - 4));
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                block_t f;
+                project(i, j, f);
+#pragma unroll
+                for (int qd = 0; qd < QPG; ++qd)
+                    f[4 * qd] += add[j][qd].x, f[4 * qd + 1] += add[j][qd].y, f[4 * qd + 2] += add[j][qd].z, f[4 * qd + 3] += add[j][qd].w;
+                stage(i, j, f);
+            }
+        }
+        store();
+        return;
+    }
     // the adapter of the lane's row in each group, and its ranks
     int id[GROUPS], first[GROUPS], rank[GROUPS];
     uint64_t with[GROUPS];
@@ -355,36 +415,8 @@ __device__ __forceinline__ void adapters_epilogue(const AdapterArgs &g, const in
     for (int i = 0; i < GROUPS; ++i) two = two && __builtin_amdgcn_ballot_w64(id[i] >= 0 && id[i] != a0 && id[i] != a1) == 0;
     two = two && rank0 <= MOST && rank1 <= MOST;
 
-    // a block's projection in the operation order of I8F_EPI_FUSED
-    auto project = [&](int i, int j, block_t &f) __attribute__((always_inline)) {
-        const float xs = s_xs[wm * C::WTM + i * GR + lrow];
-#pragma unroll
-        for (int qd = 0; qd < QPG; ++qd) {
-            const int nl = wn * C::WTN + j * CB + (M16 ? lq * 4 : qd * 8 + lhalf * 4);
-            const float4 w4 = *(const float4 *)&s_ws[nl], b4 = *(const float4 *)&s_bias[nl];
-            int a4[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if constexpr (M16) a4[e] = acc16[i >> 1][j][i & 1][e];
-                else a4[e] = acc[i][j][4 * qd + e];
-            }
-            f[4 * qd] = (float)a4[0] * (xs * w4.x) + b4.x, f[4 * qd + 1] = (float)a4[1] * (xs * w4.y) + b4.y;
-            f[4 * qd + 2] = (float)a4[2] * (xs * w4.z) + b4.z, f[4 * qd + 3] = (float)a4[3] * (xs * w4.w) + b4.w;
-        }
-    };
-
     // rows of t as a buffer (rows past the matrix load zeros)
     const auto tr = buffer_at(g.t, (int64_t)mw * g.max_rank * 2, (int64_t)min(gM - mw, C::WTM) * g.max_rank * 2);
-    constexpr int ROW_BYTES = C::WTN * 2, PITCH = ROW_BYTES + 8, CPO = ROW_BYTES / 16;
-    auto stage = [&](int i, int j, const block_t &f) __attribute__((always_inline)) {
-#pragma unroll
-        for (int qd = 0; qd < QPG; ++qd) {
-            const float v[4] = {f[4 * qd], f[4 * qd + 1], f[4 * qd + 2], f[4 * qd + 3]};
-            char *dst = ebuf + (i * GR + lrow) * PITCH + (j * CB + (M16 ? lq * 4 : qd * 8 + lhalf * 4)) * 2;
-            if constexpr (OUT == OUT_BF16) *(uint2 *)dst = make_uint2(f32x2_to_bf16x2_bits(v[0], v[1]), f32x2_to_bf16x2_bits(v[2], v[3]));
-            else *(uint2 *)dst = make_uint2(f32x2_to_f16x2_bits(v[0], v[1]), f32x2_to_f16x2_bits(v[2], v[3]));
-        }
-    };
     // (columns past the output load zeros; the lane's eight ranks from k0 on, past the adapter's last one, which may be half a step of 32, too)
     auto factor_of = [&](int f, int r) { return buffer_at(g.up, ((int64_t)gN * f + (int64_t)nw * r) * 2, (int64_t)min(gN - nw, C::WTN) * r * 2); };
     auto rank_at = [&](int k0, int r) { return k0 + lk < r ? (uint32_t)(k0 + lk) * 2u : 0x80000000u; };
@@ -550,15 +582,7 @@ __device__ __forceinline__ void adapters_epilogue(const AdapterArgs &g, const in
         }
     }
     }
-    // rows from LDS, 16 bytes to a lane
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int p = 0; p < C::WTM * CPO / 64; ++p) {
-        const int at = p * 64 + lane, row = at / CPO, cc = at % CPO;
-        const int mm = mw + row, nn = nw + cc * 8;
-        if (mm < gM && nn < gN) stream_store16((char *)gout + ((int64_t)mm * gN + nn) * 2, *(const uint4 *)(ebuf + row * PITCH + cc * 16));
-    }
+    store();
 }
 
 // KTAIL: K is not a multiple of BK (the last tile is ragged); the common case is the other kernel.

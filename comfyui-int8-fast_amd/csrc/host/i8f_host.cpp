@@ -41,7 +41,7 @@ namespace {
     X(i8f_quant_rowwise) X(i8f_quant_rowwise_prologue) X(i8f_quant_rowwise_norm_modulate) X(i8f_quant_rowwise_rms_norm)  \
     X(i8f_quant_rowwise_concat_gelu) X(i8f_rotate128) X(i8f_linear_w8a8_gated) X(i8f_linear_w8a8_grouped) X(i8f_linear_w8a16_small_m) \
     X(i8f_linear_w8a16_small_m_grouped) X(i8f_internal_w8a16_rotated) X(i8f_linear_w8a8_lora) X(i8f_internal_quant_lora)    \
-    X(i8f_adapters_down) X(i8f_adapters_down_workspace_bytes) X(i8f_linear_w8a8_adapters) X(i8f_linear_w8a8_adapters_workspace_bytes) X(i8f_linear_w8a16_small_m_adapters) X(i8f_block_norm)
+    X(i8f_adapters_by_side) X(i8f_adapters_down) X(i8f_adapters_down_workspace_bytes) X(i8f_linear_w8a8_adapters) X(i8f_linear_w8a8_adapters_workspace_bytes) X(i8f_linear_w8a16_small_m_adapters) X(i8f_block_norm)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
     I8F_ENTRY_POINTS(X)
@@ -544,7 +544,8 @@ PyObject *adapters(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const bool few = M <= PyLong_AsLongLong(a[7]);
     i8f_adapted_layer l[I8F_MAX_ADAPTED_LAYERS] = {};
     Size size[I8F_MAX_ADAPTED_LAYERS];
-    int64_t bytes = 0, t_at[I8F_MAX_ADAPTED_LAYERS], work_bytes = 0;
+    int64_t bytes = 0, t_at[I8F_MAX_ADAPTED_LAYERS], side_at[I8F_MAX_ADAPTED_LAYERS], work_bytes = 0;
+    bool by_side = !few;
     const auto take = [&](int64_t b) {   // a piece of the scratch memory
         const int64_t at = bytes;
         bytes += (b + 255) / 256 * 256;
@@ -569,10 +570,11 @@ PyObject *adapters(PyObject *, PyObject *const *a, Py_ssize_t n) {
         ad.first_rank = (const int32_t *)first->const_data_ptr(), ad.ids = (const int32_t *)ids->const_data_ptr(), ad.rows_per_id = per;
         l[i].w = o.w, l[i].w_scale = o.ws, l[i].w_scale_host = o.ws_host, l[i].scale_mode = o.mode, l[i].bias = o.bias, l[i].bias_dtype = o.bias_code, l[i].N = o.N;
         size[i] = output_size(x, o.N);
-        t_at[i] = take(2 * M * ad.max_rank);
+        by_side = by_side && lib.i8f_adapters_by_side(M, o.N, K, per);
         const int64_t need = few ? 0 : lib.i8f_linear_w8a8_adapters_workspace_bytes(M, o.N, K);
         work_bytes = need > work_bytes ? need : work_bytes;
     }
+    for (Py_ssize_t i = 0; i < count; ++i) t_at[i] = take(2 * M * l[i].adapters.max_rank), side_at[i] = by_side ? take(4 * M * l[i].N) : 0;
     // (the memory of the first products is free when the projections start)
     int64_t ranks = 0;
     for (Py_ssize_t i = 0; i < count; ++i) ranks += l[i].adapters.max_rank;
@@ -589,7 +591,7 @@ PyObject *adapters(PyObject *, PyObject *const *a, Py_ssize_t n) {
         char *base = (char *)scratch.data_ptr();
         for (Py_ssize_t i = 0; i < count; ++i) {
             y[i] = empty(size[i], type, dev);
-            l[i].t = base + t_at[i], l[i].out = y[i].data_ptr();
+            l[i].t = base + t_at[i], l[i].side = by_side ? (float *)(base + side_at[i]) : nullptr, l[i].out = y[i].data_ptr();
         }
         if (few) {
             rc = lib.i8f_adapters_down(xp, dt, M, K, ld, l, (int)count, 0, nullptr, nullptr, nullptr, 0, st.handle);

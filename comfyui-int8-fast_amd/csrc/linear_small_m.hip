@@ -590,6 +590,7 @@ extern "C" int i8f_linear_w8a16_small_m_adapters(const void *x, int x_dtype, int
     for (int i = 0; i < n_layers; ++i) {
         const i8f_adapted_layer &y = layers[i];
         if (y.N == 0) continue;
+        if (y.side) return I8F_ERR_UNSUPPORTED;
         if (!y.out || (K > 0 && !y.w) || (y.scale_mode == I8F_SCALE_ROW && !y.w_scale)) return I8F_ERR_INVALID;
         if (y.N > 0x7fffffff) return I8F_ERR_UNSUPPORTED;
         SmallMArgs a{};

@@ -97,11 +97,64 @@ int launch_rows_form(const void *x, int64_t M, int64_t K, int64_t ldx, int8_t *q
     return check_launch();
 }
 
+// ---- few rows with a side each: then their share of the result, B_a t, by a launch of its own that fills the chip, where the tiles of the
+// projection are too few to fetch as many different factors as there are rows.  A wave takes 256 columns of a row: the matrix unit's 16 x 16
+// x 32 form reads 16 rows of the factor in whole pieces, t stands in all columns of its other operand, and lane column b keeps block b's
+// result, so that a store is 1 KB in one piece.
+template <int DT>
+__global__ __launch_bounds__(256) void adapters_side_kernel(const DownLayers g) {
+    int l = 0;
+#pragma unroll
+    for (int i = 1; i < I8F_MAX_ADAPTED_LAYERS; ++i)
+        if (i < g.n && (int)blockIdx.x >= g.first_block[i]) l = i;
+    l = __builtin_amdgcn_readfirstlane(l);
+    const i8f_adapters &ad = g.ad[l];
+    const int64_t N = g.N[l];
+    const uint32_t at = blockIdx.x - g.first_block[l], pieces = (uint32_t)((N + 1023) / 1024);
+    const int64_t m = at / pieces;
+    const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
+    const int64_t n0 = (int64_t)(at % pieces) * 1024 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 256;
+    if (n0 >= N) return;
+    const int a = __builtin_amdgcn_readfirstlane(adapter_of(ad, m));
+    const int first = a < 0 ? 0 : ad.first_rank[a], rank = a < 0 ? 0 : ad.first_rank[a + 1] - first;
+    const char *t = g.t[l] + m * ad.max_rank * 2, *up = (const char *)ad.up + N * first * 2;
+    v4f keep = (v4f)0.0f;
+    for (int k = 8 * lq; k - 8 * lq < rank; k += 32) {
+        const bool in = k < rank;   // (ranks come in sixteens: the last step may be half a one)
+        const v4u tv = in ? *(const v4u *)(t + k * 2) : (v4u)0u;
+        v4u bv[16];
+#pragma unroll
+        for (int b = 0; b < 16; ++b) {
+            const int64_t row = n0 + 16 * b + l16 < N ? n0 + 16 * b + l16 : N - 1;
+            bv[b] = in ? *(const v4u *)(up + (row * rank + k) * 2) : (v4u)0u;
+        }
+#pragma unroll
+        for (int b = 0; b < 16; ++b) {
+            const v4f d = lora_mfma<DT>(bv[b], tv, (v4f)0.0f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) keep[e] = l16 == b ? keep[e] + d[e] : keep[e];
+        }
+    }
+    const int64_t n = n0 + 16 * l16 + 4 * lq;   // the four columns that the lane kept (N comes in eights)
+    if (n < N) *(v4f *)(g.side[l] + m * N + n) = keep;
+}
+
+template <int DT>
+int launch_side(int64_t M, DownLayers &g, hipStream_t st) {
+    int64_t first = 0;
+    for (int i = 0; i < g.n; ++i) g.first_block[i] = (int)first, first += M * ((g.N[i] + 1023) / 1024);
+    for (int i = g.n; i <= I8F_MAX_ADAPTED_LAYERS; ++i) g.first_block[i] = (int)first;
+    if (first == 0) return I8F_OK;
+    hipLaunchKernelGGL((adapters_side_kernel<DT>), dim3((unsigned)first), dim3(256), 0, st, g);
+    return check_launch();
+}
+
+inline bool side_in_place(int64_t M, int64_t N) { return N % 8 == 0 && M * ((N + 1023) / 1024) < (1ll << 29); }   // (four layers in a grid)
 inline bool down_by_rows(int64_t M, int64_t K) { return M <= DOWN_ROWS || M * K <= DOWN_ELEMENTS; }
 inline bool down_in_place(const void *x, int64_t K, int64_t ldx) { return K % 8 == 0 && (uintptr_t)x % 16 == 0 && ldx % 8 == 0 && ldx < (1ll << 23); }   // (32-bit offsets within 64 rows)
 
 template <int DT>
-int launch_down(const void *x, int64_t M, int64_t K, int64_t ldx, DownLayers &g, int rotate_block, int8_t *q, float *scale, void *workspace,
+int launch_first(const void *x, int64_t M, int64_t K, int64_t ldx, DownLayers &g, int rotate_block, int8_t *q, float *scale, void *workspace,
                 int64_t workspace_bytes, hipStream_t st) {
     const int64_t ranks = g.first_column[g.n];
     const bool in_place = down_in_place(x, K, ldx), by_rows = down_by_rows(M, K);
@@ -135,6 +188,13 @@ int launch_down(const void *x, int64_t M, int64_t K, int64_t ldx, DownLayers &g,
     return adapters_down_partial(x, DT, M, K, ldx, g, (float *)((char *)workspace + copy), slices, st);
 }
 
+template <int DT>
+int launch_down(const void *x, int64_t M, int64_t K, int64_t ldx, DownLayers &g, int rotate_block, int8_t *q, float *scale, void *workspace,
+                int64_t workspace_bytes, hipStream_t st) {
+    const int rc = launch_first<DT>(x, M, K, ldx, g, rotate_block, q, scale, workspace, workspace_bytes, st);
+    return rc || !g.n || !g.side[0] ? rc : launch_side<DT>(M, g, st);
+}
+
 }  // namespace
 }  // namespace i8f
 
@@ -153,8 +213,10 @@ extern "C" int i8f_adapters_down(const void *x, int x_dtype, int64_t M, int64_t 
     if (int rc = check_device()) return rc;
     DownLayers g{};
     for (int i = 0; i < n_layers; ++i)
-        if (layers[i].adapters.count > 0 && layers[i].adapters.max_rank > 0) {
-            g.ad[g.n] = for_kernel(layers[i].adapters), g.t[g.n] = (char *)layers[i].t;
+        if (layers[i].side || (layers[i].adapters.count > 0 && layers[i].adapters.max_rank > 0)) {
+            if (layers[i].side && !side_in_place(M, layers[i].N)) return I8F_ERR_UNSUPPORTED;
+            g.ad[g.n] = for_kernel(layers[i].adapters), g.t[g.n] = (char *)layers[i].t, g.side[g.n] = layers[i].side, g.N[g.n] = layers[i].N;
+            if (layers[i].adapters.max_rank == 0) g.ad[g.n].count = 0;
             g.first_column[g.n + 1] = g.first_column[g.n] + (int)layers[i].adapters.max_rank;   // (four of up to 65536)
             ++g.n;
         }
@@ -167,4 +229,11 @@ extern "C" int64_t i8f_adapters_down_workspace_bytes(int64_t M, int64_t K, int64
     if (M <= 0 || K <= 0 || ranks <= 0 || M > 0x7fffffff || K > 0x7fffffff || down_by_rows(M, K)) return 0;
     const int slices = adapters_down_slices(M, K);
     return (x_aligned && K % 8 == 0 ? 0 : adapters_copy_bytes(M, K)) + (slices < 2 ? 0 : slices * M * ranks * 4);
+}
+
+extern "C" int i8f_adapters_by_side(int64_t M, int64_t N, int64_t K, int64_t rows_per_id) {
+    // Up to 16 rows are another kernel's, and widths that the tiled kernels do not take go by way of i8f_adapters_up.  64 tokens of as many
+    // requests, 4096 -> 4096 + 1024 + 1024, ranks of 8 to 64: 33.5 us by side and 37.6 with the factors fetched by the 96 tiles; of one
+    // request the tiles' way is the faster one (64 x 4096 -> 4096, rank 64: 3 us more than without adapters, and 10 by side).
+    return rows_per_id > 0 && M / rows_per_id > 16 && M <= 128 && i8f_linear_w8a8_adapters_workspace_bytes(M, N, K) == 0;
 }

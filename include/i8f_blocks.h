@@ -44,13 +44,22 @@ typedef struct i8f_adapted_layer {
     int64_t N;
     i8f_adapters adapters;
     void *t;                   /* [M, max_rank] of the activations' type: the adapters' first product */
+    float *side;               /* NULL, or [M,N]: the adapters' whole share of the result, see i8f_adapters_down */
     void *out;                 /* [M,N] of the activations' type */
 } i8f_adapted_layer;
 
 /*
+ * Whether M rows of a W8A8 layer with K inputs and N outputs are better served by way of `side` (few rows, which may all have different
+ * adapters: their share is then computed by a launch of its own that fills the chip).
+ */
+int i8f_adapters_by_side(int64_t M, int64_t N, int64_t K, int64_t rows_per_id);
+
+/*
  * t[m, 0 ... r) = scale_a * A_a x[m] of every layer, for the adapter a of row m and its padded rank r: sums in binary32, one rounding to
  * x's type (what the matrix unit multiplies with in the second product); ranks beyond r and rows without an adapter are left as they
- * are.  Of the layers only adapters and t are looked at.  x_dtype I8F_BF16 or I8F_F16, n_layers up to I8F_MAX_ADAPTED_LAYERS.
+ * are.  Of the layers only adapters, t, side and, with it, N are looked at.
+ * Layers with a side get side[m,n] = sum_j t[m,j] B_a[n,j] in binary32 besides (zeros for rows without an adapter); i8f_linear_w8a8_adapters
+ * then adds that instead of reading t.  N is then a multiple of 8.  All layers of a call or none.  x_dtype I8F_BF16 or I8F_F16, n_layers up to I8F_MAX_ADAPTED_LAYERS.
  * q, scale: NULL, or the int8 rows of x and their scales besides, as i8f_quant_rowwise with rotate_block leaves them (the adapters take
  * x as it is).
  * workspace: any contents; i8f_adapters_down_workspace_bytes(M, K, the sum of the layers' max_rank, x_aligned) bytes let many rows' columns

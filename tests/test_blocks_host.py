@@ -80,12 +80,18 @@ def test_adapters_arguments_are_checked_before_any_launch(L):
     assert linear({"N": 9}) == INVALID and linear({"N": 9}, work=one, nbytes=20 * 9 * 4 - 1) == INVALID     # needs a workspace
     assert linear({"w": 24}) == UNSUPPORTED and linear({"out": 18}) == UNSUPPORTED and linear({}, a=ctypes.c_void_p(20)) == UNSUPPORTED
     assert linear({}, M=0) == 0 and linear() == 0
+    by_side = lib.i8f_adapters_by_side
+    assert by_side(64, 512, 256, 1) and by_side(34, 512, 256, 2) and not by_side(34, 512, 256, 34) and not by_side(64, 512, 256, 0)
+    assert not by_side(16, 512, 256, 1) and not by_side(4096, 512, 256, 1) and not by_side(64, 511, 256, 1) and not by_side(64, 512, 250, 1)
+    assert linear({"side": 24}) == INVALID and linear({"side": 16}, {}) == INVALID and linear({"side": 16, "N": 9}) == UNSUPPORTED
+    assert down({"side": 24}) == INVALID and down({}, {"side": 16}) == INVALID
 
     def small(*overs, M=4, K=64, ld=64, dt=L.BF16, x=one):
         return lib.i8f_linear_w8a16_small_m_adapters(x, dt, M, K, ld, _layers(L, *overs), len(overs), null)
 
     for bad in ({"t": None}, {"scale_mode": 3}, {"scale_mode": 1, "w_scale": None}, {"w": None}, {"out": None}, {"N": -1}):
         assert small(bad) == INVALID, bad
+    assert small({"side": 16}) == UNSUPPORTED
     assert small({}, M=17) == UNSUPPORTED and small({}, ld=32) == INVALID and small({}, dt=L.F32) == INVALID and small({}, x=null) == INVALID
     assert small({}, M=0) == 0 and small() == 0
 

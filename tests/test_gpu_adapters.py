@@ -93,6 +93,8 @@ CASES = [
     (33, 200, 100, (5, 40), torch.float16, {}),                      # K % 16: the ragged GEMM
     (40, 1024, 1001, (9, 33), torch.bfloat16, {"bias": False}),      # N % 8
     (64, 4096, 1024, (16, 8, 64, None, 32), torch.bfloat16, {"bias": False}),
+    (100, 1040, 776, (8, 1100, 40), torch.float16, {"bias": False}),  # more ranks than are kept of one row
+    (128, 2048, 4104, (32, 16, 8), torch.bfloat16, {"rotate": True}),
     (130, 384, 264, (100, 17), torch.float16, {"per_row": False}),
     (257, 640, 528, (16, 48), torch.bfloat16, {"rotate": True}),
     (300, 1536, 1536, (64,), torch.float16, {"bias": False}),
