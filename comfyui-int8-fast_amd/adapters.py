@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 from torch import Tensor, nn
 
-from . import _lib
+from . import _lib, compile_ops
 from ._comfy_compat import compute_device
 from .dynamic_lora import _factor_pair
 from .int8_quant import SMALL_BATCH_ROWS, _layers_in_place, _scale_on
@@ -147,32 +147,25 @@ def forward_adapters(layers, x: Tensor, banks, ids: Tensor):
     x2 = x.reshape(-1, x.shape[-1])
     rows = x2.shape[0]
     outs = [None] * len(layers)
+    # under torch.compile the calls go through the registered operators, in eager mode they go past the dispatcher
+    compiling = torch.compiler.is_compiling()
+    add_adapters = torch.ops.i8f.add_adapters if compiling else compile_ops.add_adapters_eager
+    linear_adapters = torch.ops.i8f.linear_adapters if compiling else compile_ops.linear_adapters_eager
     # layers of one rotation flag go together, as many as a launch takes: x quantised (or rotated) once, the adapters' first products in
     # one launch, the layers in another
     together = {}
     for i, layer in enumerate(layers):
         together.setdefault(bool(layer._use_quarot) if _quantised_here(layer, x) else None, []).append(i)
     for rotate, members in together.items():
-        q = s = rows_in = None
-        for at in range(0, len(members), _lib.MAX_ADAPTED_LAYERS):
-            part = members[at:at + _lib.MAX_ADAPTED_LAYERS]
-            some = [banks[i] for i in part]
-            if rotate is not None and rows > SMALL_BATCH_ROWS and q is None:
-                ts, q, s = _lib.adapters_down(x2, some, ids, per, quantise=True, rotate=rotate)
-            else:
-                ts = _lib.adapters_down(x2, some, ids, per)
-            if rotate is None:   # layers that go alone
-                for i, bank, t in zip(part, some, ts):
-                    outs[i] = _lib.adapters_up(layers[i](x).reshape(-1, bank.out_features), bank, ids, per, t)
-                continue
-            problems = [(layers[i].weight, _scale_on(layers[i], x.device), layers[i].bias, bank, t) for i, bank, t in zip(part, some, ts)]
-            if rows > SMALL_BATCH_ROWS:
-                got = _lib.linear_w8a8_adapters(q, s, problems, ids, per)
-            else:
-                if rows_in is None:
-                    rows_in = _lib.rotate128(x2) if rotate else x2
-                got = _lib.linear_w8a16_small_m_adapters(rows_in, problems, ids, per)
-            for i, y in zip(part, got):
-                outs[i] = y
+        if rotate is None:   # layers that go alone
+            for i in members:
+                outs[i] = add_adapters(layers[i](x).reshape(rows, banks[i].out_features), x2, ids, per, *compile_ops.bank_args(banks[i]))
+            continue
+        scales = [compile_ops.split_scale(_scale_on(layers[i], x.device)) for i in members]
+        parts = zip(*[compile_ops.bank_args(banks[i]) for i in members])
+        got = linear_adapters(x2, ids, per, rotate, [layers[i].weight for i in members], [t for t, _ in scales], [v for _, v in scales],
+                                  [layers[i].bias for i in members], *[list(p) for p in parts])
+        for i, y in zip(members, got):
+            outs[i] = y
     outs = [y.reshape(*lead, y.shape[-1]) for y in outs]
     return outs[0] if single else outs

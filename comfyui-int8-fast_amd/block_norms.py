@@ -10,9 +10,9 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from . import _lib, int8_fused_kernel
+from . import _lib, compile_ops, int8_fused_kernel
 from .adapters import _quantised_here
-from .int8_quant import SMALL_BATCH_ROWS, _layers_in_place, _project_quantised, forward_fanout
+from .int8_quant import SMALL_BATCH_ROWS, _layers_in_place, _project_quantised, _scale_on, forward_fanout
 
 
 def block_norm(y: Tensor, residual: Tensor, *, post_norm: str | None = None, post_weight: Tensor | None = None, post_bias: Tensor | None = None,
@@ -37,7 +37,14 @@ def block_norm(y: Tensor, residual: Tensor, *, post_norm: str | None = None, pos
                     residual_scale=residual_scale, branch_scale=branch_scale, pre_norm=pre_norm, pre_weight=pre_weight, pre_bias=pre_bias,
                     pre_eps=pre_eps, mod_scale=mod_scale, mod_shift=mod_shift)
     _refuse_gradients(y, residual, operands)
-    return _lib.block_norm(y, residual, **operands)
+    return _block_norm(y, residual, operands)
+
+
+def _block_norm(y, residual, operands):
+    if not torch.compiler.is_compiling():
+        return _lib.block_norm(y, residual, **operands)
+    x, h = torch.ops.i8f.block_norm(y, residual, **operands)
+    return x, None if all(operands.get(name) is None for name in ("pre_norm", "mod_scale", "mod_shift")) else h
 
 
 def _forward_native(layers, y, residual, post_norm=None, post_weight=None, post_bias=None, post_eps=1e-6, gate=None, gate_tanh=False, residual_scale=1.0,
@@ -68,9 +75,14 @@ def forward_block_norm(layers, y: Tensor, residual: Tensor, **operands):
     if (layers and y.is_cuda and y.dim() >= 2 and y.numel() // max(1, y.shape[-1]) > SMALL_BATCH_ROWS
             and y.dtype in (torch.float16, torch.bfloat16)
             and all(_quantised_here(lin, y) and bool(getattr(lin, "_use_quarot", False)) == rotate and lin.weight.shape[1] == y.shape[-1] for lin in layers)):
+        if torch.compiler.is_compiling():
+            x, q, s = torch.ops.i8f.block_norm_quantised(y, residual, rotate, **operands)
+            scales = [compile_ops.split_scale(_scale_on(lin, y.device)) for lin in layers]
+            outs = [torch.ops.i8f.linear_w8a8(q, s, lin.weight, t, v, lin.bias, y.dtype, int8_fused_kernel.DEFAULT_EPILOGUE) for lin, (t, v) in zip(layers, scales)]
+            return x, [o.reshape(*y.shape[:-1], o.shape[-1]) for o in outs]
         x, q, s = _lib.block_norm(y, residual, quantise=True, rotate=rotate, **operands)
         return x, [o.reshape(*y.shape[:-1], o.shape[-1]) for o in _project_quantised(layers, q, s, y.dtype)]
-    x, h = _lib.block_norm(y, residual, **operands)
+    x, h = _block_norm(y, residual, operands)
     return x, forward_fanout(layers, h)
 
 

@@ -14,6 +14,8 @@ the namespace `i8f` with a shape-only ("fake") implementation:
     torch.ops.i8f.int8_linear_prologue  <- int8_linear with the elementwise operation in front of the layer
                                            (adaLN modulation, tanh-GELU) applied inside the quantiser: what
                                            torch.compile's fusion into the Triton quantiser gives the reference
+    torch.ops.i8f.linear_adapters, add_adapters         the two ways of adapters.forward_adapters
+    torch.ops.i8f.block_norm, block_norm_quantised      block_norms.block_norm and the int8 form in front of layers
 
 `Int8TensorwiseOps.Linear.forward` switches to these operators while a graph is being traced
 (`torch.compiler.is_compiling()`); in eager mode it calls the library directly, which saves the
@@ -31,7 +33,8 @@ hands the graph to `inner` ("inductor" by default):
 import copy
 import logging
 import operator
-from typing import Optional, Tuple
+from types import SimpleNamespace
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 from torch import Tensor
@@ -176,8 +179,103 @@ def _(x, prologue, mod_scale, mod_shift, weight, weight_scale, weight_scale_valu
     return x.new_empty((*x.shape[:-1], width), dtype=compute_dtype)
 
 
+def bank_args(bank) -> tuple:
+    """An adapters.AdapterBank as the operators take it."""
+    return bank.down, bank.up, bank.scale, bank.first_rank, bank.count, bank.max_rank
+
+
+def _bank(x, out_features, down, up, scale, first_rank, count, max_rank):
+    return SimpleNamespace(down=down, up=up, scale=scale, first_rank=first_rank, count=count, max_rank=max_rank, dtype=down.dtype, device=down.device,
+                           in_features=x.shape[1], out_features=out_features)
+
+
+def linear_adapters_eager(x: Tensor, ids: Tensor, rows_per_id: int, rotate: bool, weights: Sequence[Tensor], weight_scales: Sequence[Optional[Tensor]],
+                    weight_scale_values: Sequence[float], biases: Sequence[Optional[Tensor]], downs: Sequence[Tensor], ups: Sequence[Tensor],
+                    scales: Sequence[Tensor], first_ranks: Sequence[Tensor], counts: Sequence[int], max_ranks: Sequence[int]) -> List[Tensor]:
+    """Layers of one rotation flag on x [M,K], with the adapters of the rows; ids has one number for each rows_per_id of them."""
+    from .int8_quant import SMALL_BATCH_ROWS
+
+    outs, q, s, rows = [], None, None, None
+    for at in range(0, len(weights), _lib.MAX_ADAPTED_LAYERS):
+        part = range(at, min(at + _lib.MAX_ADAPTED_LAYERS, len(weights)))
+        banks = [_bank(x, weights[i].shape[0], downs[i], ups[i], scales[i], first_ranks[i], counts[i], max_ranks[i]) for i in part]
+        if x.shape[0] > SMALL_BATCH_ROWS and q is None:
+            ts, q, s = _lib.adapters_down(x, banks, ids, rows_per_id, quantise=True, rotate=rotate)
+        else:
+            ts = _lib.adapters_down(x, banks, ids, rows_per_id)
+        layers = [(weights[i], _scale_arg(weight_scales[i], weight_scale_values[i]), biases[i], bank, t) for i, bank, t in zip(part, banks, ts)]
+        if x.shape[0] > SMALL_BATCH_ROWS:
+            outs += _lib.linear_w8a8_adapters(q, s, layers, ids, rows_per_id)
+        else:
+            rows = (_lib.rotate128(x) if rotate else x) if rows is None else rows
+            outs += _lib.linear_w8a16_small_m_adapters(rows, layers, ids, rows_per_id)
+    return outs
+
+
+linear_adapters = torch.library.custom_op(f"{NAMESPACE}::linear_adapters", linear_adapters_eager, mutates_args=())
+
+
+@linear_adapters.register_fake
+def _(x, ids, rows_per_id, rotate, weights, weight_scales, weight_scale_values, biases, downs, ups, scales, first_ranks, counts, max_ranks):
+    return [x.new_empty((x.shape[0], w.shape[0])) for w in weights]
+
+
+def add_adapters_eager(base: Tensor, x: Tensor, ids: Tensor, rows_per_id: int, down: Tensor, up: Tensor, scale: Tensor, first_rank: Tensor, count: int,
+                 max_rank: int) -> Tensor:
+    """round(base + the adapters' share of x), base [M,N] of x's dtype."""
+    bank = _bank(x, base.shape[1], down, up, scale, first_rank, count, max_rank)
+    return _lib.adapters_up(base, bank, ids, rows_per_id, _lib.adapters_down(x, [bank], ids, rows_per_id)[0])
+
+
+add_adapters = torch.library.custom_op(f"{NAMESPACE}::add_adapters", add_adapters_eager, mutates_args=())
+
+
+@add_adapters.register_fake
+def _(base, x, ids, rows_per_id, down, up, scale, first_rank, count, max_rank):
+    return x.new_empty(base.shape)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::block_norm", mutates_args=())
+def block_norm(y: Tensor, residual: Tensor, post_norm: Optional[str] = None, post_weight: Optional[Tensor] = None, post_bias: Optional[Tensor] = None,
+               post_eps: float = 1e-6, gate: Optional[Tensor] = None, gate_tanh: bool = False, residual_scale: float = 1.0, branch_scale: float = 1.0,
+               pre_norm: Optional[str] = None, pre_weight: Optional[Tensor] = None, pre_bias: Optional[Tensor] = None, pre_eps: float = 1e-6,
+               mod_scale: Optional[Tensor] = None, mod_shift: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+    """(x, h) of block_norms.block_norm; h has no elements where there is none."""
+    x, h = _lib.block_norm(y, residual, post_norm=post_norm, post_weight=post_weight, post_bias=post_bias, post_eps=post_eps, gate=gate,
+                           gate_tanh=gate_tanh, residual_scale=residual_scale, branch_scale=branch_scale, pre_norm=pre_norm, pre_weight=pre_weight,
+                           pre_bias=pre_bias, pre_eps=pre_eps, mod_scale=mod_scale, mod_shift=mod_shift)
+    return x, y.new_empty((0,)) if h is None else h
+
+
+@block_norm.register_fake
+def _(y, residual, post_norm=None, post_weight=None, post_bias=None, post_eps=1e-6, gate=None, gate_tanh=False, residual_scale=1.0, branch_scale=1.0,
+      pre_norm=None, pre_weight=None, pre_bias=None, pre_eps=1e-6, mod_scale=None, mod_shift=None):
+    has_h = pre_norm is not None or mod_scale is not None or mod_shift is not None
+    return y.new_empty(y.shape), y.new_empty(y.shape if has_h else (0,))
+
+
+@torch.library.custom_op(f"{NAMESPACE}::block_norm_quantised", mutates_args=())
+def block_norm_quantised(y: Tensor, residual: Tensor, rotate: bool, post_norm: Optional[str] = None, post_weight: Optional[Tensor] = None,
+                         post_bias: Optional[Tensor] = None, post_eps: float = 1e-6, gate: Optional[Tensor] = None, gate_tanh: bool = False,
+                         residual_scale: float = 1.0, branch_scale: float = 1.0, pre_norm: Optional[str] = None, pre_weight: Optional[Tensor] = None,
+                         pre_bias: Optional[Tensor] = None, pre_eps: float = 1e-6, mod_scale: Optional[Tensor] = None,
+                         mod_shift: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
+    """x of block_norms.block_norm, and h as quantize_rowwise leaves it."""
+    return _lib.block_norm(y, residual, post_norm=post_norm, post_weight=post_weight, post_bias=post_bias, post_eps=post_eps, gate=gate,
+                           gate_tanh=gate_tanh, residual_scale=residual_scale, branch_scale=branch_scale, pre_norm=pre_norm, pre_weight=pre_weight,
+                           pre_bias=pre_bias, pre_eps=pre_eps, mod_scale=mod_scale, mod_shift=mod_shift, quantise=True, rotate=rotate)
+
+
+@block_norm_quantised.register_fake
+def _(y, residual, rotate, post_norm=None, post_weight=None, post_bias=None, post_eps=1e-6, gate=None, gate_tanh=False, residual_scale=1.0,
+      branch_scale=1.0, pre_norm=None, pre_weight=None, pre_bias=None, pre_eps=1e-6, mod_scale=None, mod_shift=None):
+    K = y.shape[-1]
+    M = y.numel() // max(1, K)
+    return y.new_empty(y.shape), y.new_empty((M, K), dtype=torch.int8), y.new_empty((M, 1), dtype=torch.float32)
+
+
 OPS = ("quantize_rowwise", "quantize_rowwise_prologue", "rotate128", "linear_w8a8", "int8_linear", "int8_linear_lora",
-       "linear_w8a16_small_m", "int8_linear_prologue")
+       "linear_w8a16_small_m", "int8_linear_prologue", "linear_adapters", "add_adapters", "block_norm", "block_norm_quantised")
 
 
 # --------------------------------------------------------------------------- graph rewrite

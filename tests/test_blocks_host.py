@@ -157,3 +157,21 @@ def test_there_is_no_cpu_path(pkg):
         pkg.block_norm(torch.zeros(2, 8), torch.zeros(2, 8))
     with pytest.raises(RuntimeError, match="no CPU path"):
         pkg.forward_block_norm([lin], torch.zeros(2, 8), torch.zeros(2, 8), pre_norm="rms")
+
+
+def test_operators_of_a_traced_graph_give_shapes(pkg):
+    ops, meta = torch.ops.i8f, dict(device="meta", dtype=torch.bfloat16)
+    bank = pkg.AdapterBank([(torch.zeros(5, 40), torch.zeros(24, 5))], dtype=torch.bfloat16, device="meta")
+    x, ids = torch.empty(6, 40, **meta), torch.empty(3, dtype=torch.int32, device="meta")
+    down, up, scale, first, count, most = pkg.compile_ops.bank_args(bank)
+    w = torch.empty(24, 40, dtype=torch.int8, device="meta")
+    y, z = ops.linear_adapters(x, ids, 2, False, [w, w], [None, torch.empty(24, 1, device="meta")], [0.5, 0.0], [None, None], [down] * 2, [up] * 2,
+                               [scale] * 2, [first] * 2, [count] * 2, [most] * 2)
+    assert y.shape == z.shape == (6, 24) and y.dtype == torch.bfloat16
+    assert ops.add_adapters(y, x, ids, 2, down, up, scale, first, count, most).shape == (6, 24)
+    v = torch.empty(2, 3, 40, **meta)
+    out, h = ops.block_norm(v, v, post_norm="rms")
+    assert out.shape == v.shape and h.numel() == 0
+    assert ops.block_norm(v, v, mod_scale=torch.empty(40, **meta))[1].shape == v.shape
+    out, q, s = ops.block_norm_quantised(v, v, False, pre_norm="layer")
+    assert out.shape == v.shape and q.shape == (6, 40) and q.dtype == torch.int8 and s.shape == (6, 1) and s.dtype == torch.float32

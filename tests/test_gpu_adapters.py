@@ -331,3 +331,24 @@ def test_a_bank_of_lora_patches(pkg, dev):
     adapters = [None, ((down * 0.25).bfloat16(), up.bfloat16(), 1.0)]
     want, bound = expected(pkg, lin, x, adapters, ids)
     check(pkg.forward_adapters(lin, x, bank, ids), want, bound)
+
+
+@pytest.mark.parametrize("rows", [8, 200])
+def test_in_a_compiled_program(pkg, dev, rows):
+    """Traced without a break, also beside a layer that goes alone; more than 128 rows and up to 16 take the eager call's kernels."""
+    layers = [layer_of(pkg, 256, N, torch.bfloat16, rotate=True, seed=N) for N in (128, 72)] + [layer_of(pkg, 256, 64, torch.bfloat16, bias=False)]
+    alone = layer_of(pkg, 256, 128, torch.bfloat16, seed=9)
+    alone.weight_function = [lambda w: w]
+    layers.append(alone)
+    banks = [pkg.AdapterBank(factors_of(256, lin.out_features, (8, 20), torch.bfloat16, seed=i)) for i, lin in enumerate(layers)]
+    x, ids = torch.randn(rows, 256, device=dev).bfloat16(), ids_of("tokens", rows, 2)
+
+    def run(x, ids):
+        return pkg.forward_adapters(layers[:3], x, banks[:3], ids), pkg.forward_adapters(layers[3], x, banks[3], ids)
+
+    with torch.no_grad():
+        want, want_alone = run(x, ids)
+        got, _ = torch.compile(lambda x, ids: (pkg.forward_adapters(layers[:3], x, banks[:3], ids), 0), backend="aot_eager", fullgraph=True)(x, ids)
+        _, got_alone = torch.compile(run, backend="aot_eager")(x, ids)
+    for a, b in zip((*got, got_alone), (*want, want_alone)):
+        assert torch.equal(a, b)

@@ -316,3 +316,20 @@ def test_a_run_of_blocks(pkg, L, dev):
         assert torch.equal(x, want_x) and torch.equal(a, up[0](want_h)) and torch.equal(b, up[1](want_h))
         branch = down(a, prologue=L.PRO_SILU_GATE, mod_scale=b)
         assert torch.isfinite(branch.float()).all()
+
+
+@pytest.mark.parametrize("rows", [8, 40])
+def test_in_a_compiled_program(pkg, dev, rows):
+    layers = layers_of(pkg, 256, (128, 72), torch.bfloat16)
+    y, r = inputs((rows, 256), torch.bfloat16)
+    ops, _ = operands((rows, 256), torch.bfloat16, "rms", "layer", True)
+
+    def run(y, r):
+        return pkg.block_norm(y, r, **ops), pkg.block_norm(y, r, post_norm="rms"), pkg.forward_block_norm(layers, y, r, **ops)
+
+    with torch.no_grad():
+        want = run(y, r)
+        got = torch.compile(run, backend="aot_eager", fullgraph=True)(y, r)
+    assert got[1][1] is None and want[1][1] is None
+    pairs = [*zip(got[0], want[0]), (got[1][0], want[1][0]), (got[2][0], want[2][0]), *zip(got[2][1], want[2][1])]
+    assert all(torch.equal(a, b) for a, b in pairs)
