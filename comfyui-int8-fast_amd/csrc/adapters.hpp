@@ -51,8 +51,8 @@ __host__ __device__ inline int64_t factor_width(int64_t K) { return (K + 7) / 8 
 // A copy of x's rows with that width
 inline int64_t adapters_copy_bytes(int64_t M, int64_t K) { return (M * factor_width(K) * 2 + 255) / 256 * 256; }
 int adapters_copy_rows(const void *x, int64_t M, int64_t K, int64_t ldx, void *to, hipStream_t st);
-// Many rows (adapters_down.hip; K a multiple of eight, aligned rows): slices of the columns that a launch for M rows is split into, and the launch; partial: [slices, M,
-// first_column[n]] float where slices > 1.
+// Many rows (adapters_down.hip; K a multiple of eight, aligned rows): slices of the columns that a launch for M rows is split into, and the
+// launch.  One slice leaves t; more leave partial, [slices, M, first_column[n]] float, which adapters_combine makes t of.
 int adapters_down_slices(int64_t M, int64_t K);
 int adapters_down_partial(const void *x, int dtype, int64_t M, int64_t K, int64_t ldx, const DownLayers &g, float *partial, int slices, hipStream_t st);
 

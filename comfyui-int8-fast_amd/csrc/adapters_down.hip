@@ -2,7 +2,7 @@
 //
 // A product of M rows by a few dozen to a few hundred ranks over a long K.  What bounds it is what the CUs draw from L2 (about 35 bytes a
 // cycle each when all of them do): a workgroup reads its rows of x and the whole of the factors' slice, so 64 rows share the factors, and the
-// columns are dealt over `slices` workgroups, whose sums meet in memory (adapters_combine_kernel), until every CU has two.
+// columns are dealt over `slices` workgroups, whose sums meet in memory (adapters_combine, quant_adapters.hpp), until every CU has two.
 // 64 rows and up to 128 ranks at a time: four waves of 16 rows by all the ranks, K-tiles of 64 columns (128 bytes of a row) in LDS, fetched
 // by direct loads a few tiles ahead, with the 16-byte chunks of a row permuted by the row so that the 16 rows of a fragment are
 // read from different banks.  One barrier per K-tile: behind it the tile has landed for everyone, and everyone is done with the tile
@@ -178,30 +178,6 @@ __global__ __launch_bounds__(256) void adapters_partial_kernel(const char *__res
     }
 }
 
-// t = scale_a (the slices' sums, in order), rounded: four ranks of a row to a thread
-template <int DT>
-__global__ __launch_bounds__(256) void adapters_combine_kernel(const float *__restrict__ partial, int M, int slices, const DownLayers g) {
-    const uint32_t columns = (uint32_t)g.first_column[g.n], quads = columns / 4;
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t m = at / quads;
-    if (m >= M) return;
-    const int col = (int)(at % quads) * 4;
-    int l = 0;
-#pragma unroll
-    for (int k = 1; k < I8F_MAX_ADAPTED_LAYERS; ++k)
-        if (k < g.n && col >= g.first_column[k]) l = k;
-    const int a = adapter_of(g.ad[l], m), j = col - g.first_column[l];
-    if (a < 0 || j >= g.ad[l].first_rank[a + 1] - g.ad[l].first_rank[a]) return;
-    const float *p = partial + m * columns + col;
-    v4f sum = *(const v4f *)p;
-    for (int z = 1; z < slices; ++z) sum += *(const v4f *)(p + (int64_t)z * M * columns);
-    const float s = g.ad[l].scale[a];
-    uint2 o;
-    if constexpr (DT == I8F_BF16) o = make_uint2(f32x2_to_bf16x2_bits(sum.x * s, sum.y * s), f32x2_to_bf16x2_bits(sum.z * s, sum.w * s));
-    else o = make_uint2(f32x2_to_f16x2_bits(sum.x * s, sum.y * s), f32x2_to_f16x2_bits(sum.z * s, sum.w * s));
-    *(uint2 *)(g.t[l] + (m * g.ad[l].max_rank + j) * 2) = o;
-}
-
 // rows of 16-bit values to rows of a multiple of eight of them, zeros behind: eight to a thread
 __global__ __launch_bounds__(256) void copy_rows_kernel(const uint16_t *__restrict__ x, int64_t pieces, int K, int64_t ldx, int per_row, char *__restrict__ to) {
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -232,10 +208,6 @@ int launch(const char *x, int M, int K, int ldx_bytes, const DownLayers &g, floa
     else if (ranks <= 64) go(adapters_partial_kernel<DT, 4, 5>);
     else if (ranks <= 96) go(adapters_partial_kernel<DT, 6, 4>);
     else go(adapters_partial_kernel<DT, 8, 3>);
-    if (int rc = check_launch()) return rc;
-    if (slices == 1) return I8F_OK;
-    const int64_t threads = (int64_t)M * (ranks / 4);
-    hipLaunchKernelGGL((adapters_combine_kernel<DT>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, partial, M, slices, g);
     return check_launch();
 }
 

@@ -80,6 +80,72 @@ __global__ __launch_bounds__(256) void adapters_rows_kernel(const char *__restri
     if (lane == 0) store_from_f32<DT>(g.t[l], m * ad.max_rank + j, sum * ad.scale[a]);
 }
 
+// ---- many rows, the sums of the slices of K (adapters_down.hip): t = scale_a (the slices' sums, in order), rounded: four ranks of a row to a thread
+template <int DT>
+__device__ __forceinline__ void adapters_combine(const float *__restrict__ partial, int64_t M, int slices, int64_t block, const DownLayers &g) {
+    const uint32_t columns = (uint32_t)g.first_column[g.n], quads = columns / 4;
+    const int64_t at = block * 256 + threadIdx.x;
+    const int64_t m = at / quads;
+    if (m >= M) return;
+    const int col = (int)(at % quads) * 4;
+    int l = 0;
+#pragma unroll
+    for (int k = 1; k < I8F_MAX_ADAPTED_LAYERS; ++k)
+        if (k < g.n && col >= g.first_column[k]) l = k;
+    const int a = adapter_of(g.ad[l], m), j = col - g.first_column[l];
+    if (a < 0 || j >= g.ad[l].first_rank[a + 1] - g.ad[l].first_rank[a]) return;
+    const float *p = partial + m * columns + col;
+    v4f sum = *(const v4f *)p;
+    for (int z = 1; z < slices; ++z) sum += *(const v4f *)(p + z * M * columns);
+    const float s = g.ad[l].scale[a];
+    uint2 o;
+    if constexpr (DT == I8F_BF16) o = make_uint2(f32x2_to_bf16x2_bits(sum.x * s, sum.y * s), f32x2_to_bf16x2_bits(sum.z * s, sum.w * s));
+    else o = make_uint2(f32x2_to_f16x2_bits(sum.x * s, sum.y * s), f32x2_to_f16x2_bits(sum.z * s, sum.w * s));
+    *(uint2 *)(g.t[l] + (m * g.ad[l].max_rank + j) * 2) = o;
+}
+// and the quantiser of x beside it, by the workgroups behind (RUNS > 0, WPR waves to a row): alone the sums take 5 us, most of them the way
+// into and out of a kernel.
+template <int DT, bool ROT, int WPR, int RUNS>
+__global__ __launch_bounds__(256) void adapters_combine_kernel(const float *__restrict__ partial, int64_t M, int slices, int combine_blocks,
+                                                               const char *__restrict__ x, int64_t K, int64_t ldx, int8_t *__restrict__ q,
+                                                               float *__restrict__ scale, const DownLayers g) {
+    if constexpr (RUNS > 0) {
+        if ((int)blockIdx.x >= combine_blocks) {
+            const Prologue none{};
+            quant16_body<DT, ROT, WPR, RUNS, false, I8F_PRO_NONE, 1>(x, M, K, ldx * 2, q, scale, none, (int64_t)((int)blockIdx.x - combine_blocks) * (4 / WPR));
+            return;
+        }
+    }
+    adapters_combine<DT>(partial, M, slices, blockIdx.x, g);
+}
+
+template <int DT, bool ROT, int WPR, int RUNS>
+int launch_combine(const float *partial, int64_t M, int slices, const void *x, int64_t K, int64_t ldx, int8_t *q, float *scale, const DownLayers &g, hipStream_t st) {
+    const int64_t combine = (M * (g.first_column[g.n] / 4) + 255) / 256, quant = RUNS > 0 ? (M + 4 / WPR - 1) / (4 / WPR) : 0;
+    if (combine + quant > 0x7fffffff) return I8F_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((adapters_combine_kernel<DT, ROT, WPR, RUNS>), dim3((unsigned)(combine + quant)), dim3(256), 0, st, partial, M, slices, (int)combine, (const char *)x,
+                       K, ldx, q, scale, g);
+    return check_launch();
+}
+template <int DT, bool ROT>
+int pick_combine(const float *partial, int64_t M, int slices, const void *x, int64_t K, int64_t ldx, int8_t *q, float *scale, const DownLayers &g, hipStream_t st) {
+    const auto go = [&](auto WPR, auto RUNS) { return launch_combine<DT, ROT, decltype(WPR)::value, decltype(RUNS)::value>(partial, M, slices, x, K, ldx, q, scale, g, st); };
+    const std::integral_constant<int, 1> one;
+    const std::integral_constant<int, 2> two;
+    const std::integral_constant<int, 3> three;
+    const std::integral_constant<int, 4> four;
+    if (!q) return go(one, std::integral_constant<int, 0>{});
+    switch ((K / 16 + 63) / 64) {   // (a wave holds 64 runs of 16 values at a time; the most four times, then the row goes to four waves)
+    case 1: return go(one, one);
+    case 2: return go(one, two);
+    case 3: return go(one, three);
+    case 4: return go(one, four);
+    case 5: case 6: case 7: case 8: return go(four, two);
+    case 9: case 10: case 11: case 12: return go(four, three);
+    default: return go(four, four);
+    }
+}
+
 // Where a rank of a row is a wave of its own: few rows, whatever adapters they have, or a small x; x and a factor's row are fetched again
 // for each, so that beyond it rows share the factors (adapters_down.hip).  Not by the number of ranks: a layer's sums do not depend on the
 // layers beside it.
@@ -92,6 +158,7 @@ int launch_rows_form(const void *x, int64_t M, int64_t K, int64_t ldx, int8_t *q
     for (int i = 0; i < g.n; ++i) g.first_block[i] = (int)first, first += M * (g.ad[i].max_rank / 4);
     for (int i = g.n; i <= I8F_MAX_ADAPTED_LAYERS; ++i) g.first_block[i] = (int)first;
     if (quant_blocks + first == 0) return I8F_OK;
+    if (quant_blocks + first > 0x7fffffff) return I8F_ERR_UNSUPPORTED;
     hipLaunchKernelGGL((adapters_rows_kernel<DT, ROT, RUNS, ANY>), dim3((unsigned)(quant_blocks + first)), dim3(256), 0, st, (const char *)x, M, (int)K, ldx, q, scale,
                        (int)quant_blocks, g);
     return check_launch();
@@ -158,7 +225,6 @@ int launch_first(const void *x, int64_t M, int64_t K, int64_t ldx, DownLayers &g
                 int64_t workspace_bytes, hipStream_t st) {
     const int64_t ranks = g.first_column[g.n];
     const bool in_place = down_in_place(x, K, ldx), by_rows = down_by_rows(M, K);
-    if (by_rows && M * ranks >= (1ll << 30)) return I8F_ERR_UNSUPPORTED;
     if (by_rows && in_place && q && M <= DOWN_ROWS && K % 16 == 0 && K <= 16384 && (uintptr_t)q % 16 == 0) {   // the quantiser in the same launch
         const int64_t runs = (K / 16 + 255) / 256;
         auto go = [&](auto ROT) {
@@ -171,21 +237,26 @@ int launch_first(const void *x, int64_t M, int64_t K, int64_t ldx, DownLayers &g
         };
         return rotate_block ? go(std::true_type{}) : go(std::false_type{});
     }
-    if (q)
+    const int64_t copy = in_place ? 0 : adapters_copy_bytes(M, K);
+    int slices = adapters_down_slices(M, K);
+    if (!workspace || workspace_bytes < copy + slices * M * ranks * 4) slices = 1;
+    const bool beside = in_place && !by_rows && ranks > 0 && slices > 1 && K % 16 == 0 && K <= 16384 && (uintptr_t)q % 16 == 0;   // the quantiser goes along with the sums
+    if (q && !beside)
         if (int rc = i8f_quant_rowwise(x, DT, M, K, ldx, rotate_block, q, scale, st)) return rc;
     if (ranks == 0) return I8F_OK;
     if (by_rows)
         return in_place ? launch_rows_form<DT, false, 0>(x, M, K, ldx, q, scale, g, st) : launch_rows_form<DT, false, 0, true>(x, M, K, ldx, q, scale, g, st);
     // rows that the direct loads do not take are copied first, padded like the factors
-    const int64_t copy = in_place ? 0 : adapters_copy_bytes(M, K);
-    int slices = adapters_down_slices(M, K);
-    if (!workspace || workspace_bytes < copy + slices * M * ranks * 4) slices = 1;
     if (copy) {
         if (!workspace || workspace_bytes < copy) return launch_rows_form<DT, false, 0, true>(x, M, K, ldx, q, scale, g, st);
         if (int rc = adapters_copy_rows(x, M, K, ldx, workspace, st)) return rc;
         x = workspace, K = ldx = factor_width(K);
     }
-    return adapters_down_partial(x, DT, M, K, ldx, g, (float *)((char *)workspace + copy), slices, st);
+    const float *partial = (const float *)((char *)workspace + copy);
+    if (int rc = adapters_down_partial(x, DT, M, K, ldx, g, (float *)partial, slices, st)) return rc;
+    if (slices == 1) return I8F_OK;
+    if (!beside) q = nullptr;
+    return rotate_block ? pick_combine<DT, true>(partial, M, slices, x, K, ldx, q, scale, g, st) : pick_combine<DT, false>(partial, M, slices, x, K, ldx, q, scale, g, st);
 }
 
 template <int DT>
