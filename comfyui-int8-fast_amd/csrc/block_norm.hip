@@ -13,13 +13,15 @@ namespace {
 
 enum { H_NONE, H_STORED, H_INT8, H_INT8_ROTATED };   // what becomes of h
 
-// tanh(u) = (1 - e) / (1 + e) with e = exp(-2 |u|) on the hardware's exp2 and reciprocal: within 2e-7 of tanh, which 16-bit results do
-// not see; binary32 rows take the library's function.
+// tanh(u) = (1 - e) / (1 + e) with e = exp(-2 |u|) on the hardware's exp2 and reciprocal, within 2e-7 of it, and the first terms of the series
+// near zero (the next one, 17 u^7 / 315, is below 4e-9 u there): 4e-6 relative at the most, which 16-bit results do not see.  binary32 rows
+// take the library's function.
 template <int DT>
 __device__ __forceinline__ float gate_tanh(float u) {
     if constexpr (DT == I8F_F32) return tanhf(u);
-    const float e = __builtin_amdgcn_exp2f(fabsf(u) * -2.8853900817779268f);
-    return copysignf((1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), u);
+    const float e = __builtin_amdgcn_exp2f(fabsf(u) * -2.8853900817779268f), u2 = u * u;
+    const float near = __builtin_fmaf(u * u2, __builtin_fmaf(u2, 0.13333333f, -0.33333333f), u);   // (u - u^3 / 3 + 2 u^5 / 15: 1 - e cancels there)
+    return fabsf(u) < 0.0625f ? near : copysignf((1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), u);
 }
 
 template <int DT>
@@ -27,7 +29,8 @@ __device__ __forceinline__ float norm_operand(const void *p, int dtype, int64_t 
     return DT == I8F_F32 || dtype == I8F_F32 ? ((const float *)p)[k] : load_as_f32<DT>(p, k);
 }
 
-// ---- rows of less than a run, or too wide for registers: 256 threads to a row, which is read again for every statistic (from cache) ----------------
+// ---- rows of less than a run, or too wide for registers (more than 1024 runs): 256 threads to a row, which is read again for every statistic
+// (from cache) ----------------
 template <int DT, int H>
 __global__ __launch_bounds__(256) void block_norm_generic_kernel(const i8f_block_norm_args a) {
     __shared__ float red[4];
@@ -109,7 +112,9 @@ __global__ __launch_bounds__(256) void block_norm_generic_kernel(const i8f_block
 }
 
 // ---- rows that stay in registers --------------------------------------------------------------------------------------------
-// Both rows are read once, the sums are taken over registers: 7 or 8 bytes an element in 16 bits, which is what bounds it.
+// Both rows are read once, the sums are taken over registers: 7 or 8 bytes an element in 16 bits, which is what bounds it.  16384 x 5120 in
+// bfloat16 150 us, 4.5 TB/s, where a copy of 4 GiB runs at 4.75; 2048 x 3840 13.1 us, 4.8 TB/s, part of it from the last-level cache;
+// 4096 x 2048 in binary32 23.7 us; 4096 x 3840 with int8 rows out 28 us.  A call of two rows is 4.5 us of launch and dependent loads.
 // WPR waves share a row, a lane holds NCH runs of RUN consecutive elements (32 bytes of a 16-bit row, 16 of a binary32 one).  How many waves
 // a row gets depends on its width alone, so that a row's bits depend neither on the rows beside it nor on what becomes of h.
 template <int DT>
@@ -370,10 +375,16 @@ bool whole_runs(const i8f_block_norm_args &a, int run) {
     return all % 16 == 0 && a.K % run == 0 && a.ldy % per16 == 0 && a.ldr % per16 == 0;
 }
 
+// Waves to a row by its width, us for 2, 512, 4096 and 32768 rows with both norms, a tanh gate and a scale:
+//     1024 x 16 bits  one wave          4.1   4.9   9.6   58      four, half of them idle   4.4   5.3  19.7  128
+//     2048            two, a run each   4.4   5.3  16.0  110      one, two runs             6.3   7.5  16.7  112     four  4.3  5.5  21.8  147
+//     4096            four, a run each  4.5   6.9  27.9  217      two, two runs             6.8   8.7  29.9  212     one  10.5  12.8  35.5  251
+//     512 x 32 bits   one, two runs     4.1   4.6   8.4   54      two, a run each           3.2   3.7   8.7   58
+//     1024            four, a run each  3.4   4.2  15.0  108      two, two runs             4.3   5.1  13.9  100
 template <int DT, int H, bool ANY>
 int launch_width(const i8f_block_norm_args &a, int64_t runs, hipStream_t st) {
     if (runs <= 64) return launch_rows<DT, H, 1, 1, ANY>(a, st);
-    if (runs <= 128) return launch_rows<DT, H, 1, 2, ANY>(a, st);
+    if (runs <= 128) return launch_rows<DT, H, DT == I8F_F32 ? 1 : 2, DT == I8F_F32 ? 2 : 1, ANY>(a, st);
     if (runs <= 256) return launch_rows<DT, H, 4, 1, ANY>(a, st);
     if (runs <= 512) return launch_rows<DT, H, 4, 2, ANY>(a, st);
     if (runs <= 768) return launch_rows<DT, H, 4, 3, ANY>(a, st);

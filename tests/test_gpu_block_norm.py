@@ -333,3 +333,16 @@ def test_in_a_compiled_program(pkg, dev, rows):
     assert got[1][1] is None and want[1][1] is None
     pairs = [*zip(got[0], want[0]), (got[1][0], want[1][0]), (got[2][0], want[2][0]), *zip(got[2][1], want[2][1])]
     assert all(torch.equal(a, b) for a, b in pairs)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_a_tanh_gate_is_as_good_near_zero(pkg, dev, dtype):
+    """Relative to the result: half a step, and 4e-6 of the gate in 16 bits (2e-7 absolute from 0.0625 on, the series below), a few units of
+    binary32 else."""
+    gate = torch.tensor([0.0, 1e-6, -1e-5, 1e-3, 0.03, -0.0624, 0.0626, 0.1, -0.5, 1.0, 4.0, -9.0, 50.0, 1e-4, 0.06, -0.07], device=dev).to(dtype)
+    y = torch.linspace(0.5, 900.0, 48, device=dev).view(3, 16).to(dtype)
+    x, _ = pkg.block_norm(y, torch.zeros_like(y), gate=gate, gate_tanh=True)
+    want = gate.double().tanh() * y.double()
+    u = torch.finfo(dtype).eps / 2
+    bound = want.abs() * (u + (5e-6 if dtype != torch.float32 else 8 * V)) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    assert ((x.double() - want).abs() <= bound).all()
