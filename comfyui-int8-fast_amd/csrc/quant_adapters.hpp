@@ -146,10 +146,15 @@ int pick_combine(const float *partial, int64_t M, int slices, const void *x, int
     }
 }
 
-// Where a rank of a row is a wave of its own: few rows, whatever adapters they have, or a small x; x and a factor's row are fetched again
-// for each, so that beyond it rows share the factors (adapters_down.hip).  Not by the number of ranks: a layer's sums do not depend on the
-// layers beside it.
-constexpr int64_t DOWN_ROWS = 256, DOWN_ELEMENTS = 1 << 19;
+// Where a rank of a row is a wave of its own: few rows, whatever adapters they have, or few of those waves; x and a factor's row are fetched
+// again for each, so that beyond it rows share the factors (adapters_down.hip), which costs a pass for every adapter that occurs among 64
+// rows.  K = 4096 with the quantiser, us, rows of one adapter, of eight requests and of 32 in turn:
+//     rows x ranks   128 x 16   4.3   4.3   4.3 by waves,  11   16   60 by tiles       512 x 16    7.7   7.8   7.8 and  12   12   61
+//                    128 x 128 12.6  12.6  14.5            14   27  147               1024 x 16   14    14    14        12   12   62
+//                    256 x 128  23    22    25             15   19  146                512 x 128  42    41    46        15   15  146
+inline bool down_by_rows(int64_t M, int64_t K, int64_t ranks) {
+    return M <= 128 || (M <= 256 && M * ranks <= 1 << 15) || (M < (1 << 14) && M * ranks <= 1 << 14) || K >= (1 << 23);   // (32-bit offsets within 64 rows)
+}
 
 template <int DT, bool ROT, int RUNS, bool ANY = false>
 int launch_rows_form(const void *x, int64_t M, int64_t K, int64_t ldx, int8_t *q, float *scale, DownLayers &g, hipStream_t st) {
@@ -217,15 +222,14 @@ int launch_side(int64_t M, DownLayers &g, hipStream_t st) {
 }
 
 inline bool side_in_place(int64_t M, int64_t N) { return N % 8 == 0 && M * ((N + 1023) / 1024) < (1ll << 29); }   // (four layers in a grid)
-inline bool down_by_rows(int64_t M, int64_t K) { return M <= DOWN_ROWS || M * K <= DOWN_ELEMENTS; }
-inline bool down_in_place(const void *x, int64_t K, int64_t ldx) { return K % 8 == 0 && (uintptr_t)x % 16 == 0 && ldx % 8 == 0 && ldx < (1ll << 23); }   // (32-bit offsets within 64 rows)
+inline bool down_in_place(const void *x, int64_t K, int64_t ldx) { return K % 8 == 0 && (uintptr_t)x % 16 == 0 && ldx % 8 == 0 && ldx < (1ll << 23); }
 
 template <int DT>
 int launch_first(const void *x, int64_t M, int64_t K, int64_t ldx, DownLayers &g, int rotate_block, int8_t *q, float *scale, void *workspace,
                 int64_t workspace_bytes, hipStream_t st) {
     const int64_t ranks = g.first_column[g.n];
-    const bool in_place = down_in_place(x, K, ldx), by_rows = down_by_rows(M, K);
-    if (by_rows && in_place && q && M <= DOWN_ROWS && K % 16 == 0 && K <= 16384 && (uintptr_t)q % 16 == 0) {   // the quantiser in the same launch
+    const bool in_place = down_in_place(x, K, ldx), by_rows = down_by_rows(M, K, ranks);
+    if (by_rows && in_place && q && K % 16 == 0 && K <= 16384 && (uintptr_t)q % 16 == 0) {   // the quantiser in the same launch
         const int64_t runs = (K / 16 + 255) / 256;
         auto go = [&](auto ROT) {
             switch (runs) {
@@ -280,7 +284,7 @@ extern "C" int i8f_adapters_down(const void *x, int x_dtype, int64_t M, int64_t 
     if (int rc = validate_layers(layers, n_layers, x_dtype, M)) return rc;
     if (M == 0) return I8F_OK;
     if (ldx < K || (K > 0 && !x)) return I8F_ERR_INVALID;
-    if (M > 0x7fffffff || K > 0x7fffffff) return I8F_ERR_UNSUPPORTED;
+    if (M > 0x7fffffff || K > (1 << 30)) return I8F_ERR_UNSUPPORTED;   // (a lane's column is 32 bits, and goes a few steps past the row)
     if (int rc = check_device()) return rc;
     DownLayers g{};
     for (int i = 0; i < n_layers; ++i)
@@ -297,7 +301,7 @@ extern "C" int i8f_adapters_down(const void *x, int x_dtype, int64_t M, int64_t 
 
 extern "C" int64_t i8f_adapters_down_workspace_bytes(int64_t M, int64_t K, int64_t ranks, int x_aligned) {
     using namespace i8f;
-    if (M <= 0 || K <= 0 || ranks <= 0 || M > 0x7fffffff || K > 0x7fffffff || down_by_rows(M, K)) return 0;
+    if (M <= 0 || K <= 0 || ranks <= 0 || M > 0x7fffffff || K > (1 << 30) || down_by_rows(M, K, ranks)) return 0;
     const int slices = adapters_down_slices(M, K);
     return (x_aligned && K % 8 == 0 ? 0 : adapters_copy_bytes(M, K)) + (slices < 2 ? 0 : slices * M * ranks * 4);
 }

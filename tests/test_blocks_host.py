@@ -58,7 +58,8 @@ def test_adapters_arguments_are_checked_before_any_launch(L):
     assert size(16, 4096, 32, 1) == size(0, 64, 16, 1) == size(4096, 0, 16, 1) == size(4096, 64, 0, 1) == size(1 << 31, 64, 16, 1) == 0
     assert size(4096, 4096, 32, 1) % (4096 * 32 * 4) == 0 and size(4096, 4096, 32, 1) > 0
     assert size(4096, 4096, 32, 0) == size(4096, 4096, 32, 1) + 4096 * 4096 * 2 and size(4096, 4089, 32, 1) == size(4096, 4089, 32, 0)
-    assert down({}, M=1 << 31) == UNSUPPORTED
+    assert size(200, 4096, 128, 1) == 0 < size(200, 4096, 192, 1) and size(1000, 4096, 16, 1) == 0 < size(1100, 4096, 16, 1)
+    assert down({}, M=1 << 31) == UNSUPPORTED and down({}, K=(1 << 30) + 8, ld=(1 << 30) + 8) == UNSUPPORTED
     assert down({"ids": None, "t": None}, M=0) == 0
 
     def up(base=one, bd=L.F32, dt=L.BF16, out=ctypes.c_void_p(32), M=4, N=8, t=one):

@@ -93,7 +93,7 @@ CASES = [
     (33, 200, 100, (5, 40), torch.float16, {}),                      # K % 16: the ragged GEMM
     (40, 1024, 1001, (9, 33), torch.bfloat16, {"bias": False}),      # N % 8
     (64, 4096, 1024, (16, 8, 64, None, 32), torch.bfloat16, {"bias": False}),
-    (100, 1040, 776, (8, 1100, 40), torch.float16, {"bias": False}),  # more ranks than are kept of one row
+    (100, 1040, 776, (8, 1100, 40), torch.float16, {"bias": False}),  # a rank beyond every other
     (128, 2048, 4104, (32, 16, 8), torch.bfloat16, {"rotate": True}),
     (130, 384, 264, (100, 17), torch.float16, {"per_row": False}),
     (257, 640, 528, (16, 48), torch.bfloat16, {"rotate": True}),
@@ -352,3 +352,26 @@ def test_in_a_compiled_program(pkg, dev, rows):
         _, got_alone = torch.compile(run, backend="aot_eager")(x, ids)
     for a, b in zip((*got, got_alone), (*want, want_alone)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows", [7, 90, 300])
+def test_more_layers_than_a_launch_takes_and_one_number_for_all(pkg, dev, rows):
+    """Six layers of both rotation flags, one of them twice with one bank; ids without dimensions."""
+    dtype = torch.bfloat16
+    layers = [layer_of(pkg, 256, N, dtype, rotate=i % 3 == 0, seed=i) for i, N in enumerate((128, 72, 40, 256, 8))]
+    made = [factors_of(256, lin.out_features, (8, 20), dtype, seed=i) for i, lin in enumerate(layers)]
+    banks = [pkg.AdapterBank(f) for f in made]
+    layers, made, banks = layers + layers[1:2], made + made[1:2], banks + banks[1:2]
+    x = torch.randn(rows, 256, device=dev).to(dtype)
+    outs = pkg.forward_adapters(layers, x, banks, torch.tensor(1, dtype=torch.int32, device=dev))
+    for lin, f, y in zip(layers, made, outs):
+        check(y, *expected(pkg, lin, x, f, torch.ones(rows, dtype=torch.int32, device=dev)))
+    assert torch.equal(outs[1], outs[5])
+
+
+def test_a_single_row_without_other_dimensions(pkg, dev):
+    lin, f = layer_of(pkg, 128, 48, torch.float16), factors_of(128, 48, (8,), torch.float16)
+    x = torch.randn(128, device=dev).half()
+    y = pkg.forward_adapters(lin, x, pkg.AdapterBank(f), torch.tensor(0, dtype=torch.int32, device=dev))
+    assert y.shape == (48,)
+    check(y[None], *expected(pkg, lin, x[None], f, torch.zeros(1, dtype=torch.int32, device=dev)))
