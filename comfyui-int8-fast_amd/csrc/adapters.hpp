@@ -13,13 +13,13 @@ __device__ __forceinline__ int adapter_of(const i8f_adapters &ad, int64_t m) {
     return (uint32_t)a < (uint32_t)ad.count ? a : -1;
 }
 
-// sum_j t[m,j] B_a[n,j] over the adapter's padded ranks, pairs of 16-bit values at a time, in binary32
+// sum_j t[m,j] B_a[n,j] over the adapter's padded ranks from 8 k on, every 8 of `of` eights, pairs of 16-bit values at a time, in binary32
 template <int DT>
-__device__ __forceinline__ float adapter_term(const i8f_adapters &ad, const void *t, int64_t m, int64_t n, int64_t N, int a) {
+__device__ __forceinline__ float adapter_term(const i8f_adapters &ad, const void *t, int64_t m, int64_t n, int64_t N, int a, int k = 0, int of = 1) {
     const int first = ad.first_rank[a], r = ad.first_rank[a + 1] - first;
     const char *tp = (const char *)t + m * ad.max_rank * 2, *bp = (const char *)ad.up + (N * first + n * r) * 2;
     float sum = 0.0f;
-    for (int j = 0; j < r; j += 8) {
+    for (int j = 8 * k; j < r; j += 8 * of) {
         const uint4 tv = *(const uint4 *)(tp + j * 2), bv = *(const uint4 *)(bp + j * 2);
         const uint32_t tw[4] = {tv.x, tv.y, tv.z, tv.w}, bw[4] = {bv.x, bv.y, bv.z, bv.w};
 #pragma unroll
@@ -34,6 +34,15 @@ __device__ __forceinline__ float adapter_term(const i8f_adapters &ad, const void
         }
     }
     return sum;
+}
+
+// 16 x 16 x 32 product of two fragments of 16-bit values, eight of each to a lane, into binary32
+template <int DT, class V, class F>
+__device__ __forceinline__ F factor_mfma(V a, V b, F c) {
+    typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+    typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+    if constexpr (DT == I8F_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
 // The adapters of up to four layers, of one ids and rows_per_id, and where their first products go

@@ -23,14 +23,6 @@ using gemm::v4i;
 using gemm::waitcnt_vm;
 
 typedef float v4f __attribute__((ext_vector_type(4)));
-typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-
-template <int DT>
-__device__ __forceinline__ v4f down_mfma(v4i a, v4i b, v4f c) {
-    if constexpr (DT == I8F_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
-}
 
 // column n of an adapter's tiles: its layer, and the tile within the layer
 struct Tiles {
@@ -58,14 +50,14 @@ constexpr int ROWS = 64, BK = 64;   // rows of a workgroup, columns of a K-tile
 
 template <int DT, int RT, int STAGES>
 __global__ __launch_bounds__(256) void adapters_partial_kernel(const char *__restrict__ x, int M, int K, int ldx_bytes, float *__restrict__ partial, int slices,
-                                                               int per_slice, const DownLayers g) {
+                                                               int per_slice, int parts, const DownLayers g) {
     constexpr int STAGE = (ROWS + 16 * RT) * 128, XL = 2, AL = RT / 2, LOADS = XL + AL;   // bytes of a stage; loads of a wave for a K-tile
     static_assert(RT % 2 == 0 && STAGE * STAGES <= 80 * 1024, "two workgroups to a CU");
     __shared__ __attribute__((aligned(1024))) char smem[STAGE * STAGES];
     const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lq = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // (the slices of a block of rows are neighbours in the launch; with eight of them an XCD has the same slice of the factors for all rows)
-    const int block = blockIdx.x / slices, slice = blockIdx.x % slices, m0 = block * ROWS;
+    const int slice = blockIdx.x % slices, part = blockIdx.x / slices % parts, block = blockIdx.x / slices / parts, m0 = block * ROWS;
     const int kt_first = slice * per_slice, KT = min(per_slice, (K + BK - 1) / BK - kt_first);
     const uint32_t OOB = 0x7ffffff0u, smem_base = (uint32_t)(uintptr_t)smem;
     int64_t most = 0;
@@ -106,9 +98,14 @@ __global__ __launch_bounds__(256) void adapters_partial_kernel(const char *__res
         v4i ra[AL];   // (tiles past the adapter's last one are empty buffers: they load zeros)
     };
     Pass now, next;
+    int number = parts - part;   // passes are dealt over the parts in turn: this workgroup takes the next one at `parts`
     auto advance = [&](Pass &p) __attribute__((always_inline)) {   // (a -1 behind the last)
         p.t0 += RT;
-        while (p.t0 >= p.tl.all) {
+        while (p.t0 >= p.tl.all || number != parts) {
+            if (p.t0 < p.tl.all) {   // another workgroup's
+                p.t0 += RT, ++number;
+                continue;
+            }
             p.a = -1;
             if (!left) return;
             const int row = __builtin_ctzll(left);
@@ -121,6 +118,7 @@ __global__ __launch_bounds__(256) void adapters_partial_kernel(const char *__res
                 p.tl.until[l] = p.tl.all += __builtin_amdgcn_readlane(tiles_in[l], row);
             }
         }
+        number = 1;
 #pragma unroll
         for (int t = 0; t < AL; ++t) {
             const int n = p.t0 + 2 * t + (wave >> 1);
@@ -173,7 +171,7 @@ __global__ __launch_bounds__(256) void adapters_partial_kernel(const char *__res
 #pragma unroll
                 for (int j = 0; j < RT; ++j) {
                     const int arow = ROWS + 16 * j + l16;
-                    acc[j] = down_mfma<DT>(*(const v4i *)(st + arow * 128 + ((4 * h + lq) ^ swz<8>(arow)) * 16), xf, acc[j]);
+                    acc[j] = factor_mfma<DT>(*(const v4i *)(st + arow * 128 + ((4 * h + lq) ^ swz<8>(arow)) * 16), xf, acc[j]);
                 }
             }
         }
@@ -229,10 +227,13 @@ __global__ __launch_bounds__(256) void copy_rows_kernel(const uint16_t *__restri
 
 template <int DT>
 int launch(const char *x, int M, int K, int ldx_bytes, const DownLayers &g, float *partial, int slices, hipStream_t st) {
-    const int per = ((K + BK - 1) / BK + slices - 1) / slices;
-    const dim3 grid((unsigned)((M + ROWS - 1) / ROWS) * slices);
-    const int ranks = g.first_column[g.n];
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, x, M, K, ldx_bytes, partial, slices, per, g); };
+    const int per = ((K + BK - 1) / BK + slices - 1) / slices, ranks = g.first_column[g.n];
+    // where the rows' slices leave CUs idle, the passes of a block of rows are dealt over workgroups too (471 x 2080, 29 requests with three
+    // layers of rank 68: 52 us in one, 19 in eight); those without a pass end at once
+    const unsigned units = (unsigned)((M + ROWS - 1) / ROWS) * slices;
+    const int parts = units >= 512 ? 1 : units <= 64 ? 8 : (int)(512 / units);
+    const dim3 grid(units * parts);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, x, M, K, ldx_bytes, partial, slices, per, parts, g); };
     if (ranks <= 32) go(adapters_partial_kernel<DT, 2, 5>);
     else if (ranks <= 64) go(adapters_partial_kernel<DT, 4, 5>);
     else if (ranks <= 96) go(adapters_partial_kernel<DT, 6, 4>);

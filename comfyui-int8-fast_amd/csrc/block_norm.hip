@@ -29,7 +29,7 @@ __device__ __forceinline__ float norm_operand(const void *p, int dtype, int64_t 
     return DT == I8F_F32 || dtype == I8F_F32 ? ((const float *)p)[k] : load_as_f32<DT>(p, k);
 }
 
-// ---- rows of less than a run, or too wide for registers (more than 1024 runs): 256 threads to a row, which is read again for every statistic
+// ---- rows of less than a run, or too wide for registers (more than 16384 elements): 256 threads to a row, which is read again for every statistic
 // (from cache) ----------------
 template <int DT, int H>
 __global__ __launch_bounds__(256) void block_norm_generic_kernel(const i8f_block_norm_args a) {
@@ -388,14 +388,19 @@ int launch_width(const i8f_block_norm_args &a, int64_t runs, hipStream_t st) {
     if (runs <= 256) return launch_rows<DT, H, 4, 1, ANY>(a, st);
     if (runs <= 512) return launch_rows<DT, H, 4, 2, ANY>(a, st);
     if (runs <= 768) return launch_rows<DT, H, 4, 3, ANY>(a, st);
-    return launch_rows<DT, H, 4, 4, ANY>(a, st);
+    if (DT != I8F_F32 || runs <= 1024) return launch_rows<DT, H, 4, 4, ANY>(a, st);
+    if constexpr (DT == I8F_F32) {   // (runs of four elements: as many registers as half of that in 16 bits)
+        if (runs <= 1536) return launch_rows<DT, H, 4, 6, ANY>(a, st);
+        if (runs <= 2048) return launch_rows<DT, H, 4, 8, ANY>(a, st);
+    }
+    return launch_rows<DT, H, 4, DT == I8F_F32 ? 16 : 4, ANY>(a, st);
 }
 
 template <int DT, int H>
 int launch(const i8f_block_norm_args &a, hipStream_t st) {
     constexpr int N = Run<DT>::N;
     const int64_t runs = (a.K + N - 1) / N;
-    if (runs <= 1024 && a.K >= N) return whole_runs(a, N) ? launch_width<DT, H, false>(a, runs, st) : launch_width<DT, H, true>(a, runs, st);
+    if (runs <= (DT == I8F_F32 ? 4096 : 1024) && a.K >= N) return whole_runs(a, N) ? launch_width<DT, H, false>(a, runs, st) : launch_width<DT, H, true>(a, runs, st);
     hipLaunchKernelGGL((block_norm_generic_kernel<DT, H>), dim3((unsigned)a.M), dim3(256), 0, st, a);
     return check_launch();
 }

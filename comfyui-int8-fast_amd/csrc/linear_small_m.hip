@@ -40,14 +40,11 @@ struct WithAdapters {
     i8f_adapters ad;
     const void *t;
 };
-// the adapters' share of out[m,n]
-template <int DT, class AD>
-__device__ __forceinline__ float adapted(float v, const AD &ad, int64_t m, int64_t n, int64_t N) {
-    if constexpr (std::is_same<AD, WithAdapters>::value) {
-        const int a = adapter_of(ad.ad, m);
-        if (a >= 0) v += adapter_term<DT>(ad.ad, ad.t, m, n, N, a);
-    }
-    return v;
+// the adapters' share of out[m,n], or the part of it from ranks 8 k on, every 8 of `of` eights
+template <int DT>
+__device__ __forceinline__ float share(const WithAdapters &ad, int64_t m, int64_t n, int64_t N, int k = 0, int of = 1) {
+    const int a = adapter_of(ad.ad, m);
+    return a >= 0 ? adapter_term<DT>(ad.ad, ad.t, m, n, N, a, k, of) : 0.0f;
 }
 
 __device__ __forceinline__ float wave_sum(float v) {
@@ -97,6 +94,14 @@ __global__ __launch_bounds__(256) void small_m_kernel(const SmallMArgs a, const 
     float acc[16];
 #pragma unroll
     for (int m = 0; m < 16; ++m) acc[m] = 0.0f;
+    // the adapters' share of row lane / 4, four lanes to it (15 x 915 -> 2181 with ranks up to 51: 34 us, row after row by one lane 47)
+    constexpr bool ADAPTED = std::is_same<AD, WithAdapters>::value;
+    [[maybe_unused]] float side = 0.0f;
+    if constexpr (ADAPTED) {
+        if (lane / 4 < M) side = share<DT>(ad, lane / 4, n, a.N, lane % 4, 4);
+        side += __shfl_xor(side, 1);
+        side += __shfl_xor(side, 2);
+    }
 
     if constexpr (VEC) {
         for (int64_t k0 = (int64_t)lane * 16; k0 < a.K; k0 += 1024) {
@@ -137,8 +142,9 @@ __global__ __launch_bounds__(256) void small_m_kernel(const SmallMArgs a, const 
 #pragma unroll
     for (int m = 0; m < 16; ++m) {
         if (m < M) {
-            const float s = wave_sum(acc[m]);
-            if (lane == 0) store_from_f32<DT>(a.out, (int64_t)m * a.N + n, adapted<DT>(s + b, ad, m, n, a.N));
+            float s = wave_sum(acc[m]) + b;
+            if constexpr (ADAPTED) s += __shfl(side, 4 * m);
+            if (lane == 0) store_from_f32<DT>(a.out, (int64_t)m * a.N + n, s);
         }
     }
 }
@@ -306,7 +312,7 @@ __device__ __forceinline__ void small_m_lds_body(const SmallMArgs &a, const int6
         for (int i = 0; i < (COLS * 16 + WAVES * 64 - 1) / (WAVES * 64); ++i) {
             const int o = threadIdx.x + i * WAVES * 64, m = o / COLS;
             const int64_t n = n0 + o % COLS;
-            side[i] = o < COLS * 16 && m < (int)a.M && n < a.N ? adapted<DT>(0.0f, ad, m, n, a.N) : 0.0f;
+            side[i] = o < COLS * 16 && m < (int)a.M && n < a.N ? share<DT>(ad, m, n, a.N) : 0.0f;
         }
     }
     for (; t < nsteps; t += 2 * WAVES) {

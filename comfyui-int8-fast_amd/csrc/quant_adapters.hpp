@@ -202,7 +202,7 @@ __global__ __launch_bounds__(256) void adapters_side_kernel(const DownLayers g) 
         }
 #pragma unroll
         for (int b = 0; b < 16; ++b) {
-            const v4f d = lora_mfma<DT>(bv[b], tv, (v4f)0.0f);
+            const v4f d = factor_mfma<DT>(bv[b], tv, (v4f)0.0f);
 #pragma unroll
             for (int e = 0; e < 4; ++e) keep[e] = l16 == b ? keep[e] + d[e] : keep[e];
         }
