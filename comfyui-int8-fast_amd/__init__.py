@@ -4,11 +4,13 @@ The package replaces the W8A8 linear hot path of ComfyUI-INT8-Fast:
 
     int8_fused_kernel   quantise + GEMM + dequant pipeline   (HIP, was Triton)
     int8_quant          quantisation helpers, Int8TensorwiseOps, INT8 LoRA adapters
+    adapters            low-rank adapters of many requests beside shared projections
+    block_norms         norms, gate and residual stream between two blocks in one pass
     quarot              128-block Hadamard rotation
     compile_ops         torch.library operators (namespace i8f) for torch.compile
     nodes               ComfyUI graph nodes (model loader, LoRA loaders); ComfyUI is imported when they run
     dynamic_lora        hook for un-merged LoRA side branches
-    _lib                ctypes binding of libi8f_gfx950.so (include/i8f.h)
+    _lib                ctypes binding of libi8f_gfx950.so (include/i8f.h, include/i8f_blocks.h)
     build               build of the library (hipcc) and of the host extension (g++)
 
 The directory name is ComfyUI's convention for custom nodes and is not a Python

@@ -300,6 +300,9 @@ struct AdapterArgs {
 // over all the wave's columns, and the other rows keep what they had (a select per lane: a lane's values belong to one row, and
 // a column of the product depends on its own row of t alone; zeros in t instead would let an adapter that is not finite into every
 // row).  What counts there is the trip to memory for each adapter's factor, so the loads run RING products ahead.
+// us with the operands in place: 9216 x 3840 -> 15360, rank 128: 485 without adapters, 520 for one of them, 523 for eight ragged requests;
+// 4096 x 3840 -> 3 x 3840, rank 32: 147, 153, 158; 512 x 4096 -> 4096, rank 32: 17, 23, 23, and 47 where every row has another one.  Twelve
+// waves spill 30 to 40 registers here (4608 x 2560 -> 12288: 125, 137 to 147).
 template <class C, int OUT, class ACC, class ACC16>
 __device__ __forceinline__ void adapters_epilogue(const AdapterArgs &g, const int gM, const int gN, const int m0, const int n0, const int wm, const int wn,
                                                   const int lane, const float *s_xs, const float *s_ws, const float *s_bias, char *ebuf, ACC &acc,
