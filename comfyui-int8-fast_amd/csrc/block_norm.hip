@@ -428,6 +428,9 @@ int validate(const i8f_block_norm_args &a) {
     if (a.M == 0 || a.K == 0) return I8F_OK;   // (an empty tensor's outputs may be NULL)
     if (!a.h && !a.q && (a.pre_norm != I8F_NORM_NONE || a.mod_scale || a.mod_shift)) return I8F_ERR_INVALID;
     if (!a.y || !a.residual || !a.x_out || a.ldy < a.K || a.ldr < a.K) return I8F_ERR_INVALID;
+    for (const void *in : {a.y, a.residual})
+        if (a.x_out == in || a.h == in || (const void *)a.q == in) return I8F_ERR_INVALID;   // (a row is written while other waves read it)
+    if (a.x_out == a.h || a.x_out == (void *)a.q) return I8F_ERR_INVALID;
     return a.M > 0x7fffffff || a.K > 0x7fffffff ? I8F_ERR_UNSUPPORTED : I8F_OK;
 }
 

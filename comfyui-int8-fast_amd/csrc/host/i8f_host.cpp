@@ -666,7 +666,7 @@ PyObject *block_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
     i8f_block_norm_args g = {};
     const Stream st(y.device());
     if (!st.ok || dt < 0 || wants_gradient(yt) || wants_gradient(rt) || r.scalar_type() != y.scalar_type() || r.device() != y.device() || r.sizes() != y.sizes() ||
-        !rows_of(y, M, K, g.ldy) || !rows_of(r, Mr, Kr, g.ldr))
+        !rows_of(y, M, K, g.ldy) || !rows_of(r, Mr, Kr, g.ldr) || K < 1)
         Py_RETURN_NONE;
     g.rows_per_gate = g.rows_per_scale = g.rows_per_shift = 1;
     if (!block_norm_of(y, a + 2, &g.post_norm, &g.post_weight, &g.post_bias, &g.post_dtype, &g.post_eps) ||

@@ -108,7 +108,7 @@ int i8f_linear_w8a16_small_m_adapters(const void *x, int x_dtype, int64_t M, int
  *            given).  At most one of h and q.  pre_norm must be I8F_NORM_NONE, and the modulation absent, where both are NULL.
  *   weights and biases [K] of dtype or I8F_F32 (post_dtype, pre_dtype), each NULL when absent; an I8F_NORM_NONE has neither
  *   gate, mod_scale, mod_shift   [ceil(M / rows_per_...), K] of dtype or NULL; row m uses vector m / rows_per_...
- * x_out and h may not overlap the inputs.
+ * The outputs may overlap neither the inputs nor one another.
  */
 typedef enum i8f_norm { I8F_NORM_NONE = 0, I8F_NORM_RMS = 1, I8F_NORM_LAYER = 2 } i8f_norm;
 typedef struct i8f_block_norm_args {

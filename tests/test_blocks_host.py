@@ -99,7 +99,7 @@ def test_adapters_arguments_are_checked_before_any_launch(L):
 
 def _norm(L, **over):
     a = L._BlockNormArgs()
-    base = {"y": 16, "residual": 16, "M": 4, "K": 128, "ldy": 128, "ldr": 128, "dtype": L.BF16, "x_out": 16, "rows_per_gate": 1, "rows_per_scale": 1,
+    base = {"y": 16, "residual": 16, "M": 4, "K": 128, "ldy": 128, "ldr": 128, "dtype": L.BF16, "x_out": 32, "rows_per_gate": 1, "rows_per_scale": 1,
             "rows_per_shift": 1, "residual_scale": 1.0, "branch_scale": 1.0, "post_eps": 1e-6, "pre_eps": 1e-6}
     for k, v in {**base, **over}.items():
         setattr(a, k, v)
@@ -108,13 +108,15 @@ def _norm(L, **over):
 
 def test_block_norm_arguments_are_checked_before_any_launch(L):
     assert L.lib().i8f_block_norm(None, None) == INVALID
-    q = {"q": 16, "scale": 16}
-    for bad in ({"M": -1}, {"K": -1}, {"dtype": 5}, {"y": None}, {"residual": None}, {"x_out": None}, {"ldy": 64}, {"ldr": 64}, {"post_norm": 3}, {"pre_norm": -1, "h": 16},
-                {"post_norm": 1, "post_eps": -1.0}, {"post_norm": 1, "post_eps": float("nan")}, {"post_weight": 16}, {"pre_bias": 16, "h": 16},
-                {"post_norm": 1, "post_weight": 16, "post_dtype": L.F16}, {"gate": 16, "rows_per_gate": 0}, {"mod_scale": 16, "rows_per_scale": 0, "h": 16},
-                {"mod_shift": 16, "rows_per_shift": -1, "h": 16}, {"pre_norm": 1}, {"mod_scale": 16}, {"h": 16, **q}, {"q": 16}, {"scale": 16}, {"rotate_block": 128},
+    q = {"q": 64, "scale": 16}
+    for bad in ({"M": -1}, {"K": -1}, {"dtype": 5}, {"y": None}, {"residual": None}, {"x_out": None}, {"ldy": 64}, {"ldr": 64}, {"post_norm": 3}, {"pre_norm": -1, "h": 48},
+                {"post_norm": 1, "post_eps": -1.0}, {"post_norm": 1, "post_eps": float("nan")}, {"post_weight": 16}, {"pre_bias": 16, "h": 48},
+                {"post_norm": 1, "post_weight": 16, "post_dtype": L.F16}, {"gate": 16, "rows_per_gate": 0}, {"mod_scale": 16, "rows_per_scale": 0, "h": 48},
+                {"mod_shift": 16, "rows_per_shift": -1, "h": 48}, {"pre_norm": 1}, {"mod_scale": 16}, {"h": 48, **q}, {"q": 64}, {"scale": 16}, {"rotate_block": 128},
                 {"rotate_block": 128, "K": 100, **q}):
         assert _norm(L, **bad) == INVALID, bad
+    for alias in ({"x_out": 16}, {"h": 16}, {"h": 32}, {"q": 16, "scale": 96}, {"q": 32, "scale": 96}):
+        assert _norm(L, **alias) == INVALID, alias
     assert _norm(L, rotate_block=64, **q) == UNSUPPORTED
     assert _norm(L, M=1 << 31, ldy=128) == UNSUPPORTED
     assert _norm(L, M=0, y=None, residual=None, x_out=None) == 0
