@@ -40,12 +40,6 @@ struct WithAdapters {
     i8f_adapters ad;
     const void *t;
 };
-// the adapters' share of out[m,n], or the part of it from ranks 8 k on, every 8 of `of` eights
-template <int DT>
-__device__ __forceinline__ float share(const WithAdapters &ad, int64_t m, int64_t n, int64_t N, int k = 0, int of = 1) {
-    const int a = adapter_of(ad.ad, m);
-    return a >= 0 ? adapter_term<DT>(ad.ad, ad.t, m, n, N, a, k, of) : 0.0f;
-}
 
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
@@ -98,7 +92,8 @@ __global__ __launch_bounds__(256) void small_m_kernel(const SmallMArgs a, const 
     constexpr bool ADAPTED = std::is_same<AD, WithAdapters>::value;
     [[maybe_unused]] float side = 0.0f;
     if constexpr (ADAPTED) {
-        if (lane / 4 < M) side = share<DT>(ad, lane / 4, n, a.N, lane % 4, 4);
+        const int own = lane / 4 < M ? adapter_of(ad.ad, lane / 4) : -1;
+        if (own >= 0) side = adapter_term<DT>(ad.ad, ad.t, lane / 4, n, a.N, own, lane % 4, 4);
         side += __shfl_xor(side, 1);
         side += __shfl_xor(side, 2);
     }
@@ -302,21 +297,31 @@ __device__ __forceinline__ void small_m_lds_body(const SmallMArgs &a, const int6
             for (int j = 0; j < 4; ++j) acc[b] = mma8<DT>(wa[b][j].x, wa[b][j].y, xk[j], wsn[b], acc[b]);
     };
 
-    int t = wave;
-    if (t < nsteps) fetch(t, 0);
-    // (the adapters' share of this thread's outputs, a chain of four dependent loads, while the first weights are on their way)
+    // The adapters' share of this thread's outputs, a chain of dependent loads, while the first weights are on their way: the adapter's number
+    // is asked for ahead of them (loads return in order), the rest behind those of two steps.
     constexpr bool ADAPTED = std::is_same<AD, WithAdapters>::value;
-    [[maybe_unused]] float side[(COLS * 16 + WAVES * 64 - 1) / (WAVES * 64)];
+    constexpr int OWN = (COLS * 16 + WAVES * 64 - 1) / (WAVES * 64);
+    [[maybe_unused]] float side[OWN];
+    [[maybe_unused]] int own[OWN];
     if constexpr (ADAPTED) {
 #pragma unroll
-        for (int i = 0; i < (COLS * 16 + WAVES * 64 - 1) / (WAVES * 64); ++i) {
+        for (int i = 0; i < OWN; ++i) {
             const int o = threadIdx.x + i * WAVES * 64, m = o / COLS;
-            const int64_t n = n0 + o % COLS;
-            side[i] = o < COLS * 16 && m < (int)a.M && n < a.N ? share<DT>(ad, m, n, a.N) : 0.0f;
+            own[i] = o < COLS * 16 && m < (int)a.M && n0 + o % COLS < a.N ? adapter_of(ad.ad, m) : -1;
+        }
+    }
+    int t = wave;
+    if (t < nsteps) fetch(t, 0);
+    if constexpr (ADAPTED) {
+        if (t + WAVES < nsteps) fetch(t + WAVES, 1);
+#pragma unroll
+        for (int i = 0; i < OWN; ++i) {
+            const int o = threadIdx.x + i * WAVES * 64;
+            side[i] = own[i] >= 0 ? adapter_term<DT>(ad.ad, ad.t, o / COLS, n0 + o % COLS, a.N, own[i]) : 0.0f;
         }
     }
     for (; t < nsteps; t += 2 * WAVES) {
-        if (t + WAVES < nsteps) fetch(t + WAVES, 1);
+        if (t + WAVES < nsteps && (!ADAPTED || t > wave)) fetch(t + WAVES, 1);
         compute(0);
         if (t + WAVES < nsteps) {
             if (t + 2 * WAVES < nsteps) fetch(t + 2 * WAVES, 0);
