@@ -20,11 +20,11 @@ __device__ __forceinline__ float dot8(v4u a, v4u b, float sum) {
     return sum;
 }
 
-// ---- few rows: every rank of every row is a wave of its own, with 16-byte loads, eight of each operand under way at once; what counts is
+// ---- few rows: every rank of every row (or two of them) is a wave of its own, with 16-byte loads, eight of each operand under way at once; what counts is
 // the one trip to memory.  The first quant_blocks workgroups quantise a row of x each (RUNS > 0).
 // ANY: x of any width and alignment (a row's last eight elements, where it has fewer of them, are fetched one by one; the factors' rows
 // are padded).
-template <int DT, bool ROT, int RUNS, bool ANY>
+template <int DT, bool ROT, int RUNS, bool ANY, int PER>
 __global__ __launch_bounds__(256) void adapters_rows_kernel(const char *__restrict__ x, int64_t M, int K, int64_t ldx, int8_t *__restrict__ q,
                                                             float *__restrict__ scale, int quant_blocks, const DownLayers g) {
     if constexpr (RUNS > 0) {
@@ -41,17 +41,17 @@ __global__ __launch_bounds__(256) void adapters_rows_kernel(const char *__restri
         if (i < g.n && block >= g.first_block[i]) l = i;
     l = __builtin_amdgcn_readfirstlane(l);
     const i8f_adapters &ad = g.ad[l];
-    const uint32_t quads = (uint32_t)ad.max_rank / 4, at = (uint32_t)(block - g.first_block[l]);   // a workgroup takes four ranks of a row
-    const int64_t m = at / quads;
-    const int lane = threadIdx.x & 63, j = (int)(at % quads) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t groups = (uint32_t)ad.max_rank / (4 * PER), at = (uint32_t)(block - g.first_block[l]);   // a workgroup takes 4 PER ranks of a row
+    const int64_t m = at / groups;
+    const int lane = threadIdx.x & 63, j = ((int)(at % groups) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * PER;
     const int a = __builtin_amdgcn_readfirstlane(adapter_of(ad, m));
     if (a < 0) return;
     const int first = ad.first_rank[a];
     if (j >= ad.first_rank[a + 1] - first) return;
     const char *xp = x + m * ldx * 2, *ap = (const char *)ad.down + (int64_t)(first + j) * factor_width(K) * 2;
-    float sum = 0.0f;
+    float sum[PER] = {};
     for (int k0 = lane * 8; k0 < K; k0 += 8 * 512) {
-        v4u xv[8], av[8];
+        v4u xv[8], av[PER][8];
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
             const int k = k0 + c * 512;
@@ -61,7 +61,8 @@ __global__ __launch_bounds__(256) void adapters_rows_kernel(const char *__restri
             } else {
                 xv[c] = k < K ? *(const v4u *)(xp + (int64_t)k * 2) : (v4u)0u;
             }
-            av[c] = k < K ? *(const v4u *)(ap + (int64_t)k * 2) : (v4u)0u;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) av[i][c] = k < K ? *(const v4u *)(ap + (i * factor_width(K) + k) * 2) : (v4u)0u;
         }
         if constexpr (ANY) {
             const int c = (K - k0) / 512, k = k0 + c * 512;   // the piece that holds the row's end, if it is this lane's
@@ -74,10 +75,16 @@ __global__ __launch_bounds__(256) void adapters_rows_kernel(const char *__restri
             }
         }
 #pragma unroll
-        for (int c = 0; c < 8; ++c) sum = dot8<DT>(xv[c], av[c], sum);
+        for (int c = 0; c < 8; ++c)
+#pragma unroll
+            for (int i = 0; i < PER; ++i) sum[i] = dot8<DT>(xv[c], av[i][c], sum[i]);
     }
-    sum = wave_sum_all(sum);
-    if (lane == 0) store_from_f32<DT>(g.t[l], m * ad.max_rank + j, sum * ad.scale[a]);
+    const float s = ad.scale[a];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        sum[i] = wave_sum_all(sum[i]);
+        if (lane == 0) store_from_f32<DT>(g.t[l], m * ad.max_rank + j + i, sum[i] * s);
+    }
 }
 
 // ---- many rows, the sums of the slices of K (adapters_down.hip): t = scale_a (the slices' sums, in order), rounded: four ranks of a row to a thread
@@ -150,23 +157,32 @@ int pick_combine(const float *partial, int64_t M, int slices, const void *x, int
 // again for each, so that beyond it rows share the factors (adapters_down.hip), which costs a pass for every adapter that occurs among 64
 // rows.  K = 4096 with the quantiser, us, rows of one adapter, of eight requests and of 32 in turn:
 //     rows x ranks   128 x 16   4.3   4.3   4.3 by waves,  11   16   60 by tiles       512 x 16    7.7   7.8   7.8 and  12   12   61
-//                    128 x 128 12.6  12.6  14.5            14   27  147               1024 x 16   14    14    14        12   12   62
-//                    256 x 128  23    22    25             15   19  146                512 x 128  42    41    46        15   15  146
+//                    128 x 128 11.5  11.4  14.1            14   27  147               1024 x 16   12    13    12        12   12   62
+//                    256 x 128  20    20    24             15   19  146                512 x 128  42    41    46        17   17   61
+// (the tiles' figures but the last ones are of passes that one workgroup took; dealt over idle ones they cost about half where they are many)
 inline bool down_by_rows(int64_t M, int64_t K, int64_t ranks) {
     return M <= 128 || (M <= 256 && M * ranks <= 1 << 15) || (M < (1 << 14) && M * ranks <= 1 << 14) || K >= (1 << 23);   // (32-bit offsets within 64 rows)
 }
 
-template <int DT, bool ROT, int RUNS, bool ANY = false>
-int launch_rows_form(const void *x, int64_t M, int64_t K, int64_t ldx, int8_t *q, float *scale, DownLayers &g, hipStream_t st) {
+template <int DT, bool ROT, int RUNS, bool ANY, int PER>
+int launch_rows_of(const void *x, int64_t M, int64_t K, int64_t ldx, int8_t *q, float *scale, DownLayers &g, hipStream_t st) {
     const int64_t quant_blocks = RUNS > 0 ? M : 0;
     int64_t first = 0;
-    for (int i = 0; i < g.n; ++i) g.first_block[i] = (int)first, first += M * (g.ad[i].max_rank / 4);
+    for (int i = 0; i < g.n; ++i) g.first_block[i] = (int)first, first += M * (g.ad[i].max_rank / (4 * PER));
     for (int i = g.n; i <= I8F_MAX_ADAPTED_LAYERS; ++i) g.first_block[i] = (int)first;
     if (quant_blocks + first == 0) return I8F_OK;
     if (quant_blocks + first > 0x7fffffff) return I8F_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((adapters_rows_kernel<DT, ROT, RUNS, ANY>), dim3((unsigned)(quant_blocks + first)), dim3(256), 0, st, (const char *)x, M, (int)K, ldx, q, scale,
+    hipLaunchKernelGGL((adapters_rows_kernel<DT, ROT, RUNS, ANY, PER>), dim3((unsigned)(quant_blocks + first)), dim3(256), 0, st, (const char *)x, M, (int)K, ldx, q, scale,
                        (int)quant_blocks, g);
     return check_launch();
+}
+
+template <int DT, bool ROT, int RUNS, bool ANY = false>
+int launch_rows_form(const void *x, int64_t M, int64_t K, int64_t ldx, int8_t *q, float *scale, DownLayers &g, hipStream_t st) {
+    // two ranks to a wave, which share the row of x, where there are waves enough: K = 4096, 128 x 128 12.6 and 11.5 us, 1024 x 16 14.2 and 12.0;
+    // 128 x 16 4.3 and 4.7
+    return M * g.first_column[g.n] >= 1 << 14 ? launch_rows_of<DT, ROT, RUNS, ANY, 2>(x, M, K, ldx, q, scale, g, st)
+                                           : launch_rows_of<DT, ROT, RUNS, ANY, 1>(x, M, K, ldx, q, scale, g, st);
 }
 
 // ---- few rows with a side each: then their share of the result, B_a t, by a launch of its own that fills the chip, where the tiles of the
