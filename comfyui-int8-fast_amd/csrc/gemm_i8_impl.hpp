@@ -304,7 +304,7 @@ struct AdapterArgs {
 // 4096 x 3840 -> 3 x 3840, rank 32: 147, 153, 158; 512 x 4096 -> 4096, rank 32: 17, 23, 23, and 47 where every row has another one.  Twelve
 // waves spill 30 to 40 registers here (4608 x 2560 -> 12288: 125, 137 to 147).
 template <class C, int OUT, class ACC, class ACC16>
-__device__ __forceinline__ void adapters_epilogue(const AdapterArgs &g, const int gM, const int gN, const int m0, const int n0, const int wm, const int wn,
+__device__ __forceinline__ void adapters_epilogue(const AdapterArgs &g, const int (&ids)[(C::WTM + 63) / 64], const int gM, const int gN, const int m0, const int n0, const int wm, const int wn,
                                                   const int lane, const float *s_xs, const float *s_ws, const float *s_bias, char *ebuf, ACC &acc,
                                                   ACC16 &acc16, void *gout) {
     static_assert(OUT == OUT_BF16 || OUT == OUT_F16, "16-bit factors");
@@ -384,7 +384,7 @@ __device__ __forceinline__ void adapters_epilogue(const AdapterArgs &g, const in
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i) {
         const int m = mw + i * GR + lrow;
-        const int a = g.ids[(uint32_t)min(m, gM - 1) / (uint32_t)g.rows_per_id];
+        const int a = __shfl(ids[i * GR / 64], i * GR % 64 + lrow);
         id[i] = m < gM && (uint32_t)a < (uint32_t)g.count ? a : -1;
     }
 #pragma unroll
@@ -913,6 +913,13 @@ __device__ __forceinline__ void gemm_i8_body(const int8_t *gx, const int8_t *gw,
         }
     };
     if constexpr (SIDE_EARLY) side_fetch(tid);
+    // the adapters' numbers of the wave's rows, a row to a lane
+    constexpr int IDS_PER = (C::WTM + 63) / 64;
+    [[maybe_unused]] int ids_r[IDS_PER];
+    if constexpr (ADAPT) {
+#pragma unroll
+        for (int u = 0; u < IDS_PER; ++u) ids_r[u] = adapters->ids[(uint32_t)min(m0 + wm * C::WTM + u * 64 + lane, gM - 1) / (uint32_t)adapters->rows_per_id];
+    }
 
     __builtin_amdgcn_s_waitcnt(waitcnt_vm(SPREAD_DMA ? (PRE - 1) * C::LOADS : (ASYM ? C::LOADS : cut(1))));  // younger tiles may be in flight
     __builtin_amdgcn_s_barrier();  // tile 0 is in LDS for everyone (no fence: nothing else has been written)
@@ -1415,7 +1422,7 @@ __device__ __forceinline__ void gemm_i8_body(const int8_t *gx, const int8_t *gw,
     if constexpr (OUT == OUT_I32) {
         run_epilogue(O0{}, F_{}, F_{}, S0{}, F_{});  // (the raw product: no gate and no addend)
     } else if constexpr (ADAPT) {
-        adapters_epilogue<C, OUT>(*adapters, gM, gN, m0, n0, wm, wn, lane, s_xs, s_ws, s_bias, ebuf, acc, acc16, gout);
+        adapters_epilogue<C, OUT>(*adapters, ids_r, gM, gN, m0, n0, wm, wn, lane, s_xs, s_ws, s_bias, ebuf, acc, acc16, gout);
     } else if constexpr (SIDE) {  // (no gate and no addend beside a side branch)
         if (g.side_rank > 32) choose(std::integral_constant<int, 4>{});
         else choose(std::integral_constant<int, 2>{});
