@@ -300,11 +300,13 @@ struct AdapterArgs {
 // over all the wave's columns, and the other rows keep what they had (a select per lane: a lane's values belong to one row, and
 // a column of the product depends on its own row of t alone; zeros in t instead would let an adapter that is not finite into every
 // row).  What counts there is the trip to memory for each adapter's factor, so the loads run RING products ahead.
-// us with the operands in place: 9216 x 3840 -> 15360, rank 128: 485 without adapters, 520 for one of them, 523 for eight ragged requests;
-// 4096 x 3840 -> 3 x 3840, rank 32: 147, 153, 158; 512 x 4096 -> 4096, rank 32: 17, 23, 23, and 47 where every row has another one.  Twelve
-// waves spill 30 to 40 registers here (4608 x 2560 -> 12288: 125, 137 to 147).
+// The rows' numbers and where their factors are have been requested behind the first tiles of the main loop, a row to a lane.
+// us with the operands in place: 9216 x 3840 -> 15360, rank 128: 484 without adapters, 500 for one of them, 503 for eight ragged requests;
+// 4096 x 3840 -> 3 x 3840, rank 32: 141, 146, 151; 512 x 4096 -> 4096, rank 32: 16, 19, 21, and 44 where every row has another one.  Twelve
+// waves spill some 30 registers here (4608 x 2560 -> 12288: 123, 131 to 143).
 template <class C, int OUT, class ACC, class ACC16>
-__device__ __forceinline__ void adapters_epilogue(const AdapterArgs &g, const int (&ids)[(C::WTM + 63) / 64], const int gM, const int gN, const int m0, const int n0, const int wm, const int wn,
+__device__ __forceinline__ void adapters_epilogue(const AdapterArgs &g, const int (&ids)[(C::WTM + 63) / 64], const int (&firsts)[(C::WTM + 63) / 64],
+                                                  const int (&ends)[(C::WTM + 63) / 64], const int gM, const int gN, const int m0, const int n0, const int wm, const int wn,
                                                   const int lane, const float *s_xs, const float *s_ws, const float *s_bias, char *ebuf, ACC &acc,
                                                   ACC16 &acc16, void *gout) {
     static_assert(OUT == OUT_BF16 || OUT == OUT_F16, "16-bit factors");
@@ -383,15 +385,9 @@ __device__ __forceinline__ void adapters_epilogue(const AdapterArgs &g, const in
     uint64_t with[GROUPS];
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i) {
-        const int m = mw + i * GR + lrow;
-        const int a = __shfl(ids[i * GR / 64], i * GR % 64 + lrow);
-        id[i] = m < gM && (uint32_t)a < (uint32_t)g.count ? a : -1;
-    }
-#pragma unroll
-    for (int i = 0; i < GROUPS; ++i) {
+        const int u = i * GR / 64, from = i * GR % 64 + lrow;
+        id[i] = __shfl(ids[u], from), first[i] = __shfl(firsts[u], from), rank[i] = __shfl(ends[u], from) - first[i];
         with[i] = __builtin_amdgcn_ballot_w64(id[i] >= 0);
-        first[i] = rank[i] = 0;
-        if (id[i] >= 0) first[i] = g.first_rank[id[i]], rank[i] = g.first_rank[id[i] + 1] - first[i];
     }
     int a0 = -1, first0 = 0, rank0 = 0;   // the first of them
 #pragma unroll
@@ -931,6 +927,16 @@ __device__ __forceinline__ void gemm_i8_body(const int8_t *gx, const int8_t *gw,
     // right away, and tile kt+1 is known to have landed, so its first fragments can be fetched.
     v4i xa[XF] = {}, wa[WF] = {}, xb[XF] = {}, wb[WF] = {};
     if (KT > 0) load_frags(smem, smem + C::W_BASE, 0, xa, wa);
+    // and where their factors are
+    [[maybe_unused]] int first_r[IDS_PER], rank_r[IDS_PER];
+    if constexpr (ADAPT) {
+#pragma unroll
+        for (int u = 0; u < IDS_PER; ++u) {
+            const bool has = m0 + wm * C::WTM + u * 64 + lane < gM && (uint32_t)ids_r[u] < (uint32_t)adapters->count;
+            ids_r[u] = has ? ids_r[u] : -1;
+            first_r[u] = has ? adapters->first_rank[ids_r[u]] : 0, rank_r[u] = has ? adapters->first_rank[ids_r[u] + 1] : 0;
+        }
+    }
     // Drain scalar loads (kernel arguments) here: a scalar load still pending at the loop header
     // would turn every LDS wait inside the loop into a full lgkmcnt(0).
     __builtin_amdgcn_s_waitcnt(0xC07F);
@@ -1422,7 +1428,7 @@ __device__ __forceinline__ void gemm_i8_body(const int8_t *gx, const int8_t *gw,
     if constexpr (OUT == OUT_I32) {
         run_epilogue(O0{}, F_{}, F_{}, S0{}, F_{});  // (the raw product: no gate and no addend)
     } else if constexpr (ADAPT) {
-        adapters_epilogue<C, OUT>(*adapters, ids_r, gM, gN, m0, n0, wm, wn, lane, s_xs, s_ws, s_bias, ebuf, acc, acc16, gout);
+        adapters_epilogue<C, OUT>(*adapters, ids_r, first_r, rank_r, gM, gN, m0, n0, wm, wn, lane, s_xs, s_ws, s_bias, ebuf, acc, acc16, gout);
     } else if constexpr (SIDE) {  // (no gate and no addend beside a side branch)
         if (g.side_rank > 32) choose(std::integral_constant<int, 4>{});
         else choose(std::integral_constant<int, 2>{});
