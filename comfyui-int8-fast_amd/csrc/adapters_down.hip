@@ -229,9 +229,9 @@ template <int DT>
 int launch(const char *x, int M, int K, int ldx_bytes, const DownLayers &g, float *partial, int slices, hipStream_t st) {
     const int per = ((K + BK - 1) / BK + slices - 1) / slices, ranks = g.first_column[g.n];
     // where the rows' slices leave CUs idle, the passes of a block of rows are dealt over workgroups too (471 x 2080, 29 requests with three
-    // layers of rank 68: 52 us in one, 19 in eight); those without a pass end at once
+    // layers of rank 68: 52 us in one, 19 in eight; 188 x 1141, 85 requests, rank 82: 43 in eight, 22 in 32); those without a pass end at once
     const unsigned units = (unsigned)((M + ROWS - 1) / ROWS) * slices;
-    const int parts = units >= 512 ? 1 : units <= 64 ? 8 : (int)(512 / units);
+    const int parts = units >= 512 ? 1 : units <= 16 ? 32 : (int)(512 / units);
     const dim3 grid(units * parts);
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, x, M, K, ldx_bytes, partial, slices, per, parts, g); };
     if (ranks <= 32) go(adapters_partial_kernel<DT, 2, 5>);
