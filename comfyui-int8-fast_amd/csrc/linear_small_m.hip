@@ -334,12 +334,10 @@ __device__ __forceinline__ void small_m_lds_body(const SmallMArgs &a, const int6
 #pragma unroll
         for (int i = 0; i < 4; ++i) red[wave][b * 16 + 4 * g + i][r] = acc[b][i];
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < (COLS * 16 + WAVES * 64 - 1) / (WAVES * 64); ++i) {
-        const int o = threadIdx.x + i * WAVES * 64;
+    auto finish = [&](int o, float share) __attribute__((always_inline)) {
         const int m = o / COLS, c = o % COLS;
         const int64_t n = n0 + c;
-        if (o < COLS * 16 && m < (int)a.M && n < a.N) {
+        if (m < (int)a.M && n < a.N) {
             float s = red[0][c][m];
 #pragma unroll
             for (int w = 1; w < WAVES; ++w) s += red[w][c][m];
@@ -351,9 +349,16 @@ __device__ __forceinline__ void small_m_lds_body(const SmallMArgs &a, const int6
                 bv = round_to_dtype<DT>(bv);
             }
             s = s + bv;
-            if constexpr (ADAPTED) s = s + side[i];
+            if constexpr (ADAPTED) s = s + share;
             store_from_f32<DT>(a.out, (int64_t)m * a.N + n, s);
         }
+    };
+    if constexpr (ADAPTED) {
+#pragma unroll
+        for (int i = 0; i < OWN; ++i)
+            if ((int)threadIdx.x + i * WAVES * 64 < COLS * 16) finish(threadIdx.x + i * WAVES * 64, side[i]);
+    } else {
+        for (int o = threadIdx.x; o < COLS * 16; o += WAVES * 64) finish(o, 0.0f);
     }
 }
 
