@@ -188,7 +188,8 @@ int launch_rows_form(const void *x, int64_t M, int64_t K, int64_t ldx, int8_t *q
 // ---- few rows with a side each: then their share of the result, B_a t, by a launch of its own that fills the chip, where the tiles of the
 // projection are too few to fetch as many different factors as there are rows.  A wave takes 256 columns of a row: the matrix unit's 16 x 16
 // x 32 form reads 16 rows of the factor in whole pieces, t stands in all columns of its other operand, and lane column b keeps block b's
-// result, so that a store is 1 KB in one piece.
+// result, so that a store is 1 KB in one piece.  64 rows x 6144 columns, ranks of 8 to 64: 12 us, 4 of them the factors' bytes, the rest the way
+// to a row's number, its factor and back.
 template <int DT>
 __global__ __launch_bounds__(256) void adapters_side_kernel(const DownLayers g) {
     int l = 0;

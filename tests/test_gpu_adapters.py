@@ -375,3 +375,41 @@ def test_a_single_row_without_other_dimensions(pkg, dev):
     y = pkg.forward_adapters(lin, x, pkg.AdapterBank(f), torch.tensor(0, dtype=torch.int32, device=dev))
     assert y.shape == (48,)
     check(y[None], *expected(pkg, lin, x[None], f, torch.zeros(1, dtype=torch.int32, device=dev)))
+
+
+@pytest.mark.parametrize("kind", ["tokens", "runs"])
+@pytest.mark.parametrize("rows,K,N", [(9, 250, 33), (64, 256, 192), (100, 200, 101), (700, 512, 200), (700, 515, 201), (1100, 512, 2304)])
+def test_not_finite_values_stay_in_their_rows_in_every_form(pkg, dev, rows, K, N, kind):
+    """By waves and by tiles, by way of a side tensor, of the epilogue and of the second product's own launch."""
+    lin = layer_of(pkg, K, N, torch.float16)
+    adapters = factors_of(K, N, (40, 20, 16, 33), torch.float16)
+    x = torch.randn(rows, K, device=dev).half()
+    ids = (torch.arange(rows, device=dev) % 5 - 1 if kind == "tokens" else (torch.arange(rows, device=dev) * 9 // rows) % 5 - 1).to(torch.int32)
+    want = pkg.forward_adapters(lin, x, pkg.AdapterBank(adapters), ids)
+    adapters[1][0][3, 5] = float("inf")
+    adapters[1][1][7] = float("nan")
+    x[rows // 2] = float("nan")
+    got = pkg.forward_adapters(lin, x, pkg.AdapterBank(adapters), ids)
+    fine = (ids != 1) & (torch.arange(rows, device=dev) != rows // 2)
+    assert torch.equal(got[fine], want[fine]) and torch.isfinite(want.float()).all()
+    assert not torch.isfinite(got[ids == 1][:, 7].float()).any()
+
+
+@pytest.mark.parametrize("rows,K,N,ranks", [(40, 200, 101, (16, 8)), (90, 512, 384, (64, 16)), (400, 1024, 384, (64, 16, 8)), (700, 1003, 96, (40, 16))])
+def test_captured_calls_of_the_other_forms(pkg, dev, rows, K, N, ranks):
+    lin, bank = layer_of(pkg, K, N, torch.bfloat16), pkg.AdapterBank(factors_of(K, N, ranks, torch.bfloat16))
+    x, ids = torch.randn(rows, K, device=dev).bfloat16(), torch.zeros(rows, dtype=torch.int32, device=dev)
+    pkg.forward_adapters(lin, x, bank, ids)
+    graphs, ys = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for g in graphs:
+        with torch.cuda.graph(g):
+            ys.append(pkg.forward_adapters(lin, x, bank, ids))
+    for i in range(4):
+        x.copy_(torch.randn(rows, K, device=dev))
+        ids.copy_(torch.randint(-1, len(ranks), (rows,), device=dev))
+        want = pkg.forward_adapters(lin, x, bank, ids)
+        for g, y in zip(graphs, ys):
+            y.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want), f"replay {i}"
