@@ -70,7 +70,8 @@ class AdapterBank:
         self.scale = torch.tensor([0.0 if e is None else e[2] for e in entries], dtype=torch.float32, device=device)
         self.first_rank = torch.tensor(offsets, dtype=torch.int32, device=device)
         self.device = down_all.device
-        self._native = (self.down, self.up, self.scale, self.first_rank, self.count, self.max_rank)   # (as the host path takes it)
+        # (as the host path takes it)
+        self._native = (self.down, self.up, self.scale, self.first_rank, self.count, self.max_rank, self.in_features, self.out_features)
 
     @classmethod
     def from_patches(cls, patches, **kwargs):

@@ -522,7 +522,7 @@ int64_t rows_to_element(const at::Tensor &t, const at::Tensor &v) {
 }
 
 // adapters(x, ids, weights, scales, biases, per_row, rotate, small_rows, banks): tuples with an entry for each layer, a bank being (down,
-// up, scale, first_rank, count, max_rank) -> list of outputs.
+// up, scale, first_rank, count, max_rank, in features, out features) -> list of outputs.
 PyObject *adapters(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (n != 9) return PyErr_Format(PyExc_TypeError, "adapters takes 9 arguments, got %zd", n);
     const at::Tensor *xt = tensor(a[0]), *ids = tensor(a[1]);
@@ -557,7 +557,9 @@ PyObject *adapters(PyObject *, PyObject *const *a, Py_ssize_t n) {
         if (!layer_of(PyTuple_GET_ITEM(a[2], i), PyTuple_GET_ITEM(a[3], i), PyTuple_GET_ITEM(a[4], i), PyTuple_GET_ITEM(a[5], i) == Py_True, x.device(), o) || o.K != K)
             Py_RETURN_NONE;
         PyObject *bank = PyTuple_GET_ITEM(a[8], i);
-        if (!PyTuple_Check(bank) || PyTuple_GET_SIZE(bank) != 6) Py_RETURN_NONE;
+        if (!PyTuple_Check(bank) || PyTuple_GET_SIZE(bank) != 8) Py_RETURN_NONE;
+        // (a factor's rows are padded in memory: 249 to 256 columns look the same there)
+        if (PyLong_AsLongLong(PyTuple_GET_ITEM(bank, 6)) != K || PyLong_AsLongLong(PyTuple_GET_ITEM(bank, 7)) != o.N) Py_RETURN_NONE;
         const at::Tensor *down = tensor(PyTuple_GET_ITEM(bank, 0)), *up = tensor(PyTuple_GET_ITEM(bank, 1)), *scale = tensor(PyTuple_GET_ITEM(bank, 2)),
                          *first = tensor(PyTuple_GET_ITEM(bank, 3));
         i8f_adapters &ad = l[i].adapters;
