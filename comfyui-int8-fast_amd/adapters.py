@@ -23,6 +23,9 @@ class AdapterBank:
     dtype:    torch.bfloat16 or torch.float16, the activations' (default: the first factor's); factors are rounded to it once.
     device:   where the layer runs (default: the first factor's device if that is a GPU, else ComfyUI's compute device).
     in_features / out_features: needed where no entry has factors.
+
+    A bank is laid out once.  Its tensors may be written into (captured graphs follow that too); assigning another one to an attribute is
+    refused, because the host path keeps the tensors that the kernels are given.
     """
 
     def __init__(self, adapters, dtype: torch.dtype | None = None, device=None, in_features: int | None = None, out_features: int | None = None):
@@ -72,6 +75,11 @@ class AdapterBank:
         self.device = down_all.device
         # (as the host path takes it)
         self._native = (self.down, self.up, self.scale, self.first_rank, self.count, self.max_rank, self.in_features, self.out_features)
+
+    def __setattr__(self, name, value):
+        if "_native" in self.__dict__:
+            raise AttributeError(f"a bank is laid out once: make another one instead of assigning {name}")
+        super().__setattr__(name, value)
 
     @classmethod
     def from_patches(cls, patches, **kwargs):
