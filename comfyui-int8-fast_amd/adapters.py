@@ -132,7 +132,8 @@ def forward_adapters(layers, x: Tensor, banks, ids: Tensor):
     order of binary32 sums.  The adapter acts on x itself,
     also where the layer rotates its activations (a dynamic LoRA of the layer gets them rotated).  Layers whose own kernels cannot take
     the adapters (not quantised, weights that ComfyUI casts or moves for the call, a dynamic LoRA attached) run by themselves, and
-    their rounded result gets the adapters' share.  No gradients: under grad mode an input that asks for one is refused."""
+    their rounded result gets the adapters' share.  No gradients: under grad mode an input that asks for one is refused, and so is a layer
+    with trainable parameters that goes alone."""
     single = isinstance(layers, nn.Module)
     layers, banks = ([layers], [banks]) if single else (list(layers), list(banks))
     if type(x) is Tensor and x.is_cuda and 0 < len(layers) == len(banks) <= _lib.MAX_ADAPTED_LAYERS and not torch.compiler.is_compiling():
@@ -168,7 +169,9 @@ def forward_adapters(layers, x: Tensor, banks, ids: Tensor):
     for rotate, members in together.items():
         if rotate is None:   # layers that go alone
             for i in members:
-                outs[i] = add_adapters(layers[i](x).reshape(rows, banks[i].out_features), x2, ids, per, *compile_ops.bank_args(banks[i]))
+                base = layers[i](x)
+                _lib.refuse_gradients(**{"the layer's result": base})   # (of trainable parameters: it would end here)
+                outs[i] = add_adapters(base.reshape(rows, banks[i].out_features), x2, ids, per, *compile_ops.bank_args(banks[i]))
             continue
         scales = [compile_ops.split_scale(_scale_on(layers[i], x.device)) for i in members]
         parts = zip(*[compile_ops.bank_args(banks[i]) for i in members])

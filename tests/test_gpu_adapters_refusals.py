@@ -27,3 +27,31 @@ def test_a_bank_without_factors_of_another_width(pkg, dev, rows):
     for inputs, outputs in ((256, 64), (250, 128)):
         with pytest.raises(ValueError, match="features"):
             pkg.forward_adapters(lin, x, pkg.AdapterBank([None], in_features=inputs, out_features=outputs, device=dev), ids)
+
+
+@pytest.mark.parametrize("rows", [5, 40])
+def test_a_gradient_that_a_layer_going_alone_would_have(pkg, dev, rows):
+    x, ids = torch.randn(rows, 256, device=dev).bfloat16(), torch.zeros(rows, dtype=torch.int32, device=dev)
+    bank = pkg.AdapterBank(factors_of(256, 128, (16,), torch.bfloat16))
+    lora = layer_of(pkg, 256, 128, torch.bfloat16)
+    lora.lora_A, lora.lora_B = (torch.nn.Parameter(torch.randn(s, device=dev).bfloat16()) for s in ((16, 256), (128, 16)))
+    for lin in (torch.nn.Linear(256, 128, device=dev, dtype=torch.bfloat16), lora):
+        with torch.no_grad():
+            want, base = pkg.forward_adapters(lin, x, bank, ids), lin(x)
+        if not lin(x).requires_grad:   # (the layer itself has no gradient to lose)
+            continue
+        with pytest.raises(RuntimeError, match="gradient"):
+            pkg.forward_adapters(lin, x, bank, ids)
+        assert want.shape == base.shape
+    assert torch.nn.Linear(256, 128, device=dev, dtype=torch.bfloat16)(x).requires_grad
+
+
+def test_a_layer_with_parameters_that_ask_for_nothing_goes_on(pkg, dev):
+    """Frozen parameters, or no grad mode: the call is as before."""
+    x, ids = torch.randn(20, 256, device=dev).bfloat16(), torch.zeros(20, dtype=torch.int32, device=dev)
+    bank = pkg.AdapterBank(factors_of(256, 128, (16,), torch.bfloat16))
+    lin = torch.nn.Linear(256, 128, device=dev, dtype=torch.bfloat16)
+    with torch.no_grad():
+        want = pkg.forward_adapters(lin, x, bank, ids)
+    lin.requires_grad_(False)
+    assert torch.equal(pkg.forward_adapters(lin, x, bank, ids), want)
