@@ -12,6 +12,7 @@ import importlib.util
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from .build import host_lib
 
@@ -154,11 +155,14 @@ def _dev(t: torch.Tensor, name: str) -> None:
 
 
 def refuse_gradients(**tensors) -> None:
-    """For operators without a backward pass: under grad mode an operand that asks for a gradient would silently get none."""
-    if torch.is_grad_enabled():
-        for name, t in tensors.items():
-            if isinstance(t, torch.Tensor) and t.requires_grad:
+    """For operators without derivatives: under grad mode an operand that asks for a gradient would silently get none, and one with a
+    tangent (torch.autograd.forward_ad) would silently lose it."""
+    for name, t in tensors.items():
+        if isinstance(t, torch.Tensor):
+            if t.requires_grad and torch.is_grad_enabled():
                 raise RuntimeError(f"{name} asks for a gradient, which this operator does not have: call it under torch.no_grad()")
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{name} has a tangent, and this operator no forward derivative: call it with the primal")
 
 
 class _Nop:

@@ -133,7 +133,7 @@ def forward_adapters(layers, x: Tensor, banks, ids: Tensor):
     also where the layer rotates its activations (a dynamic LoRA of the layer gets them rotated).  Layers whose own kernels cannot take
     the adapters (not quantised, weights that ComfyUI casts or moves for the call, a dynamic LoRA attached) run by themselves, and
     their rounded result gets the adapters' share.  No gradients: under grad mode an input that asks for one is refused, and so is a layer
-    with trainable parameters that goes alone."""
+    with trainable parameters that goes alone; an input with a tangent always."""
     single = isinstance(layers, nn.Module)
     layers, banks = ([layers], [banks]) if single else (list(layers), list(banks))
     if type(x) is Tensor and x.is_cuda and 0 < len(layers) == len(banks) <= _lib.MAX_ADAPTED_LAYERS and not torch.compiler.is_compiling():

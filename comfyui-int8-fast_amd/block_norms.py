@@ -27,7 +27,8 @@ def block_norm(y: Tensor, residual: Tensor, *, post_norm: str | None = None, pos
     Norms: "rms", "layer" or None over the last dimension, with weight and bias [K] of y's dtype or float32.
     y, residual: tensors alike, bfloat16, float16 or float32.  gate, mod_scale, mod_shift: of y's dtype, [K] or y's shape with ones from
     some leading dimension on ([batch, 1, K] for one vector to an image).  Everything is computed in binary32, h from x before its
-    rounding; x and h are rounded once.  No gradients: under grad mode an input that asks for one is refused."""
+    rounding; x and h are rounded once.  No gradients: under grad mode an input that asks for one is refused, one with a
+    tangent always."""
     if type(y) is Tensor and y.is_cuda and not torch.compiler.is_compiling():
         out = _lib.host().block_norm(y, residual, post_norm, post_weight, post_bias, post_eps, gate, gate_tanh, residual_scale, branch_scale, pre_norm,
                                      pre_weight, pre_bias, pre_eps, mod_scale, mod_shift, None, None, None, None, False, 0, None)

@@ -507,8 +507,8 @@ PyObject *vector_fanout(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return list_of(y, count);
 }
 
-// Whether an operand asks for a gradient that these operators do not have: the general path words the refusal.
-bool wants_gradient(const at::Tensor *t) { return t && t->requires_grad() && c10::GradMode::is_enabled(); }
+// Whether an operand has or asks for a derivative that these operators do not have: the general path words the refusal.
+bool wants_gradient(const at::Tensor *t) { return t && ((t->requires_grad() && c10::GradMode::is_enabled()) || t->_fw_grad(0).defined()); }
 
 // v has the shape of t's leading dimensions, all of them but the last or fewer: the rows of t to an element of v, 0 if it has not.
 int64_t rows_to_element(const at::Tensor &t, const at::Tensor &v) {

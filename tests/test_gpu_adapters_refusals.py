@@ -1,6 +1,7 @@
 """Calls that the adapters and the norms between blocks refuse, whichever path takes them."""
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from test_gpu_adapters import factors_of, layer_of
 
@@ -55,3 +56,27 @@ def test_a_layer_with_parameters_that_ask_for_nothing_goes_on(pkg, dev):
         want = pkg.forward_adapters(lin, x, bank, ids)
     lin.requires_grad_(False)
     assert torch.equal(pkg.forward_adapters(lin, x, bank, ids), want)
+
+
+@pytest.mark.parametrize("rows", [5, 40])
+def test_a_tangent_is_not_dropped(pkg, dev, rows):
+    """Forward-mode derivatives, with and without grad mode, on either path."""
+    lin, bank = layer_of(pkg, 256, 128, torch.bfloat16), pkg.AdapterBank(factors_of(256, 128, (16,), torch.bfloat16))
+    x, ids = torch.randn(rows, 256, device=dev).bfloat16(), torch.zeros(rows, dtype=torch.int32, device=dev)
+    w = torch.ones(256, device=dev).bfloat16()
+    want = pkg.forward_adapters(lin, x, bank, ids), pkg.block_norm(x, x, pre_norm="rms", pre_weight=w)
+    plain = torch.nn.Linear(256, 128, device=dev, dtype=torch.bfloat16).requires_grad_(False)
+    with forward_ad.dual_level():
+        dual, dual_w = forward_ad.make_dual(x, torch.ones_like(x)), forward_ad.make_dual(w, torch.ones_like(w))
+        calls = [lambda: pkg.forward_adapters(lin, dual, bank, ids), lambda: pkg.forward_adapters(plain, dual, bank, ids),
+                 lambda: pkg.forward_adapters(lin, dual, bank, ids.view(rows, 1)[:, 0].expand(rows)), lambda: pkg.block_norm(dual, x), lambda: pkg.block_norm(x, dual),
+                 lambda: pkg.block_norm(x, x, gate=dual), lambda: pkg.block_norm(x, x, pre_norm="rms", pre_weight=dual_w),
+                 lambda: pkg.forward_block_norm([lin], dual, x, pre_norm="rms"), lambda: pkg.forward_block_norm([lin], x, x, pre_norm="rms", pre_weight=dual_w)]
+        for i, call in enumerate(calls):
+            with pytest.raises(RuntimeError, match="tangent"):
+                call()
+                pytest.fail(f"call {i} dropped a tangent")
+            with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):
+                call()
+        got = pkg.forward_adapters(lin, x, bank, ids), pkg.block_norm(x, x, pre_norm="rms", pre_weight=w)   # (others of the same level go on)
+    assert torch.equal(got[0], want[0]) and all(torch.equal(a, b) for a, b in zip(got[1], want[1]))
