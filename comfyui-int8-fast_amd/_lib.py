@@ -902,8 +902,8 @@ def _adapters_arg(bank, ids, rows_per_id):
 
 
 def adapters_down(x, banks, ids, rows_per_id=1, quantise=False, rotate=False):
-    """The first product of every bank's adapters, [t [M, bank.max_rank], ...] of x [M,K]: row m holds scale_a * A_a x[m] for its adapter
-    a = ids[m // rows_per_id] in its first ranks; what lies behind them, and rows without an adapter, are not written.  ids: int32,
+    """The first product of every bank's adapters, [t [M, bank.max_rank], ...] of x [M,K]: row m holds scale_a * A_a x[m], with the scale
+    that the bank holds, for its adapter a = ids[m // rows_per_id] in its first ranks; what lies behind them, and rows without an adapter, are not written.  ids: int32,
     contiguous, one for each rows_per_id rows.  quantise: (ts, int8 rows, their scales) as quant_rowwise(x, rotate) besides."""
     _dev(x, "x")
     x = _rows(x, "x")

@@ -6,6 +6,8 @@ adapters of a layer lie in an `AdapterBank`, and a call names the adapter of eve
 """
 from __future__ import annotations
 
+import math
+
 import torch
 from torch import Tensor, nn
 
@@ -13,6 +15,22 @@ from . import _lib, compile_ops
 from ._comfy_compat import compute_device
 from .dynamic_lora import _factor_pair
 from .int8_quant import SMALL_BATCH_ROWS, _layers_in_place, _scale_on
+
+
+def _second_factor_exponent(up: Tensor, scale: float) -> int:
+    """e for which up * 2^e and scale * 2^-e are laid out in float16: the largest element of up comes to between 1 and 2.
+
+    The kernels round t = scale * down @ x to 16 bits for the matrix unit, and float16 ends at 65504 above and has fewer bits below 2^-14.
+    With up near 1 a t is beyond the type only where one rank's share of some output is as well, and what a t below 2^-14 loses
+    is at most 2^-25 of up: r * 2^-24 of an output, steps of the smallest numbers.  Powers of two change no other rounding."""
+    top = up.detach().abs().max().float().item() if up.numel() else 0.0
+    if not 0.0 < top < math.inf:
+        return 0
+    e = 1 - math.frexp(top)[1]
+    if scale != 0.0 and math.isfinite(scale):   # (which stays a normal float32)
+        at = math.frexp(scale)[1]
+        e = min(max(e, at - 128), at + 125)
+    return min(max(e, -126), 126)
 
 
 class AdapterBank:
@@ -24,6 +42,7 @@ class AdapterBank:
     device:   where the layer runs (default: the first factor's device if that is a GPU, else ComfyUI's compute device).
     in_features / out_features: needed where no entry has factors.
 
+    In float16 an adapter's up is kept times a power of two and its scale times the inverse (_second_factor_exponent).
     A bank is laid out once.  Its tensors may be written into (captured graphs follow that too); assigning another one to an attribute is
     refused, because the host path keeps the tensors that the kernels are given.
     """
@@ -64,13 +83,18 @@ class AdapterBank:
         with torch.no_grad():
             down_all = torch.zeros((offsets[-1], -(-in_features // 8) * 8), dtype=dtype, device=device)   # (whole 16-byte pieces)
             up_all = torch.zeros((offsets[-1] * out_features,), dtype=dtype, device=device)
-            for entry, at, r in zip(entries, offsets, padded):
+            scales = [0.0 if e is None else e[2] for e in entries]
+            for i, (entry, at, r) in enumerate(zip(entries, offsets, padded)):
                 if entry is not None and entry[0].shape[0]:
-                    down, up, _ = entry
+                    down, up, scale = entry
                     down_all[at:at + down.shape[0], :in_features] = down.detach().to(device=device, dtype=dtype)
-                    up_all[at * out_features:(at + r) * out_features].view(out_features, r)[:, :up.shape[1]] = up.detach().to(device=device, dtype=dtype)
+                    up = up.detach().to(device=device)
+                    e = _second_factor_exponent(up, scale) if dtype == torch.float16 else 0
+                    if e:
+                        up, scales[i] = up.float() * 2.0 ** e, math.ldexp(scale, -e)
+                    up_all[at * out_features:(at + r) * out_features].view(out_features, r)[:, :up.shape[1]] = up.to(dtype)
         self.down, self.up = down_all, up_all
-        self.scale = torch.tensor([0.0 if e is None else e[2] for e in entries], dtype=torch.float32, device=device)
+        self.scale = torch.tensor(scales, dtype=torch.float32, device=device)
         self.first_rank = torch.tensor(offsets, dtype=torch.int32, device=device)
         self.device = down_all.device
         # (as the host path takes it)

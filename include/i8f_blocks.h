@@ -56,8 +56,9 @@ int i8f_adapters_by_side(int64_t M, int64_t N, int64_t K, int64_t rows_per_id);
 
 /*
  * t[m, 0 ... r) = scale_a * A_a x[m] of every layer, for the adapter a of row m and its padded rank r: sums in binary32, one rounding to
- * x's type (what the matrix unit multiplies with in the second product); ranks beyond r and rows without an adapter are left as they
- * are.  Of the layers only adapters, t, side and, with it, N are looked at.
+ * x's type (what the matrix unit multiplies with in the second product; binary16 ends at 65504 and has fewer bits below 2^-14, so a
+ * caller lets the largest element of B be about 1 there and puts the rest into the scale); ranks beyond r and rows without an adapter are
+ * left as they are.  Of the layers only adapters, t, side and, with it, N are looked at.
  * Layers with a side get side[m,n] = sum_j t[m,j] B_a[n,j] in binary32 besides (zeros for rows without an adapter); i8f_linear_w8a8_adapters
  * then adds that instead of reading t.  N is then a multiple of 8.  All layers of a call or none.  x_dtype I8F_BF16 or I8F_F16, n_layers up to I8F_MAX_ADAPTED_LAYERS.
  * q, scale: NULL, or the int8 rows of x and their scales besides, as i8f_quant_rowwise with rotate_block leaves them (the adapters take

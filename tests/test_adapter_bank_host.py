@@ -36,3 +36,32 @@ def test_what_is_written_into_a_bank_is_in_both(pkg):
     bank.scale[0] = 4.0
     bank.down.mul_(2)
     assert bank._native[2][0] == 4.0 and torch.equal(bank._native[0], parts(pkg, bank)[0])
+
+
+@pytest.mark.parametrize("given", [torch.float16, torch.bfloat16, torch.float32, torch.float64])
+@pytest.mark.parametrize("size,scale", [(1.0, 1.0), (2.0 ** -13, 2.0 ** 20), (300.0, 1e-6), (1e-9, 3e9), (1e6, -1e-7), (1e-30, 1e30), (1.0, 1e-38), (1.0, 3e38)])
+def test_second_factors_of_a_binary16_bank_are_near_one(pkg, given, size, scale):
+    """scale * up is what it was, up to one rounding of up to binary16; up reaches 1 where the scale leaves it room."""
+    if given == torch.float16 and not 2.0 ** -14 <= size <= 300:
+        pytest.skip("no binary16 number")
+    up, down = (torch.linspace(-1.0, 1.7, 60).view(12, 5) * size).to(given), torch.ones(5, 8)
+    bank = pkg.AdapterBank([(down, up, scale), None, (down, up * 0, scale), (down, up, 0.0)], dtype=torch.float16, device="cpu")
+    got = bank.up.view(-1)[:12 * 16].view(12, 16)[:, :5].double() * bank.scale[0].double()
+    want = up.double() * scale
+    top = want.abs().max()
+    assert torch.isfinite(bank.scale).all() and bank.scale[0] != 0
+    assert ((got - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -23 * want.abs() + 2.0 ** -25 * top).all()
+    assert 1.0 <= bank.up.abs().max() <= 2.0
+    assert not bank.up.view(-1)[12 * 16:2 * 12 * 16].any() and bank.scale[3] == 0
+
+
+def test_second_factors_of_a_bfloat16_bank_and_of_no_finite_ones_stay(pkg):
+    up, down = torch.full((6, 3), 2.0 ** -10), torch.ones(3, 8)
+    bank = pkg.AdapterBank([(down, up, 7.0)], dtype=torch.bfloat16, device="cpu")
+    assert bank.scale[0] == 7.0 and bank.up.max() == 2.0 ** -10
+    for value in (float("inf"), float("nan")):
+        up[2, 1] = value
+        bank = pkg.AdapterBank([(down, up, 7.0)], dtype=torch.float16, device="cpu")
+        assert bank.scale[0] == 7.0 and bank.up[0] == 2.0 ** -10
+    bank = pkg.AdapterBank([(torch.ones(0, 8), torch.ones(6, 0), 7.0)], dtype=torch.float16, device="cpu")
+    assert bank.max_rank == 0 and bank.scale[0] == 7.0
