@@ -32,9 +32,9 @@ __device__ __forceinline__ float norm_operand(const void *p, int dtype, int64_t 
 // ---- rows of less than a run, or too wide for registers (more than 16384 elements): 256 threads to a row, which is read again for every statistic
 // (from cache) ----------------
 template <int DT, int H>
-__global__ __launch_bounds__(256) void block_norm_generic_kernel(const i8f_block_norm_args a) {
+__global__ __launch_bounds__(256) void block_norm_generic_kernel(const i8f_block_norm_args a, const int64_t first_row) {
     __shared__ float red[4];
-    const int64_t m = blockIdx.x, K = a.K;
+    const int64_t m = first_row + blockIdx.x, K = a.K;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t yb = m * a.ldy, rb = m * a.ldr;
     const int64_t gb = a.gate ? m / a.rows_per_gate * K : 0, sb = a.mod_scale ? m / a.rows_per_scale * K : 0;
@@ -191,13 +191,13 @@ __device__ __forceinline__ void operand_run(const void *p, int dtype, int64_t k,
 // ANY: rows of any width (a run at least) and alignment.  A row's last run then ends with it and begins in the run before, whose elements it
 // computes again and leaves out of the sums, which are the same ones in the same order.
 template <int DT, int H, int WPR, int NCH, bool ANY>
-__global__ __launch_bounds__(256) void block_norm_kernel(const i8f_block_norm_args a) {
+__global__ __launch_bounds__(256) void block_norm_kernel(const i8f_block_norm_args a, const int64_t first_row) {
     constexpr int N = Run<DT>::N, TPR = 64 * WPR, ROWS = 4 / WPR, SIZE = DT == I8F_F32 ? 4 : 2;
     __shared__ float red[5][ROWS][WPR];
     const int t = threadIdx.x % TPR, rb = threadIdx.x / TPR, lane = threadIdx.x & 63;
     const int64_t K = a.K;
     const int runs = (int)((K + N - 1) / N);
-    const int64_t own = (int64_t)blockIdx.x * ROWS + rb;
+    const int64_t own = first_row + (int64_t)blockIdx.x * ROWS + rb;
     const bool ok = own < a.M;
     const int64_t m = ok ? own : a.M - 1;   // (a wave past the last row computes it again and stores nothing)
     // which of its runs a lane holds: its own, or where the rotation pairs lanes by DPP the one that it wants there (rotate_run16,
@@ -359,11 +359,20 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const i8f_block_norm_ar
     }
 }
 
+// ROWS rows to a workgroup, in as many launches as it takes: one has fewer than 2^32 threads
+template <int ROWS, class KERNEL>
+int launch_ranges(KERNEL kernel, const i8f_block_norm_args &a, hipStream_t st) {
+    constexpr int64_t MOST = (int64_t)ROWS << 23;
+    for (int64_t m0 = 0; m0 < a.M; m0 += MOST) {
+        const int64_t rows = a.M - m0 < MOST ? a.M - m0 : MOST;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + ROWS - 1) / ROWS)), dim3(256), 0, st, a, m0);
+        if (int rc = check_launch()) return rc;
+    }
+    return I8F_OK;
+}
 template <int DT, int H, int WPR, int NCH, bool ANY>
 int launch_rows(const i8f_block_norm_args &a, hipStream_t st) {
-    constexpr int ROWS = 4 / WPR;
-    hipLaunchKernelGGL((block_norm_kernel<DT, H, WPR, NCH, ANY>), dim3((unsigned)((a.M + ROWS - 1) / ROWS)), dim3(256), 0, st, a);
-    return check_launch();
+    return launch_ranges<4 / WPR>(block_norm_kernel<DT, H, WPR, NCH, ANY>, a, st);
 }
 
 // Aligned rows of whole runs; 16-byte pieces of every operand
@@ -401,8 +410,7 @@ int launch(const i8f_block_norm_args &a, hipStream_t st) {
     constexpr int N = Run<DT>::N;
     const int64_t runs = (a.K + N - 1) / N;
     if (runs <= (DT == I8F_F32 ? 4096 : 1024) && a.K >= N) return whole_runs(a, N) ? launch_width<DT, H, false>(a, runs, st) : launch_width<DT, H, true>(a, runs, st);
-    hipLaunchKernelGGL((block_norm_generic_kernel<DT, H>), dim3((unsigned)a.M), dim3(256), 0, st, a);
-    return check_launch();
+    return launch_ranges<1>(block_norm_generic_kernel<DT, H>, a, st);
 }
 
 template <int DT>
