@@ -72,6 +72,7 @@ __global__ __launch_bounds__(256) void adapters_up_kernel(const void *base, cons
 
 template <int DT, int BASE>
 int launch_up(const void *base, const i8f_adapters &ad, const void *t, void *out, int64_t M, int64_t N, hipStream_t st) {
+    if (!grid_fits((N + 127) / 128, 256)) return I8F_ERR_UNSUPPORTED;
     constexpr int64_t MOST = 16 * 65535;   // (the second dimension of a grid ends there)
     for (int64_t m0 = 0; m0 < M; m0 += MOST) {
         const dim3 grid((unsigned)((N + 127) / 128), (unsigned)(((M - m0 < MOST ? M - m0 : MOST) + 15) / 16));

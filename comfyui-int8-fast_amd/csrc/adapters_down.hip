@@ -232,6 +232,7 @@ int launch(const char *x, int M, int K, int ldx_bytes, const DownLayers &g, floa
     // layers of rank 68: 52 us in one, 19 in eight; 188 x 1141, 85 requests, rank 82: 43 in eight, 22 in 32); those without a pass end at once
     const unsigned units = (unsigned)((M + ROWS - 1) / ROWS) * slices;
     const int parts = units >= 512 ? 1 : units <= 16 ? 32 : (int)(512 / units);
+    if (!grid_fits((int64_t)units * parts, 256)) return I8F_ERR_UNSUPPORTED;
     const dim3 grid(units * parts);
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, x, M, K, ldx_bytes, partial, slices, per, parts, g); };
     if (ranks <= 32) go(adapters_partial_kernel<DT, 2, 5>);
@@ -256,7 +257,7 @@ int adapters_down_slices(int64_t M, int64_t K) {
 
 int adapters_copy_rows(const void *x, int64_t M, int64_t K, int64_t ldx, void *to, hipStream_t st) {
     const int64_t per_row = factor_width(K) / 8, pieces = M * per_row;
-    if ((pieces + 255) / 256 > 0x7fffffff) return I8F_ERR_UNSUPPORTED;
+    if (!grid_fits((pieces + 255) / 256, 256)) return I8F_ERR_UNSUPPORTED;
     hipLaunchKernelGGL(copy_rows_kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, st, (const uint16_t *)x, pieces, (int)K, ldx, (int)per_row, (char *)to);
     return check_launch();
 }

@@ -1590,7 +1590,7 @@ int launch_cfg_adapted(AdaptedLayers &l, const int8_t *x, const float *xs, int M
         l.first_tile[i] = (int)first;
         first += (int64_t)tiles_m * l.tiles_n[i];
     }
-    if (first > 0x7fffffff) return I8F_ERR_UNSUPPORTED;
+    if (!grid_fits(first, C::NT)) return I8F_ERR_UNSUPPORTED;
     for (int i = l.n; i <= MAX_ADAPTED; ++i) l.first_tile[i] = (int)first;
     GemmArgs g{};
     g.order = I8F_EPI_FUSED;

@@ -39,6 +39,9 @@ inline int check_launch() {
     return I8F_OK;
 }
 
+// Whether a launch can have that many workgroups: its threads are counted in 32 bits.
+inline bool grid_fits(int64_t blocks, int threads) { return blocks <= 0x7fffffff && blocks * threads < (1ll << 32); }
+
 // I8F_OK if the current device is a gfx950, I8F_ERR_DEVICE otherwise (cached per device).
 int check_device();
 

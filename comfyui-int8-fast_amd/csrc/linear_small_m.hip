@@ -466,6 +466,7 @@ int launch_adapted(const SmallMArgs *as, const WithAdapters *ads, int n, hipStre
             l.a[l.n] = a, l.ad[l.n++] = ads[i];
             continue;
         }
+        if (!grid_fits((a.N + 3) / 4, 256)) return I8F_ERR_UNSUPPORTED;
         hipLaunchKernelGGL((small_m_kernel<DT, false, WithAdapters>), dim3((unsigned)((a.N + 3) / 4)), dim3(256), 0, st, a, ads[i]);
         if (int rc = check_launch()) return rc;
     }
@@ -473,7 +474,7 @@ int launch_adapted(const SmallMArgs *as, const WithAdapters *ads, int n, hipStre
     const int together = blocks_to_workgroup(l.a, l.n);
     int64_t first = 0;
     for (int i = 0; i < l.n; ++i) l.first_block[i] = (int)first, first += (l.a[i].N + 16 * together - 1) / (16 * together);
-    if (first > 0x7fffffff) return I8F_ERR_UNSUPPORTED;
+    if (!grid_fits(first, 512)) return I8F_ERR_UNSUPPORTED;
     for (int i = l.n; i <= I8F_MAX_ADAPTED_LAYERS; ++i) l.first_block[i] = (int)first;
     if (together == 3) hipLaunchKernelGGL((small_m_adapters_kernel<DT, 3, 8>), dim3((unsigned)first), dim3(512), 0, st, l);
     else if (together == 2) hipLaunchKernelGGL((small_m_adapters_kernel<DT, 2, 8>), dim3((unsigned)first), dim3(512), 0, st, l);

@@ -129,7 +129,7 @@ __global__ __launch_bounds__(256) void adapters_combine_kernel(const float *__re
 template <int DT, bool ROT, int WPR, int RUNS>
 int launch_combine(const float *partial, int64_t M, int slices, const void *x, int64_t K, int64_t ldx, int8_t *q, float *scale, const DownLayers &g, hipStream_t st) {
     const int64_t combine = (M * (g.first_column[g.n] / 4) + 255) / 256, quant = RUNS > 0 ? (M + 4 / WPR - 1) / (4 / WPR) : 0;
-    if (combine + quant > 0x7fffffff) return I8F_ERR_UNSUPPORTED;
+    if (!grid_fits(combine + quant, 256)) return I8F_ERR_UNSUPPORTED;
     hipLaunchKernelGGL((adapters_combine_kernel<DT, ROT, WPR, RUNS>), dim3((unsigned)(combine + quant)), dim3(256), 0, st, partial, M, slices, (int)combine, (const char *)x,
                        K, ldx, q, scale, g);
     return check_launch();
@@ -171,7 +171,7 @@ int launch_rows_of(const void *x, int64_t M, int64_t K, int64_t ldx, int8_t *q, 
     for (int i = 0; i < g.n; ++i) g.first_block[i] = (int)first, first += M * (g.ad[i].max_rank / (4 * PER));
     for (int i = g.n; i <= I8F_MAX_ADAPTED_LAYERS; ++i) g.first_block[i] = (int)first;
     if (quant_blocks + first == 0) return I8F_OK;
-    if (quant_blocks + first > 0x7fffffff) return I8F_ERR_UNSUPPORTED;
+    if (!grid_fits(quant_blocks + first, 256)) return I8F_ERR_UNSUPPORTED;
     hipLaunchKernelGGL((adapters_rows_kernel<DT, ROT, RUNS, ANY, PER>), dim3((unsigned)(quant_blocks + first)), dim3(256), 0, st, (const char *)x, M, (int)K, ldx, q, scale,
                        (int)quant_blocks, g);
     return check_launch();
@@ -238,7 +238,7 @@ int launch_side(int64_t M, DownLayers &g, hipStream_t st) {
     return check_launch();
 }
 
-inline bool side_in_place(int64_t M, int64_t N) { return N % 8 == 0 && M * ((N + 1023) / 1024) < (1ll << 29); }   // (four layers in a grid)
+inline bool side_in_place(int64_t M, int64_t N) { return N % 8 == 0 && M * ((N + 1023) / 1024) < (1ll << 22); }   // (four layers in a grid)
 inline bool down_in_place(const void *x, int64_t K, int64_t ldx) { return K % 8 == 0 && (uintptr_t)x % 16 == 0 && ldx % 8 == 0 && ldx < (1ll << 23); }
 
 template <int DT>
@@ -327,5 +327,5 @@ extern "C" int i8f_adapters_by_side(int64_t M, int64_t N, int64_t K, int64_t row
     // Up to 16 rows are another kernel's, and widths that the tiled kernels do not take go by way of i8f_adapters_up.  64 tokens of as many
     // requests, 4096 -> 4096 + 1024 + 1024, ranks of 8 to 64: 33.5 us by side and 37.6 with the factors fetched by the 96 tiles; of one
     // request the tiles' way is the faster one (64 x 4096 -> 4096, rank 64: 3 us more than without adapters, and 10 by side).
-    return rows_per_id > 0 && M / rows_per_id > 16 && M <= 128 && i8f_linear_w8a8_adapters_workspace_bytes(M, N, K) == 0;
+    return rows_per_id > 0 && M / rows_per_id > 16 && M <= 128 && i8f::side_in_place(M, N) && i8f_linear_w8a8_adapters_workspace_bytes(M, N, K) == 0;
 }
