@@ -153,7 +153,9 @@ def forward_adapters(layers, x: Tensor, banks, ids: Tensor):
 
     One rounding at the end: the projection stays in binary32 (in the order of _lib.EPI_FUSED) until the adapter's share has been
     added; down @ x is rounded to x's dtype for the matrix unit.  x is quantised once for all layers; which layers go together may change the
-    order of binary32 sums.  The adapter acts on x itself,
+    order of binary32 sums, and so may the way a call goes: for 17 to 128 rows with more than 16 numbers the native path sums the adapters'
+    share for itself, in a launch of its own, which contiguous ids of up to four layers of one rotation flag take in eager mode.
+    A row without an adapter is the layer's result in that order, not layer(x) bit for bit.  The adapter acts on x itself,
     also where the layer rotates its activations (a dynamic LoRA of the layer gets them rotated).  Layers whose own kernels cannot take
     the adapters (not quantised, weights that ComfyUI casts or moves for the call, a dynamic LoRA attached) run by themselves, and
     their rounded result gets the adapters' share.  No gradients: under grad mode an input that asks for one is refused, and so is a layer
