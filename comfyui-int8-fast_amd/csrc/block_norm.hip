@@ -331,8 +331,10 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const i8f_block_norm_ar
 #pragma unroll
             for (int w = 1; w < WPR; ++w) amax = fmaxf(amax, red[4][rb][w]);
         }
+        // (as i8f_quant_rowwise does with rows of this width: the short forms differ from these in what becomes of a value that is not finite)
+        const bool saturating = DT == I8F_F32 || (ANY && K % 16 != 0);
         float s, inv;
-        if constexpr (DT == I8F_F32) {
+        if (saturating) {
             s = amax / 127.0f;
             s = s < 1e-30f ? 1e-30f : s;
             inv = 1.0f / s;
@@ -344,12 +346,12 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const i8f_block_norm_ar
         for (int i = 0; i < NCH; ++i) {
             if (!in[i]) continue;
             int8_t *dst = a.q + m * K + at[i];
-            if constexpr (DT == I8F_F32) {
-                uint32_t w = 0;
+            if (saturating) {
+                uint32_t w[N / 4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w |= ((uint32_t)quant_i8(x[i][e] * inv) & 0xffu) << (8 * e);
-                __builtin_memcpy(dst, &w, 4);
-            } else {
+                for (int e = 0; e < N; ++e) w[e / 4] = (e % 4 ? w[e / 4] : 0u) | ((uint32_t)quant_i8(x[i][e] * inv) & 0xffu) << (8 * (e % 4));
+                __builtin_memcpy(dst, w, N);
+            } else if constexpr (DT != I8F_F32) {
                 const uint4 o = quant16_magic(x[i], inv);
                 if constexpr (ANY) __builtin_memcpy(dst, &o, 16);
                 else stream_store16(dst, o);
