@@ -32,7 +32,7 @@ __device__ __forceinline__ float norm_operand(const void *p, int dtype, int64_t 
 // ---- rows of less than a run, or too wide for registers (more than 16384 elements): 256 threads to a row, which is read again for every statistic
 // (from cache) ----------------
 template <int DT, int H>
-__global__ __launch_bounds__(256) void block_norm_generic_kernel(const i8f_block_norm_args a, const int64_t first_row) {
+__global__ __launch_bounds__(256) void block_norm_generic_kernel(const int64_t first_row, const i8f_block_norm_args a) {
     __shared__ float red[4];
     const int64_t m = first_row + blockIdx.x, K = a.K;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -191,7 +191,7 @@ __device__ __forceinline__ void operand_run(const void *p, int dtype, int64_t k,
 // ANY: rows of any width (a run at least) and alignment.  A row's last run then ends with it and begins in the run before, whose elements it
 // computes again and leaves out of the sums, which are the same ones in the same order.
 template <int DT, int H, int WPR, int NCH, bool ANY>
-__global__ __launch_bounds__(256) void block_norm_kernel(const i8f_block_norm_args a, const int64_t first_row) {
+__global__ __launch_bounds__(256) void block_norm_kernel(const int64_t first_row, const i8f_block_norm_args a) {
     constexpr int N = Run<DT>::N, TPR = 64 * WPR, ROWS = 4 / WPR, SIZE = DT == I8F_F32 ? 4 : 2;
     __shared__ float red[5][ROWS][WPR];
     const int t = threadIdx.x % TPR, rb = threadIdx.x / TPR, lane = threadIdx.x & 63;
@@ -362,12 +362,13 @@ __global__ __launch_bounds__(256) void block_norm_kernel(const i8f_block_norm_ar
 }
 
 // ROWS rows to a workgroup, in as many launches as it takes: one has fewer than 2^32 threads
+// (the first row comes ahead of the structure, among the arguments that are in registers when a wave starts: 2048 x 3840 13.7 us, 14.1 behind it)
 template <int ROWS, class KERNEL>
 int launch_ranges(KERNEL kernel, const i8f_block_norm_args &a, hipStream_t st) {
     constexpr int64_t MOST = (int64_t)ROWS << 23;
     for (int64_t m0 = 0; m0 < a.M; m0 += MOST) {
         const int64_t rows = a.M - m0 < MOST ? a.M - m0 : MOST;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + ROWS - 1) / ROWS)), dim3(256), 0, st, a, m0);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + ROWS - 1) / ROWS)), dim3(256), 0, st, m0, a);
         if (int rc = check_launch()) return rc;
     }
     return I8F_OK;
