@@ -13,7 +13,7 @@ from torch import Tensor, nn
 
 from . import _lib, compile_ops
 from ._comfy_compat import compute_device
-from .dynamic_lora import _factor_pair
+from .dynamic_lora import _factors
 from .int8_quant import SMALL_BATCH_ROWS, _layers_in_place, _scale_on
 
 
@@ -108,8 +108,8 @@ class AdapterBank:
     @classmethod
     def from_patches(cls, patches, **kwargs):
         """A bank of ComfyUI LoRA patches of one layer: (adapter, strength) for each adapter number or None, as the entries of
-        the dynamic LoRA loaders hold them; alpha, rank and strength make the scale."""
-        return cls([None if p is None else _factor_pair(*p) for p in patches], **kwargs)
+        the dynamic LoRA loaders hold them; alpha, rank and strength make the scale, which stays out of the rounded factors."""
+        return cls([None if p is None else _factors(*p) for p in patches], **kwargs)
 
 
 def _adapter_rows(x: Tensor, ids: Tensor) -> tuple[Tensor, int]:

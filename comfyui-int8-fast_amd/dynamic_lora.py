@@ -28,14 +28,20 @@ def _entries_signature(entries):
     return tuple((id(e["patches"]), float(e["strength"])) for e in entries)
 
 
-def _factor_pair(adapter, strength):
-    """(A, B) of one LoRA patch: A = scaled down-projection (through `mid` if present), B = up."""
+def _factors(adapter, strength):
+    """(down, up, scale) of one LoRA patch: the down-projection through `mid` if present, and alpha, rank and strength."""
     up, down, alpha, mid = adapter.weights[0], adapter.weights[1], adapter.weights[2], adapter.weights[3]
     rank = down.shape[0] if down.ndim >= 2 else 1
     scale = strength if alpha is None else (alpha / rank) * strength
     a = down
     if mid is not None:
         a = torch.mm(mid.flatten(1), down.flatten(1)).reshape(down.shape)
+    return a, up, scale
+
+
+def _factor_pair(adapter, strength):
+    """(A, B) of one LoRA patch: A = scaled down-projection, B = up."""
+    a, up, scale = _factors(adapter, strength)
     return a * scale, up
 
 

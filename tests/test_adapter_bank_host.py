@@ -65,3 +65,18 @@ def test_second_factors_of_a_bfloat16_bank_and_of_no_finite_ones_stay(pkg):
         assert bank.scale[0] == 7.0 and bank.up[0] == 2.0 ** -10
     bank = pkg.AdapterBank([(torch.ones(0, 8), torch.ones(6, 0), 7.0)], dtype=torch.float16, device="cpu")
     assert bank.max_rank == 0 and bank.scale[0] == 7.0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("alpha,strength", [(3.0, 0.7), (None, 1e-5), (None, -1.3)])
+def test_a_patch_s_strength_does_not_go_through_16_bits(pkg, dtype, alpha, strength):
+    """Factors of a patch in the activations' type are kept as they are; alpha, rank and strength are the scale."""
+    g = torch.Generator().manual_seed(5)
+    up, down, mid = (torch.randn(s, generator=g).to(dtype) for s in ((6, 4), (4, 10), (4, 4)))
+    for middle in (None, mid):
+        patch = pkg.INT8LoRAPatchAdapter(set(), (up, down, alpha, middle, None, None), 0.01)
+        bank = pkg.AdapterBank.from_patches([None, (patch, strength)], dtype=dtype, device="cpu")
+        scale = strength if alpha is None else alpha / 4 * strength
+        assert torch.equal(bank.down[:4, :10], down if middle is None else mid @ down) and bank.ranks == [0, 4]
+        got = bank.up.view(6, 16)[:, :4].double() * bank.scale[1].double()
+        assert (got - up.double() * scale).abs().max() <= 2.0 ** -23 * (up.double() * scale).abs().max()
