@@ -17,13 +17,12 @@ from .dynamic_lora import _factors
 from .int8_quant import SMALL_BATCH_ROWS, _layers_in_place, _scale_on
 
 
-def _second_factor_exponent(up: Tensor, scale: float) -> int:
-    """e for which up * 2^e and scale * 2^-e are laid out in float16: the largest element of up comes to between 1 and 2.
+def _second_factor_exponent(top: float, scale: float) -> int:
+    """e for which up * 2^e and scale * 2^-e are laid out in float16, top being the largest element of up: it comes to between 1 and 2.
 
     The kernels round t = scale * down @ x to 16 bits for the matrix unit, and float16 ends at 65504 above and has fewer bits below 2^-14.
     With up near 1 a t is beyond the type only where one rank's share of some output is as well, and what a t below 2^-14 loses
     is at most 2^-25 of up: r * 2^-24 of an output, steps of the smallest numbers.  Powers of two change no other rounding."""
-    top = up.detach().abs().max().float().item() if up.numel() else 0.0
     if not 0.0 < top < math.inf:
         return 0
     e = 1 - math.frexp(top)[1]
@@ -80,19 +79,26 @@ class AdapterBank:
             offsets.append(offsets[-1] + r)
         if offsets[-1] >= 1 << 31 or self.max_rank > 65536:
             raise ValueError(f"the ranks of a bank add up to less than 2^31 and stay within 65536, got {offsets[-1]} and {self.max_rank}")
+        scales = [0.0 if e is None else e[2] for e in entries]
         with torch.no_grad():
             down_all = torch.zeros((offsets[-1], -(-in_features // 8) * 8), dtype=dtype, device=device)   # (whole 16-byte pieces)
-            up_all = torch.zeros((offsets[-1] * out_features,), dtype=dtype, device=device)
-            scales = [0.0 if e is None else e[2] for e in entries]
-            for i, (entry, at, r) in enumerate(zip(entries, offsets, padded)):
+            # (float16 factors are scaled before they are rounded)
+            wide = dtype == torch.float16 and any(e is not None and e[1].dtype != torch.float16 for e in entries)
+            up_all = torch.zeros((offsets[-1] * out_features,), dtype=torch.float32 if wide else dtype, device=device)
+            for entry, at, r in zip(entries, offsets, padded):
                 if entry is not None and entry[0].shape[0]:
-                    down, up, scale = entry
+                    down, up, _ = entry
                     down_all[at:at + down.shape[0], :in_features] = down.detach().to(device=device, dtype=dtype)
-                    up = up.detach().to(device=device)
-                    e = _second_factor_exponent(up, scale) if dtype == torch.float16 else 0
-                    if e:
-                        up, scales[i] = up.float() * 2.0 ** e, math.ldexp(scale, -e)
-                    up_all[at * out_features:(at + r) * out_features].view(out_features, r)[:, :up.shape[1]] = up.to(dtype)
+                    up_all[at * out_features:(at + r) * out_features].view(out_features, r)[:, :up.shape[1]] = up.detach().to(device=device, dtype=up_all.dtype)
+            if dtype == torch.float16 and up_all.numel():
+                pieces = up_all.view(-1, 16 * out_features)   # (each of one adapter)
+                tops = torch.maximum(pieces.amax(1), -pieces.amin(1)).tolist()
+                exponents = [_second_factor_exponent(max(tops[at // 16:(at + r) // 16], key=lambda v: (v != v, v)), scale) if r else 0
+                             for at, r, scale in zip(offsets, padded, scales)]
+                if any(exponents):
+                    scales = [math.ldexp(scale, -e) for scale, e in zip(scales, exponents)]
+                    pieces.mul_(torch.tensor([2.0 ** e for e, r in zip(exponents, padded) for _ in range(r // 16)], dtype=torch.float32, device=device)[:, None])
+                up_all = up_all.to(dtype)
         self.down, self.up = down_all, up_all
         self.scale = torch.tensor(scales, dtype=torch.float32, device=device)
         self.first_rank = torch.tensor(offsets, dtype=torch.int32, device=device)
