@@ -21,8 +21,9 @@ def _second_factor_exponent(top: float, scale: float) -> int:
     """e for which up * 2^e and scale * 2^-e are laid out in float16, top being the largest element of up: it comes to between 1 and 2.
 
     The kernels round t = scale * down @ x to 16 bits for the matrix unit, and float16 ends at 65504 above and has fewer bits below 2^-14.
-    With up near 1 a t is beyond the type only where one rank's share of some output is as well, and what a t below 2^-14 loses
-    is at most 2^-25 of up: r * 2^-24 of an output, steps of the smallest numbers.  Powers of two change no other rounding."""
+    With up near 1 a t is beyond the type only where its share of an output is as well (in a rank whose column of up is as large as the
+    others'), and what a t below 2^-14 loses is at most 2^-25 of up: r * 2^-24 of an output, steps of the smallest numbers.  Powers of
+    two change no other rounding."""
     if not 0.0 < top < math.inf:
         return 0
     e = 1 - math.frexp(top)[1]

@@ -113,8 +113,9 @@ __global__ __launch_bounds__(256) void block_norm_generic_kernel(const int64_t f
 
 // ---- rows that stay in registers --------------------------------------------------------------------------------------------
 // Both rows are read once, the sums are taken over registers: 7 or 8 bytes an element in 16 bits, which is what bounds it.  16384 x 5120 in
-// bfloat16 150 us, 4.5 TB/s, where a copy of 4 GiB runs at 4.75; 2048 x 3840 13.1 us, 4.8 TB/s, part of it from the last-level cache;
-// 4096 x 2048 in binary32 23.7 us; 4096 x 3840 with int8 rows out 28 us.  A call of two rows is 4.5 us of launch and dependent loads.
+// bfloat16 153 us (149 to 159 from card to card), 4.4 TB/s, where a copy of 4 GiB runs at 4.75; 2048 x 3840 13.7 us, 4.6 TB/s;
+// 4096 x 2048 in binary32 23.8 us, 5.6 TB/s, part of it from the last-level cache; 4096 x 3840 with int8 rows out 29 us.  A launch of two rows is
+// 2.8 to 3.4 us, 4.5 in a row, of dependent loads.
 // WPR waves share a row, a lane holds NCH runs of RUN consecutive elements (32 bytes of a 16-bit row, 16 of a binary32 one).  How many waves
 // a row gets depends on its width alone, so that a row's bits depend neither on the rows beside it nor on what becomes of h.
 template <int DT>
