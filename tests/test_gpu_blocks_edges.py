@@ -84,3 +84,29 @@ def test_int8_rows_of_values_that_are_not_finite(pkg, L, dev, K, rotate, dtype):
         assert torch.equal(x.nan_to_num(1.0), x8.nan_to_num(1.0))
         off = ((s != want_s) & ~(s.isnan() & want_s.isnan())).view(-1) | (q != want_q).any(1)
         assert not off.any(), f"rows {off.nonzero().view(-1).tolist()}"
+
+
+def test_threads_with_and_without_streams_of_their_own(pkg, dev):
+    """The host path gives the interpreter's lock back while it launches."""
+    import concurrent.futures
+
+    layers = layers_of(pkg, 1024, (512, 264), torch.bfloat16)
+    banks = [pkg.AdapterBank(factors_of(1024, n, (16, 40), torch.bfloat16)) for n in (512, 264)]
+    cases = []
+    for rows in (4, 60, 300):
+        x = torch.randn(rows, 1024, device=dev).bfloat16()
+        ids = (torch.arange(rows, device=dev) % 3 - 1).to(torch.int32)
+        cases.append((x, ids, pkg.forward_adapters(layers, x, banks, ids), pkg.forward_block_norm(layers, x, x, post_norm="rms", pre_norm="layer")))
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream() if i % 2 else torch.cuda.default_stream()):
+            for k in range(12):
+                x, ids, want, (want_x, want_h) = cases[(i + k) % len(cases)]
+                got, (got_x, got_h) = pkg.forward_adapters(layers, x, banks, ids), pkg.forward_block_norm(layers, x, x, post_norm="rms", pre_norm="layer")
+                if not all(torch.equal(a, b) for a, b in zip((*got, got_x, *got_h), (*want, want_x, *want_h))):
+                    return f"thread {i}, call {k}"
+        return None
+
+    with concurrent.futures.ThreadPoolExecutor(max_workers=6) as pool:
+        assert [r for r in pool.map(work, range(6)) if r] == []
