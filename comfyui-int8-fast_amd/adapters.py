@@ -43,8 +43,8 @@ class AdapterBank:
     in_features / out_features: needed where no entry has factors.
 
     In float16 an adapter's up is kept times a power of two and its scale times the inverse (_second_factor_exponent).
-    A bank is laid out once.  Its tensors may be written into (captured graphs follow that too); assigning another one to an attribute is
-    refused, because the host path keeps the tensors that the kernels are given.
+    A bank is laid out once.  Its tensors may be written into (captured graphs follow that too); assigning another one to an attribute of
+    the layout is refused, because the host path keeps the tensors that the kernels are given.
     """
 
     def __init__(self, adapters, dtype: torch.dtype | None = None, device=None, in_features: int | None = None, out_features: int | None = None):
@@ -91,7 +91,7 @@ class AdapterBank:
                     down, up, _ = entry
                     down_all[at:at + down.shape[0], :in_features] = down.detach().to(device=device, dtype=dtype)
                     up_all[at * out_features:(at + r) * out_features].view(out_features, r)[:, :up.shape[1]] = up.detach().to(device=device, dtype=up_all.dtype)
-            if dtype == torch.float16 and up_all.numel():
+            if dtype == torch.float16 and up_all.numel() and not up_all.is_meta:
                 pieces = up_all.view(-1, 16 * out_features)   # (each of one adapter)
                 tops = torch.maximum(pieces.amax(1), -pieces.amin(1)).tolist()
                 exponents = [_second_factor_exponent(max(tops[at // 16:(at + r) // 16], key=lambda v: (v != v, v)), scale) if r else 0
@@ -99,7 +99,7 @@ class AdapterBank:
                 if any(exponents):
                     scales = [math.ldexp(scale, -e) for scale, e in zip(scales, exponents)]
                     pieces.mul_(torch.tensor([2.0 ** e for e, r in zip(exponents, padded) for _ in range(r // 16)], dtype=torch.float32, device=device)[:, None])
-                up_all = up_all.to(dtype)
+            up_all = up_all.to(dtype)
         self.down, self.up = down_all, up_all
         self.scale = torch.tensor(scales, dtype=torch.float32, device=device)
         self.first_rank = torch.tensor(offsets, dtype=torch.int32, device=device)
@@ -107,8 +107,10 @@ class AdapterBank:
         # (as the host path takes it)
         self._native = (self.down, self.up, self.scale, self.first_rank, self.count, self.max_rank, self.in_features, self.out_features)
 
+    _LAID_OUT = frozenset(("down", "up", "scale", "first_rank", "count", "max_rank", "in_features", "out_features", "dtype", "device", "ranks", "_native"))
+
     def __setattr__(self, name, value):
-        if "_native" in self.__dict__:
+        if name in self._LAID_OUT and "_native" in self.__dict__:
             raise AttributeError(f"a bank is laid out once: make another one instead of assigning {name}")
         super().__setattr__(name, value)
 

@@ -20,12 +20,12 @@ def test_the_host_path_and_the_general_one_take_the_same_tensors(pkg):
         assert all(a is b for a, b in zip(bank._native, parts(pkg, bank))) and bank._native[6:] == (10, 6)
 
 
-@pytest.mark.parametrize("name", ["down", "up", "scale", "first_rank", "count", "max_rank", "in_features", "out_features", "dtype", "device", "ranks", "other"])
+@pytest.mark.parametrize("name", ["down", "up", "scale", "first_rank", "count", "max_rank", "in_features", "out_features", "dtype", "device", "ranks"])
 def test_nothing_is_assigned_to_a_bank(pkg, name):
     """A tensor that took another's place would be used by one path and not by the other."""
     bank = bank_of(pkg)
     kept = dict(bank.__dict__)
-    value = getattr(bank, name, 1)
+    value = getattr(bank, name)
     with pytest.raises(AttributeError, match=name):
         setattr(bank, name, value.clone() if isinstance(value, torch.Tensor) else value)
     assert bank.__dict__.keys() == kept.keys() and all(bank.__dict__[k] is v for k, v in kept.items())
@@ -80,3 +80,23 @@ def test_a_patch_s_strength_does_not_go_through_16_bits(pkg, dtype, alpha, stren
         assert torch.equal(bank.down[:4, :10], down if middle is None else mid @ down) and bank.ranks == [0, 4]
         got = bank.up.view(6, 16)[:, :4].double() * bank.scale[1].double()
         assert (got - up.double() * scale).abs().max() <= 2.0 ** -23 * (up.double() * scale).abs().max()
+
+
+def test_a_bank_of_one_s_own_kind_has_attributes_of_its_own(pkg):
+    class Named(pkg.AdapterBank):
+        def __init__(self, *args, **kwargs):
+            super().__init__(*args, **kwargs)
+            self.name = "a"
+
+    bank = Named([(torch.ones(3, 8), torch.ones(6, 3))], dtype=torch.bfloat16, device="cpu")
+    bank.name = "b"
+    assert bank.name == "b"
+    with pytest.raises(AttributeError, match="up"):
+        bank.up = bank.up.clone()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_bank_of_shapes_alone(pkg, dtype):
+    """On the meta device there are no values to look at."""
+    bank = pkg.AdapterBank([(torch.ones(3, 8, device="meta"), torch.ones(6, 3, device="meta")), None], dtype=dtype, device="meta")
+    assert bank.up.is_meta and bank.up.shape == (96,) and bank.up.dtype == dtype and bank.scale.shape == (2,)
