@@ -6,11 +6,12 @@ The package replaces the W8A8 linear hot path of ComfyUI-INT8-Fast:
     int8_quant          quantisation helpers, Int8TensorwiseOps, INT8 LoRA adapters
     adapters            low-rank adapters of many requests beside shared projections
     block_norms         norms, gate and residual stream between two blocks in one pass
+    attention           norms and rotation of heads, attention over an encoder's states
     quarot              128-block Hadamard rotation
     compile_ops         torch.library operators (namespace i8f) for torch.compile
     nodes               ComfyUI graph nodes (model loader, LoRA loaders); ComfyUI is imported when they run
     dynamic_lora        hook for un-merged LoRA side branches
-    _lib                ctypes binding of libi8f_gfx950.so (include/i8f.h, include/i8f_blocks.h)
+    _lib                ctypes binding of libi8f_gfx950.so (include/i8f*.h)
     build               build of the library (hipcc) and of the host extension (g++)
 
 The directory name is ComfyUI's convention for custom nodes and is not a Python
@@ -48,6 +49,7 @@ from .int8_quant import (  # noqa: F401
     stochastic_round_int8_delta,
 )
 
+from .attention import RotaryAxes, cross_attention, forward_cross_attention, norm_heads, rotate_heads  # noqa: F401
 from .adapters import AdapterBank, forward_adapters  # noqa: F401
 from .block_norms import block_norm, forward_block_norm  # noqa: F401
 from .nodes import NODE_CLASS_MAPPINGS, NODE_DISPLAY_NAME_MAPPINGS  # noqa: E402,F401

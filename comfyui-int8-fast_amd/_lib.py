@@ -95,7 +95,11 @@ def lib() -> ctypes.CDLL:
     L.i8f_linear_w8a16_small_m_adapters.argtypes = [vp, i32, i64, i64, i64, vp, i32, vp]
     L.i8f_adapters_by_side.argtypes = [i64, i64, i64, i64]
     L.i8f_block_norm.argtypes = [vp, vp]
-    for name in BLOCK_EXPORTS:
+    L.i8f_norm_rotate.argtypes = [vp, vp, i32, vp]
+    L.i8f_attention.argtypes = [vp, vp]
+    L.i8f_attention_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i64]
+    L.i8f_attention_workspace_bytes.restype = i64
+    for name in (*BLOCK_EXPORTS, *ATTENTION_EXPORTS):
         if not name.endswith("_bytes"):
             getattr(L, name).restype = i32
     for name in ("i8f_quant_rowwise_concat_gelu", "i8f_quant_rowwise_rms_norm", "i8f_linear_w8a8_gated", "i8f_quant_rowwise", "i8f_quant_rowwise_grouped", "i8f_quant_rowwise_prologue", "i8f_quant_rowwise_norm_modulate", "i8f_quant_tensorwise", "i8f_quant_tensorwise_static", "i8f_rotate128", "i8f_gemm_i32", "i8f_linear_w8a8", "i8f_linear_w8a8_add", "i8f_linear_w8a8_splitk", "i8f_linear_w8a8_grouped", "i8f_linear_w8a8_lora",
@@ -136,6 +140,9 @@ EXPORTS = (
 # the entry points of include/i8f_blocks.h
 BLOCK_EXPORTS = ("i8f_adapters_by_side", "i8f_adapters_down_workspace_bytes", "i8f_adapters_down", "i8f_adapters_up", "i8f_linear_w8a8_adapters_workspace_bytes", "i8f_linear_w8a8_adapters",
                  "i8f_linear_w8a16_small_m_adapters", "i8f_block_norm")
+
+# the entry points of include/i8f_attention.h
+ATTENTION_EXPORTS = ("i8f_norm_rotate", "i8f_attention_workspace_bytes", "i8f_attention")
 
 ERR_UNSUPPORTED = -2   # I8F_ERR_UNSUPPORTED
 
@@ -1083,6 +1090,135 @@ def block_norm(y, residual, *, post_norm=None, post_weight=None, post_bias=None,
     with _on(y.device):
         _check(lib().i8f_block_norm(ctypes.byref(arg), _stream(y)), "i8f_block_norm")
     return (x, q, scale) if quantise else (x, h)
+
+
+MAX_HEAD_GROUPS, MAX_AXES, MAX_NORM_WIDTH, MAX_HEAD_WIDTH = 4, 4, 512, 256
+_POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
+_MASKS = {torch.bool: 0, torch.bfloat16: 1, torch.float16: 2, torch.float32: 3}
+
+
+class _Heads(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("batch_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("heads", ctypes.c_int64), ("weight", ctypes.c_void_p), ("weight_dtype", ctypes.c_int), ("out", ctypes.c_void_p)]
+
+
+class _NormRotateArgs(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int64), ("tokens", ctypes.c_int64), ("width", ctypes.c_int64), ("dtype", ctypes.c_int), ("norm", ctypes.c_int),
+                ("eps", ctypes.c_float), ("axes", ctypes.c_int), ("first_pair", ctypes.c_int * (MAX_AXES + 1)), ("apart", ctypes.c_int),
+                ("positions_type", ctypes.c_int), ("rates", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("position_batch", ctypes.c_int64),
+                ("position_token", ctypes.c_int64), ("position_axis", ctypes.c_int64)]
+
+
+class _AttentionArgs(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                *((n, ctypes.c_int64) for n in ("batch", "queries", "keys", "heads", "kv_heads", "width", "q_batch", "q_token", "q_head", "k_batch",
+                                                "k_token", "k_head", "v_batch", "v_token", "v_head")),
+                ("dtype", ctypes.c_int), ("scale", ctypes.c_float), ("key_lengths", ctypes.c_void_p), ("lengths_type", ctypes.c_int),
+                ("mask_type", ctypes.c_int), ("key_mask", ctypes.c_void_p), ("mask_batch", ctypes.c_int64), ("mask_key", ctypes.c_int64),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64)]
+
+
+def _unit_stride(t):
+    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def norm_rotate(xs, weights, norm, eps, rates, dims, apart, positions):
+    """i8f_norm_rotate on tensors of heads [batch, tokens, heads, width] or [tokens, heads, width]; rates [sum(dims) / 2] float64 and positions,
+    or neither (attention.norm_heads has the operands).  -> list of contiguous tensors."""
+    if not xs:
+        return []
+    first = xs[0]
+    for i, x in enumerate(xs):
+        _dev(x, f"xs[{i}]")
+        if x.dim() not in (3, 4) or x.dim() != first.dim() or x.shape[:-2] != first.shape[:-2] or x.shape[-1] != first.shape[-1]:
+            raise ValueError(f"heads must be [batch, tokens, heads, width] or [tokens, heads, width] of the same tokens and width, got {[list(x.shape) for x in xs]}")
+        if x.dtype != first.dtype or x.device != first.device:
+            raise TypeError(f"xs[{i}] is {x.dtype} on {x.device}, xs[0] {first.dtype} on {first.device}")
+    code, width, device = dtype_code(first.dtype), first.shape[-1], first.device
+    if not 1 <= width <= MAX_NORM_WIDTH:
+        raise ValueError(f"heads must be 1 to {MAX_NORM_WIDTH} elements wide, got {width}")
+    if not eps >= 0.0:
+        raise ValueError("eps must not be negative")
+    batch, tokens = first.shape[0] if first.dim() == 4 else 1, first.shape[-3]
+    arg = _NormRotateArgs(batch=batch, tokens=tokens, width=width, dtype=code, norm=int(bool(norm)), eps=eps, apart=int(bool(apart)))
+    if positions is not None:
+        _dev(positions, "positions")
+        _dev(rates, "rates")
+        if positions.dtype not in _POSITIONS or positions.device != device or rates.device != device:
+            raise TypeError(f"positions must be int32, int64, float32 or float64 and lie on {device} as the axes' rates: {positions.dtype} on {positions.device}, rates on {rates.device}")
+        p = positions.unsqueeze(0) if positions.dim() == 2 else positions
+        if p.dim() != 3 or p.shape[0] not in (1, batch) or p.shape[1] != tokens or p.shape[2] != len(dims):
+            raise ValueError(f"positions must be [{tokens}, {len(dims)}] or [{batch}, {tokens}, {len(dims)}], got {list(positions.shape)}")
+        if sum(dims) > width or rates.dtype != torch.float64 or rates.numel() * 2 != sum(dims) or not rates.is_contiguous():
+            raise ValueError(f"{sum(dims)} elements are turned by {rates.numel()} rates of {rates.dtype}, the heads have {width}")
+        ends = [0]
+        for n in dims:
+            ends.append(ends[-1] + n // 2)
+        arg.axes, arg.first_pair, arg.positions_type = len(dims), (ctypes.c_int * (MAX_AXES + 1))(*ends), _POSITIONS[positions.dtype]
+        arg.rates, arg.positions, arg.position_batch = _addr(rates), _addr(p), p.stride(0) if p.shape[0] == batch and batch > 1 else 0
+        arg.position_token, arg.position_axis = p.stride(1), p.stride(2)
+    outs, keep = [], []
+    groups = (_Heads * len(xs))()
+    for i, (x, w, g) in enumerate(zip(xs, weights, groups)):
+        if w is not None:
+            _dev(w, f"weights[{i}]")
+            if tuple(w.shape) != (width,) or w.dtype not in (x.dtype, torch.float32) or w.device != device:
+                raise ValueError(f"weights[{i}] must be [{width}] of {x.dtype} or float32 on {device}, got {list(w.shape)} of {w.dtype} on {w.device}")
+            w = w.contiguous()
+            g.weight, g.weight_dtype = _addr(w), dtype_code(w.dtype)
+        x = _unit_stride(x)
+        out = torch.empty(x.shape, dtype=x.dtype, device=device)
+        g.x, g.out, g.heads = _addr(x), _addr(out), x.shape[-2]
+        g.batch_stride, g.token_stride, g.head_stride = x.stride(0) if x.dim() == 4 else 0, x.stride(-3), x.stride(-2)
+        outs.append(out)
+        keep.append((x, w))
+    with _on(device):
+        for at in range(0, len(xs), MAX_HEAD_GROUPS):
+            n = min(MAX_HEAD_GROUPS, len(xs) - at)
+            _check(lib().i8f_norm_rotate(ctypes.byref(arg), ctypes.byref(groups, at * ctypes.sizeof(_Heads)), n, _stream(first)), "i8f_norm_rotate")
+    return outs
+
+
+def attention(q, k, v, key_lengths=None, key_mask=None, scale=None):
+    """i8f_attention on tensors (attention.cross_attention has the formula and the operands)."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _dev(t, name)
+        if t.dim() != 4:
+            raise ValueError(f"{name} must be [batch, tokens, heads, width], got {list(t.shape)}")
+        if t.dtype != q.dtype or t.device != q.device or t.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"q, k and v must be bfloat16 or float16, alike, on one device: {name} is {t.dtype} on {t.device}, q {q.dtype} on {q.device}")
+    batch, queries, heads, width = q.shape
+    keys, kv_heads = k.shape[1], k.shape[2]
+    if k.shape != v.shape or k.shape[0] != batch or k.shape[3] != width:
+        raise ValueError(f"k and v must be [{batch}, keys, kv heads, {width}] alike, got {list(k.shape)} and {list(v.shape)}")
+    if heads and (kv_heads == 0 or heads % kv_heads):
+        raise ValueError(f"{heads} heads cannot share {kv_heads} of the states")
+    if not 1 <= width <= MAX_HEAD_WIDTH:
+        raise ValueError(f"heads must be 1 to {MAX_HEAD_WIDTH} elements wide, got {width}")
+    scale = width ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale <= torch.finfo(torch.float32).max:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    q, k, v = _unit_stride(q), _unit_stride(k), _unit_stride(v)
+    out = torch.empty((batch, queries, heads, width), dtype=q.dtype, device=q.device)
+    arg = _AttentionArgs(_addr(q), _addr(k), _addr(v), _addr(out), batch, queries, keys, heads, kv_heads, width, *q.stride()[:3], *k.stride()[:3],
+                         *v.stride()[:3], dtype_code(q.dtype), scale)
+    if key_lengths is not None:
+        _dev(key_lengths, "key_lengths")
+        if key_lengths.dtype not in (torch.int32, torch.int64) or key_lengths.device != q.device or tuple(key_lengths.shape) != (batch,):
+            raise ValueError(f"key_lengths must be int32 or int64 [{batch}] on {q.device}, got {list(key_lengths.shape)} of {key_lengths.dtype} on {key_lengths.device}")
+        key_lengths = key_lengths.contiguous()
+        arg.key_lengths, arg.lengths_type = _addr(key_lengths), int(key_lengths.dtype == torch.int64)
+    if key_mask is not None:
+        _dev(key_mask, "key_mask")
+        if key_mask.dtype not in _MASKS or key_mask.device != q.device or tuple(key_mask.shape) != (batch, keys):
+            raise ValueError(f"key_mask must be bool or a floating type [{batch}, {keys}] on {q.device}, got {list(key_mask.shape)} of {key_mask.dtype} on {key_mask.device}")
+        arg.key_mask, arg.mask_type, arg.mask_batch, arg.mask_key = _addr(key_mask), _MASKS[key_mask.dtype], *key_mask.stride()
+    nbytes = lib().i8f_attention_workspace_bytes(batch, queries, keys, heads, kv_heads, width)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    arg.workspace, arg.workspace_bytes = _addr(work), nbytes
+    with _on(q.device):
+        _check(lib().i8f_attention(ctypes.byref(arg), _stream(q)), "i8f_attention")
+    return out
 
 
 def version() -> int:

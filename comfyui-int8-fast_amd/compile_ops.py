@@ -16,6 +16,8 @@ the namespace `i8f` with a shape-only ("fake") implementation:
                                            torch.compile's fusion into the Triton quantiser gives the reference
     torch.ops.i8f.linear_adapters, add_adapters         the two ways of adapters.forward_adapters
     torch.ops.i8f.block_norm, block_norm_quantised      block_norms.block_norm and the int8 form in front of layers
+    torch.ops.i8f.norm_rotate_heads                     attention.norm_heads and rotate_heads
+    torch.ops.i8f.cross_attention                       attention.cross_attention
 
 `Int8TensorwiseOps.Linear.forward` switches to these operators while a graph is being traced
 (`torch.compiler.is_compiling()`); in eager mode it calls the library directly, which saves the
@@ -274,8 +276,31 @@ def _(y, residual, rotate, post_norm=None, post_weight=None, post_bias=None, pos
     return y.new_empty(y.shape), y.new_empty((M, K), dtype=torch.int8), y.new_empty((M, 1), dtype=torch.float32)
 
 
+@torch.library.custom_op(f"{NAMESPACE}::norm_rotate_heads", mutates_args=())
+def norm_rotate_heads(xs: Sequence[Tensor], weights: Sequence[Optional[Tensor]], norm: bool, eps: float, rates: Optional[Tensor], dims: Sequence[int],
+                      apart: bool, positions: Optional[Tensor]) -> List[Tensor]:
+    return _lib.norm_rotate(xs, weights, norm, eps, rates, dims, apart, positions)
+
+
+@norm_rotate_heads.register_fake
+def _(xs, weights, norm, eps, rates, dims, apart, positions):
+    return [x.new_empty(x.shape) for x in xs]
+
+
+@torch.library.custom_op(f"{NAMESPACE}::cross_attention", mutates_args=())
+def cross_attention(q: Tensor, k: Tensor, v: Tensor, key_lengths: Optional[Tensor] = None, key_mask: Optional[Tensor] = None,
+                    scale: Optional[float] = None) -> Tensor:
+    return _lib.attention(q, k, v, key_lengths, key_mask, scale)
+
+
+@cross_attention.register_fake
+def _(q, k, v, key_lengths=None, key_mask=None, scale=None):
+    return q.new_empty(q.shape)
+
+
 OPS = ("quantize_rowwise", "quantize_rowwise_prologue", "rotate128", "linear_w8a8", "int8_linear", "int8_linear_lora",
-       "linear_w8a16_small_m", "int8_linear_prologue", "linear_adapters", "add_adapters", "block_norm", "block_norm_quantised")
+       "linear_w8a16_small_m", "int8_linear_prologue", "linear_adapters", "add_adapters", "block_norm", "block_norm_quantised",
+       "norm_rotate_heads", "cross_attention")
 
 
 # --------------------------------------------------------------------------- graph rewrite
