@@ -97,7 +97,7 @@ def lib() -> ctypes.CDLL:
     L.i8f_block_norm.argtypes = [vp, vp]
     L.i8f_norm_rotate.argtypes = [vp, vp, i32, vp]
     L.i8f_attention.argtypes = [vp, vp]
-    L.i8f_attention_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i64]
+    L.i8f_attention_workspace_bytes.argtypes = [vp]
     L.i8f_attention_workspace_bytes.restype = i64
     for name in (*BLOCK_EXPORTS, *ATTENTION_EXPORTS):
         if not name.endswith("_bytes"):
@@ -1213,7 +1213,7 @@ def attention(q, k, v, key_lengths=None, key_mask=None, scale=None):
         if key_mask.dtype not in _MASKS or key_mask.device != q.device or tuple(key_mask.shape) != (batch, keys):
             raise ValueError(f"key_mask must be bool or a floating type [{batch}, {keys}] on {q.device}, got {list(key_mask.shape)} of {key_mask.dtype} on {key_mask.device}")
         arg.key_mask, arg.mask_type, arg.mask_batch, arg.mask_key = _addr(key_mask), _MASKS[key_mask.dtype], *key_mask.stride()
-    nbytes = lib().i8f_attention_workspace_bytes(batch, queries, keys, heads, kv_heads, width)
+    nbytes = lib().i8f_attention_workspace_bytes(ctypes.byref(arg))
     work = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     arg.workspace, arg.workspace_bytes = _addr(work), nbytes
     with _on(q.device):

@@ -1,7 +1,15 @@
 // Attention over an encoder's states (include/i8f_attention.h has the formula).
+//
+// A wave takes 32 rows and goes over the states in tiles, keeping the running maximum and sum of a softmax.  A row is a query of one of the
+// heads that share a head of the states, so that one token's 32 heads over 8 fill eight waves' rows by fours and every state is read once.
+// Both products are computed transposed: S^T = K Q^T leaves a lane with 16 scores of ONE row in every 32 x 32 block, so that maximum and sum are
+// in-lane but for one exchange of wave halves, and rounded to 16 bits the scores' weights already are the second operand of
+// O^T = V^T P^T, the contraction index being free to run in the order in which a lane happens to hold the states; the first operand comes
+// out of row-major V by LDS reads that transpose (ds_read_b64_tr_b16).
 #include <initializer_list>
 #include <utility>
 
+#include "dma.hpp"
 #include "i8f_common.hpp"
 
 #include "../../include/i8f_attention.h"
@@ -9,57 +17,484 @@
 namespace i8f {
 namespace {
 
-// Whether state j of batch b counts, and its addend.
-__device__ __forceinline__ bool counts(const i8f_attention_args &a, int64_t b, int64_t j, float &m) {
-    m = 0.0f;
-    if (!a.key_mask) return true;
-    const int64_t at = b * a.mask_batch + j * a.mask_key;
-    switch (a.mask_type) {
-    case I8F_MASK_BYTES: return ((const uint8_t *)a.key_mask)[at] != 0;
-    case I8F_MASK_BF16: m = load_as_f32<I8F_BF16>(a.key_mask, at); return !(m <= -3.3895313892515355e38f);
-    case I8F_MASK_F16: m = load_as_f32<I8F_F16>(a.key_mask, at); return !(m <= -65504.0f);
-    default: m = ((const float *)a.key_mask)[at]; return !(m <= -3.4028234663852886e38f);
+using gemm::dma16;
+using gemm::make_rsrc;
+using gemm::v4i;
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef short v8s __attribute__((ext_vector_type(8)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+
+constexpr float LOWEST = -3.4028234663852886e38f, TO_LOG2 = 1.4426950408889634f;
+
+struct Launch {
+    i8f_attention_args a;
+    uint32_t share, rows;        // heads to one of the states', rows = queries * share to (batch, state head)
+    uint32_t row_tiles, splits;  // of a (batch, state head)
+    uint32_t tiles;              // of a split, in tiles of the kernel
+    uint32_t loaded;             // elements of a row in memory, whole pieces of eight
+    uint32_t wide_out;           // rows of the result may be written four elements at a time
+    float *partial;             // splits > 1: [batch * kv_heads, splits, rows, padded width], then [.., rows, 2]: maximum and sum
+    float *stats;
+};
+
+template <int DT>
+__device__ __forceinline__ v16f mfma(v8s a, v8s b, v16f c) {
+    if constexpr (DT == I8F_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+// two weights rounded to the type, and their sum as they were rounded added to `sum`
+template <int DT>
+__device__ __forceinline__ uint32_t round_weights(float lo, float hi, float &sum) {
+    if constexpr (DT == I8F_BF16) {
+        const uint32_t w = f32x2_to_bf16x2_bits(lo, hi);
+        sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w), __builtin_bit_cast(v2bf, 0x3f803f80u), sum, false);
+        return w;
+    } else {
+        const uint32_t w = f32x2_to_f16x2_bits(lo, hi);
+        sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, w), __builtin_bit_cast(half2v, 0x3c003c00u), sum, false);
+        return w;
     }
 }
+// the other half of the wave's value beside the own
+__device__ __forceinline__ float max_of_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_of_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 
-// A wave to a query's head: 64 states at a time, a lane to a state for the scores and a lane to every 64th element for the result.
-template <int DT>
-__global__ __launch_bounds__(256) void attention_kernel(const i8f_attention_args a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= a.batch * a.queries * a.heads) return;
-    const int64_t h = row % a.heads, i = row / a.heads % a.queries, b = row / a.heads / a.queries, g = h / (a.heads / a.kv_heads);
-    const int64_t qb = b * a.q_batch + i * a.q_token + h * a.q_head, kb = b * a.k_batch + g * a.k_head, vb = b * a.v_batch + g * a.v_head;
+// Whether state j of batch b counts, and its addend in units of log 2.
+__device__ __forceinline__ bool counts(const i8f_attention_args &a, int64_t b, int64_t j, float &m) {
+    const int64_t at = b * a.mask_batch + j * a.mask_key;
+    m = 0.0f;
+    bool on;
+    switch (a.mask_type) {
+    case I8F_MASK_BYTES: return ((const uint8_t *)a.key_mask)[at] != 0;
+    case I8F_MASK_BF16: m = load_as_f32<I8F_BF16>(a.key_mask, at), on = !(m <= -3.3895313892515355e38f); break;
+    case I8F_MASK_F16: m = load_as_f32<I8F_F16>(a.key_mask, at), on = !(m <= -65504.0f); break;
+    default: m = ((const float *)a.key_mask)[at], on = !(m <= LOWEST); break;
+    }
+    m = on ? fmaxf(m * TO_LOG2, LOWEST) : 0.0f;
+    return on;
+}
+
+// The 16-byte pieces of a row are exchanged within it by a function of the row, so that the lanes of an LDS read are spread over the banks.
+// K is read by eight rows' same piece at a time (ds_read_b128), V by four rows' same 64 bytes (ds_read_b64_tr_b16); rows of 192 bytes lie
+// three quarters of the banks apart by themselves.
+template <int DP>
+__device__ __forceinline__ int k_piece(int row, int piece) {
+    if constexpr (DP == 96) return piece ^ ((row >> 2) & 1);
+    else if constexpr (DP % 128 == 0) return piece ^ (row & 7);
+    else return piece ^ ((row >> 1) & 7);
+}
+template <int DP>
+__device__ __forceinline__ int v_quad(int row) {   // what the number of a row's 64-byte quarter is exchanged by
+    if constexpr (DP == 96) return 0;
+    else if constexpr (DP % 128 == 0) return row & 3;
+    else return (row >> 1) & 1;
+}
+
+// DP: the width, padded.  APART: the waves of a workgroup have the same rows and a tile of 32 states each, by themselves; otherwise 32 rows
+// each and a tile of 64 states together.
+template <int DT, int DP, bool APART, bool MASK>
+struct Shape {
+    static constexpr int WAVES = APART && DP > 128 ? 2 : 4, KT = APART ? 32 : 64, PIECES = DP / 8, TILE = KT * DP * 2;
+    static constexpr int LOADS = KT * PIECES / 64 / (APART ? 1 : WAVES);       // a wave's of a tile of K, or of V
+    static constexpr int SETS = APART ? WAVES : 1, LDS = SETS * 4 * TILE;      // two stages of K and V
+    static constexpr int ROWS = APART ? 32 : 32 * WAVES;
+};
+
+template <int DT, int DP, bool APART, bool MASK>
+__global__ __launch_bounds__((Shape<DT, DP, APART, MASK>::WAVES * 64), (Shape<DT, DP, APART, MASK>::LDS <= 80 * 1024 ? 2 : 1)) void attention_kernel(const Launch p) {
+    using S = Shape<DT, DP, APART, MASK>;
+    constexpr int KT = S::KT, KB = KT / 32, NK = DP / 16, ND = DP / 32, WAVES = S::WAVES;
+    __shared__ __attribute__((aligned(16))) char lds[S::LDS + (MASK ? WAVES * 64 * 4 : 0)];
+    const i8f_attention_args &a = p.a;
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // the workgroups of an XCD (number mod 8) take consecutive row tiles of the same states
+    const unsigned per = gridDim.x / 8, extra = gridDim.x % 8, xcd = blockIdx.x % 8;
+    const unsigned id = xcd * per + (xcd < extra ? xcd : extra) + blockIdx.x / 8;
+    const unsigned row_tile = id % p.row_tiles, split = id / p.row_tiles % p.splits, bg = id / p.row_tiles / p.splits;
+    const int64_t b = bg / (unsigned)a.kv_heads, g = bg % (unsigned)a.kv_heads;
     int64_t n = a.keys;
     if (a.key_lengths) {
         const int64_t given = a.lengths_type ? ((const int64_t *)a.key_lengths)[b] : ((const int32_t *)a.key_lengths)[b];
         n = given < 0 ? 0 : given < n ? given : n;
     }
-    const float to_log2 = 1.4426950408889634f;
-    float top = -3.4028234663852886e38f, total = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int64_t j0 = 0; j0 < n; j0 += 64) {
-        float s = -__builtin_inff(), m;
-        const int64_t j = j0 + lane;
-        const bool in = j < n && counts(a, b, j, m);
-        if (in) {
-            float dot = 0.0f;
-            for (int e = 0; e < a.width; ++e) dot = __builtin_fmaf(load_as_f32<DT>(a.q, qb + e), load_as_f32<DT>(a.k, kb + j * a.k_token + e), dot);
-            s = __builtin_fmaf(dot, a.scale * to_log2, m * to_log2);
-        }
-        const float new_top = fmaxf(top, wave_max(s)), fade = __builtin_amdgcn_exp2f(top - new_top);
-        const float p = in ? __builtin_amdgcn_exp2f(s - new_top) : 0.0f;
-        top = new_top, total = total * fade + p;
-        for (int e = 0; e < 4; ++e) o[e] *= fade;
-        for (uint64_t left = __ballot(in); left; left &= left - 1) {
-            const int x = __builtin_ctzll(left);
-            const float px = round_to_dtype<DT>(__shfl(p, x));
-            for (int e = 0; e < 4; ++e)
-                if (e * 64 + lane < a.width) o[e] = __builtin_fmaf(px, load_as_f32<DT>(a.v, vb + (j0 + x) * a.v_token + e * 64 + lane), o[e]);
+    int64_t last_tile = (n + KT - 1) / KT, tile = (int64_t)split * p.tiles;
+    last_tile = last_tile < tile + p.tiles ? last_tile : tile + p.tiles;
+    if constexpr (APART) tile += wave;   // (every WAVES-th tile)
+    constexpr int STEP = APART ? WAVES : 1;
+
+    // a wave's 32 rows, a lane's in both halves
+    const unsigned row = row_tile * S::ROWS + (APART ? 0 : wave * 32) + (lane & 31), real = row < p.rows ? row : p.rows - 1;
+    const int64_t query = real / p.share, head = g * p.share + real % p.share;
+    v8s q[NK];
+    {
+        const uint16_t *qp = (const uint16_t *)a.q + b * a.q_batch + query * a.q_token + head * a.q_head;
+#pragma unroll
+        for (int s = 0; s < NK; ++s) {
+            const unsigned e = s * 16 + half * 8;
+            q[s] = e < p.loaded ? *(const v8s *)(qp + e) : v8s{};
         }
     }
-    for (int x = 1; x < 64; x *= 2) total += __shfl_xor(total, x);
-    for (int e = 0; e < 4; ++e)
-        if (e * 64 + lane < a.width) store_from_f32<DT>(a.out, row * a.width + e * 64 + lane, total > 0.0f ? o[e] / total : total);
+    const float to_log2 = a.scale * TO_LOG2;
+
+    // where a lane's pieces of a tile come from: LDS is filled in order, 16 bytes a lane
+    constexpr uint32_t NOWHERE = 0x80000000u;   // (behind the buffer's end: such a piece is zeros)
+    uint32_t from_k[S::LOADS], from_v[S::LOADS];
+    auto piece_at = [&](int i) { return (APART ? i : i * WAVES + wave) * 64 + lane; };
+#pragma unroll
+    for (int i = 0; i < S::LOADS; ++i) {
+        const int at = piece_at(i), r = at / S::PIECES, c = at % S::PIECES;
+        const unsigned ck = k_piece<DP>(r, c), cv = c ^ (v_quad<DP>(r) << 2);
+        from_k[i] = ck * 8 < p.loaded ? (uint32_t)(r * a.k_token + ck * 8) * 2u : NOWHERE;
+        from_v[i] = cv * 8 < p.loaded ? (uint32_t)(r * a.v_token + cv * 8) * 2u : NOWHERE;
+    }
+    const uint16_t *kp = (const uint16_t *)a.k + b * a.k_batch + g * a.k_head, *vp = (const uint16_t *)a.v + b * a.v_batch + g * a.v_head;
+    const uint32_t lds_at = (uint32_t)(uintptr_t)(gemm::lds_ptr_t)lds + (APART ? wave * 4 * S::TILE : 0);   // stage s: K at s * 2 * TILE, V behind it
+
+    // which states of tile t count: bit j for the tile's state j; with a mask a lane's own addend besides
+    auto on_of = [&](int64_t t, float &add) -> uint64_t {
+        const int64_t left = n - t * KT;
+        if constexpr (!MASK) {
+            return left >= 64 ? ~0ull : left <= 0 ? 0ull : KT == 32 && left >= 32 ? 0xffffffffull : (1ull << left) - 1;
+        } else {
+            const int64_t j = t * KT + lane;
+            bool on = lane < KT && lane < left;
+            add = 0.0f;
+            if (on) on = counts(a, b, j, add);
+            return __ballot(on);
+        }
+    };
+    constexpr uint64_t ALL = KT == 64 ? ~0ull : 0xffffffffull;
+    auto request = [&](int64_t t, int stage, uint64_t on) {
+        const v4i kr = make_rsrc(kp + t * KT * a.k_token, 0x7ffffff0u), vr = make_rsrc(vp + t * KT * a.v_token, 0x7ffffff0u);
+        const uint32_t to = lds_at + stage * 2 * S::TILE + (APART ? 0 : wave * 1024);
+        if ((on & ALL) == ALL) {
+#pragma unroll
+            for (int i = 0; i < S::LOADS; ++i) dma16(kr, to + i * (APART ? 1 : WAVES) * 1024, from_k[i], 0);
+#pragma unroll
+            for (int i = 0; i < S::LOADS; ++i) dma16(vr, to + S::TILE + i * (APART ? 1 : WAVES) * 1024, from_v[i], 0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < S::LOADS; ++i) {
+                const bool in = on >> (piece_at(i) / S::PIECES) & 1;
+                dma16(kr, to + i * (APART ? 1 : WAVES) * 1024, in ? from_k[i] : NOWHERE, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < S::LOADS; ++i) {
+                const bool in = on >> (piece_at(i) / S::PIECES) & 1;
+                dma16(vr, to + S::TILE + i * (APART ? 1 : WAVES) * 1024, in ? from_v[i] : NOWHERE, 0);
+            }
+        }
+    };
+
+    v16f o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[d] = v16f{};
+    float top = LOWEST, sum = 0.0f;
+    constexpr float RAISE = DT == I8F_F16 ? 6.0f : 0.0f;   // (binary16 weights lie between 2^6 and 2^14 for the largest: see below)
+
+    // where a lane reads: K row (lane & 31) of a block, V's four rows from 4 half on by 16 elements
+    const int k_row = (lane & 31) * DP * 2;
+    const int v_row = (4 * half + ((lane >> 2) & 3)) * DP * 2 + (2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) * 16 + (lane & 1) * 8;
+    const int v_x = v_quad<DP>((lane >> 2) & 3);
+    float *const adds = (float *)(lds + S::LDS) + wave * 64;
+
+    float add = 0.0f;
+    uint64_t on = 0;
+    auto next_tile = [&](int64_t t) {   // the first tile from t on with a state that counts
+        while (t < last_tile && (on = on_of(t, add)) == 0) t += STEP;
+        return t;
+    };
+    tile = next_tile(tile);
+    if (tile < last_tile) request(tile, 0, on);
+    int stage = 0;
+    while (tile < last_tile) {
+        const uint64_t now = on;
+        if constexpr (MASK) adds[lane] = add;
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if constexpr (!APART) __builtin_amdgcn_s_barrier();   // everyone's pieces of the tile are there, and the other stage has been read
+        asm volatile("" ::: "memory");
+        const int64_t next = next_tile(tile + STEP);
+        if (next < last_tile) request(next, stage ^ 1, on);
+
+        const char *ks = lds + (APART ? wave * 4 * S::TILE : 0) + stage * 2 * S::TILE, *vs = ks + S::TILE;
+        v16f s[KB];
+#pragma unroll
+        for (int k = 0; k < KB; ++k) s[k] = v16f{};
+#pragma unroll
+        for (int e = 0; e < NK; ++e)
+#pragma unroll
+            for (int k = 0; k < KB; ++k)
+                s[k] = mfma<DT>(*(const v8s *)(ks + k * 32 * DP * 2 + k_row + k_piece<DP>(lane & 31, 2 * e + half) * 16), q[e], s[k]);
+        // scores: times the scale in the exponential's argument, or here where addends come on top
+        float factor = to_log2;
+        if constexpr (MASK) {
+            if (a.mask_type != I8F_MASK_BYTES) {
+#pragma unroll
+                for (int k = 0; k < KB; ++k)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[k][i] = __builtin_fmaf(s[k][i], to_log2, adds[k * 32 + 8 * (i / 4) + 4 * half + i % 4]);
+                factor = 1.0f;
+            }
+        }
+        if ((now & ALL) != ALL) {
+#pragma unroll
+            for (int k = 0; k < KB; ++k) {
+                const uint32_t mine = (uint32_t)(now >> (32 * k)) >> (4 * half);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[k][i] = mine >> (8 * (i / 4) + i % 4) & 1 ? s[k][i] : -__builtin_inff();
+            }
+        }
+        float most = s[0][0];
+#pragma unroll
+        for (int k = 0; k < KB; ++k)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) most = fmaxf(most, s[k][i]);
+        most = max_of_halves(most) * factor;
+        // The reference of the exponentials follows the maximum only where that has grown by 2^8: the weights are below 2^8 then, which costs
+        // no bits, and the result is divided by their sum either way.
+        if (__any(most > top + 8.0f)) {
+            const float to = fmaxf(top, most), fade = __builtin_amdgcn_exp2f(top - to);
+            top = to;
+            sum *= fade;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[d] *= fade;
+        }
+        const float from = RAISE - top;
+#pragma unroll
+        for (int k = 0; k < KB; ++k)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    w[i] = round_weights<DT>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[k][8 * j + 2 * i], factor, from)),
+                                             __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][8 * j + 2 * i + 1], factor, from)), sum);
+                const v8s weights = __builtin_bit_cast(v8s, (v4i){(int)w[0], (int)w[1], (int)w[2], (int)w[3]});
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    typedef __attribute__((address_space(3))) v4s *v4s_lds;
+                    const char *at = vs + (k * 32 + j * 16) * DP * 2 + v_row + (d ^ v_x) * 64;
+                    const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s_lds)(gemm::lds_ptr_t)at);
+                    const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s_lds)(gemm::lds_ptr_t)(at + 8 * DP * 2));
+                    o[d] = mfma<DT>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), weights, o[d]);
+                }
+            }
+        tile = next, stage ^= 1;
+    }
+
+    // a lane has elements 32 d + 8 (i / 4) + 4 half + i % 4 of its row
+    sum = sum_of_halves(sum);
+    if constexpr (APART) {   // the waves' results meet in LDS, in the place of their tiles
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __syncthreads();
+        float *const others = (float *)lds;   // [WAVES][32][DP + 4]
+        constexpr int PITCH = DP + 4;
+        static_assert(WAVES * 32 * (PITCH + 2) * 4 <= S::LDS, "");
+        float *const heads = others + WAVES * 32 * PITCH;   // [WAVES][32][2]
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float4 v = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+                *(float4 *)(others + (wave * 32 + (lane & 31)) * PITCH + 32 * d + 8 * i + 4 * half) = v;
+            }
+        if (half == 0) heads[(wave * 32 + lane) * 2] = top, heads[(wave * 32 + lane) * 2 + 1] = sum;
+        __syncthreads();
+        constexpr int QUADS = DP / 4;
+        for (int at = threadIdx.x; at < 32 * QUADS; at += WAVES * 64) {
+            const int r = at / QUADS, e = at % QUADS * 4;
+            const unsigned own = row_tile * 32 + r;
+            if (own >= p.rows) continue;
+            float best = LOWEST, total = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) best = fmaxf(best, heads[(w * 32 + r) * 2]);
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                const float f = __builtin_amdgcn_exp2f(heads[(w * 32 + r) * 2] - best);
+                total = __builtin_fmaf(heads[(w * 32 + r) * 2 + 1], f, total);
+                const float4 x = *(const float4 *)(others + (w * 32 + r) * PITCH + e);
+                v[0] = __builtin_fmaf(x.x, f, v[0]), v[1] = __builtin_fmaf(x.y, f, v[1]), v[2] = __builtin_fmaf(x.z, f, v[2]), v[3] = __builtin_fmaf(x.w, f, v[3]);
+            }
+            if (p.splits > 1) {
+                const int64_t at_row = ((int64_t)bg * p.splits + split) * p.rows + own;
+                *(float4 *)(p.partial + at_row * DP + e) = make_float4(v[0], v[1], v[2], v[3]);
+                if (e == 0) p.stats[at_row * 2] = best, p.stats[at_row * 2 + 1] = total;
+            } else {
+                const int64_t to = ((b * a.queries + own / p.share) * a.heads + g * p.share + own % p.share) * a.width;
+                for (int i = 0; i < 4; ++i)
+                    if (e + i < a.width) store_from_f32<DT>(a.out, to + e + i, total == 0.0f ? 0.0f : v[i] / total);
+            }
+        }
+    } else {
+        if (row >= p.rows) return;
+        if (p.splits > 1) {
+            const int64_t at_row = ((int64_t)bg * p.splits + split) * p.rows + row;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *(float4 *)(p.partial + at_row * DP + 32 * d + 8 * i + 4 * half) = make_float4(o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]);
+            if (half == 0) p.stats[at_row * 2] = top, p.stats[at_row * 2 + 1] = sum;
+            return;
+        }
+        const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+        uint16_t *const to = (uint16_t *)a.out + ((b * a.queries + query) * a.heads + head) * a.width;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int e = 32 * d + 8 * i + 4 * half;
+                if (p.wide_out) {
+                    if (e < a.width) {
+                        const float x = o[d][4 * i] * by, y = o[d][4 * i + 1] * by, z = o[d][4 * i + 2] * by, w = o[d][4 * i + 3] * by;
+                        const uint2 v = DT == I8F_BF16 ? make_uint2(f32x2_to_bf16x2_bits(x, y), f32x2_to_bf16x2_bits(z, w)) : make_uint2(f32x2_to_f16x2_bits(x, y), f32x2_to_f16x2_bits(z, w));
+                        stream_store8(to + e, v);
+                    }
+                } else {
+                    for (int j = 0; j < 4; ++j)
+                        if (e + j < a.width) store_from_f32<DT>(to, e + j, o[d][4 * i + j] * by);
+                }
+            }
+    }
+}
+
+// The splits' results of a row joined: a wave to a row.
+template <int DT>
+__global__ __launch_bounds__(256) void join_kernel(const Launch p, const int padded) {
+    const i8f_attention_args &a = p.a;
+    const int lane = threadIdx.x & 63;
+    const unsigned at = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (at >= a.batch * a.kv_heads * p.rows) return;
+    const unsigned row = at % p.rows;
+    const int64_t bg = at / p.rows, b = bg / a.kv_heads, g = bg % a.kv_heads;
+    float best = LOWEST;
+    for (unsigned s = lane; s < p.splits; s += 64) best = fmaxf(best, p.stats[((bg * p.splits + s) * p.rows + row) * 2]);
+    best = wave_max(best);
+    float total = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (unsigned s = 0; s < p.splits; ++s) {
+        const int64_t r = (bg * p.splits + s) * p.rows + row;
+        const float f = __builtin_amdgcn_exp2f(p.stats[r * 2] - best);
+        total = __builtin_fmaf(p.stats[r * 2 + 1], f, total);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i * 64 + lane < padded) v[i] = __builtin_fmaf(p.partial[r * padded + i * 64 + lane], f, v[i]);
+    }
+    const int64_t to = ((b * a.queries + row / p.share) * a.heads + g * p.share + row % p.share) * a.width;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i * 64 + lane < a.width) store_from_f32<DT>(a.out, to + i * 64 + lane, total == 0.0f ? 0.0f : v[i] / total);
+}
+
+// [batch, tokens, heads, width] of any strides and alignment as contiguous rows of whole 16-byte pieces, the rest of them zeros.
+struct Pack {
+    const uint16_t *x;
+    uint16_t *out;
+    int64_t rows, tokens, heads, batch_stride, token_stride, head_stride;
+    int width, padded;
+};
+struct Packs {
+    Pack p[3];
+};
+__global__ __launch_bounds__(256) void pack_kernel(const Packs packs) {
+    const Pack &p = packs.p[blockIdx.y];
+    const int pieces = p.padded / 8;
+    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < p.rows * pieces; at += (int64_t)gridDim.x * 256) {
+        const int64_t row = at / pieces, h = row % p.heads, t = row / p.heads % p.tokens, b = row / p.heads / p.tokens;
+        const int e = (int)(at % pieces) * 8;
+        const uint16_t *x = p.x + b * p.batch_stride + t * p.token_stride + h * p.head_stride + e;
+        uint16_t v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = e + i < p.width ? x[i] : (uint16_t)0;
+        uint4 o;
+        __builtin_memcpy(&o, v, 16);
+        *(uint4 *)(p.out + at * 8) = o;
+    }
+}
+
+// ---- how a call is cut ------------------------------------------------------------------------------------------------------------
+struct Plan {
+    int padded;               // width of the kernels
+    bool apart;               // few rows: the waves of a workgroup take the states in turn
+    int64_t row_tiles, splits, tiles;
+    int64_t partial_bytes;    // of results and statistics of the splits
+};
+int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+Plan plan_of(int64_t batch, int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads, int64_t width) {
+    Plan p = {};
+    p.padded = width <= 64 ? 64 : width <= 96 ? 96 : width <= 128 ? 128 : width <= 192 ? 192 : 256;
+    const int64_t rows = queries * (heads / kv_heads), sets = batch * kv_heads;
+    p.apart = rows <= 32;
+    const int waves = p.apart && p.padded > 128 ? 2 : 4;
+    p.row_tiles = p.apart ? (rows + 31) / 32 : (rows + 127) / 128;
+    const int64_t tile = p.apart ? 32 : 64, all = (keys + tile - 1) / tile, groups = sets * p.row_tiles;
+    // as many splits as make 512 workgroups, of at least 4 tiles to a wave
+    const int64_t least = 4 * (p.apart ? waves : 1);
+    p.splits = groups >= 256 || all < 2 * least ? 1 : (512 + groups - 1) / groups;
+    if (p.splits > all / least) p.splits = all / least;
+    if (p.splits < 1) p.splits = 1;
+    p.tiles = round_up((all + p.splits - 1) / p.splits, p.apart ? waves : 1);
+    if (p.tiles < 1) p.tiles = 1;
+    p.splits = all ? (all + p.tiles - 1) / p.tiles : 1;
+    p.partial_bytes = p.splits > 1 ? sets * p.splits * rows * (p.padded + 2) * 4 : 0;
+    return p;
+}
+
+// The kernels read 16-byte pieces, and a tile's rows by 32-bit offsets.
+constexpr int64_t MOST_STRIDE = 1 << 22;
+bool in_pieces(const void *x, int64_t width, std::initializer_list<int64_t> strides, int64_t token) {
+    if ((uintptr_t)x % 16 || width % 8 || token > MOST_STRIDE) return false;
+    for (int64_t s : strides)
+        if (s % 8) return false;
+    return true;
+}
+// Which of q, k and v (bits 0 to 2) have to be copied into whole pieces first, and the bytes of the copies.
+int to_pack(const i8f_attention_args &a, int64_t (&bytes)[3]) {
+    const bool in[3] = {in_pieces(a.q, a.width, {a.q_batch, a.q_token, a.q_head}, 0), in_pieces(a.k, a.width, {a.k_batch, a.k_token, a.k_head}, a.k_token),
+                        in_pieces(a.v, a.width, {a.v_batch, a.v_token, a.v_head}, a.v_token)};
+    const int64_t states = a.batch * a.keys * a.kv_heads, rows[3] = {a.batch * a.queries * a.heads, states, states};
+    int which = 0;
+    for (int i = 0; i < 3; ++i) bytes[i] = in[i] ? 0 : rows[i] * round_up(a.width, 8) * 2, which |= in[i] ? 0 : 1 << i;
+    return which;
+}
+
+template <int DT, int DP, bool APART, bool MASK>
+int launch_tiles(const Launch &p, int64_t groups, hipStream_t st) {
+    using S = Shape<DT, DP, APART, MASK>;
+    if (!grid_fits(groups, S::WAVES * 64)) return I8F_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((attention_kernel<DT, DP, APART, MASK>), dim3((unsigned)groups), dim3(S::WAVES * 64), 0, st, p);
+    return check_launch();
+}
+template <int DT, int DP>
+int launch_form(const Launch &p, bool apart, int64_t groups, hipStream_t st) {
+    if (p.a.key_mask) return apart ? launch_tiles<DT, DP, true, true>(p, groups, st) : launch_tiles<DT, DP, false, true>(p, groups, st);
+    return apart ? launch_tiles<DT, DP, true, false>(p, groups, st) : launch_tiles<DT, DP, false, false>(p, groups, st);
+}
+template <int DT>
+int launch(const Launch &p, const Plan &plan, hipStream_t st) {
+    const int64_t groups = p.a.batch * p.a.kv_heads * p.row_tiles * p.splits;
+    int rc;
+    switch (plan.padded) {
+    case 64: rc = launch_form<DT, 64>(p, plan.apart, groups, st); break;
+    case 96: rc = launch_form<DT, 96>(p, plan.apart, groups, st); break;
+    case 128: rc = launch_form<DT, 128>(p, plan.apart, groups, st); break;
+    case 192: rc = launch_form<DT, 192>(p, plan.apart, groups, st); break;
+    default: rc = launch_form<DT, 256>(p, plan.apart, groups, st); break;
+    }
+    if (rc || p.splits == 1) return rc;
+    const int64_t rows = p.a.batch * p.a.kv_heads * p.rows;
+    hipLaunchKernelGGL((join_kernel<DT>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p, plan.padded);
+    return check_launch();
 }
 
 // The elements that a strided tensor reaches to from its first one, 0 for one without elements, -1 past 2^62.
@@ -87,7 +522,7 @@ int validate(const i8f_attention_args &a) {
     for (int64_t n : {a.batch, a.queries, a.keys, a.heads})
         if (n > 0x7fffffff) return I8F_ERR_UNSUPPORTED;
     const int64_t rows = a.batch * a.queries;
-    if (rows && a.heads > ((int64_t)1 << 33) / rows) return I8F_ERR_UNSUPPORTED;
+    if (rows && a.heads > 0x7fffffff / rows) return I8F_ERR_UNSUPPORTED;   // (rows are counted in 32 bits)
     if (a.key_lengths && a.lengths_type != 0 && a.lengths_type != 1) return I8F_ERR_INVALID;
     if (a.key_mask && (a.mask_type < I8F_MASK_BYTES || a.mask_type > I8F_MASK_F32 || a.mask_batch < 0 || a.mask_key < 0)) return I8F_ERR_INVALID;
     const int64_t out = rows * a.heads * a.width, q = extent({{a.batch, a.q_batch}, {a.queries, a.q_token}, {a.heads, a.q_head}, {a.width, 1}});
@@ -103,18 +538,52 @@ int validate(const i8f_attention_args &a) {
 }  // namespace
 }  // namespace i8f
 
-extern "C" int64_t i8f_attention_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t) { return 0; }
+extern "C" int64_t i8f_attention_workspace_bytes(const i8f_attention_args *args) {
+    using namespace i8f;
+    if (!args || validate(*args) || !args->batch || !args->queries || !args->keys || !args->heads) return 0;
+    const i8f_attention_args &a = *args;
+    int64_t bytes[3];
+    to_pack(a, bytes);
+    return plan_of(a.batch, a.queries, a.keys, a.heads, a.kv_heads, a.width).partial_bytes + bytes[0] + bytes[1] + bytes[2];
+}
 
 extern "C" int i8f_attention(const i8f_attention_args *args, void *stream) {
     using namespace i8f;
     if (!args) return I8F_ERR_INVALID;
     const i8f_attention_args &a = *args;
     if (int rc = validate(a)) return rc;
-    const int64_t rows = a.batch * a.queries * a.heads;
-    if (!rows) return I8F_OK;
-    if (!grid_fits((rows + 3) / 4, 256)) return I8F_ERR_UNSUPPORTED;
+    if (!a.batch || !a.queries || !a.heads) return I8F_OK;
+    const int64_t need = i8f_attention_workspace_bytes(args);
+    if (need && (!a.workspace || a.workspace_bytes < need || (uintptr_t)a.workspace % 16)) return I8F_ERR_INVALID;
+    const Plan plan = plan_of(a.batch, a.queries, a.keys, a.heads, a.kv_heads, a.width);
+    const int64_t share = a.heads / a.kv_heads;
     if (int rc = check_device()) return rc;
-    if (a.dtype == I8F_BF16) hipLaunchKernelGGL((attention_kernel<I8F_BF16>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL((attention_kernel<I8F_F16>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a);
-    return check_launch();
+    hipStream_t st = (hipStream_t)stream;
+    Launch p = {a, (uint32_t)share, (uint32_t)(a.queries * share), (uint32_t)plan.row_tiles, (uint32_t)plan.splits, (uint32_t)plan.tiles, (uint32_t)round_up(a.width, 8)};
+    p.wide_out = a.width % 4 == 0 && (uintptr_t)a.out % 8 == 0;
+    p.partial = (float *)a.workspace;
+    p.stats = p.partial ? p.partial + plan.partial_bytes / 4 / (plan.padded + 2) * plan.padded : nullptr;
+    int64_t bytes[3];
+    const int which = to_pack(a, bytes);
+    if (which && a.keys) {
+        Packs packs = {};
+        char *at = (char *)a.workspace + plan.partial_bytes;
+        int count = 0;
+        int64_t most = 0;
+        auto pack = [&](int i, const void *&x, int64_t tokens, int64_t heads, int64_t &batch_stride, int64_t &token_stride, int64_t &head_stride) {
+            if (!(which >> i & 1)) return;
+            const int64_t padded = round_up(a.width, 8);
+            packs.p[count++] = {(const uint16_t *)x, (uint16_t *)at, a.batch * tokens * heads, tokens, heads, batch_stride, token_stride, head_stride, (int)a.width, (int)padded};
+            x = at, head_stride = padded, token_stride = heads * padded, batch_stride = tokens * heads * padded;
+            most = bytes[i] > most ? bytes[i] : most;
+            at += bytes[i];
+        };
+        pack(0, p.a.q, a.queries, a.heads, p.a.q_batch, p.a.q_token, p.a.q_head);
+        pack(1, p.a.k, a.keys, a.kv_heads, p.a.k_batch, p.a.k_token, p.a.k_head);
+        pack(2, p.a.v, a.keys, a.kv_heads, p.a.v_batch, p.a.v_token, p.a.v_head);
+        const int64_t blocks = (most / 16 + 255) / 256;
+        hipLaunchKernelGGL(pack_kernel, dim3((unsigned)(blocks < 8192 ? blocks : 8192), count), dim3(256), 0, st, packs);
+        if (int rc = check_launch()) return rc;
+    }
+    return a.dtype == I8F_BF16 ? launch<I8F_BF16>(p, plan, st) : launch<I8F_F16>(p, plan, st);
 }

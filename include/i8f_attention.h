@@ -64,8 +64,9 @@ int i8f_norm_rotate(const i8f_norm_rotate_args *args, const i8f_heads *groups, i
  *   key_lengths  [batch] of int32 (lengths_type 0) or int64 (1), or NULL; values outside 0 ... keys count as the nearer of the two
  *   key_mask     NULL or element (b, j) at mask_batch b + mask_key j of mask_type
  *   scale        positive and finite
- *   workspace    any contents, i8f_attention_workspace_bytes() of these sizes; less, or NULL, is refused where that is not 0.  Calls that
- *                overlap in time do not share it.
+ *   workspace    any contents, 16-byte aligned, i8f_attention_workspace_bytes() of these arguments (which looks at all but workspace and
+ *                key_lengths' and key_mask's contents); less, or NULL, is refused where that is not 0.  Calls that overlap in time do not share it.
+ * batch * queries * heads is below 2^31.
  */
 typedef enum i8f_key_mask { I8F_MASK_BYTES = 0, I8F_MASK_BF16 = 1, I8F_MASK_F16 = 2, I8F_MASK_F32 = 3 } i8f_key_mask;
 typedef struct i8f_attention_args {
@@ -83,7 +84,7 @@ typedef struct i8f_attention_args {
     void *workspace;
     int64_t workspace_bytes;
 } i8f_attention_args;
-int64_t i8f_attention_workspace_bytes(int64_t batch, int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads, int64_t width);
+int64_t i8f_attention_workspace_bytes(const i8f_attention_args *args);
 int i8f_attention(const i8f_attention_args *args, void *stream);
 
 #ifdef __cplusplus

@@ -55,13 +55,17 @@ def test_norm_rotate_arguments_are_checked_before_any_launch(L):
     assert _heads(L, None, {"heads": 0, "x": None, "out": None}) == 0 and _heads(L) == 0
 
 
-def _attention(L, **over):
+def _attention_args(L, **over):
     base = {"q": 1 << 20, "k": 1 << 22, "v": 1 << 23, "out": 1 << 24, "batch": 2, "queries": 3, "keys": 5, "heads": 4, "kv_heads": 2, "width": 8, "q_batch": 96, "q_token": 32,
             "q_head": 8, "k_batch": 80, "k_token": 16, "k_head": 8, "v_batch": 80, "v_token": 16, "v_head": 8, "dtype": L.BF16, "scale": 0.5, **over}
     a = L._AttentionArgs()
     for k, v in base.items():
         setattr(a, k, v)
-    return L.lib().i8f_attention(ctypes.byref(a), None)
+    return a
+
+
+def _attention(L, **over):
+    return L.lib().i8f_attention(ctypes.byref(_attention_args(L, **over)), None)
 
 
 def test_attention_arguments_are_checked_before_any_launch(L):
@@ -75,9 +79,16 @@ def test_attention_arguments_are_checked_before_any_launch(L):
     for bad in ({"dtype": L.F32}, {"width": 257}, {"batch": 1 << 31}, {"queries": 1 << 31}, {"keys": 1 << 31}, {"heads": 1 << 31}, {"k_token": 1 << 61}):
         assert _attention(L, **bad) == UNSUPPORTED, bad
     assert _attention(L, batch=0, q=None, out=None) == 0 and _attention(L, queries=0) == 0 and _attention(L, heads=0, kv_heads=0) == 0
-    size = L.lib().i8f_attention_workspace_bytes
-    for sizes in ((0, 3, 5, 4, 2, 8), (2, 0, 5, 4, 2, 8), (2, 3, 5, 0, 0, 8), (2, 3, 5, 4, 0, 8), (2, 3, 0, 4, 2, 8), (-1, 3, 5, 4, 2, 8), (2, 3, 5, 4, 3, 8), (2, 3, 5, 4, 2, 300)):
-        assert size(*sizes) == 0, sizes
+    size = lambda **over: L.lib().i8f_attention_workspace_bytes(ctypes.byref(_attention_args(L, **over)))  # noqa: E731
+    for bad in ({}, {"batch": 0}, {"queries": 0}, {"heads": 0, "kv_heads": 0}, {"keys": 0, "width": 7}, {"batch": -1}, {"kv_heads": 3}, {"width": 300}):
+        assert size(**bad) == 0, bad
+    assert L.lib().i8f_attention_workspace_bytes(None) == 0
+    # rows that are not whole aligned pieces are copied: q [2, 3, 4, 8], k and v [2, 5, 2, 8]
+    assert size(q=(1 << 20) + 2) == 2 * 3 * 4 * 16 and size(k=(1 << 22) + 8) == size(v_head=9) == 2 * 5 * 2 * 16 and size(width=5) == 2 * 3 * 4 * 16 + 2 * 2 * 5 * 2 * 16
+    assert size(k_token=(1 << 22) + 8, k_batch=1 << 40, out=1 << 50) == 2 * 5 * 2 * 16
+    assert _attention(L, width=5) == INVALID and _attention(L, width=5, workspace=16, workspace_bytes=1023) == INVALID and _attention(L, width=5, workspace=24, workspace_bytes=1 << 20) == INVALID
+    long = {"keys": 100000, "k_batch": 1600000, "v_batch": 1600000, "v": 1 << 30, "out": 1 << 40}
+    assert size(**long) > 0 and _attention(L, **long) == INVALID and _attention(L, **long, workspace=16, workspace_bytes=size(**long) - 1) == INVALID
 
 
 def test_a_rotation_keeps_turns_to_a_unit(pkg):
