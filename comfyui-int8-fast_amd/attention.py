@@ -56,8 +56,8 @@ def norm_heads(xs, weights=None, *, eps: float = 1e-6, rotary: RotaryAxes | None
     Everything is computed in binary32, the angles in binary64, and rounded once.  The results are contiguous.  No gradients: under grad
     mode an input that asks for one is refused, one with a tangent always."""
     single = isinstance(xs, Tensor)
-    xs = [xs] if single else list(xs)
-    weights = [None] * len(xs) if weights is None else [weights] if single and isinstance(weights, Tensor) else list(weights)
+    xs = (xs,) if single else tuple(xs)
+    weights = (None,) * len(xs) if weights is None else (weights,) if single and isinstance(weights, Tensor) else tuple(weights)
     if len(weights) != len(xs):
         raise ValueError(f"{len(xs)} tensors of heads and {len(weights)} weights")
     outs = _norm_rotate(xs, weights, True, eps, rotary, positions)
@@ -67,20 +67,25 @@ def norm_heads(xs, weights=None, *, eps: float = 1e-6, rotary: RotaryAxes | None
 def rotate_heads(xs, rotary: RotaryAxes, positions: Tensor):
     """Heads turned by their tokens' positions, without a norm: norm_heads describes xs, positions and the result."""
     single = isinstance(xs, Tensor)
-    xs = [xs] if single else list(xs)
+    xs = (xs,) if single else tuple(xs)
     if rotary is None:
         raise ValueError("a rotation needs its axes")
-    outs = _norm_rotate(xs, [None] * len(xs), False, 0.0, rotary, positions)
+    outs = _norm_rotate(xs, (None,) * len(xs), False, 0.0, rotary, positions)
     return outs[0] if single else outs
 
 
 def _norm_rotate(xs, weights, norm, eps, rotary, positions):
     if (rotary is None) != (positions is None):
         raise ValueError("rotary and positions go together")
+    rates, dims, apart = (None, (), False) if rotary is None else (rotary.rates, rotary.dims, not rotary.interleaved)
+    compiling = torch.compiler.is_compiling()
+    if xs and xs[0].is_cuda and not compiling:
+        outs = _lib.host().norm_rotate(xs, weights, norm, eps, rates, dims, apart, positions)
+        if outs is not None:
+            return outs
     _lib.refuse_gradients(**{f"xs[{i}]": x for i, x in enumerate(xs)}, **{f"weights[{i}]": w for i, w in enumerate(weights)}, positions=positions)
-    rates, dims, apart = (None, [], False) if rotary is None else (rotary.rates, list(rotary.dims), not rotary.interleaved)
-    if torch.compiler.is_compiling():
-        return torch.ops.i8f.norm_rotate_heads(xs, weights, norm, eps, rates, dims, apart, positions)
+    if compiling:
+        return torch.ops.i8f.norm_rotate_heads(list(xs), list(weights), norm, eps, rates, list(dims), apart, positions)
     return _lib.norm_rotate(xs, weights, norm, eps, rates, dims, apart, positions)
 
 
@@ -98,8 +103,13 @@ def cross_attention(q: Tensor, k: Tensor, v: Tensor, *, key_lengths: Tensor | No
     (NaN, infinities) reaches nothing.  Scores, maximum and sums are in binary32, the weights are rounded to q's type for the second product,
     the result is rounded once.  Both are read on the device: a captured graph follows what is written into them.  No gradients: under
     grad mode an input that asks for one is refused, one with a tangent always."""
+    compiling = torch.compiler.is_compiling()
+    if type(q) is Tensor and q.is_cuda and not compiling:
+        out = _lib.host().attention(q, k, v, key_lengths, key_mask, scale)
+        if out is not None:
+            return out
     _lib.refuse_gradients(q=q, k=k, v=v, key_mask=key_mask)
-    if torch.compiler.is_compiling():
+    if compiling:
         return torch.ops.i8f.cross_attention(q, k, v, key_lengths, key_mask, scale)
     return _lib.attention(q, k, v, key_lengths, key_mask, scale)
 
@@ -135,11 +145,11 @@ def forward_cross_attention(x: Tensor, context: Tensor | None, to_q, to_k, to_v,
     q, k, v = q.unflatten(-1, (heads, -1)), k.unflatten(-1, (kv_heads, -1)), v.unflatten(-1, (kv_heads, -1))
     norm = q_weight is not None
     if context is None and (norm or rotary is not None):
-        q, k = _norm_rotate([q, k], [q_weight, k_weight], norm, eps, rotary, positions)
+        q, k = _norm_rotate((q, k), (q_weight, k_weight), norm, eps, rotary, positions)
     else:
         if norm or positions is not None:
-            q, = _norm_rotate([q], [q_weight], norm, eps, rotary, positions)
+            q, = _norm_rotate((q,), (q_weight,), norm, eps, rotary, positions)
         if norm or context_positions is not None:
-            k, = _norm_rotate([k], [k_weight], norm, eps, rotary if context_positions is not None else None, context_positions)
+            k, = _norm_rotate((k,), (k_weight,), norm, eps, rotary if context_positions is not None else None, context_positions)
     out = cross_attention(q, k, v, key_lengths=key_lengths, key_mask=key_mask, scale=scale).flatten(-2)
     return out if to_out is None else to_out(out) if gate is None and residual is None else to_out(out, gate=gate, residual=residual)

@@ -9,6 +9,8 @@
 //   vector_fanout(...)          several small-batch layers that read the same rows, in one launch
 //   adapters(...)               layers that read the same rows, with a low-rank adapter for each of them
 //   block_norm(...)             what lies between two blocks, and the next one's projections where they are given
+//   norm_rotate(...)            norms and rotation of heads
+//   attention(...)              attention over an encoder's states
 //
 // Every function takes the cases it can decide on cheaply and returns None for all others (tensors of other types,
 // devices or layouts, operands that need a cast or a copy, errors): the caller then goes the general way in Python, which
@@ -27,9 +29,11 @@
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
+#include <cmath>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../../include/i8f.h"
+#include "../../../include/i8f_attention.h"
 #include "../../../include/i8f_blocks.h"
 #include "../quant_lora_entry.hpp"
 #include "../w8a16_rotated.hpp"
@@ -41,7 +45,8 @@ namespace {
     X(i8f_quant_rowwise) X(i8f_quant_rowwise_prologue) X(i8f_quant_rowwise_norm_modulate) X(i8f_quant_rowwise_rms_norm)  \
     X(i8f_quant_rowwise_concat_gelu) X(i8f_rotate128) X(i8f_linear_w8a8_gated) X(i8f_linear_w8a8_grouped) X(i8f_linear_w8a16_small_m) \
     X(i8f_linear_w8a16_small_m_grouped) X(i8f_internal_w8a16_rotated) X(i8f_linear_w8a8_lora) X(i8f_internal_quant_lora)    \
-    X(i8f_adapters_by_side) X(i8f_adapters_down) X(i8f_adapters_down_workspace_bytes) X(i8f_linear_w8a8_adapters) X(i8f_linear_w8a8_adapters_workspace_bytes) X(i8f_linear_w8a16_small_m_adapters) X(i8f_block_norm)
+    X(i8f_adapters_by_side) X(i8f_adapters_down) X(i8f_adapters_down_workspace_bytes) X(i8f_linear_w8a8_adapters) X(i8f_linear_w8a8_adapters_workspace_bytes) X(i8f_linear_w8a16_small_m_adapters) X(i8f_block_norm) \
+    X(i8f_norm_rotate) X(i8f_attention) X(i8f_attention_workspace_bytes)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
     I8F_ENTRY_POINTS(X)
@@ -739,6 +744,141 @@ PyObject *block_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return PyTuple_Pack(2, first.p, second.p);
 }
 
+// Heads [.., tokens, heads, width] with contiguous elements; batch, token and head strides in elements.
+bool heads_of(const at::Tensor &x, int64_t &batch_stride, int64_t &token_stride, int64_t &head_stride) {
+    const int64_t d = x.dim();
+    if (d < 3 || d > 4 || (x.size(d - 1) > 1 && x.stride(d - 1) != 1)) return false;
+    batch_stride = d == 4 ? x.stride(0) : 0, token_stride = x.stride(d - 3), head_stride = x.stride(d - 2);
+    return true;
+}
+
+// norm_rotate(xs, weights, norm, eps, rates, dims, apart, positions): tuples of heads and of their weights or None, the axes' rates and elements
+// and the positions or None -> list of the results
+PyObject *norm_rotate(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 8) return PyErr_Format(PyExc_TypeError, "norm_rotate takes 8 arguments, got %zd", n);
+    const Py_ssize_t count = PyTuple_Check(a[0]) ? PyTuple_GET_SIZE(a[0]) : 0;
+    if (!lib.bound || count < 1 || count > I8F_MAX_HEAD_GROUPS || !PyTuple_Check(a[1]) || PyTuple_GET_SIZE(a[1]) != count) Py_RETURN_NONE;
+    const at::Tensor *first = tensor(PyTuple_GET_ITEM(a[0], 0));
+    if (!first || !first->is_cuda() || first->dim() < 3) Py_RETURN_NONE;
+    const at::ScalarType type = first->scalar_type();
+    const at::Device dev = first->device();
+    const int64_t d = first->dim();
+    i8f_norm_rotate_args g = {};
+    i8f_heads h[I8F_MAX_HEAD_GROUPS] = {};
+    Size size[I8F_MAX_HEAD_GROUPS];
+    const Stream st(dev);
+    g.dtype = code_of(type);
+    if (!st.ok || g.dtype < 0) Py_RETURN_NONE;
+    g.batch = d == 4 ? first->size(0) : 1, g.tokens = first->size(d - 3), g.width = first->size(d - 1);
+    g.norm = a[2] == Py_True, g.eps = (float)PyFloat_AsDouble(a[3]);
+    if (PyErr_Occurred()) return nullptr;
+    if (g.width > 512) Py_RETURN_NONE;
+    for (Py_ssize_t i = 0; i < count; ++i) {
+        const at::Tensor *x = tensor(PyTuple_GET_ITEM(a[0], i));
+        if (!x || wants_gradient(x) || x->scalar_type() != type || x->device() != dev || x->dim() != d || x->size(d - 1) != g.width || x->size(d - 3) != g.tokens ||
+            (d == 4 && x->size(0) != g.batch) || !heads_of(*x, h[i].batch_stride, h[i].token_stride, h[i].head_stride))
+            Py_RETURN_NONE;
+        h[i].x = x->const_data_ptr(), h[i].heads = x->size(d - 2);
+        size[i] = Size(x->sizes().begin(), x->sizes().end());
+        if (PyTuple_GET_ITEM(a[1], i) == Py_None) continue;
+        const at::Tensor *w = tensor(PyTuple_GET_ITEM(a[1], i));
+        if (!w || wants_gradient(w) || (w->scalar_type() != type && w->scalar_type() != at::kFloat) || w->device() != dev || w->dim() != 1 || w->size(0) != g.width ||
+            !w->is_contiguous())
+            Py_RETURN_NONE;
+        h[i].weight = w->const_data_ptr(), h[i].weight_dtype = code_of(w->scalar_type());
+    }
+    if (a[7] != Py_None) {
+        const at::Tensor *rates = tensor(a[4]), *p = tensor(a[7]);
+        const Py_ssize_t axes = PyTuple_Check(a[5]) ? PyTuple_GET_SIZE(a[5]) : 0;
+        if (!rates || !p || wants_gradient(p) || axes < 1 || axes > I8F_MAX_AXES || rates->device() != dev || p->device() != dev || rates->scalar_type() != at::kDouble ||
+            !rates->is_contiguous() || p->dim() < 2 || p->dim() > 3)
+            Py_RETURN_NONE;
+        switch (p->scalar_type()) {
+        case at::kInt: g.positions_type = I8F_POSITION_I32; break;
+        case at::kLong: g.positions_type = I8F_POSITION_I64; break;
+        case at::kFloat: g.positions_type = I8F_POSITION_F32; break;
+        case at::kDouble: g.positions_type = I8F_POSITION_F64; break;
+        default: Py_RETURN_NONE;
+        }
+        g.axes = (int)axes, g.apart = a[6] == Py_True;
+        for (Py_ssize_t i = 0; i < axes; ++i) g.first_pair[i + 1] = g.first_pair[i] + (int)(PyLong_AsLong(PyTuple_GET_ITEM(a[5], i)) / 2);
+        if (PyErr_Occurred()) return nullptr;
+        const int64_t lead = p->dim() - 2;   // (a batch dimension in front)
+        if (rates->numel() != g.first_pair[axes] || p->size(lead) != g.tokens || p->size(lead + 1) != axes || (lead && p->size(0) != 1 && p->size(0) != g.batch)) Py_RETURN_NONE;
+        g.position_batch = lead && p->size(0) == g.batch && g.batch > 1 ? p->stride(0) : 0, g.position_token = p->stride(lead), g.position_axis = p->stride(lead + 1);
+        g.rates = (const double *)rates->const_data_ptr(), g.positions = p->const_data_ptr();
+    } else if (a[4] != Py_None) {
+        Py_RETURN_NONE;
+    }
+    at::Tensor y[I8F_MAX_HEAD_GROUPS];
+    int rc;
+    {
+        const WithoutGil released;
+        for (Py_ssize_t i = 0; i < count; ++i) {
+            y[i] = empty(size[i], type, dev);
+            h[i].out = y[i].data_ptr();
+        }
+        rc = lib.i8f_norm_rotate(&g, h, (int)count, st.handle);
+    }
+    if (rc) Py_RETURN_NONE;
+    return list_of(y, count);
+}
+
+// attention(q, k, v, key_lengths, key_mask, scale): lengths, mask and scale may be None -> the result
+PyObject *attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 6) return PyErr_Format(PyExc_TypeError, "attention takes 6 arguments, got %zd", n);
+    const at::Tensor *q = tensor(a[0]), *k = tensor(a[1]), *v = tensor(a[2]);
+    if (!lib.bound || !q || !k || !v || !q->is_cuda()) Py_RETURN_NONE;
+    const at::ScalarType type = q->scalar_type();
+    const at::Device dev = q->device();
+    const Stream st(dev);
+    i8f_attention_args g = {};
+    g.dtype = code_of(type);
+    if (!st.ok || (g.dtype != I8F_BF16 && g.dtype != I8F_F16)) Py_RETURN_NONE;
+    for (const at::Tensor *t : {q, k, v})
+        if (wants_gradient(t) || t->scalar_type() != type || t->device() != dev || t->dim() != 4) Py_RETURN_NONE;
+    if (!heads_of(*q, g.q_batch, g.q_token, g.q_head) || !heads_of(*k, g.k_batch, g.k_token, g.k_head) || !heads_of(*v, g.v_batch, g.v_token, g.v_head)) Py_RETURN_NONE;
+    g.batch = q->size(0), g.queries = q->size(1), g.heads = q->size(2), g.width = q->size(3), g.keys = k->size(1), g.kv_heads = k->size(2);
+    if (k->sizes() != v->sizes() || k->size(0) != g.batch || k->size(3) != g.width || g.width < 1) Py_RETURN_NONE;
+    const double scale = a[5] == Py_None ? 1.0 / std::sqrt((double)g.width) : PyFloat_AsDouble(a[5]);
+    if (PyErr_Occurred()) return nullptr;
+    g.scale = (float)scale;
+    if (a[3] != Py_None) {
+        const at::Tensor *t = tensor(a[3]);
+        if (!t || (t->scalar_type() != at::kInt && t->scalar_type() != at::kLong) || t->device() != dev || t->dim() != 1 || t->size(0) != g.batch || !t->is_contiguous()) Py_RETURN_NONE;
+        g.key_lengths = t->const_data_ptr(), g.lengths_type = t->scalar_type() == at::kLong;
+    }
+    if (a[4] != Py_None) {
+        const at::Tensor *t = tensor(a[4]);
+        if (!t || wants_gradient(t) || t->device() != dev || t->dim() != 2 || t->size(0) != g.batch || t->size(1) != g.keys) Py_RETURN_NONE;
+        switch (t->scalar_type()) {
+        case at::kBool: g.mask_type = I8F_MASK_BYTES; break;
+        case at::kBFloat16: g.mask_type = I8F_MASK_BF16; break;
+        case at::kHalf: g.mask_type = I8F_MASK_F16; break;
+        case at::kFloat: g.mask_type = I8F_MASK_F32; break;
+        default: Py_RETURN_NONE;
+        }
+        g.key_mask = t->const_data_ptr(), g.mask_batch = t->stride(0), g.mask_key = t->stride(1);
+    }
+    g.q = q->const_data_ptr(), g.k = k->const_data_ptr(), g.v = v->const_data_ptr();
+    const Size size(q->sizes().begin(), q->sizes().end());
+    at::Tensor out, work;
+    int rc;
+    {
+        const WithoutGil released;
+        out = empty(size, type, dev);
+        g.out = out.data_ptr();
+        g.workspace_bytes = lib.i8f_attention_workspace_bytes(&g);
+        if (g.workspace_bytes > 0) {
+            work = empty({g.workspace_bytes}, at::kByte, dev);
+            g.workspace = work.data_ptr();
+        }
+        rc = lib.i8f_attention(&g, st.handle);
+    }
+    if (rc) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(out));
+}
+
 // No C++ exception leaves an entry point: an allocator that has nothing left, say, becomes the general path's to report.
 template <PyObject *(*F)(PyObject *, PyObject *const *, Py_ssize_t)>
 PyObject *guarded(PyObject *self, PyObject *const *a, Py_ssize_t n) {
@@ -763,6 +903,8 @@ PyMethodDef methods[] = {
     {"vector_fanout", (PyCFunction)(void (*)(void))guarded<vector_fanout>, METH_FASTCALL, "several small-batch layers, or None"},
     {"adapters", (PyCFunction)(void (*)(void))guarded<adapters>, METH_FASTCALL, "quantised layers with an adapter for each row, or None"},
     {"block_norm", (PyCFunction)(void (*)(void))guarded<block_norm>, METH_FASTCALL, "what lies between two blocks, or None"},
+    {"norm_rotate", (PyCFunction)(void (*)(void))guarded<norm_rotate>, METH_FASTCALL, "norms and rotation of heads, or None"},
+    {"attention", (PyCFunction)(void (*)(void))guarded<attention>, METH_FASTCALL, "attention over an encoder's states, or None"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_i8f_host", "Native host path of the INT8 linear layers.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,6 +1,7 @@
 // Queries and keys between their projection and the attention: the norm of every head and the rotation by the token's positions, in one
 // pass (include/i8f_attention.h has the formula).
 #include <initializer_list>
+#include <type_traits>
 #include <utility>
 
 #include "i8f_common.hpp"
@@ -108,8 +109,187 @@ int launch_any(const i8f_norm_rotate_args &a, const Groups &groups, hipStream_t 
     return I8F_OK;
 }
 
+// ---- heads of whole aligned pieces: a lane holds eight elements of a head, LPH lanes a head ------------------------------------------
+// Pairs that lie apart are in one lane as well: it takes four elements of either half.
+template <int DT>
+struct Eight {
+    uint4 v[DT == I8F_F32 ? 2 : 1];
+};
+template <int DT, bool APART>
+__device__ __forceinline__ Eight<DT> load_eight(const char *p, int e0, int e1) {
+    Eight<DT> r;
+    if constexpr (DT == I8F_F32) {
+        r.v[0] = *(const uint4 *)(p + e0 * 4), r.v[1] = *(const uint4 *)(p + e1 * 4);
+    } else if constexpr (APART) {
+        const uint2 lo = *(const uint2 *)(p + e0 * 2), hi = *(const uint2 *)(p + e1 * 2);
+        r.v[0] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+    } else {
+        r.v[0] = *(const uint4 *)(p + e0 * 2);
+    }
+    return r;
+}
+template <int DT>
+__device__ __forceinline__ void expand_eight(const Eight<DT> &r, float (&v)[8]) {
+    if constexpr (DT == I8F_F32) {
+        __builtin_memcpy(v, &r, 32);
+    } else {
+        const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = DT == I8F_BF16 ? __uint_as_float(w[i] << 16) : f16_bits_to_f32(w[i] & 0xffffu);
+            v[2 * i + 1] = DT == I8F_BF16 ? __uint_as_float(w[i] & 0xffff0000u) : f16_bits_to_f32(w[i] >> 16);
+        }
+    }
+}
+template <int DT, bool APART>
+__device__ __forceinline__ void store_eight(char *p, int e0, int e1, const float (&v)[8]) {
+    if constexpr (DT == I8F_F32) {
+        uint4 lo, hi;
+        __builtin_memcpy(&lo, v, 16);
+        __builtin_memcpy(&hi, v + 4, 16);
+        stream_store16(p + e0 * 4, lo), stream_store16(p + e1 * 4, hi);
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = DT == I8F_BF16 ? f32x2_to_bf16x2_bits(v[2 * i], v[2 * i + 1]) : f32x2_to_f16x2_bits(v[2 * i], v[2 * i + 1]);
+        if constexpr (APART) stream_store8(p + e0 * 2, make_uint2(w[0], w[1])), stream_store8(p + e1 * 2, make_uint2(w[2], w[3]));
+        else stream_store16(p + e0 * 2, make_uint4(w[0], w[1], w[2], w[3]));
+    }
+}
+// a sum over LPH neighbouring lanes, in every one of them
+template <int LPH>
+__device__ __forceinline__ float sum_of_lanes(float v) {
+    auto add = [&](auto ctrl) __attribute__((always_inline)) {
+        v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    using std::integral_constant;
+    if constexpr (LPH > 1) add(integral_constant<int, 0xb1>{});     // quad_perm [1,0,3,2]
+    if constexpr (LPH > 2) add(integral_constant<int, 0x4e>{});     // quad_perm [2,3,0,1]
+    if constexpr (LPH > 4) add(integral_constant<int, 0x141>{});    // row_half_mirror
+    if constexpr (LPH > 8) add(integral_constant<int, 0x140>{});    // row_mirror
+    if constexpr (LPH > 16) v += __shfl_xor(v, 16);
+    if constexpr (LPH > 32) v += __shfl_xor(v, 32);
+    return v;
+}
+
+constexpr int DEEP = 4;   // passes that a wave requests at a time
+// A wave takes `per` passes of one token, a pass being 64 / LPH heads: the angles are the same for all of them.
+template <int DT, int LPH, bool APART>
+__global__ __launch_bounds__(256) void norm_rotate_kernel(const int64_t first, const unsigned chunks, const int per, const i8f_norm_rotate_args a, const Groups groups) {
+    constexpr int HPP = 64 / LPH, SIZE = DT == I8F_F32 ? 4 : 2;
+    const int lane = threadIdx.x & 63, sub = lane / LPH, l = lane % LPH;
+    const int64_t id = first + (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t bt = id / chunks;
+    if (bt >= a.batch * a.tokens) return;
+    const int start = (int)(id % chunks) * per;
+    const int64_t b = bt / a.tokens, t = bt % a.tokens;
+    const int width = (int)a.width, pairs = a.axes ? a.first_pair[a.axes] : 0;
+    const bool low = APART && l < pairs / 4;   // (lanes behind the turned pairs hold eight neighbours in either form)
+    const int e0 = !APART ? 8 * l : low ? 4 * l : 2 * pairs + 8 * (l - pairs / 4), e1 = low ? pairs + 4 * l : e0 + 4;
+    const bool in = e0 < width;
+    float c[4], s[4];
+    if (pairs) {
+        double pos[I8F_MAX_AXES];
+        token_positions(a, bt, pos);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (4 * l + i < pairs) turn(a, pos, 4 * l + i, c[i], s[i]);
+    }
+    int before = 0;
+    for (int g = 0; g < groups.n; ++g) {
+        const i8f_heads &h = groups.g[g];
+        const int passes = ((int)h.heads + HPP - 1) / HPP, lo = start - before > 0 ? start - before : 0, hi = start + per - before < passes ? start + per - before : passes;
+        before += passes;
+        if (lo >= hi) continue;
+        float w[8];
+        if (h.weight && in) {
+            if (DT == I8F_F32 || h.weight_dtype == I8F_F32) expand_eight<I8F_F32>(load_eight<I8F_F32, APART>((const char *)h.weight, e0, e1), w);
+            else expand_eight<DT>(load_eight<DT, APART>((const char *)h.weight, e0, e1), w);
+        }
+        const char *x = (const char *)h.x + (b * h.batch_stride + t * h.token_stride) * SIZE;
+        char *out = (char *)h.out + bt * h.heads * width * SIZE;
+        for (int pass = lo; pass < hi; pass += DEEP) {
+            Eight<DT> raw[DEEP];
+#pragma unroll
+            for (int i = 0; i < DEEP; ++i) {
+                const int head = (pass + i) * HPP + sub;
+                if (pass + i < hi && in && head < h.heads) raw[i] = load_eight<DT, APART>(x + head * h.head_stride * SIZE, e0, e1);
+                else raw[i] = {};
+            }
+#pragma unroll
+            for (int i = 0; i < DEEP; ++i) {
+                if (pass + i >= hi) break;
+                const int head = (pass + i) * HPP + sub;
+                float v[8];
+                expand_eight<DT>(raw[i], v);
+                if (a.norm) {
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(v[e], v[e], sum);
+                    const float rstd = 1.0f / sqrtf(sum_of_lanes<LPH>(sum) / (float)width + a.eps);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] *= rstd;
+                    if (h.weight) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] *= w[e];
+                    }
+                }
+                if (pairs) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float &v0 = v[APART ? e : 2 * e], &v1 = v[APART ? e + 4 : 2 * e + 1];
+                        const float y0 = __builtin_fmaf(v0, c[e], -(v1 * s[e])), y1 = __builtin_fmaf(v0, s[e], v1 * c[e]);
+                        if (4 * l + e < pairs) v0 = y0, v1 = y1;   // (the others as they are: 0 times an infinity is none)
+                    }
+                }
+                if (in && head < h.heads) store_eight<DT, APART>(out + (int64_t)head * width * SIZE, e0, e1, v);
+            }
+        }
+    }
+}
+
+// All operands in 16-byte pieces, and with pairs that lie apart the turned and the other elements in whole lanes.
+bool in_pieces(const i8f_norm_rotate_args &a, const Groups &groups) {
+    const int64_t per16 = 16 / (int64_t)dtype_size(a.dtype);
+    if (a.width % 8 || (a.axes && a.apart && a.first_pair[a.axes] % 4)) return false;
+    for (int i = 0; i < groups.n; ++i) {
+        const i8f_heads &g = groups.g[i];
+        if (((uintptr_t)g.x | (uintptr_t)g.weight | (uintptr_t)g.out) % 16 || g.batch_stride % per16 || g.token_stride % per16 || g.head_stride % per16) return false;
+    }
+    return true;
+}
+
+template <int DT, int LPH, bool APART>
+int launch_pieces(const i8f_norm_rotate_args &a, const Groups &groups, hipStream_t st) {
+    int64_t passes = 0;
+    for (int i = 0; i < groups.n; ++i) passes += (groups.g[i].heads + 64 / LPH - 1) / (64 / LPH);
+    if (passes > 0x7fffffff) return I8F_ERR_UNSUPPORTED;
+    // As many passes to a wave as it requests at a time: us for 4096 tokens of 30 + 30 heads of 128 and 32760 of 40 + 40, 1 pass 45 and 239, 4 or 5
+    // 24.1 and 238, 8 24.6 and 246, a whole token 24.8 and 248.  Fewer where the waves would be few.
+    const int64_t tokens = a.batch * a.tokens, total = tokens * passes;
+    int64_t per = total / 4096;
+    per = per < 1 ? 1 : per > DEEP ? DEEP : per;
+    const int64_t chunks = (passes + per - 1) / per;
+    per = (passes + chunks - 1) / chunks;
+    const int64_t waves = tokens * chunks, most = (int64_t)4 << 23;   // (a launch has fewer than 2^32 threads)
+    for (int64_t w = 0; w < waves; w += most) {
+        const int64_t n = waves - w < most ? waves - w : most;
+        hipLaunchKernelGGL((norm_rotate_kernel<DT, LPH, APART>), dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, w, (unsigned)chunks, (int)per, a, groups);
+        if (int rc = check_launch()) return rc;
+    }
+    return I8F_OK;
+}
+template <int DT, bool APART>
+int launch_lanes(const i8f_norm_rotate_args &a, const Groups &groups, hipStream_t st) {
+    if (a.width <= 64) return launch_pieces<DT, 8, APART>(a, groups, st);
+    if (a.width <= 128) return launch_pieces<DT, 16, APART>(a, groups, st);
+    if (a.width <= 256) return launch_pieces<DT, 32, APART>(a, groups, st);
+    return launch_pieces<DT, 64, APART>(a, groups, st);
+}
+
 template <int DT>
 int launch(const i8f_norm_rotate_args &a, const Groups &groups, hipStream_t st) {
+    if (in_pieces(a, groups)) return a.axes && a.apart ? launch_lanes<DT, true>(a, groups, st) : launch_lanes<DT, false>(a, groups, st);
     const int64_t pairs = (a.width + 1) / 2;
     if (pairs <= 64) return launch_any<DT, 1>(a, groups, st);
     if (pairs <= 128) return launch_any<DT, 2>(a, groups, st);
