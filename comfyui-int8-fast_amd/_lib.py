@@ -1092,7 +1092,7 @@ def block_norm(y, residual, *, post_norm=None, post_weight=None, post_bias=None,
     return (x, q, scale) if quantise else (x, h)
 
 
-MAX_HEAD_GROUPS, MAX_AXES, MAX_NORM_WIDTH, MAX_HEAD_WIDTH = 4, 4, 512, 256
+MAX_HEAD_GROUPS, MAX_AXES, MAX_HEAD_WIDTH = 4, 4, 256
 _POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
 _MASKS = {torch.bool: 0, torch.bfloat16: 1, torch.float16: 2, torch.float32: 3}
 
@@ -1135,8 +1135,8 @@ def norm_rotate(xs, weights, norm, eps, rates, dims, apart, positions):
         if x.dtype != first.dtype or x.device != first.device:
             raise TypeError(f"xs[{i}] is {x.dtype} on {x.device}, xs[0] {first.dtype} on {first.device}")
     code, width, device = dtype_code(first.dtype), first.shape[-1], first.device
-    if not 1 <= width <= MAX_NORM_WIDTH:
-        raise ValueError(f"heads must be 1 to {MAX_NORM_WIDTH} elements wide, got {width}")
+    if not 1 <= width <= MAX_HEAD_WIDTH:
+        raise ValueError(f"heads must be 1 to {MAX_HEAD_WIDTH} elements wide, got {width}")
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
     batch, tokens = first.shape[0] if first.dim() == 4 else 1, first.shape[-3]

@@ -48,7 +48,7 @@ def norm_heads(xs, weights=None, *, eps: float = 1e-6, rotary: RotaryAxes | None
     """x / sqrt(mean(x^2) + eps) * weight over the last dimension of every head, turned by its token's positions where `rotary` is given.
 
     xs:        heads [batch, tokens, heads, width] or [tokens, heads, width], or a list of tensors of the same tokens (queries and keys, of
-               unlike numbers of heads; then the result is a list).  bfloat16, float16 or float32, width up to 512.  Views of a fused
+               unlike numbers of heads; then the result is a list).  bfloat16, float16 or float32, width up to 256.  Views of a fused
                projection are taken as they are.
     weights:   [width] of their type or float32, one for each of xs (None for none), or None for none at all.
     positions: [tokens, axes], or [batch, tokens, axes] (a batch of 1 for all), int32, int64, float32 or float64, on xs' device.

@@ -772,7 +772,7 @@ PyObject *norm_rotate(PyObject *, PyObject *const *a, Py_ssize_t n) {
     g.batch = d == 4 ? first->size(0) : 1, g.tokens = first->size(d - 3), g.width = first->size(d - 1);
     g.norm = a[2] == Py_True, g.eps = (float)PyFloat_AsDouble(a[3]);
     if (PyErr_Occurred()) return nullptr;
-    if (g.width > 512) Py_RETURN_NONE;
+    if (g.width > 256) Py_RETURN_NONE;
     for (Py_ssize_t i = 0; i < count; ++i) {
         const at::Tensor *x = tensor(PyTuple_GET_ITEM(a[0], i));
         if (!x || wants_gradient(x) || x->scalar_type() != type || x->device() != dev || x->dim() != d || x->size(d - 1) != g.width || x->size(d - 3) != g.tokens ||

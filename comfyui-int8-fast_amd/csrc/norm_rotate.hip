@@ -41,90 +41,41 @@ __device__ __forceinline__ void token_positions(const i8f_norm_rotate_args &a, i
     for (int x = 0; x < I8F_MAX_AXES; ++x) pos[x] = x < a.axes ? position_at(a.positions, a.positions_type, at + x * a.position_axis) : 0.0;
 }
 
-// ---- any width, alignment and pairing: a wave to a token, a lane to every 64th pair -----------------------------------------------
-// (elements behind the turned ones go in pairs too, which are not turned; the last may be one element)
-template <int DT, int NP>
-__global__ __launch_bounds__(256) void norm_rotate_any_kernel(const int64_t first, const i8f_norm_rotate_args a, const Groups groups) {
-    const int lane = threadIdx.x & 63;
-    const int64_t bt = first + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (bt >= a.batch * a.tokens) return;
-    const int width = (int)a.width, pairs = a.axes ? a.first_pair[a.axes] : 0;
-    double pos[I8F_MAX_AXES];
-    token_positions(a, bt, pos);
-    float c[NP], s[NP];
-    int e0[NP], e1[NP];
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-        const int j = i * 64 + lane;
-        c[i] = 1.0f, s[i] = 0.0f;
-        e0[i] = j >= pairs || !a.apart ? 2 * j : j;
-        e1[i] = j >= pairs || !a.apart ? 2 * j + 1 : j + pairs;
-        if (j < pairs) turn(a, pos, j, c[i], s[i]);
-    }
-    for (int g = 0; g < groups.n; ++g) {
-        const i8f_heads &h = groups.g[g];
-        const int64_t xb = bt / a.tokens * h.batch_stride + bt % a.tokens * h.token_stride;
-        for (int64_t head = 0; head < h.heads; ++head) {
-            float v0[NP], v1[NP], sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                v0[i] = e0[i] < width ? load_as_f32<DT>(h.x, xb + head * h.head_stride + e0[i]) : 0.0f;
-                v1[i] = e1[i] < width ? load_as_f32<DT>(h.x, xb + head * h.head_stride + e1[i]) : 0.0f;
-                sum = __builtin_fmaf(v0[i], v0[i], __builtin_fmaf(v1[i], v1[i], sum));
-            }
-            if (a.norm) {
-#pragma unroll
-                for (int x = 1; x < 64; x *= 2) sum += __shfl_xor(sum, x);
-                const float rstd = 1.0f / sqrtf(sum / (float)width + a.eps);
-#pragma unroll
-                for (int i = 0; i < NP; ++i) {
-                    v0[i] *= rstd, v1[i] *= rstd;
-                    if (h.weight) {
-                        const bool wide = DT == I8F_F32 || h.weight_dtype == I8F_F32;
-                        if (e0[i] < width) v0[i] *= wide ? ((const float *)h.weight)[e0[i]] : load_as_f32<DT>(h.weight, e0[i]);
-                        if (e1[i] < width) v1[i] *= wide ? ((const float *)h.weight)[e1[i]] : load_as_f32<DT>(h.weight, e1[i]);
-                    }
-                }
-            }
-            const int64_t ob = (bt * h.heads + head) * width;
-#pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                const bool turned = i * 64 + lane < pairs;   // (the others as they are: 0 times an infinity is none)
-                const float y0 = turned ? __builtin_fmaf(v0[i], c[i], -(v1[i] * s[i])) : v0[i], y1 = turned ? __builtin_fmaf(v0[i], s[i], v1[i] * c[i]) : v1[i];
-                if (e0[i] < width) store_from_f32<DT>(h.out, ob + e0[i], y0);
-                if (e1[i] < width) store_from_f32<DT>(h.out, ob + e1[i], y1);
-            }
-        }
-    }
-}
-
-template <int DT, int NP>
-int launch_any(const i8f_norm_rotate_args &a, const Groups &groups, hipStream_t st) {
-    const int64_t rows = a.batch * a.tokens, most = (int64_t)4 << 23;   // (a launch has fewer than 2^32 threads)
-    for (int64_t r = 0; r < rows; r += most) {
-        const int64_t n = rows - r < most ? rows - r : most;
-        hipLaunchKernelGGL((norm_rotate_any_kernel<DT, NP>), dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, r, a, groups);
-        if (int rc = check_launch()) return rc;
-    }
-    return I8F_OK;
-}
-
-// ---- heads of whole aligned pieces: a lane holds eight elements of a head, LPH lanes a head ------------------------------------------
-// Pairs that lie apart are in one lane as well: it takes four elements of either half.
+// A lane holds eight elements of a head: neighbours, or of pairs that lie apart four elements of either half.  They move in 16 or 8 bytes from
+// whatever address they have.  The last lane of a width or of a half that is no multiple begins further back, in elements that the lane before
+// it has too, which it computes again and leaves out of the sum (SHIFTED); where that would tear pairs of neighbours or leave the head
+// its elements move one by one (SINGLE).
+enum { FULL, SHIFTED, SINGLE };
+typedef v4u_t any4_t __attribute__((aligned(2)));
+typedef v2u_t any2_t __attribute__((aligned(2)));
 template <int DT>
 struct Eight {
-    uint4 v[DT == I8F_F32 ? 2 : 1];
+    v4u_t v[DT == I8F_F32 ? 2 : 1];
 };
 template <int DT, bool APART>
 __device__ __forceinline__ Eight<DT> load_eight(const char *p, int e0, int e1) {
     Eight<DT> r;
     if constexpr (DT == I8F_F32) {
-        r.v[0] = *(const uint4 *)(p + e0 * 4), r.v[1] = *(const uint4 *)(p + e1 * 4);
+        r.v[0] = *(const any4_t *)(p + e0 * 4), r.v[1] = *(const any4_t *)(p + e1 * 4);
     } else if constexpr (APART) {
-        const uint2 lo = *(const uint2 *)(p + e0 * 2), hi = *(const uint2 *)(p + e1 * 2);
-        r.v[0] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        const v2u_t lo = *(const any2_t *)(p + e0 * 2), hi = *(const any2_t *)(p + e1 * 2);
+        r.v[0] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3);
     } else {
-        r.v[0] = *(const uint4 *)(p + e0 * 2);
+        r.v[0] = *(const any4_t *)(p + e0 * 2);
+    }
+    return r;
+}
+// the first n of each four (of a lane's pairs that lie apart), or of eight neighbours; the others are zeros
+template <int DT>
+__device__ __forceinline__ Eight<DT> load_some(const char *p, int e0, int e1, int n0, int n1) {
+    Eight<DT> r = {};
+    uint32_t *w = (uint32_t *)&r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if (e % 4 >= (e < 4 ? n0 : n1)) continue;
+        const int at = (e < 4 ? e0 : e1) + e % 4;
+        if constexpr (DT == I8F_F32) w[e] = *(const uint32_t *)(p + at * 4);
+        else w[e / 2] |= (uint32_t)*(const uint16_t *)(p + at * 2) << (16 * (e % 2));
     }
     return r;
 }
@@ -133,27 +84,45 @@ __device__ __forceinline__ void expand_eight(const Eight<DT> &r, float (&v)[8]) 
     if constexpr (DT == I8F_F32) {
         __builtin_memcpy(v, &r, 32);
     } else {
-        const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            v[2 * i] = DT == I8F_BF16 ? __uint_as_float(w[i] << 16) : f16_bits_to_f32(w[i] & 0xffffu);
-            v[2 * i + 1] = DT == I8F_BF16 ? __uint_as_float(w[i] & 0xffff0000u) : f16_bits_to_f32(w[i] >> 16);
+            const uint32_t w = r.v[0][i];
+            v[2 * i] = DT == I8F_BF16 ? __uint_as_float(w << 16) : f16_bits_to_f32(w & 0xffffu);
+            v[2 * i + 1] = DT == I8F_BF16 ? __uint_as_float(w & 0xffff0000u) : f16_bits_to_f32(w >> 16);
         }
     }
 }
-template <int DT, bool APART>
-__device__ __forceinline__ void store_eight(char *p, int e0, int e1, const float (&v)[8]) {
+template <int DT>
+__device__ __forceinline__ Eight<DT> round_eight(const float (&v)[8]) {
+    Eight<DT> r;
     if constexpr (DT == I8F_F32) {
-        uint4 lo, hi;
-        __builtin_memcpy(&lo, v, 16);
-        __builtin_memcpy(&hi, v + 4, 16);
-        stream_store16(p + e0 * 4, lo), stream_store16(p + e1 * 4, hi);
+        __builtin_memcpy(&r, v, 32);
     } else {
-        uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = DT == I8F_BF16 ? f32x2_to_bf16x2_bits(v[2 * i], v[2 * i + 1]) : f32x2_to_f16x2_bits(v[2 * i], v[2 * i + 1]);
-        if constexpr (APART) stream_store8(p + e0 * 2, make_uint2(w[0], w[1])), stream_store8(p + e1 * 2, make_uint2(w[2], w[3]));
-        else stream_store16(p + e0 * 2, make_uint4(w[0], w[1], w[2], w[3]));
+        for (int i = 0; i < 4; ++i) r.v[0][i] = DT == I8F_BF16 ? f32x2_to_bf16x2_bits(v[2 * i], v[2 * i + 1]) : f32x2_to_f16x2_bits(v[2 * i], v[2 * i + 1]);
+    }
+    return r;
+}
+template <int DT, bool APART>
+__device__ __forceinline__ void store_eight(char *p, int e0, int e1, const Eight<DT> &r) {
+    if constexpr (DT == I8F_F32) {
+        __builtin_nontemporal_store(r.v[0], (any4_t *)(p + e0 * 4)), __builtin_nontemporal_store(r.v[1], (any4_t *)(p + e1 * 4));
+    } else if constexpr (APART) {
+        __builtin_nontemporal_store(__builtin_shufflevector(r.v[0], r.v[0], 0, 1), (any2_t *)(p + e0 * 2));
+        __builtin_nontemporal_store(__builtin_shufflevector(r.v[0], r.v[0], 2, 3), (any2_t *)(p + e1 * 2));
+    } else {
+        __builtin_nontemporal_store(r.v[0], (any4_t *)(p + e0 * 2));
+    }
+}
+template <int DT>
+__device__ __forceinline__ void store_some(char *p, int e0, int e1, int n0, int n1, const Eight<DT> &r) {
+    const uint32_t *w = (const uint32_t *)&r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if (e % 4 >= (e < 4 ? n0 : n1)) continue;
+        const int at = (e < 4 ? e0 : e1) + e % 4;
+        if constexpr (DT == I8F_F32) *(uint32_t *)(p + at * 4) = w[e];
+        else *(uint16_t *)(p + at * 2) = (uint16_t)(w[e / 2] >> (16 * (e % 2)));
     }
 }
 // a sum over LPH neighbouring lanes, in every one of them
@@ -174,7 +143,7 @@ __device__ __forceinline__ float sum_of_lanes(float v) {
 
 constexpr int DEEP = 4;   // passes that a wave requests at a time
 // A wave takes `per` passes of one token, a pass being 64 / LPH heads: the angles are the same for all of them.
-template <int DT, int LPH, bool APART>
+template <int DT, int LPH, bool APART, int ENDS>
 __global__ __launch_bounds__(256) void norm_rotate_kernel(const int64_t first, const unsigned chunks, const int per, const i8f_norm_rotate_args a, const Groups groups) {
     constexpr int HPP = 64 / LPH, SIZE = DT == I8F_F32 ? 4 : 2;
     const int lane = threadIdx.x & 63, sub = lane / LPH, l = lane % LPH;
@@ -184,16 +153,28 @@ __global__ __launch_bounds__(256) void norm_rotate_kernel(const int64_t first, c
     const int start = (int)(id % chunks) * per;
     const int64_t b = bt / a.tokens, t = bt % a.tokens;
     const int width = (int)a.width, pairs = a.axes ? a.first_pair[a.axes] : 0;
-    const bool low = APART && l < pairs / 4;   // (lanes behind the turned pairs hold eight neighbours in either form)
-    const int e0 = !APART ? 8 * l : low ? 4 * l : 2 * pairs + 8 * (l - pairs / 4), e1 = low ? pairs + 4 * l : e0 + 4;
-    const bool in = e0 < width;
+    const int lows = (pairs + 3) / 4;
+    const bool low = APART && l < lows;   // (lanes behind the turned pairs hold eight neighbours in either form)
+    int e0 = !APART ? 8 * l : low ? 4 * l : 2 * pairs + 8 * (l - lows), e1 = low ? pairs + 4 * l : e0 + 4;
+    int n0 = low ? pairs - 4 * l : width - e0, n1 = low ? n0 : n0 - 4;   // elements from e0 and e1 on, up to four of them the lane's
+    const bool in = n0 > 0;
+    int pair = low || !APART ? 4 * l : pairs, again = 0;   // the lane's first pair; elements (of each four, or of eight) of the lane before
+    if constexpr (ENDS != FULL) {
+        const int need = low ? 4 : 8, back = need - n0, begin = APART && !low ? 2 * pairs : 0;
+        if (in && back > 0 && back <= e0 - begin && (APART || back % 2 == 0)) {
+            again = back, e0 -= back, e1 -= back, n0 = 4, n1 = 4;
+            if (low) pair -= back;
+            else if (!APART) pair -= back / 2;
+        }
+    }
+    const bool whole = ENDS != SINGLE || (n0 >= 4 && n1 >= 4);
     float c[4], s[4];
     if (pairs) {
         double pos[I8F_MAX_AXES];
         token_positions(a, bt, pos);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (4 * l + i < pairs) turn(a, pos, 4 * l + i, c[i], s[i]);
+            if (pair + i < pairs) turn(a, pos, pair + i, c[i], s[i]);
     }
     int before = 0;
     for (int g = 0; g < groups.n; ++g) {
@@ -203,8 +184,9 @@ __global__ __launch_bounds__(256) void norm_rotate_kernel(const int64_t first, c
         if (lo >= hi) continue;
         float w[8];
         if (h.weight && in) {
-            if (DT == I8F_F32 || h.weight_dtype == I8F_F32) expand_eight<I8F_F32>(load_eight<I8F_F32, APART>((const char *)h.weight, e0, e1), w);
-            else expand_eight<DT>(load_eight<DT, APART>((const char *)h.weight, e0, e1), w);
+            const char *p = (const char *)h.weight;
+            if (DT == I8F_F32 || h.weight_dtype == I8F_F32) expand_eight<I8F_F32>(whole ? load_eight<I8F_F32, APART>(p, e0, e1) : load_some<I8F_F32>(p, e0, e1, n0, n1), w);
+            else expand_eight<DT>(whole ? load_eight<DT, APART>(p, e0, e1) : load_some<DT>(p, e0, e1, n0, n1), w);
         }
         const char *x = (const char *)h.x + (b * h.batch_stride + t * h.token_stride) * SIZE;
         char *out = (char *)h.out + bt * h.heads * width * SIZE;
@@ -213,8 +195,11 @@ __global__ __launch_bounds__(256) void norm_rotate_kernel(const int64_t first, c
 #pragma unroll
             for (int i = 0; i < DEEP; ++i) {
                 const int head = (pass + i) * HPP + sub;
-                if (pass + i < hi && in && head < h.heads) raw[i] = load_eight<DT, APART>(x + head * h.head_stride * SIZE, e0, e1);
-                else raw[i] = {};
+                raw[i] = {};
+                if (pass + i < hi && in && head < h.heads) {
+                    if (whole) raw[i] = load_eight<DT, APART>(x + head * h.head_stride * SIZE, e0, e1);
+                    else raw[i] = load_some<DT>(x + head * h.head_stride * SIZE, e0, e1, n0, n1);
+                }
             }
 #pragma unroll
             for (int i = 0; i < DEEP; ++i) {
@@ -225,7 +210,7 @@ __global__ __launch_bounds__(256) void norm_rotate_kernel(const int64_t first, c
                 if (a.norm) {
                     float sum = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(v[e], v[e], sum);
+                    for (int e = 0; e < 8; ++e) sum = ENDS != FULL && (low ? e % 4 : e) < again ? sum : __builtin_fmaf(v[e], v[e], sum);
                     const float rstd = 1.0f / sqrtf(sum_of_lanes<LPH>(sum) / (float)width + a.eps);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[e] *= rstd;
@@ -239,28 +224,20 @@ __global__ __launch_bounds__(256) void norm_rotate_kernel(const int64_t first, c
                     for (int e = 0; e < 4; ++e) {
                         float &v0 = v[APART ? e : 2 * e], &v1 = v[APART ? e + 4 : 2 * e + 1];
                         const float y0 = __builtin_fmaf(v0, c[e], -(v1 * s[e])), y1 = __builtin_fmaf(v0, s[e], v1 * c[e]);
-                        if (4 * l + e < pairs) v0 = y0, v1 = y1;   // (the others as they are: 0 times an infinity is none)
+                        if (pair + e < pairs) v0 = y0, v1 = y1;   // (the others as they are: 0 times an infinity is none)
                     }
                 }
-                if (in && head < h.heads) store_eight<DT, APART>(out + (int64_t)head * width * SIZE, e0, e1, v);
+                if (in && head < h.heads) {
+                    if (whole) store_eight<DT, APART>(out + (int64_t)head * width * SIZE, e0, e1, round_eight<DT>(v));
+                    else store_some<DT>(out + (int64_t)head * width * SIZE, e0, e1, n0, n1, round_eight<DT>(v));
+                }
             }
         }
     }
 }
 
-// All operands in 16-byte pieces, and with pairs that lie apart the turned and the other elements in whole lanes.
-bool in_pieces(const i8f_norm_rotate_args &a, const Groups &groups) {
-    const int64_t per16 = 16 / (int64_t)dtype_size(a.dtype);
-    if (a.width % 8 || (a.axes && a.apart && a.first_pair[a.axes] % 4)) return false;
-    for (int i = 0; i < groups.n; ++i) {
-        const i8f_heads &g = groups.g[i];
-        if (((uintptr_t)g.x | (uintptr_t)g.weight | (uintptr_t)g.out) % 16 || g.batch_stride % per16 || g.token_stride % per16 || g.head_stride % per16) return false;
-    }
-    return true;
-}
-
-template <int DT, int LPH, bool APART>
-int launch_pieces(const i8f_norm_rotate_args &a, const Groups &groups, hipStream_t st) {
+template <int DT, int LPH, bool APART, int ENDS>
+int launch_passes(const i8f_norm_rotate_args &a, const Groups &groups, hipStream_t st) {
     int64_t passes = 0;
     for (int i = 0; i < groups.n; ++i) passes += (groups.g[i].heads + 64 / LPH - 1) / (64 / LPH);
     if (passes > 0x7fffffff) return I8F_ERR_UNSUPPORTED;
@@ -274,26 +251,29 @@ int launch_pieces(const i8f_norm_rotate_args &a, const Groups &groups, hipStream
     const int64_t waves = tokens * chunks, most = (int64_t)4 << 23;   // (a launch has fewer than 2^32 threads)
     for (int64_t w = 0; w < waves; w += most) {
         const int64_t n = waves - w < most ? waves - w : most;
-        hipLaunchKernelGGL((norm_rotate_kernel<DT, LPH, APART>), dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, w, (unsigned)chunks, (int)per, a, groups);
+        hipLaunchKernelGGL((norm_rotate_kernel<DT, LPH, APART, ENDS>), dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, w, (unsigned)chunks, (int)per, a, groups);
         if (int rc = check_launch()) return rc;
     }
     return I8F_OK;
 }
+template <int DT, int LPH, bool APART>
+int launch_ends(const i8f_norm_rotate_args &a, const Groups &groups, hipStream_t st) {
+    const int64_t pairs = APART ? a.first_pair[a.axes] : 0, rest = a.width - 2 * pairs;
+    if (pairs % 4 == 0 && rest % 8 == 0) return launch_passes<DT, LPH, APART, FULL>(a, groups, st);
+    const bool halves = pairs % 4 == 0 || pairs >= 4, end = rest % 8 == 0 || (rest >= 8 && (APART || rest % 2 == 0));
+    return halves && end ? launch_passes<DT, LPH, APART, SHIFTED>(a, groups, st) : launch_passes<DT, LPH, APART, SINGLE>(a, groups, st);
+}
 template <int DT, bool APART>
 int launch_lanes(const i8f_norm_rotate_args &a, const Groups &groups, hipStream_t st) {
-    if (a.width <= 64) return launch_pieces<DT, 8, APART>(a, groups, st);
-    if (a.width <= 128) return launch_pieces<DT, 16, APART>(a, groups, st);
-    if (a.width <= 256) return launch_pieces<DT, 32, APART>(a, groups, st);
-    return launch_pieces<DT, 64, APART>(a, groups, st);
+    const int64_t pairs = APART ? a.first_pair[a.axes] : 0, lanes = (pairs + 3) / 4 + (a.width - 2 * pairs + 7) / 8;   // (33 at the most)
+    if (lanes <= 8) return launch_ends<DT, 8, APART>(a, groups, st);
+    if (lanes <= 16) return launch_ends<DT, 16, APART>(a, groups, st);
+    if (lanes <= 32) return launch_ends<DT, 32, APART>(a, groups, st);
+    return launch_ends<DT, 64, APART>(a, groups, st);
 }
-
 template <int DT>
 int launch(const i8f_norm_rotate_args &a, const Groups &groups, hipStream_t st) {
-    if (in_pieces(a, groups)) return a.axes && a.apart ? launch_lanes<DT, true>(a, groups, st) : launch_lanes<DT, false>(a, groups, st);
-    const int64_t pairs = (a.width + 1) / 2;
-    if (pairs <= 64) return launch_any<DT, 1>(a, groups, st);
-    if (pairs <= 128) return launch_any<DT, 2>(a, groups, st);
-    return launch_any<DT, 4>(a, groups, st);
+    return a.axes && a.apart ? launch_lanes<DT, true>(a, groups, st) : launch_lanes<DT, false>(a, groups, st);
 }
 
 // The elements that a strided tensor reaches to from its first one, -1 past 2^62.
@@ -314,7 +294,7 @@ int validate(const i8f_norm_rotate_args &a, const i8f_heads *groups, int n) {
     if (a.batch < 0 || a.tokens < 0 || a.width < 1 || !valid_dtype(a.dtype) || n < 0 || (n && !groups)) return I8F_ERR_INVALID;
     if (a.norm && !(a.eps >= 0.0f)) return I8F_ERR_INVALID;
     if (a.axes < 0) return I8F_ERR_INVALID;
-    if (a.axes > I8F_MAX_AXES || n > I8F_MAX_HEAD_GROUPS || a.width > 512) return I8F_ERR_UNSUPPORTED;
+    if (a.axes > I8F_MAX_AXES || n > I8F_MAX_HEAD_GROUPS || a.width > 256) return I8F_ERR_UNSUPPORTED;
     if (a.batch > 0x7fffffff || a.tokens > 0x7fffffff || (a.batch && a.tokens > ((int64_t)1 << 40) / a.batch)) return I8F_ERR_UNSUPPORTED;
     const bool any = a.batch && a.tokens;
     if (a.axes) {

@@ -47,7 +47,7 @@ def test_norm_rotate_arguments_are_checked_before_any_launch(L):
     assert _heads(L, {"norm": 0}, {"weight": 16, "weight_dtype": L.BF16}) == INVALID     # a weight without a norm
     assert _heads(L, None, {"out": 1 << 24}, {"out": (1 << 24) + 94}) == INVALID          # outputs that overlap
     assert _heads(L, None, {}, {}, n=-1) == INVALID and L.lib().i8f_norm_rotate(ctypes.byref(L._NormRotateArgs(width=8)), None, 1, None) == INVALID
-    assert _heads(L, {"axes": 5}, {}) == UNSUPPORTED and _heads(L, {"width": 513}, {}) == UNSUPPORTED and _heads(L, None, *[{}] * 5) == UNSUPPORTED
+    assert _heads(L, {"axes": 5}, {}) == UNSUPPORTED and _heads(L, {"width": 257}, {}) == UNSUPPORTED and _heads(L, None, *[{}] * 5) == UNSUPPORTED
     assert _heads(L, {"batch": 1 << 31}, {}) == UNSUPPORTED and _heads(L, {"tokens": 1 << 31}, {}) == UNSUPPORTED
     assert _heads(L, None, {"token_stride": 1 << 62}) == UNSUPPORTED
     for empty in ({"batch": 0}, {"tokens": 0}):

@@ -72,7 +72,7 @@ def grid(tokens, axes, dtype=torch.int64):
 # (batch, tokens, heads of each tensor, width, elements to an axis)
 SHAPES = [(1, 1, (1,), 1, ()), (2, 1, (3,), 2, (2,)), (1, 5, (1, 2), 7, (2, 4)), (3, 4, (5,), 16, (8, 8)), (1, 77, (5, 5), 37, (10, 14)), (2, 33, (4, 1), 64, (20, 22, 22)),
           (1, 9, (3,), 64, (2, 2, 2, 58)), (2, 130, (16,), 72, (16, 20)), (1, 64, (7, 7), 96, (32, 32, 32)), (2, 300, (6, 2), 128, (16, 56, 56)), (1, 3000, (10, 10), 128, (44, 42, 42)),
-          (1, 40, (3, 3), 120, (40,)), (1, 17, (2,), 130, (60, 70)), (2, 21, (3, 1), 256, (64, 64)), (1, 10, (2,), 255, (250,)), (1, 6, (2, 2), 512, (128, 128, 256)), (1, 6, (2,), 511, (2,)),
+          (1, 40, (3, 3), 120, (40,)), (1, 17, (2,), 130, (60, 70)), (2, 21, (3, 1), 256, (64, 64)), (1, 10, (2,), 255, (250,)), (1, 6, (2, 2), 256, (62, 64, 128)), (1, 6, (2,), 255, (2,)), (2, 5, (3,), 256, (254,)), (1, 9, (2, 5), 64, (62,)), (1, 9, (2,), 66, (64,)),
           (1, 3, (70, 3), 128, (64, 32, 32)), (40000, 1, (1,), 8, (8,))]
 
 
@@ -175,7 +175,7 @@ def test_refusals(pkg, dev):
                 lambda: pkg.rotate_heads(x, r, p[:2]), lambda: pkg.rotate_heads(x, r, p[:, :1]), lambda: pkg.rotate_heads(x, r, p[None].expand(3, -1, -1)),
                 lambda: pkg.rotate_heads(x, r, p.half()), lambda: pkg.rotate_heads(x, r, p.cpu()), lambda: pkg.rotate_heads(x, pkg.RotaryAxes((8, 10)), p),
                 lambda: pkg.rotate_heads(x, pkg.RotaryAxes((8, 4), device="cpu"), p), lambda: pkg.norm_heads([x, x.half()], **ok), lambda: pkg.norm_heads(x.double(), **ok),
-                lambda: pkg.norm_heads(torch.zeros(1, 1, 1, 513, device="cuda")), lambda: pkg.norm_heads(torch.zeros(1, 1, 1, 0, device="cuda"))):
+                lambda: pkg.norm_heads(torch.zeros(1, 1, 1, 257, device="cuda")), lambda: pkg.norm_heads(torch.zeros(1, 1, 1, 0, device="cuda"))):
         with pytest.raises((ValueError, TypeError, RuntimeError)):
             bad()
 
