@@ -36,7 +36,7 @@ struct Launch {
     uint32_t row_tiles, splits;  // of a (batch, state head)
     uint32_t tiles;              // of a split, in tiles of the kernel
     uint32_t loaded;             // elements of a row in memory, whole pieces of eight
-    uint32_t wide_out;           // rows of the result may be written four elements at a time
+    uint32_t wide_out;           // rows of the result are whole aligned pieces
     float *partial;             // splits > 1: [batch * kv_heads, splits, rows, padded width], then [.., rows, 2]: maximum and sum
     float *stats;
 };
@@ -336,8 +336,8 @@ __global__ __launch_bounds__((Shape<DT, DP, APART, MASK>::WAVES * 64), (Shape<DT
             }
         }
     } else {
-        if (row >= p.rows) return;
         if (p.splits > 1) {
+            if (row >= p.rows) return;
             const int64_t at_row = ((int64_t)bg * p.splits + split) * p.rows + row;
 #pragma unroll
             for (int d = 0; d < ND; ++d)
@@ -347,24 +347,38 @@ __global__ __launch_bounds__((Shape<DT, DP, APART, MASK>::WAVES * 64), (Shape<DT
             if (half == 0) p.stats[at_row * 2] = top, p.stats[at_row * 2 + 1] = sum;
             return;
         }
+        // A lane has pieces of one row, memory wants whole lines: the rows change places in LDS.  The stage that the last tile is not in has been
+        // read by everyone and nothing is under way to it, and is as large as the workgroup's rows.
         const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
-        uint16_t *const to = (uint16_t *)a.out + ((b * a.queries + query) * a.heads + head) * a.width;
+        static_assert(WAVES * 32 * DP * 2 <= 2 * S::TILE, "");
+        char *const mine = lds + stage * 2 * S::TILE + wave * 32 * DP * 2;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int e = 32 * d + 8 * i + 4 * half;
-                if (p.wide_out) {
-                    if (e < a.width) {
-                        const float x = o[d][4 * i] * by, y = o[d][4 * i + 1] * by, z = o[d][4 * i + 2] * by, w = o[d][4 * i + 3] * by;
-                        const uint2 v = DT == I8F_BF16 ? make_uint2(f32x2_to_bf16x2_bits(x, y), f32x2_to_bf16x2_bits(z, w)) : make_uint2(f32x2_to_f16x2_bits(x, y), f32x2_to_f16x2_bits(z, w));
-                        stream_store8(to + e, v);
-                    }
-                } else {
-                    for (int j = 0; j < 4; ++j)
-                        if (e + j < a.width) store_from_f32<DT>(to, e + j, o[d][4 * i + j] * by);
-                }
+                const float x = o[d][4 * i] * by, y = o[d][4 * i + 1] * by, z = o[d][4 * i + 2] * by, w = o[d][4 * i + 3] * by;
+                const uint2 v = DT == I8F_BF16 ? make_uint2(f32x2_to_bf16x2_bits(x, y), f32x2_to_bf16x2_bits(z, w)) : make_uint2(f32x2_to_f16x2_bits(x, y), f32x2_to_f16x2_bits(z, w));
+                *(uint2 *)(mine + k_row + k_piece<DP>(lane & 31, 4 * d + i) * 16 + half * 8) = v;
             }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        const unsigned first = row_tile * S::ROWS + wave * 32;
+#pragma unroll
+        for (int i = 0; i < 32 * S::PIECES / 64; ++i) {
+            const int at = i * 64 + lane, r = at / S::PIECES, c = at % S::PIECES;
+            const unsigned own = first + r;
+            if (own >= p.rows || c * 8 >= a.width) continue;
+            const uint4 v = *(const uint4 *)(mine + r * DP * 2 + k_piece<DP>(r, c) * 16);
+            const int64_t q_at = p.share == 1 ? own : own / p.share, h_at = p.share == 1 ? g : g * p.share + own % p.share;
+            uint16_t *const to = (uint16_t *)a.out + ((b * a.queries + q_at) * a.heads + h_at) * a.width + c * 8;
+            if (p.wide_out) {
+                stream_store16(to, v);
+            } else {
+                uint16_t e[8];
+                __builtin_memcpy(e, &v, 16);
+                for (int j = 0; j < 8; ++j)
+                    if (c * 8 + j < a.width) to[j] = e[j];
+            }
+        }
     }
 }
 
@@ -560,7 +574,7 @@ extern "C" int i8f_attention(const i8f_attention_args *args, void *stream) {
     if (int rc = check_device()) return rc;
     hipStream_t st = (hipStream_t)stream;
     Launch p = {a, (uint32_t)share, (uint32_t)(a.queries * share), (uint32_t)plan.row_tiles, (uint32_t)plan.splits, (uint32_t)plan.tiles, (uint32_t)round_up(a.width, 8)};
-    p.wide_out = a.width % 4 == 0 && (uintptr_t)a.out % 8 == 0;
+    p.wide_out = a.width % 8 == 0 && (uintptr_t)a.out % 16 == 0;
     p.partial = (float *)a.workspace;
     p.stats = p.partial ? p.partial + plan.partial_bytes / 4 / (plan.padded + 2) * plan.padded : nullptr;
     int64_t bytes[3];
