@@ -249,7 +249,8 @@ __global__ __launch_bounds__((Shape<DT, DP, APART, MASK>::WAVES * 64), (Shape<DT
         if ((now & ALL) != ALL) {
 #pragma unroll
             for (int k = 0; k < KB; ++k) {
-                const uint32_t mine = (uint32_t)(now >> (32 * k)) >> (4 * half);
+                uint32_t mine = (uint32_t)(now >> (32 * k)) >> (4 * half);
+                asm volatile("" : "+v"(mine));   // (keeps what follows in this branch: the last tile's, or a mask's)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[k][i] = mine >> (8 * (i / 4) + i % 4) & 1 ? s[k][i] : -__builtin_inff();
             }
@@ -258,7 +259,7 @@ __global__ __launch_bounds__((Shape<DT, DP, APART, MASK>::WAVES * 64), (Shape<DT
 #pragma unroll
         for (int k = 0; k < KB; ++k)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) most = fmaxf(most, s[k][i]);
+            for (int i = 0; i < 16; ++i) most = __builtin_elementwise_maximum(most, s[k][i]);
         most = max_of_halves(most) * factor;
         // The reference of the exponentials follows the maximum only where that has grown by 2^8: the weights are below 2^8 then, which costs
         // no bits, and the result is divided by their sum either way.
