@@ -7,6 +7,7 @@
 // O^T = V^T P^T, the contraction index being free to run in the order in which a lane happens to hold the states; the first operand comes
 // out of row-major V by LDS reads that transpose (ds_read_b64_tr_b16).
 #include <initializer_list>
+#include <type_traits>
 #include <utility>
 
 #include "dma.hpp"
@@ -85,12 +86,12 @@ __device__ __forceinline__ bool counts(const i8f_attention_args &a, int64_t b, i
 }
 
 // The 16-byte pieces of a row are exchanged within it by a function of the row, so that the lanes of an LDS read are spread over the banks.
-// K is read by eight rows' same piece at a time (ds_read_b128), V by four rows' same 64 bytes (ds_read_b64_tr_b16); rows of 192 bytes lie
-// three quarters of the banks apart by themselves.
+// K is read by 32 rows' same piece at a time (ds_read_b128): sixteen rows that differ in their number's last four bits are on different
+// banks.  V is read by four rows' same 64 bytes (ds_read_b64_tr_b16); rows of 192 bytes lie three quarters of the banks apart by themselves.
 template <int DP>
 __device__ __forceinline__ int k_piece(int row, int piece) {
-    if constexpr (DP == 96) return piece ^ ((row >> 2) & 1);
-    else if constexpr (DP % 128 == 0) return piece ^ (row & 7);
+    if constexpr (DP == 96) return piece ^ ((row >> 2) & 3);
+    else if constexpr (DP % 128 == 0) return piece ^ (row & 15);
     else return piece ^ ((row >> 1) & 7);
 }
 template <int DP>
@@ -122,15 +123,14 @@ __global__ __launch_bounds__((Shape<DT, DP, APART, MASK>::WAVES * 64), (Shape<DT
     const unsigned id = xcd * per + (xcd < extra ? xcd : extra) + blockIdx.x / 8;
     const unsigned row_tile = id % p.row_tiles, split = id / p.row_tiles % p.splits, bg = id / p.row_tiles / p.splits;
     const int64_t b = bg / (unsigned)a.kv_heads, g = bg % (unsigned)a.kv_heads;
-    int64_t n = a.keys;
+    int n = (int)a.keys;
     if (a.key_lengths) {
         const int64_t given = a.lengths_type ? ((const int64_t *)a.key_lengths)[b] : ((const int32_t *)a.key_lengths)[b];
-        n = given < 0 ? 0 : given < n ? given : n;
+        n = given < 0 ? 0 : given < n ? (int)given : n;
     }
-    int64_t last_tile = (n + KT - 1) / KT, tile = (int64_t)split * p.tiles;
-    last_tile = last_tile < tile + p.tiles ? last_tile : tile + p.tiles;
-    if constexpr (APART) tile += wave;   // (every WAVES-th tile)
-    constexpr int STEP = APART ? WAVES : 1;
+    const int from_tile = (int)(split * p.tiles) + (APART ? wave : 0), all_tiles = (n - 1 + KT) / KT, to_tile = (int)((split + 1) * p.tiles);
+    const int last_tile = all_tiles < to_tile ? all_tiles : to_tile;
+    constexpr int STEP = APART ? WAVES : 1;   // (apart, every WAVES-th tile is a wave's)
 
     // a wave's 32 rows, a lane's in both halves
     const unsigned row = row_tile * S::ROWS + (APART ? 0 : wave * 32) + (lane & 31), real = row < p.rows ? row : p.rows - 1;
@@ -160,43 +160,51 @@ __global__ __launch_bounds__((Shape<DT, DP, APART, MASK>::WAVES * 64), (Shape<DT
     const uint16_t *kp = (const uint16_t *)a.k + b * a.k_batch + g * a.k_head, *vp = (const uint16_t *)a.v + b * a.v_batch + g * a.v_head;
     const uint32_t lds_at = (uint32_t)(uintptr_t)(gemm::lds_ptr_t)lds + (APART ? wave * 4 * S::TILE : 0);   // stage s: K at s * 2 * TILE, V behind it
 
-    // which states of tile t count: bit j for the tile's state j; with a mask a lane's own addend besides
-    auto on_of = [&](int64_t t, float &add) -> uint64_t {
-        const int64_t left = n - t * KT;
-        if constexpr (!MASK) {
-            return left >= 64 ? ~0ull : left <= 0 ? 0ull : KT == 32 && left >= 32 ? 0xffffffffull : (1ull << left) - 1;
-        } else {
-            const int64_t j = t * KT + lane;
-            bool on = lane < KT && lane < left;
-            add = 0.0f;
-            if (on) on = counts(a, b, j, add);
-            return __ballot(on);
-        }
+    // A tile, which of its states count (bit j for its state j) and with a mask a lane's own addend.
+    struct Tile {
+        int at;
+        uint64_t on;
+        float add;
     };
     constexpr uint64_t ALL = KT == 64 ? ~0ull : 0xffffffffull;
-    auto request = [&](int64_t t, int stage, uint64_t on) {
-        const v4i kr = make_rsrc(kp + t * KT * a.k_token, 0x7ffffff0u), vr = make_rsrc(vp + t * KT * a.v_token, 0x7ffffff0u);
-        const uint32_t to = lds_at + stage * 2 * S::TILE + (APART ? 0 : wave * 1024);
-        if ((on & ALL) == ALL) {
-#pragma unroll
-            for (int i = 0; i < S::LOADS; ++i) dma16(kr, to + i * (APART ? 1 : WAVES) * 1024, from_k[i], 0);
-#pragma unroll
-            for (int i = 0; i < S::LOADS; ++i) dma16(vr, to + S::TILE + i * (APART ? 1 : WAVES) * 1024, from_v[i], 0);
-        } else {
-#pragma unroll
-            for (int i = 0; i < S::LOADS; ++i) {
-                const bool in = on >> (piece_at(i) / S::PIECES) & 1;
-                dma16(kr, to + i * (APART ? 1 : WAVES) * 1024, in ? from_k[i] : NOWHERE, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < S::LOADS; ++i) {
-                const bool in = on >> (piece_at(i) / S::PIECES) & 1;
-                dma16(vr, to + S::TILE + i * (APART ? 1 : WAVES) * 1024, in ? from_v[i] : NOWHERE, 0);
+    auto tile_from = [&](int at) {   // the first tile from `at` on with a state that counts, or one past the last
+        Tile t = {at, ALL, 0.0f};
+        for (; t.at < last_tile; t.at += STEP) {
+            const int left = n - t.at * KT;
+            if constexpr (!MASK) {
+                if (left < KT) t.on = (1ull << left) - 1;
+                break;
+            } else {
+                bool on = lane < KT && lane < left;
+                t.add = 0.0f;
+                if (on) on = counts(a, b, (int64_t)t.at * KT + lane, t.add);
+                if ((t.on = __ballot(on)) != 0) break;
             }
         }
+        return t;
+    };
+    // the wave's pieces of a tile of K (or of V) on their way into a stage; those of states that do not count are zeros
+    auto request = [&](const Tile &t, const uint16_t *x, int64_t token, const uint32_t (&from)[S::LOADS], uint32_t to) {
+        if (t.at >= last_tile) return;
+        const v4i r = make_rsrc(x + (int64_t)t.at * KT * token, 0x7ffffff0u);
+        if (t.on == ALL) {
+#pragma unroll
+            for (int i = 0; i < S::LOADS; ++i) dma16(r, to + i * (APART ? 1 : WAVES) * 1024, from[i], 0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < S::LOADS; ++i) dma16(r, to + i * (APART ? 1 : WAVES) * 1024, t.on >> (piece_at(i) / S::PIECES) & 1 ? from[i] : NOWHERE, 0);
+        }
+    };
+    const uint32_t lds_to = lds_at + (APART ? 0 : wave * 1024);
+    auto request_k = [&](const Tile &t, int stage) { request(t, kp, a.k_token, from_k, lds_to + stage * 2 * S::TILE); };
+    auto request_v = [&](const Tile &t, int stage) { request(t, vp, a.v_token, from_v, lds_to + stage * 2 * S::TILE + S::TILE); };
+    auto all_here = [&]() {   // what was requested has arrived, and (together) everyone has read what may now be overwritten
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if constexpr (!APART) __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
     };
 
-    v16f o[ND];
+    v16f o[ND], s[KB];
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = v16f{};
     float top = LOWEST, sum = 0.0f;
@@ -206,39 +214,29 @@ __global__ __launch_bounds__((Shape<DT, DP, APART, MASK>::WAVES * 64), (Shape<DT
     const int k_row = (lane & 31) * DP * 2;
     const int v_row = (4 * half + ((lane >> 2) & 3)) * DP * 2 + (2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) * 16 + (lane & 1) * 8;
     const int v_x = v_quad<DP>((lane >> 2) & 3);
+    char *const tiles = lds + (APART ? wave * 4 * S::TILE : 0);
     float *const adds = (float *)(lds + S::LDS) + wave * 64;
+    auto k_part = [&](const char *ks, int e, int k) { return *(const v8s *)(ks + k * 32 * DP * 2 + k_row + k_piece<DP>(lane & 31, 2 * e + half) * 16); };
 
-    float add = 0.0f;
-    uint64_t on = 0;
-    auto next_tile = [&](int64_t t) {   // the first tile from t on with a state that counts
-        while (t < last_tile && (on = on_of(t, add)) == 0) t += STEP;
-        return t;
-    };
-    tile = next_tile(tile);
-    if (tile < last_tile) request(tile, 0, on);
+    Tile now = tile_from(from_tile), next = tile_from(now.at + STEP);
+    request_k(now, 0), request_v(now, 0), request_k(next, 1);
     int stage = 0;
-    while (tile < last_tile) {
-        const uint64_t now = on;
-        if constexpr (MASK) adds[lane] = add;
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        if constexpr (!APART) __builtin_amdgcn_s_barrier();   // everyone's pieces of the tile are there, and the other stage has been read
-        asm volatile("" ::: "memory");
-        const int64_t next = next_tile(tile + STEP);
-        if (next < last_tile) request(next, stage ^ 1, on);
-
-        const char *ks = lds + (APART ? wave * 4 * S::TILE : 0) + stage * 2 * S::TILE, *vs = ks + S::TILE;
-        v16f s[KB];
+    if (now.at < last_tile) {
+        all_here();
 #pragma unroll
         for (int k = 0; k < KB; ++k) s[k] = v16f{};
 #pragma unroll
         for (int e = 0; e < NK; ++e)
 #pragma unroll
-            for (int k = 0; k < KB; ++k)
-                s[k] = mfma<DT>(*(const v8s *)(ks + k * 32 * DP * 2 + k_row + k_piece<DP>(lane & 31, 2 * e + half) * 16), q[e], s[k]);
-        // scores: times the scale in the exponential's argument, or here where addends come on top
-        float factor = to_log2;
+            for (int k = 0; k < KB; ++k) s[k] = mfma<DT>(k_part(tiles, e, k), q[e], s[k]);
+    }
+    // One tile: its scores are there, the next tile's are formed on the matrix unit (MORE) while the vector units have the exponentials.
+    auto step = [&](auto more) __attribute__((always_inline)) {
+        constexpr bool MORE = decltype(more)::value;
+        float factor = to_log2;   // scores are scaled in the exponential's argument, or here where addends come on top
         if constexpr (MASK) {
             if (a.mask_type != I8F_MASK_BYTES) {
+                adds[lane] = now.add;
 #pragma unroll
                 for (int k = 0; k < KB; ++k)
 #pragma unroll
@@ -246,10 +244,10 @@ __global__ __launch_bounds__((Shape<DT, DP, APART, MASK>::WAVES * 64), (Shape<DT
                 factor = 1.0f;
             }
         }
-        if ((now & ALL) != ALL) {
+        if (now.on != ALL) {
 #pragma unroll
             for (int k = 0; k < KB; ++k) {
-                uint32_t mine = (uint32_t)(now >> (32 * k)) >> (4 * half);
+                uint32_t mine = (uint32_t)(now.on >> (32 * k)) >> (4 * half);
                 asm volatile("" : "+v"(mine));   // (keeps what follows in this branch: the last tile's, or a mask's)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[k][i] = mine >> (8 * (i / 4) + i % 4) & 1 ? s[k][i] : -__builtin_inff();
@@ -271,27 +269,48 @@ __global__ __launch_bounds__((Shape<DT, DP, APART, MASK>::WAVES * 64), (Shape<DT
             for (int d = 0; d < ND; ++d) o[d] *= fade;
         }
         const float from = RAISE - top;
+        all_here();   // the tile's V and the next one's K
+        const Tile after = MORE ? tile_from(next.at + STEP) : next;
+        if constexpr (MORE) request_k(after, stage), request_v(next, stage ^ 1);
+        const char *vs = tiles + stage * 2 * S::TILE + S::TILE, *ks = tiles + (stage ^ 1) * 2 * S::TILE;
+        v16f t[KB];
+        if constexpr (MORE) {
 #pragma unroll
-        for (int k = 0; k < KB; ++k)
+            for (int k = 0; k < KB; ++k) t[k] = v16f{};
+        }
+        constexpr int PARTS = 2 * KB;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                uint32_t w[4];
+        for (int part = 0; part < PARTS; ++part) {
+            const int k = part / 2, j = part % 2;
+            if constexpr (MORE) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    w[i] = round_weights<DT>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[k][8 * j + 2 * i], factor, from)),
-                                             __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][8 * j + 2 * i + 1], factor, from)), sum);
-                const v8s weights = __builtin_bit_cast(v8s, (v4i){(int)w[0], (int)w[1], (int)w[2], (int)w[3]});
+                for (int e = NK * part / PARTS; e < NK * (part + 1) / PARTS; ++e)
 #pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    typedef __attribute__((address_space(3))) v4s *v4s_lds;
-                    const char *at = vs + (k * 32 + j * 16) * DP * 2 + v_row + (d ^ v_x) * 64;
-                    const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s_lds)(gemm::lds_ptr_t)at);
-                    const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s_lds)(gemm::lds_ptr_t)(at + 8 * DP * 2));
-                    o[d] = mfma<DT>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), weights, o[d]);
-                }
+                    for (int x = 0; x < KB; ++x) t[x] = mfma<DT>(k_part(ks, e, x), q[e], t[x]);
             }
-        tile = next, stage ^= 1;
-    }
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                w[i] = round_weights<DT>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[k][8 * j + 2 * i], factor, from)),
+                                         __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][8 * j + 2 * i + 1], factor, from)), sum);
+            const v8s weights = __builtin_bit_cast(v8s, (v4i){(int)w[0], (int)w[1], (int)w[2], (int)w[3]});
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                typedef __attribute__((address_space(3))) v4s *v4s_lds;
+                const char *at = vs + (k * 32 + j * 16) * DP * 2 + v_row + (d ^ v_x) * 64;
+                const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s_lds)(gemm::lds_ptr_t)at);
+                const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s_lds)(gemm::lds_ptr_t)(at + 8 * DP * 2));
+                o[d] = mfma<DT>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), weights, o[d]);
+            }
+        }
+        if constexpr (MORE) {
+#pragma unroll
+            for (int k = 0; k < KB; ++k) s[k] = t[k];
+        }
+        now = next, next = after, stage ^= 1;
+    };
+    while (next.at < last_tile) step(std::integral_constant<bool, true>{});
+    if (now.at < last_tile) step(std::integral_constant<bool, false>{});
 
     // a lane has elements 32 d + 8 (i / 4) + 4 half + i % 4 of its row
     sum = sum_of_halves(sum);
