@@ -221,8 +221,11 @@ __global__ __launch_bounds__((Shape<DT, DP, APART, MASK>::WAVES * 64), (Shape<DT
     Tile now = tile_from(from_tile), next = tile_from(now.at + STEP);
     request_k(now, 0), request_v(now, 0), request_k(next, 1);
     int stage = 0;
+    all_here();
+    // (the rows have arrived as well: without this the compiler waits for them, and with them for the tiles under way, in every step)
+#pragma unroll
+    for (int e = 0; e < NK; ++e) asm volatile("" : "+v"(q[e]));
     if (now.at < last_tile) {
-        all_here();
 #pragma unroll
         for (int k = 0; k < KB; ++k) s[k] = v16f{};
 #pragma unroll
