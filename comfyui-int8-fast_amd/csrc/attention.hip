@@ -31,6 +31,14 @@ typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 
 constexpr float LOWEST = -3.4028234663852886e38f, TO_LOG2 = 1.4426950408889634f;
 
+// Division of a number below 2^31 by a fixed one: with 2^(s-1) < d <= 2^s and m = floor(2^(31+s) / d) + 1 the product is too large by less
+// than a d-th.
+struct Divisor {
+    uint32_t m, s;
+    Divisor(uint32_t d = 1) : s(d > 1 ? 32 - __builtin_clz(d - 1) : 0) { m = (uint32_t)((1ull << (31 + s)) / d + 1); }
+    __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return (uint32_t)(((uint64_t)x * m) >> (31 + s)); }
+};
+
 struct Launch {
     i8f_attention_args a;
     uint32_t share, rows;        // heads to one of the states', rows = queries * share to (batch, state head)
@@ -38,6 +46,7 @@ struct Launch {
     uint32_t tiles;              // of a split, in tiles of the kernel
     uint32_t loaded;             // elements of a row in memory, whole pieces of eight
     uint32_t wide_out;           // rows of the result are whole aligned pieces
+    Divisor by_share, by_row_tiles, by_splits, by_kv_heads;
     float *partial;             // splits > 1: [batch * kv_heads, splits, rows, padded width], then [.., rows, 2]: maximum and sum
     float *stats;
 };
@@ -70,19 +79,23 @@ __device__ __forceinline__ float sum_of_halves(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Whether state j of batch b counts, and its addend in units of log 2.
-__device__ __forceinline__ bool counts(const i8f_attention_args &a, int64_t b, int64_t j, float &m) {
+// A state's element of the mask as it is in memory, and whether it counts by it, with its addend in units of log 2.
+__device__ __forceinline__ uint32_t mask_bits(const i8f_attention_args &a, int64_t b, int64_t j) {
     const int64_t at = b * a.mask_batch + j * a.mask_key;
-    m = 0.0f;
-    bool on;
     switch (a.mask_type) {
-    case I8F_MASK_BYTES: return ((const uint8_t *)a.key_mask)[at] != 0;
-    case I8F_MASK_BF16: m = load_as_f32<I8F_BF16>(a.key_mask, at), on = !(m <= -3.3895313892515355e38f); break;
-    case I8F_MASK_F16: m = load_as_f32<I8F_F16>(a.key_mask, at), on = !(m <= -65504.0f); break;
-    default: m = ((const float *)a.key_mask)[at], on = !(m <= LOWEST); break;
+    case I8F_MASK_BYTES: return ((const uint8_t *)a.key_mask)[at];
+    case I8F_MASK_F32: return ((const uint32_t *)a.key_mask)[at];
+    default: return ((const uint16_t *)a.key_mask)[at];
     }
-    m = on ? fmaxf(m * TO_LOG2, LOWEST) : 0.0f;
-    return on;
+}
+__device__ __forceinline__ bool counts(int type, uint32_t bits, float &add) {
+    add = 0.0f;
+    if (type == I8F_MASK_BYTES) return bits != 0;
+    const float m = type == I8F_MASK_BF16 ? bf16_bits_to_f32(bits) : type == I8F_MASK_F16 ? f16_bits_to_f32(bits) : __uint_as_float(bits);
+    const float lowest = type == I8F_MASK_BF16 ? -3.3895313892515355e38f : type == I8F_MASK_F16 ? -65504.0f : LOWEST;
+    if (m <= lowest) return false;
+    add = fmaxf(m * TO_LOG2, LOWEST);
+    return true;
 }
 
 // The 16-byte pieces of a row are exchanged within it by a function of the row, so that the lanes of an LDS read are spread over the banks.
@@ -101,28 +114,30 @@ __device__ __forceinline__ int v_quad(int row) {   // what the number of a row's
     else return (row >> 1) & 1;
 }
 
-// DP: the width, padded.  APART: the waves of a workgroup have the same rows and a tile of 32 states each, by themselves; otherwise 32 rows
+// DP: the width, padded.  WAVES of a workgroup; APART: they have the same 32 rows and a tile of 32 states each, by themselves; otherwise 32 rows
 // each and a tile of 64 states together.
-template <int DT, int DP, bool APART, bool MASK>
+template <int DT, int DP, int WAVES, bool APART, bool MASK>
 struct Shape {
-    static constexpr int WAVES = APART && DP > 128 ? 2 : 4, KT = APART ? 32 : 64, PIECES = DP / 8, TILE = KT * DP * 2;
+    static constexpr int KT = APART ? 32 : 64, PIECES = DP / 8, TILE = KT * DP * 2;
     static constexpr int LOADS = KT * PIECES / 64 / (APART ? 1 : WAVES);       // a wave's of a tile of K, or of V
+    static_assert(KT * PIECES % (64 * (APART ? 1 : WAVES)) == 0, "");
     static constexpr int SETS = APART ? WAVES : 1, LDS = SETS * 4 * TILE;      // two stages of K and V
     static constexpr int ROWS = APART ? 32 : 32 * WAVES;
+    static constexpr int PER_SIMD = WAVES == 8 || LDS <= 80 * 1024 ? 2 : 1;    // waves
 };
 
-template <int DT, int DP, bool APART, bool MASK>
-__global__ __launch_bounds__((Shape<DT, DP, APART, MASK>::WAVES * 64), (Shape<DT, DP, APART, MASK>::LDS <= 80 * 1024 ? 2 : 1)) void attention_kernel(const Launch p) {
-    using S = Shape<DT, DP, APART, MASK>;
-    constexpr int KT = S::KT, KB = KT / 32, NK = DP / 16, ND = DP / 32, WAVES = S::WAVES;
+template <int DT, int DP, int WAVES, bool APART, bool MASK>
+__global__ __launch_bounds__(WAVES * 64, (Shape<DT, DP, WAVES, APART, MASK>::PER_SIMD)) void attention_kernel(const Launch p) {
+    using S = Shape<DT, DP, WAVES, APART, MASK>;
+    constexpr int KT = S::KT, KB = KT / 32, NK = DP / 16, ND = DP / 32;
     __shared__ __attribute__((aligned(16))) char lds[S::LDS + (MASK ? WAVES * 64 * 4 : 0)];
     const i8f_attention_args &a = p.a;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // the workgroups of an XCD (number mod 8) take consecutive row tiles of the same states
     const unsigned per = gridDim.x / 8, extra = gridDim.x % 8, xcd = blockIdx.x % 8;
-    const unsigned id = xcd * per + (xcd < extra ? xcd : extra) + blockIdx.x / 8;
-    const unsigned row_tile = id % p.row_tiles, split = id / p.row_tiles % p.splits, bg = id / p.row_tiles / p.splits;
-    const int64_t b = bg / (unsigned)a.kv_heads, g = bg % (unsigned)a.kv_heads;
+    const unsigned id = xcd * per + (xcd < extra ? xcd : extra) + blockIdx.x / 8, set = p.by_row_tiles(id), row_tile = id - set * p.row_tiles;
+    const unsigned bg = p.by_splits(set), split = set - bg * p.splits;
+    const int64_t b = p.by_kv_heads(bg), g = bg - (unsigned)b * (unsigned)a.kv_heads;
     int n = (int)a.keys;
     if (a.key_lengths) {
         const int64_t given = a.lengths_type ? ((const int64_t *)a.key_lengths)[b] : ((const int32_t *)a.key_lengths)[b];
@@ -131,19 +146,6 @@ __global__ __launch_bounds__((Shape<DT, DP, APART, MASK>::WAVES * 64), (Shape<DT
     const int from_tile = (int)(split * p.tiles) + (APART ? wave : 0), all_tiles = (n - 1 + KT) / KT, to_tile = (int)((split + 1) * p.tiles);
     const int last_tile = all_tiles < to_tile ? all_tiles : to_tile;
     constexpr int STEP = APART ? WAVES : 1;   // (apart, every WAVES-th tile is a wave's)
-
-    // a wave's 32 rows, a lane's in both halves
-    const unsigned row = row_tile * S::ROWS + (APART ? 0 : wave * 32) + (lane & 31), real = row < p.rows ? row : p.rows - 1;
-    const int64_t query = real / p.share, head = g * p.share + real % p.share;
-    v8s q[NK];
-    {
-        const uint16_t *qp = (const uint16_t *)a.q + b * a.q_batch + query * a.q_token + head * a.q_head;
-#pragma unroll
-        for (int s = 0; s < NK; ++s) {
-            const unsigned e = s * 16 + half * 8;
-            q[s] = e < p.loaded ? *(const v8s *)(qp + e) : v8s{};
-        }
-    }
     const float to_log2 = a.scale * TO_LOG2;
 
     // where a lane's pieces of a tile come from: LDS is filled in order, 16 bytes a lane
@@ -154,8 +156,8 @@ __global__ __launch_bounds__((Shape<DT, DP, APART, MASK>::WAVES * 64), (Shape<DT
     for (int i = 0; i < S::LOADS; ++i) {
         const int at = piece_at(i), r = at / S::PIECES, c = at % S::PIECES;
         const unsigned ck = k_piece<DP>(r, c), cv = c ^ (v_quad<DP>(r) << 2);
-        from_k[i] = ck * 8 < p.loaded ? (uint32_t)(r * a.k_token + ck * 8) * 2u : NOWHERE;
-        from_v[i] = cv * 8 < p.loaded ? (uint32_t)(r * a.v_token + cv * 8) * 2u : NOWHERE;
+        from_k[i] = ck * 8 < p.loaded ? ((uint32_t)r * (uint32_t)a.k_token + ck * 8) * 2u : NOWHERE;
+        from_v[i] = cv * 8 < p.loaded ? ((uint32_t)r * (uint32_t)a.v_token + cv * 8) * 2u : NOWHERE;
     }
     const uint16_t *kp = (const uint16_t *)a.k + b * a.k_batch + g * a.k_head, *vp = (const uint16_t *)a.v + b * a.v_batch + g * a.v_head;
     const uint32_t lds_at = (uint32_t)(uintptr_t)(gemm::lds_ptr_t)lds + (APART ? wave * 4 * S::TILE : 0);   // stage s: K at s * 2 * TILE, V behind it
@@ -167,7 +169,12 @@ __global__ __launch_bounds__((Shape<DT, DP, APART, MASK>::WAVES * 64), (Shape<DT
         float add;
     };
     constexpr uint64_t ALL = KT == 64 ? ~0ull : 0xffffffffull;
-    auto tile_from = [&](int at) {   // the first tile from `at` on with a state that counts, or one past the last
+    // a lane's state of a tile in the mask; it is asked for a step before it is looked at
+    auto peek = [&](int at) -> uint32_t {
+        const int j = at * KT + lane;
+        return MASK && at < last_tile && lane < KT && j < n ? mask_bits(a, b, j) : 0u;
+    };
+    auto tile_from = [&](int at, uint32_t bits) {   // the first tile from `at` on (whose mask is there) with a state that counts, or one past the last
         Tile t = {at, ALL, 0.0f};
         for (; t.at < last_tile; t.at += STEP) {
             const int left = n - t.at * KT;
@@ -175,9 +182,8 @@ __global__ __launch_bounds__((Shape<DT, DP, APART, MASK>::WAVES * 64), (Shape<DT
                 if (left < KT) t.on = (1ull << left) - 1;
                 break;
             } else {
-                bool on = lane < KT && lane < left;
-                t.add = 0.0f;
-                if (on) on = counts(a, b, (int64_t)t.at * KT + lane, t.add);
+                if (t.at != at) bits = peek(t.at);
+                const bool on = counts(a.mask_type, bits, t.add) && lane < KT && lane < left;
                 if ((t.on = __ballot(on)) != 0) break;
             }
         }
@@ -204,63 +210,81 @@ __global__ __launch_bounds__((Shape<DT, DP, APART, MASK>::WAVES * 64), (Shape<DT
         asm volatile("" ::: "memory");
     };
 
+    Tile now = tile_from(from_tile, peek(from_tile)), next = tile_from(now.at + STEP, peek(now.at + STEP));
+    uint32_t ahead = peek(next.at + STEP);
+    request_k(now, 0), request_v(now, 0), request_k(next, 1);
+
+    // a wave's 32 rows, a lane's in both halves
+    const unsigned first_row = row_tile * S::ROWS + (APART ? 0 : wave * 32);
+    v8s q[NK];
+    {
+        const unsigned row = first_row + (lane & 31), real = row < p.rows ? row : p.rows - 1, query = p.by_share(real);
+        const uint16_t *qp = (const uint16_t *)a.q + b * a.q_batch + query * a.q_token + (g * p.share + (real - query * p.share)) * a.q_head;
+#pragma unroll
+        for (int e = 0; e < NK; ++e) {
+            const unsigned at = e * 16 + half * 8;
+            q[e] = at < p.loaded ? *(const v8s *)(qp + at) : v8s{};
+        }
+    }
     v16f o[ND], s[KB];
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = v16f{};
-    float top = LOWEST, sum = 0.0f;
+    float top = LOWEST, sum = 0.0f, most = LOWEST;
     constexpr float RAISE = DT == I8F_F16 ? 6.0f : 0.0f;   // (binary16 weights lie between 2^6 and 2^14 for the largest: see below)
 
     // where a lane reads: K row (lane & 31) of a block, V's four rows from 4 half on by 16 elements
+    char *const tiles = lds + (APART ? wave * 4 * S::TILE : 0);
     const int k_row = (lane & 31) * DP * 2;
     const int v_row = (4 * half + ((lane >> 2) & 3)) * DP * 2 + (2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) * 16 + (lane & 1) * 8;
     const int v_x = v_quad<DP>((lane >> 2) & 3);
-    char *const tiles = lds + (APART ? wave * 4 * S::TILE : 0);
     float *const adds = (float *)(lds + S::LDS) + wave * 64;
     auto k_part = [&](const char *ks, int e, int k) { return *(const v8s *)(ks + k * 32 * DP * 2 + k_row + k_piece<DP>(lane & 31, 2 * e + half) * 16); };
+    auto largest = [&](const v16f (&x)[KB]) {   // (of the wave half's states)
+        float m = x[0][0];
+#pragma unroll
+        for (int k = 0; k < KB; ++k)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) m = __builtin_elementwise_maximum(m, x[k][i]);
+        return m;
+    };
 
-    Tile now = tile_from(from_tile), next = tile_from(now.at + STEP);
-    request_k(now, 0), request_v(now, 0), request_k(next, 1);
-    int stage = 0;
     all_here();
     // (the rows have arrived as well: without this the compiler waits for them, and with them for the tiles under way, in every step)
 #pragma unroll
     for (int e = 0; e < NK; ++e) asm volatile("" : "+v"(q[e]));
     if (now.at < last_tile) {
 #pragma unroll
-        for (int k = 0; k < KB; ++k) s[k] = v16f{};
-#pragma unroll
         for (int e = 0; e < NK; ++e)
 #pragma unroll
-            for (int k = 0; k < KB; ++k) s[k] = mfma<DT>(k_part(tiles, e, k), q[e], s[k]);
+            for (int k = 0; k < KB; ++k) s[k] = mfma<DT>(k_part(tiles, e, k), q[e], e ? s[k] : v16f{});
+        most = largest(s);
     }
-    // One tile: its scores are there, the next tile's are formed on the matrix unit (MORE) while the vector units have the exponentials.
+    // One tile: its scores and their maximum are there; the next tile's scores are formed on the matrix unit (MORE) while the vector units have
+    // this one's exponentials, and their maximum beside this one's last products.
+    int stage = 0;
     auto step = [&](auto more) __attribute__((always_inline)) {
         constexpr bool MORE = decltype(more)::value;
         float factor = to_log2;   // scores are scaled in the exponential's argument, or here where addends come on top
-        if constexpr (MASK) {
-            if (a.mask_type != I8F_MASK_BYTES) {
-                adds[lane] = now.add;
-#pragma unroll
-                for (int k = 0; k < KB; ++k)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[k][i] = __builtin_fmaf(s[k][i], to_log2, adds[k * 32 + 8 * (i / 4) + 4 * half + i % 4]);
-                factor = 1.0f;
+        const bool added = MASK && a.mask_type != I8F_MASK_BYTES;
+        if (added || now.on != ALL) {
+            if constexpr (MASK) {
+                if (added) adds[lane] = now.add, factor = 1.0f;
             }
-        }
-        if (now.on != ALL) {
 #pragma unroll
             for (int k = 0; k < KB; ++k) {
                 uint32_t mine = (uint32_t)(now.on >> (32 * k)) >> (4 * half);
                 asm volatile("" : "+v"(mine));   // (keeps what follows in this branch: the last tile's, or a mask's)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[k][i] = mine >> (8 * (i / 4) + i % 4) & 1 ? s[k][i] : -__builtin_inff();
+                for (int i = 0; i < 16; ++i) {
+                    float x = s[k][i];
+                    if constexpr (MASK) {
+                        if (added) x = __builtin_fmaf(x, to_log2, adds[k * 32 + 8 * (i / 4) + 4 * half + i % 4]);
+                    }
+                    s[k][i] = mine >> (8 * (i / 4) + i % 4) & 1 ? x : -__builtin_inff();
+                }
             }
+            most = largest(s);
         }
-        float most = s[0][0];
-#pragma unroll
-        for (int k = 0; k < KB; ++k)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) most = __builtin_elementwise_maximum(most, s[k][i]);
         most = max_of_halves(most) * factor;
         // The reference of the exponentials follows the maximum only where that has grown by 2^8: the weights are below 2^8 then, which costs
         // no bits, and the result is divided by their sum either way.
@@ -273,40 +297,45 @@ __global__ __launch_bounds__((Shape<DT, DP, APART, MASK>::WAVES * 64), (Shape<DT
         }
         const float from = RAISE - top;
         all_here();   // the tile's V and the next one's K
-        const Tile after = MORE ? tile_from(next.at + STEP) : next;
-        if constexpr (MORE) request_k(after, stage), request_v(next, stage ^ 1);
+        const Tile after = MORE ? tile_from(next.at + STEP, ahead) : next;
+        if constexpr (MORE) request_k(after, stage), request_v(next, stage ^ 1), ahead = peek(after.at + STEP);
         const char *vs = tiles + stage * 2 * S::TILE + S::TILE, *ks = tiles + (stage ^ 1) * 2 * S::TILE;
         v16f t[KB];
-        if constexpr (MORE) {
-#pragma unroll
-            for (int k = 0; k < KB; ++k) t[k] = v16f{};
-        }
-        constexpr int PARTS = 2 * KB;
-#pragma unroll
-        for (int part = 0; part < PARTS; ++part) {
-            const int k = part / 2, j = part % 2;
+        constexpr int PARTS = 2 * KB;   // of 16 states
+        auto score = [&](int part) __attribute__((always_inline)) {
             if constexpr (MORE) {
 #pragma unroll
                 for (int e = NK * part / PARTS; e < NK * (part + 1) / PARTS; ++e)
 #pragma unroll
-                    for (int x = 0; x < KB; ++x) t[x] = mfma<DT>(k_part(ks, e, x), q[e], t[x]);
+                    for (int k = 0; k < KB; ++k) t[k] = mfma<DT>(k_part(ks, e, k), q[e], e ? t[k] : v16f{});
             }
+        };
+        auto weigh = [&](int part) __attribute__((always_inline)) {
+            const v16f &x = s[part / 2];
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                w[i] = round_weights<DT>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[k][8 * j + 2 * i], factor, from)),
-                                         __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][8 * j + 2 * i + 1], factor, from)), sum);
-            const v8s weights = __builtin_bit_cast(v8s, (v4i){(int)w[0], (int)w[1], (int)w[2], (int)w[3]});
+                w[i] = round_weights<DT>(__builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * (part % 2) + 2 * i], factor, from)),
+                                         __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * (part % 2) + 2 * i + 1], factor, from)), sum);
+            return __builtin_bit_cast(v8s, (v4i){(int)w[0], (int)w[1], (int)w[2], (int)w[3]});
+        };
+        score(0);
+        v8s weights = weigh(0);
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+            const v8s mine = weights;
+            if (part + 1 < PARTS) score(part + 1), weights = weigh(part + 1);
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
                 typedef __attribute__((address_space(3))) v4s *v4s_lds;
-                const char *at = vs + (k * 32 + j * 16) * DP * 2 + v_row + (d ^ v_x) * 64;
+                const char *at = vs + part * 16 * DP * 2 + v_row + (d ^ v_x) * 64;
                 const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s_lds)(gemm::lds_ptr_t)at);
                 const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s_lds)(gemm::lds_ptr_t)(at + 8 * DP * 2));
-                o[d] = mfma<DT>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), weights, o[d]);
+                o[d] = mfma<DT>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), mine, o[d]);
             }
         }
         if constexpr (MORE) {
+            most = largest(t);
 #pragma unroll
             for (int k = 0; k < KB; ++k) s[k] = t[k];
         }
@@ -353,13 +382,14 @@ __global__ __launch_bounds__((Shape<DT, DP, APART, MASK>::WAVES * 64), (Shape<DT
                 *(float4 *)(p.partial + at_row * DP + e) = make_float4(v[0], v[1], v[2], v[3]);
                 if (e == 0) p.stats[at_row * 2] = best, p.stats[at_row * 2 + 1] = total;
             } else {
-                const int64_t to = ((b * a.queries + own / p.share) * a.heads + g * p.share + own % p.share) * a.width;
+                const int64_t to = ((b * a.queries + p.by_share(own)) * a.heads + g * p.share + (own - p.by_share(own) * p.share)) * a.width;
                 for (int i = 0; i < 4; ++i)
                     if (e + i < a.width) store_from_f32<DT>(a.out, to + e + i, total == 0.0f ? 0.0f : v[i] / total);
             }
         }
     } else {
         if (p.splits > 1) {
+            const unsigned row = first_row + (lane & 31);
             if (row >= p.rows) return;
             const int64_t at_row = ((int64_t)bg * p.splits + split) * p.rows + row;
 #pragma unroll
@@ -371,10 +401,11 @@ __global__ __launch_bounds__((Shape<DT, DP, APART, MASK>::WAVES * 64), (Shape<DT
             return;
         }
         // A lane has pieces of one row, memory wants whole lines: the rows change places in LDS.  The stage that the last tile is not in has been
-        // read by everyone and nothing is under way to it, and is as large as the workgroup's rows.
+        // read by everyone and nothing is under way to it; it holds the rows of four waves, those of eight take both.
+        static_assert(WAVES * 32 * DP * 2 <= (WAVES == 8 ? S::LDS : 2 * S::TILE), "");
+        if constexpr (WAVES == 8) __syncthreads();
+        char *const mine = lds + (WAVES == 8 ? 0 : stage * 2 * S::TILE) + wave * 32 * DP * 2;
         const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
-        static_assert(WAVES * 32 * DP * 2 <= 2 * S::TILE, "");
-        char *const mine = lds + stage * 2 * S::TILE + wave * 32 * DP * 2;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -384,15 +415,14 @@ __global__ __launch_bounds__((Shape<DT, DP, APART, MASK>::WAVES * 64), (Shape<DT
                 *(uint2 *)(mine + k_row + k_piece<DP>(lane & 31, 4 * d + i) * 16 + half * 8) = v;
             }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        const unsigned first = row_tile * S::ROWS + wave * 32;
 #pragma unroll
         for (int i = 0; i < 32 * S::PIECES / 64; ++i) {
-            const int at = i * 64 + lane, r = at / S::PIECES, c = at % S::PIECES;
-            const unsigned own = first + r;
+            const int at = i * 64 + lane, x = at / S::PIECES, c = at % S::PIECES;
+            const unsigned own = first_row + x;
             if (own >= p.rows || c * 8 >= a.width) continue;
-            const uint4 v = *(const uint4 *)(mine + r * DP * 2 + k_piece<DP>(r, c) * 16);
-            const int64_t q_at = p.share == 1 ? own : own / p.share, h_at = p.share == 1 ? g : g * p.share + own % p.share;
-            uint16_t *const to = (uint16_t *)a.out + ((b * a.queries + q_at) * a.heads + h_at) * a.width + c * 8;
+            const uint4 v = *(const uint4 *)(mine + x * DP * 2 + k_piece<DP>(x, c) * 16);
+            const unsigned query = p.by_share(own);
+            uint16_t *const to = (uint16_t *)a.out + ((b * a.queries + query) * a.heads + g * p.share + (own - query * p.share)) * a.width + c * 8;
             if (p.wide_out) {
                 stream_store16(to, v);
             } else {
@@ -405,31 +435,52 @@ __global__ __launch_bounds__((Shape<DT, DP, APART, MASK>::WAVES * 64), (Shape<DT
     }
 }
 
-// The splits' results of a row joined: a wave to a row.
-template <int DT>
-__global__ __launch_bounds__(256) void join_kernel(const Launch p, const int padded) {
+// The splits' results of a row joined: a workgroup to a row, its threads by four elements and by splits, so that all of them are requested at once.
+constexpr int MOST_SPLITS = 256;
+template <int DT, int DP>
+__global__ __launch_bounds__(256) void join_kernel(const Launch p) {
+    constexpr int QUADS = DP / 4, PARTS = 256 / QUADS;
+    __shared__ float weight[MOST_SPLITS], red[4];
+    __shared__ float4 sums[PARTS][QUADS];
     const i8f_attention_args &a = p.a;
-    const int lane = threadIdx.x & 63;
-    const unsigned at = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (at >= a.batch * a.kv_heads * p.rows) return;
-    const unsigned row = at % p.rows;
-    const int64_t bg = at / p.rows, b = bg / a.kv_heads, g = bg % a.kv_heads;
-    float best = LOWEST;
-    for (unsigned s = lane; s < p.splits; s += 64) best = fmaxf(best, p.stats[((bg * p.splits + s) * p.rows + row) * 2]);
-    best = wave_max(best);
-    float total = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (unsigned s = 0; s < p.splits; ++s) {
-        const int64_t r = (bg * p.splits + s) * p.rows + row;
-        const float f = __builtin_amdgcn_exp2f(p.stats[r * 2] - best);
-        total = __builtin_fmaf(p.stats[r * 2 + 1], f, total);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quad = tid % QUADS, part = tid / QUADS, splits = (int)p.splits;
+    const unsigned row = blockIdx.x % p.rows;
+    const int64_t bg = blockIdx.x / p.rows, b = bg / a.kv_heads, g = bg % a.kv_heads, first = bg * p.splits * p.rows + row;
+    const bool mine = tid < splits;
+    const float2 own = mine ? *(const float2 *)(p.stats + 2 * (first + (int64_t)tid * p.rows)) : make_float2(LOWEST, 0.0f);
+    float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    const float top = wave_max(own.x);
+    if (lane == 0) red[wave] = top;
+    __syncthreads();
+    const float best = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float f = mine ? __builtin_amdgcn_exp2f(own.x - best) : 0.0f;
+    weight[tid] = f;
+    float total = own.y * f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i * 64 + lane < padded) v[i] = __builtin_fmaf(p.partial[r * padded + i * 64 + lane], f, v[i]);
+    for (int x = 1; x < 64; x *= 2) total += __shfl_xor(total, x);
+    __syncthreads();
+    if (lane == 0) red[wave] = total;
+    if (part < PARTS) {
+#pragma unroll 8
+        for (int s = part; s < splits; s += PARTS) {
+            const float4 x = *(const float4 *)(p.partial + (first + (int64_t)s * p.rows) * DP + quad * 4);
+            const float w = weight[s];
+            v.x = __builtin_fmaf(x.x, w, v.x), v.y = __builtin_fmaf(x.y, w, v.y), v.z = __builtin_fmaf(x.z, w, v.z), v.w = __builtin_fmaf(x.w, w, v.w);
+        }
+        sums[part][quad] = v;
     }
-    const int64_t to = ((b * a.queries + row / p.share) * a.heads + g * p.share + row % p.share) * a.width;
+    __syncthreads();
+    if (tid >= QUADS) return;
+    total = (red[0] + red[1]) + (red[2] + red[3]);
+    v = sums[0][tid];
+#pragma unroll
+    for (int i = 1; i < PARTS; ++i) v.x += sums[i][tid].x, v.y += sums[i][tid].y, v.z += sums[i][tid].z, v.w += sums[i][tid].w;
+    const unsigned query = p.by_share(row);
+    const int64_t to = ((b * a.queries + query) * a.heads + g * p.share + (row - query * p.share)) * a.width + tid * 4;
+    const float o[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        if (i * 64 + lane < a.width) store_from_f32<DT>(a.out, to + i * 64 + lane, total == 0.0f ? 0.0f : v[i] / total);
+        if (tid * 4 + i < a.width) store_from_f32<DT>(a.out, to + i, total == 0.0f ? 0.0f : o[i] / total);
 }
 
 // [batch, tokens, heads, width] of any strides and alignment as contiguous rows of whole 16-byte pieces, the rest of them zeros.
@@ -462,6 +513,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const Packs packs) {
 struct Plan {
     int padded;               // width of the kernels
     bool apart;               // few rows: the waves of a workgroup take the states in turn
+    int waves;                // of a workgroup
     int64_t row_tiles, splits, tiles;
     int64_t partial_bytes;    // of results and statistics of the splits
 };
@@ -472,15 +524,20 @@ Plan plan_of(int64_t batch, int64_t queries, int64_t keys, int64_t heads, int64_
     p.padded = width <= 64 ? 64 : width <= 96 ? 96 : width <= 128 ? 128 : width <= 192 ? 192 : 256;
     const int64_t rows = queries * (heads / kv_heads), sets = batch * kv_heads;
     p.apart = rows <= 32;
-    const int waves = p.apart && p.padded > 128 ? 2 : 4;
-    p.row_tiles = p.apart ? (rows + 31) / 32 : (rows + 127) / 128;
+    p.waves = p.apart ? (p.padded > 128 ? 2 : 4) : 4;
+    // Eight waves read the states half as often, which is energy, and the card runs at its power limit in long calls; four start and end beside
+    // another workgroup.  us with four and eight for 40 heads of 128: 8192 x 8192 1338 and 1284, 32768 x 4096 2603 and 2546, 32768 x 2048 1333 and
+    // 1333, 32768 x 512 419 and 449, 4096 x 4096 336 and 356.
+    if (!p.apart && (p.padded == 64 || p.padded == 128) && keys >= 4096 && sets * ((rows + 255) / 256) >= 1024) p.waves = 8;
+    const int64_t to_group = p.apart ? 32 : 32 * p.waves;
+    p.row_tiles = (rows + to_group - 1) / to_group;
     const int64_t tile = p.apart ? 32 : 64, all = (keys + tile - 1) / tile, groups = sets * p.row_tiles;
-    // as many splits as make 512 workgroups, of at least 4 tiles to a wave
-    const int64_t least = 4 * (p.apart ? waves : 1);
-    p.splits = groups >= 256 || all < 2 * least ? 1 : (512 + groups - 1) / groups;
+    // as many splits as make a workgroup to a CU (one token over 65536 states of 8 heads: 256 workgroups 59 us, 512 81), of at least 4 tiles to a wave
+    const int64_t least = 4 * (p.apart ? p.waves : 1);
+    p.splits = groups >= 256 || all < 2 * least ? 1 : (256 + groups - 1) / groups;
     if (p.splits > all / least) p.splits = all / least;
     if (p.splits < 1) p.splits = 1;
-    p.tiles = round_up((all + p.splits - 1) / p.splits, p.apart ? waves : 1);
+    p.tiles = round_up((all + p.splits - 1) / p.splits, p.apart ? p.waves : 1);
     if (p.tiles < 1) p.tiles = 1;
     p.splits = all ? (all + p.tiles - 1) / p.tiles : 1;
     p.partial_bytes = p.splits > 1 ? sets * p.splits * rows * (p.padded + 2) * 4 : 0;
@@ -505,33 +562,42 @@ int to_pack(const i8f_attention_args &a, int64_t (&bytes)[3]) {
     return which;
 }
 
-template <int DT, int DP, bool APART, bool MASK>
+template <int DT, int DP, int WAVES, bool APART, bool MASK>
 int launch_tiles(const Launch &p, int64_t groups, hipStream_t st) {
-    using S = Shape<DT, DP, APART, MASK>;
-    if (!grid_fits(groups, S::WAVES * 64)) return I8F_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((attention_kernel<DT, DP, APART, MASK>), dim3((unsigned)groups), dim3(S::WAVES * 64), 0, st, p);
+    if (!grid_fits(groups, WAVES * 64)) return I8F_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((attention_kernel<DT, DP, WAVES, APART, MASK>), dim3((unsigned)groups), dim3(WAVES * 64), 0, st, p);
     return check_launch();
 }
+template <int DT, int DP, bool MASK>
+int launch_masked(const Launch &p, const Plan &plan, int64_t groups, hipStream_t st) {
+    if (plan.apart) return launch_tiles<DT, DP, DP <= 128 ? 4 : 2, true, MASK>(p, groups, st);
+    if constexpr (DP == 64 || DP == 128) {
+        if (plan.waves == 8) return launch_tiles<DT, DP, 8, false, MASK>(p, groups, st);
+    }
+    return launch_tiles<DT, DP, 4, false, MASK>(p, groups, st);
+}
 template <int DT, int DP>
-int launch_form(const Launch &p, bool apart, int64_t groups, hipStream_t st) {
-    if (p.a.key_mask) return apart ? launch_tiles<DT, DP, true, true>(p, groups, st) : launch_tiles<DT, DP, false, true>(p, groups, st);
-    return apart ? launch_tiles<DT, DP, true, false>(p, groups, st) : launch_tiles<DT, DP, false, false>(p, groups, st);
+int launch_form(const Launch &p, const Plan &plan, int64_t groups, hipStream_t st) {
+    return p.a.key_mask ? launch_masked<DT, DP, true>(p, plan, groups, st) : launch_masked<DT, DP, false>(p, plan, groups, st);
+}
+template <int DT, int DP>
+int launch_width(const Launch &p, const Plan &plan, hipStream_t st) {
+    const int64_t sets = p.a.batch * p.a.kv_heads;
+    const int rc = launch_form<DT, DP>(p, plan, sets * p.row_tiles * p.splits, st);
+    if (rc || p.splits == 1) return rc;
+    if (!grid_fits(sets * p.rows, 256)) return I8F_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((join_kernel<DT, DP>), dim3((unsigned)(sets * p.rows)), dim3(256), 0, st, p);
+    return check_launch();
 }
 template <int DT>
 int launch(const Launch &p, const Plan &plan, hipStream_t st) {
-    const int64_t groups = p.a.batch * p.a.kv_heads * p.row_tiles * p.splits;
-    int rc;
     switch (plan.padded) {
-    case 64: rc = launch_form<DT, 64>(p, plan.apart, groups, st); break;
-    case 96: rc = launch_form<DT, 96>(p, plan.apart, groups, st); break;
-    case 128: rc = launch_form<DT, 128>(p, plan.apart, groups, st); break;
-    case 192: rc = launch_form<DT, 192>(p, plan.apart, groups, st); break;
-    default: rc = launch_form<DT, 256>(p, plan.apart, groups, st); break;
+    case 64: return launch_width<DT, 64>(p, plan, st);
+    case 96: return launch_width<DT, 96>(p, plan, st);
+    case 128: return launch_width<DT, 128>(p, plan, st);
+    case 192: return launch_width<DT, 192>(p, plan, st);
+    default: return launch_width<DT, 256>(p, plan, st);
     }
-    if (rc || p.splits == 1) return rc;
-    const int64_t rows = p.a.batch * p.a.kv_heads * p.rows;
-    hipLaunchKernelGGL((join_kernel<DT>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p, plan.padded);
-    return check_launch();
 }
 
 // The elements that a strided tensor reaches to from its first one, 0 for one without elements, -1 past 2^62.
@@ -598,6 +664,7 @@ extern "C" int i8f_attention(const i8f_attention_args *args, void *stream) {
     hipStream_t st = (hipStream_t)stream;
     Launch p = {a, (uint32_t)share, (uint32_t)(a.queries * share), (uint32_t)plan.row_tiles, (uint32_t)plan.splits, (uint32_t)plan.tiles, (uint32_t)round_up(a.width, 8)};
     p.wide_out = a.width % 8 == 0 && (uintptr_t)a.out % 16 == 0;
+    p.by_share = Divisor(p.share), p.by_row_tiles = Divisor(p.row_tiles), p.by_splits = Divisor(p.splits), p.by_kv_heads = Divisor((uint32_t)a.kv_heads);
     p.partial = (float *)a.workspace;
     p.stats = p.partial ? p.partial + plan.partial_bytes / 4 / (plan.padded + 2) * plan.padded : nullptr;
     int64_t bytes[3];
