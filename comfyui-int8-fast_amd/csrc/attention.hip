@@ -130,7 +130,7 @@ template <int DT, int DP, int WAVES, bool APART, bool MASK>
 __global__ __launch_bounds__(WAVES * 64, (Shape<DT, DP, WAVES, APART, MASK>::PER_SIMD)) void attention_kernel(const Launch p) {
     using S = Shape<DT, DP, WAVES, APART, MASK>;
     constexpr int KT = S::KT, KB = KT / 32, NK = DP / 16, ND = DP / 32;
-    __shared__ __attribute__((aligned(16))) char lds[S::LDS + (MASK ? WAVES * 64 * 4 : 0)];
+    __shared__ __attribute__((aligned(16))) char lds[S::LDS + (MASK ? WAVES * 128 * 4 : 0)];
     const i8f_attention_args &a = p.a;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // the workgroups of an XCD (number mod 8) take consecutive row tiles of the same states
@@ -237,7 +237,21 @@ __global__ __launch_bounds__(WAVES * 64, (Shape<DT, DP, WAVES, APART, MASK>::PER
     const int k_row = (lane & 31) * DP * 2;
     const int v_row = (4 * half + ((lane >> 2) & 3)) * DP * 2 + (2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) * 16 + (lane & 1) * 8;
     const int v_x = v_quad<DP>((lane >> 2) & 3);
-    float *const adds = (float *)(lds + S::LDS) + wave * 64;
+    // With a mask the scores' sums begin at 0 or, of states that do not count, at -inf: their K is zeros, so that is what they stay, without a
+    // vector instruction.  A lane has states 8 (i / 4) + 4 half + i % 4 of a block.
+    float *const begins = (float *)(lds + S::LDS) + wave * 128, *const adds = begins + 64;
+    auto begin = [&](const Tile &t, int k) {
+        v16f x = {};
+        if constexpr (MASK) {
+            if (k == 0) begins[lane] = t.on >> lane & 1 ? 0.0f : -__builtin_inff();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float4 y = *(const float4 *)(begins + k * 32 + 8 * i + 4 * half);
+                x[4 * i] = y.x, x[4 * i + 1] = y.y, x[4 * i + 2] = y.z, x[4 * i + 3] = y.w;
+            }
+        }
+        return x;
+    };
     auto k_part = [&](const char *ks, int e, int k) { return *(const v8s *)(ks + k * 32 * DP * 2 + k_row + k_piece<DP>(lane & 31, 2 * e + half) * 16); };
     auto largest = [&](const v16f (&x)[KB]) {   // (of the wave half's states)
         float m = x[0][0];
@@ -256,7 +270,7 @@ __global__ __launch_bounds__(WAVES * 64, (Shape<DT, DP, WAVES, APART, MASK>::PER
 #pragma unroll
         for (int e = 0; e < NK; ++e)
 #pragma unroll
-            for (int k = 0; k < KB; ++k) s[k] = mfma<DT>(k_part(tiles, e, k), q[e], e ? s[k] : v16f{});
+            for (int k = 0; k < KB; ++k) s[k] = mfma<DT>(k_part(tiles, e, k), q[e], e ? s[k] : begin(now, k));
         most = largest(s);
     }
     // One tile: its scores and their maximum are there; the next tile's scores are formed on the matrix unit (MORE) while the vector units have
@@ -265,23 +279,22 @@ __global__ __launch_bounds__(WAVES * 64, (Shape<DT, DP, WAVES, APART, MASK>::PER
     auto step = [&](auto more) __attribute__((always_inline)) {
         constexpr bool MORE = decltype(more)::value;
         float factor = to_log2;   // scores are scaled in the exponential's argument, or here where addends come on top
-        const bool added = MASK && a.mask_type != I8F_MASK_BYTES;
-        if (added || now.on != ALL) {
-            if constexpr (MASK) {
-                if (added) adds[lane] = now.add, factor = 1.0f;
+        if constexpr (MASK) {
+            if (a.mask_type != I8F_MASK_BYTES) {
+                adds[lane] = now.add, factor = 1.0f;
+#pragma unroll
+                for (int k = 0; k < KB; ++k)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[k][i] = __builtin_fmaf(s[k][i], to_log2, adds[k * 32 + 8 * (i / 4) + 4 * half + i % 4]);
+                most = largest(s);
             }
+        } else if (now.on != ALL) {   // (the last tile)
 #pragma unroll
             for (int k = 0; k < KB; ++k) {
                 uint32_t mine = (uint32_t)(now.on >> (32 * k)) >> (4 * half);
-                asm volatile("" : "+v"(mine));   // (keeps what follows in this branch: the last tile's, or a mask's)
+                asm volatile("" : "+v"(mine));   // (keeps what follows in this branch)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float x = s[k][i];
-                    if constexpr (MASK) {
-                        if (added) x = __builtin_fmaf(x, to_log2, adds[k * 32 + 8 * (i / 4) + 4 * half + i % 4]);
-                    }
-                    s[k][i] = mine >> (8 * (i / 4) + i % 4) & 1 ? x : -__builtin_inff();
-                }
+                for (int i = 0; i < 16; ++i) s[k][i] = mine >> (8 * (i / 4) + i % 4) & 1 ? s[k][i] : -__builtin_inff();
             }
             most = largest(s);
         }
@@ -307,7 +320,7 @@ __global__ __launch_bounds__(WAVES * 64, (Shape<DT, DP, WAVES, APART, MASK>::PER
 #pragma unroll
                 for (int e = NK * part / PARTS; e < NK * (part + 1) / PARTS; ++e)
 #pragma unroll
-                    for (int k = 0; k < KB; ++k) t[k] = mfma<DT>(k_part(ks, e, k), q[e], e ? t[k] : v16f{});
+                    for (int k = 0; k < KB; ++k) t[k] = mfma<DT>(k_part(ks, e, k), q[e], e ? t[k] : begin(next, k));
             }
         };
         auto weigh = [&](int part) __attribute__((always_inline)) {
