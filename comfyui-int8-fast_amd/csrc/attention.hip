@@ -10,6 +10,7 @@
 #include <type_traits>
 #include <utility>
 
+#include "divisor.hpp"
 #include "dma.hpp"
 #include "i8f_common.hpp"
 
@@ -30,14 +31,6 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 
 constexpr float LOWEST = -3.4028234663852886e38f, TO_LOG2 = 1.4426950408889634f;
-
-// Division of a number below 2^31 by a fixed one: with 2^(s-1) < d <= 2^s and m = floor(2^(31+s) / d) + 1 the product is too large by less
-// than a d-th.
-struct Divisor {
-    uint32_t m, s;
-    Divisor(uint32_t d = 1) : s(d > 1 ? 32 - __builtin_clz(d - 1) : 0) { m = (uint32_t)((1ull << (31 + s)) / d + 1); }
-    __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return (uint32_t)(((uint64_t)x * m) >> (31 + s)); }
-};
 
 struct Launch {
     i8f_attention_args a;

@@ -4,6 +4,7 @@
 #include <type_traits>
 #include <utility>
 
+#include "divisor.hpp"
 #include "i8f_common.hpp"
 
 #include "../../include/i8f_attention.h"
@@ -35,8 +36,8 @@ __device__ __forceinline__ void turn(const i8f_norm_rotate_args &a, const double
     sincospif((float)(2.0 * (t - __builtin_rint(t))), &s, &c);
 }
 
-__device__ __forceinline__ void token_positions(const i8f_norm_rotate_args &a, int64_t bt, double (&pos)[I8F_MAX_AXES]) {
-    const int64_t at = bt / a.tokens * a.position_batch + bt % a.tokens * a.position_token;
+__device__ __forceinline__ void token_positions(const i8f_norm_rotate_args &a, unsigned b, unsigned t, double (&pos)[I8F_MAX_AXES]) {
+    const int64_t at = b * a.position_batch + t * a.position_token;
 #pragma unroll
     for (int x = 0; x < I8F_MAX_AXES; ++x) pos[x] = x < a.axes ? position_at(a.positions, a.positions_type, at + x * a.position_axis) : 0.0;
 }
@@ -144,14 +145,14 @@ __device__ __forceinline__ float sum_of_lanes(float v) {
 constexpr int DEEP = 4;   // passes that a wave requests at a time
 // A wave takes `per` passes of one token, a pass being 64 / LPH heads: the angles are the same for all of them.
 template <int DT, int LPH, bool APART, int ENDS>
-__global__ __launch_bounds__(256) void norm_rotate_kernel(const int64_t first, const unsigned chunks, const int per, const i8f_norm_rotate_args a, const Groups groups) {
+__global__ __launch_bounds__(256) void norm_rotate_kernel(const unsigned first, const unsigned tokens, const unsigned chunks, const int per, const Divisor by_chunks,
+                                                          const Divisor by_tokens, const i8f_norm_rotate_args a, const Groups groups) {
     constexpr int HPP = 64 / LPH, SIZE = DT == I8F_F32 ? 4 : 2;
     const int lane = threadIdx.x & 63, sub = lane / LPH, l = lane % LPH;
-    const int64_t id = first + (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t bt = id / chunks;
-    if (bt >= a.batch * a.tokens) return;
-    const int start = (int)(id % chunks) * per;
-    const int64_t b = bt / a.tokens, t = bt % a.tokens;
+    const unsigned id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), at = by_chunks(id);
+    if (at >= tokens) return;
+    const unsigned bt = first + at, b = by_tokens(bt), t = bt - b * (unsigned)a.tokens;
+    const int start = (int)(id - at * chunks) * per;
     const int width = (int)a.width, pairs = a.axes ? a.first_pair[a.axes] : 0;
     const int lows = (pairs + 3) / 4;
     const bool low = APART && l < lows;   // (lanes behind the turned pairs hold eight neighbours in either form)
@@ -171,7 +172,7 @@ __global__ __launch_bounds__(256) void norm_rotate_kernel(const int64_t first, c
     float c[4], s[4];
     if (pairs) {
         double pos[I8F_MAX_AXES];
-        token_positions(a, bt, pos);
+        token_positions(a, b, t, pos);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (pair + i < pairs) turn(a, pos, pair + i, c[i], s[i]);
@@ -189,7 +190,7 @@ __global__ __launch_bounds__(256) void norm_rotate_kernel(const int64_t first, c
             else expand_eight<DT>(whole ? load_eight<DT, APART>(p, e0, e1) : load_some<DT>(p, e0, e1, n0, n1), w);
         }
         const char *x = (const char *)h.x + (b * h.batch_stride + t * h.token_stride) * SIZE;
-        char *out = (char *)h.out + bt * h.heads * width * SIZE;
+        char *out = (char *)h.out + (int64_t)bt * h.heads * width * SIZE;
         for (int pass = lo; pass < hi; pass += DEEP) {
             Eight<DT> raw[DEEP];
 #pragma unroll
@@ -248,10 +249,12 @@ int launch_passes(const i8f_norm_rotate_args &a, const Groups &groups, hipStream
     per = per < 1 ? 1 : per > DEEP ? DEEP : per;
     const int64_t chunks = (passes + per - 1) / per;
     per = (passes + chunks - 1) / chunks;
-    const int64_t waves = tokens * chunks, most = (int64_t)4 << 23;   // (a launch has fewer than 2^32 threads)
-    for (int64_t w = 0; w < waves; w += most) {
-        const int64_t n = waves - w < most ? waves - w : most;
-        hipLaunchKernelGGL((norm_rotate_kernel<DT, LPH, APART, ENDS>), dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, w, (unsigned)chunks, (int)per, a, groups);
+    const int64_t most = ((int64_t)4 << 23) / chunks;   // tokens to a launch, which has fewer than 2^32 threads
+    if (most < 1) return I8F_ERR_UNSUPPORTED;
+    for (int64_t t = 0; t < tokens; t += most) {
+        const int64_t n = tokens - t < most ? tokens - t : most;
+        hipLaunchKernelGGL((norm_rotate_kernel<DT, LPH, APART, ENDS>), dim3((unsigned)((n * chunks + 3) / 4)), dim3(256), 0, st, (unsigned)t, (unsigned)n,
+                           (unsigned)chunks, (int)per, Divisor((uint32_t)chunks), Divisor((uint32_t)a.tokens), a, groups);
         if (int rc = check_launch()) return rc;
     }
     return I8F_OK;
@@ -295,7 +298,7 @@ int validate(const i8f_norm_rotate_args &a, const i8f_heads *groups, int n) {
     if (a.norm && !(a.eps >= 0.0f)) return I8F_ERR_INVALID;
     if (a.axes < 0) return I8F_ERR_INVALID;
     if (a.axes > I8F_MAX_AXES || n > I8F_MAX_HEAD_GROUPS || a.width > 256) return I8F_ERR_UNSUPPORTED;
-    if (a.batch > 0x7fffffff || a.tokens > 0x7fffffff || (a.batch && a.tokens > ((int64_t)1 << 40) / a.batch)) return I8F_ERR_UNSUPPORTED;
+    if (a.batch > 0x7fffffff || a.tokens > 0x7fffffff || (a.batch && a.tokens > 0x7fffffff / a.batch)) return I8F_ERR_UNSUPPORTED;
     const bool any = a.batch && a.tokens;
     if (a.axes) {
         if (a.positions_type < I8F_POSITION_I32 || a.positions_type > I8F_POSITION_F64 || a.first_pair[0] != 0) return I8F_ERR_INVALID;

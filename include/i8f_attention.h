@@ -33,7 +33,7 @@ typedef struct i8f_heads {
  * and a whole number of turns is taken off before it is rounded to binary32.
  *   rates      [pairs] binary64, turns to a unit; pairs = first_pair[axes], 2 pairs <= width
  *   positions  of positions_type, element strides position_batch, position_token, position_axis (the batch's may be 0)
- * axes 0: nothing is turned.  width up to 256.  The outputs overlap neither the inputs nor one another.
+ * axes 0: nothing is turned.  width up to 256, batch * tokens below 2^31.  The outputs overlap neither the inputs nor one another.
  */
 #define I8F_MAX_HEAD_GROUPS 4
 #define I8F_MAX_AXES 4
