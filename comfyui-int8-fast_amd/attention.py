@@ -123,7 +123,9 @@ def forward_cross_attention(x: Tensor, context: Tensor | None, to_q, to_k, to_v,
     x [batch, queries, features], context [batch, keys, features] or None for x itself; layers that read one tensor quantise it once
     (int8_quant.forward_fanout).  q_weight, k_weight [head width]: the norms of the heads (both or neither); rotary with `positions` of x's tokens
     and `context_positions` of the context's (None: its keys are not turned; without a context those of x).  gate and residual as
-    Linear.forward takes them, applied behind to_out; without to_out the heads side by side are returned."""
+    Linear.forward takes them, applied behind to_out; without to_out the heads side by side are returned.  No gradients: under grad mode an
+    input that asks for one is refused, and layers of queries, keys and values with trainable parameters; an input with a tangent always."""
+    _lib.refuse_gradients(x=x, context=context, gate=gate, residual=residual)
     kv_heads = heads if kv_heads is None else kv_heads
     if (q_weight is None) != (k_weight is None):
         raise ValueError("the norms of queries and keys go together")

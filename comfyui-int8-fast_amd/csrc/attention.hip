@@ -629,7 +629,7 @@ int validate(const i8f_attention_args &a) {
     for (int64_t s : {a.q_batch, a.q_token, a.q_head, a.k_batch, a.k_token, a.k_head, a.v_batch, a.v_token, a.v_head})
         if (s < 0) return I8F_ERR_INVALID;
     for (int64_t n : {a.batch, a.queries, a.keys, a.heads})
-        if (n > 0x7fffffff) return I8F_ERR_UNSUPPORTED;
+        if (n > 1 << 30) return I8F_ERR_UNSUPPORTED;
     const int64_t rows = a.batch * a.queries;
     if (rows && a.heads > 0x7fffffff / rows) return I8F_ERR_UNSUPPORTED;   // (rows are counted in 32 bits)
     if (a.key_lengths && a.lengths_type != 0 && a.lengths_type != 1) return I8F_ERR_INVALID;
