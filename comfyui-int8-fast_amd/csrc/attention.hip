@@ -6,6 +6,16 @@
 // in-lane but for one exchange of wave halves, and rounded to 16 bits the scores' weights already are the second operand of
 // O^T = V^T P^T, the contraction index being free to run in the order in which a lane happens to hold the states; the first operand comes
 // out of row-major V by LDS reads that transpose (ds_read_b64_tr_b16).
+//
+// What bounds it.  Long calls the card's power: 8192 x 8192, 40 heads of 128, 1270 us, 1.08 PFLOP/s, the matrix unit 53 % busy at 1.95 of 2.4 GHz
+// (eight waves; four: 55 % at 1.8 GHz, 1340 us); 1.58 PFLOP/s is what a large library product reaches.  A wave's 64 states are 32 matrix
+// instructions of 32 cycles and 124 vector instructions of arithmetic (32 exponentials among them, 8 cycles each), which share the issue with
+// them.  Calls over few states their start and end, in which nothing multiplies: 32760 x 512 420 us (0.82), over 64 states 181 us, 3.7 TB/s.  One
+// token memory: 65536 states of 8 heads 58 us with the join, 4.6 TB/s; small ones the latencies of a launch (5 us).
+// Measured and not kept: 64 rows to a wave, which halve the LDS reads but leave one wave to a SIMD and a third of the vector instructions
+// moving scores between register files (1450 us for 8192 x 8192); tiles of 32 states with three waves to a SIMD (405 against 419 us for 32768 x 512,
+// 1320 against 1290 for 8192 x 8192, 82 to 107 for 1024 x 4096 of 32 heads); LDS reads three products ahead of their use in a fixed order (no
+// faster); two steps unrolled so that addresses are constants (registers spilled).
 #include <initializer_list>
 #include <type_traits>
 #include <utility>
@@ -441,7 +451,8 @@ __global__ __launch_bounds__(WAVES * 64, (Shape<DT, DP, WAVES, APART, MASK>::PER
     }
 }
 
-// The splits' results of a row joined: a workgroup to a row, its threads by four elements and by splits, so that all of them are requested at once.
+// The splits' results of a row joined: a workgroup to a row, its threads by four elements and by splits, so that all of them are requested at once
+// (4 us for 32 rows of 32 splits; a wave to a row, split after split, was 25).
 constexpr int MOST_SPLITS = 256;
 template <int DT, int DP>
 __global__ __launch_bounds__(256) void join_kernel(const Launch p) {
@@ -518,7 +529,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const Packs packs) {
 // ---- how a call is cut ------------------------------------------------------------------------------------------------------------
 struct Plan {
     int padded;               // width of the kernels
-    bool apart;               // few rows: the waves of a workgroup take the states in turn
+    bool apart;               // the waves of a workgroup take the states in turn
     int waves;                // of a workgroup
     int64_t row_tiles, splits, tiles;
     int64_t partial_bytes;    // of results and statistics of the splits
@@ -529,8 +540,11 @@ Plan plan_of(int64_t batch, int64_t queries, int64_t keys, int64_t heads, int64_
     Plan p = {};
     p.padded = width <= 64 ? 64 : width <= 96 ? 96 : width <= 128 ? 128 : width <= 192 ? 192 : 256;
     const int64_t rows = queries * (heads / kv_heads), sets = batch * kv_heads;
-    p.apart = rows <= 32;
-    p.waves = p.apart ? (p.padded > 128 ? 2 : 4) : 4;
+    // Apart, four waves to 32 rows, where 128 rows together leave waves idle or CUs.  us together and apart: 16 heads of 64, 64 rows over 512 states
+    // 10.3 and 6.5, 96 over 512 10.8 and 6.0, over 4096 13.9 and 13.5, over 32768 36 and 40; 32 heads of 128, 96 rows over 512 16.2 and 9.3, over
+    // 4096 28 and 35; 256 heads of 64, 77 rows over 512 11.7 and 15.0.
+    p.apart = rows <= 32 || (sets * ((rows + 31) / 32) <= 128 && keys <= 2048);
+    p.waves = p.apart && p.padded > 128 ? 2 : 4;
     // Eight waves read the states half as often, which is energy, and the card runs at its power limit in long calls; four start and end beside
     // another workgroup.  us with four and eight for 40 heads of 128: 8192 x 8192 1338 and 1284, 32768 x 4096 2603 and 2546, 32768 x 2048 1333 and
     // 1333, 32768 x 512 419 and 449, 4096 x 4096 336 and 356.
