@@ -526,6 +526,11 @@ __global__ __launch_bounds__(256) void pack_kernel(const Packs packs) {
     }
 }
 
+// No states at all: zeros.
+__global__ __launch_bounds__(256) void zeros_kernel(uint16_t *out, const int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) out[i] = 0;
+}
+
 // ---- how a call is cut ------------------------------------------------------------------------------------------------------------
 struct Plan {
     int padded;               // width of the kernels
@@ -682,6 +687,11 @@ extern "C" int i8f_attention(const i8f_attention_args *args, void *stream) {
     const int64_t share = a.heads / a.kv_heads;
     if (int rc = check_device()) return rc;
     hipStream_t st = (hipStream_t)stream;
+    if (!a.keys) {
+        const int64_t n = a.batch * a.queries * a.heads * a.width, blocks = (n + 2047) / 2048;
+        hipLaunchKernelGGL(zeros_kernel, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st, (uint16_t *)a.out, n);
+        return check_launch();
+    }
     Launch p = {a, (uint32_t)share, (uint32_t)(a.queries * share), (uint32_t)plan.row_tiles, (uint32_t)plan.splits, (uint32_t)plan.tiles, (uint32_t)round_up(a.width, 8)};
     p.wide_out = a.width % 8 == 0 && (uintptr_t)a.out % 16 == 0;
     p.by_share = Divisor(p.share), p.by_row_tiles = Divisor(p.row_tiles), p.by_splits = Divisor(p.splits), p.by_kv_heads = Divisor((uint32_t)a.kv_heads);
@@ -689,7 +699,7 @@ extern "C" int i8f_attention(const i8f_attention_args *args, void *stream) {
     p.stats = p.partial ? p.partial + plan.partial_bytes / 4 / (plan.padded + 2) * plan.padded : nullptr;
     int64_t bytes[3];
     const int which = to_pack(a, bytes);
-    if (which && a.keys) {
+    if (which) {
         Packs packs = {};
         char *at = (char *)a.workspace + plan.partial_bytes;
         int count = 0;

@@ -199,8 +199,13 @@ def test_rows_of_nothing(pkg, dev):
     for shape in ((0, 3, 5, 2, 2, 64), (2, 0, 5, 2, 2, 64), (2, 3, 5, 0, 0, 64)):
         q, k, v = inputs(*shape, torch.bfloat16)
         assert pkg.cross_attention(q, k, v).shape == q.shape
+    for width in (64, 37, 256):
+        for queries in (3, 500):
+            q, k, v = inputs(2, queries, 0, 4, 2, width, torch.bfloat16)
+            torch.empty_like(q).fill_(7.0)   # (what the result's memory may have held)
+            got = pkg.cross_attention(q[..., :], k, v)
+            assert got.shape == q.shape and torch.equal(got, torch.zeros_like(q))
     q, k, v = inputs(2, 3, 0, 4, 2, 64, torch.bfloat16)
-    assert not pkg.cross_attention(q, k, v).any() and pkg.cross_attention(q, k, v).shape == q.shape
     assert not pkg.cross_attention(q, k, v, key_mask=torch.zeros(2, 0, dtype=torch.bool, device="cuda"), key_lengths=torch.ones(2, dtype=torch.int64, device="cuda")).any()
 
 
