@@ -97,7 +97,7 @@ __device__ __forceinline__ bool counts(int type, uint32_t bits, float &add) {
     const float m = type == I8F_MASK_BF16 ? bf16_bits_to_f32(bits) : type == I8F_MASK_F16 ? f16_bits_to_f32(bits) : __uint_as_float(bits);
     const float lowest = type == I8F_MASK_BF16 ? -3.3895313892515355e38f : type == I8F_MASK_F16 ? -65504.0f : LOWEST;
     if (m <= lowest) return false;
-    add = fmaxf(m * TO_LOG2, LOWEST);
+    add = m * TO_LOG2 < LOWEST ? LOWEST : m * TO_LOG2;   // (a NaN stays one)
     return true;
 }
 

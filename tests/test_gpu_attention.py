@@ -195,6 +195,35 @@ def test_addends_that_are_large_but_count(pkg, dev):
         check(pkg.cross_attention(q, k, v, key_mask=torch.full_like(m, big)), expected(q, k, v, key_mask=torch.full_like(m, big)))
 
 
+def test_an_addend_that_is_no_number_ends_its_batch_only(pkg, dev):
+    q, k, v = inputs(2, 50, 200, 2, 2, 128, torch.bfloat16)
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        m = torch.zeros(2, 200, dtype=dtype, device="cuda")
+        want = pkg.cross_attention(q, k, v, key_mask=m)
+        m[1, 77] = math.nan
+        got = pkg.cross_attention(q, k, v, key_mask=m)
+        assert torch.equal(got[0], want[0]) and torch.isnan(got[1]).all()
+
+
+def test_values_that_are_not_finite_stay_in_their_rows(pkg, dev):
+    """A query that is no number ends itself, a state that counts ends the queries of its batch and head."""
+    for queries, keys in ((200, 300), (3, 300), (1, 3000)):
+        q, k, v = inputs(2, queries, keys, 2, 2, 64, torch.bfloat16)
+        want = pkg.cross_attention(q, k, v)
+        bad = q.clone()
+        bad[0, queries // 2, 1, 5] = math.nan
+        got = pkg.cross_attention(bad, k, v)
+        same = torch.ones(q.shape[:3], dtype=torch.bool, device="cuda")
+        same[0, queries // 2, 1] = False
+        assert torch.equal(got[same], want[same]) and torch.isnan(got[~same]).all()
+        bad = v.clone()
+        bad[1, keys - 1, 0, 3] = math.inf
+        got = pkg.cross_attention(q, k, bad)
+        same = torch.ones(q.shape, dtype=torch.bool, device="cuda")
+        same[1, :, 0, 3] = False
+        assert torch.equal(got[same], want[same]) and not torch.isfinite(got[~same].float()).any()
+
+
 def test_rows_of_nothing(pkg, dev):
     for shape in ((0, 3, 5, 2, 2, 64), (2, 0, 5, 2, 2, 64), (2, 3, 5, 0, 0, 64)):
         q, k, v = inputs(*shape, torch.bfloat16)
