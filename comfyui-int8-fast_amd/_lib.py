@@ -1196,8 +1196,8 @@ def attention(q, k, v, key_lengths=None, key_mask=None, scale=None):
     if not 1 <= width <= MAX_HEAD_WIDTH:
         raise ValueError(f"heads must be 1 to {MAX_HEAD_WIDTH} elements wide, got {width}")
     scale = width ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale <= torch.finfo(torch.float32).max:
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if not 0.0 < scale <= 2.0 ** 126:
+        raise ValueError(f"scale must be positive and at most 2^126, got {scale}")
     q, k, v = _unit_stride(q), _unit_stride(k), _unit_stride(v)
     out = torch.empty((batch, queries, heads, width), dtype=q.dtype, device=q.device)
     arg = _AttentionArgs(_addr(q), _addr(k), _addr(v), _addr(out), batch, queries, keys, heads, kv_heads, width, *q.stride()[:3], *k.stride()[:3],

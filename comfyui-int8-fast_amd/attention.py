@@ -7,6 +7,7 @@ bear the steps of int8 rows.  forward_cross_attention is the whole path, project
 from __future__ import annotations
 
 import math
+import operator
 
 import torch
 from torch import Tensor
@@ -27,7 +28,7 @@ class RotaryAxes:
     Laid out once: assigning to its attributes is refused."""
 
     def __init__(self, dims, theta=10000.0, *, interleaved: bool = True, device=None):
-        dims = tuple(int(n) for n in dims)
+        dims = tuple(operator.index(n) for n in dims)
         if not 1 <= len(dims) <= _lib.MAX_AXES or any(n < 2 or n % 2 for n in dims):
             raise ValueError(f"dims must be one to {_lib.MAX_AXES} even numbers from 2 on, got {list(dims)}")
         thetas = tuple(float(t) for t in theta) if isinstance(theta, (tuple, list)) else (float(theta),) * len(dims)
@@ -77,6 +78,11 @@ def rotate_heads(xs, rotary: RotaryAxes, positions: Tensor):
 def _norm_rotate(xs, weights, norm, eps, rotary, positions):
     if (rotary is None) != (positions is None):
         raise ValueError("rotary and positions go together")
+    if rotary is not None and not isinstance(rotary, RotaryAxes):
+        raise TypeError(f"rotary must be a RotaryAxes, not {type(rotary).__name__}")
+    for x in xs:
+        if not isinstance(x, Tensor):
+            raise TypeError(f"heads must be tensors, not {type(x).__name__}")
     rates, dims, apart = (None, (), False) if rotary is None else (rotary.rates, rotary.dims, not rotary.interleaved)
     compiling = torch.compiler.is_compiling()
     if xs and xs[0].is_cuda and not compiling:
@@ -97,7 +103,7 @@ def cross_attention(q: Tensor, k: Tensor, v: Tensor, *, key_lengths: Tensor | No
     key_lengths: int32 or int64 [batch]: only the first so many states count (all of them for a larger number, none for a negative one).
     key_mask:    [batch, keys], bool (True: the state counts) or bfloat16, float16, float32 added to the scores; a state whose addend is -inf
                  or the lowest value of its type does not count.  With lengths both hold.
-    scale:       positive; width ** -0.5 by default.
+    scale:       positive, at most 2^126; width ** -0.5 by default.
 
     -> [batch, queries, heads, width], contiguous.  A query over which no state counts gets zeros, and what the states that do not count hold
     (NaN, infinities) reaches nothing.  Scores, maximum and sums are in binary32, the weights are rounded to q's type for the second product,

@@ -643,7 +643,8 @@ int validate(const i8f_attention_args &a) {
     if (a.batch < 0 || a.queries < 0 || a.keys < 0 || a.heads < 0 || a.kv_heads < 0 || a.width < 1) return I8F_ERR_INVALID;
     if (a.dtype != I8F_BF16 && a.dtype != I8F_F16) return valid_dtype(a.dtype) ? I8F_ERR_UNSUPPORTED : I8F_ERR_INVALID;
     if (a.heads && (!a.kv_heads || a.heads % a.kv_heads)) return I8F_ERR_INVALID;
-    if (!(a.scale > 0.0f) || !(a.scale <= 3.4028234663852886e38f)) return I8F_ERR_INVALID;
+    if (!(a.scale > 0.0f) || !(a.scale <= 0x1p126f)) return I8F_ERR_INVALID;   // (times log2 e it stays finite)
+    if (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out) % 2) return I8F_ERR_INVALID;
     if (a.width > 256) return I8F_ERR_UNSUPPORTED;
     for (int64_t s : {a.q_batch, a.q_token, a.q_head, a.k_batch, a.k_token, a.k_head, a.v_batch, a.v_token, a.v_head})
         if (s < 0) return I8F_ERR_INVALID;

@@ -321,6 +321,7 @@ int validate(const i8f_norm_rotate_args &a, const i8f_heads *groups, int n) {
         out[i] = extent({{a.batch, a.tokens * g.heads * a.width}, {a.tokens, g.heads * a.width}, {g.heads, a.width}, {a.width, 1}});
         if (in[i] < 0 || out[i] < 0) return I8F_ERR_UNSUPPORTED;
         if (in[i] && (!g.x || !g.out)) return I8F_ERR_INVALID;
+        if (((uintptr_t)g.x | (uintptr_t)g.out) % size) return I8F_ERR_INVALID;
     }
     for (int i = 0; i < n; ++i)
         for (int j = 0; j < n; ++j)   // (a head is written while other waves read)

@@ -63,9 +63,10 @@ int i8f_norm_rotate(const i8f_norm_rotate_args *args, const i8f_heads *groups, i
  *   out          [batch, queries, heads, width], contiguous; overlaps no input
  *   key_lengths  [batch] of int32 (lengths_type 0) or int64 (1), or NULL; values outside 0 ... keys count as the nearer of the two
  *   key_mask     NULL or element (b, j) at mask_batch b + mask_key j of mask_type
- *   scale        positive and finite
+ *   scale        positive, at most 2^126
  *   workspace    any contents, 16-byte aligned, i8f_attention_workspace_bytes() of these arguments (which looks at all but workspace and
- *                key_lengths' and key_mask's contents); less, or NULL, is refused where that is not 0.  Calls that overlap in time do not share it.
+ *                key_lengths' and key_mask's contents); less, or NULL, is refused where that is not 0.  It overlaps nothing else, and calls that overlap in
+ *                time do not share it.
  * batch * queries * heads is below 2^31, keys at most 2^30; more workgroups than a launch has (2^24 of 128 rows, of 32 where there are fewer) are
  * I8F_ERR_UNSUPPORTED.
  */

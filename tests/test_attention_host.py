@@ -40,7 +40,7 @@ def test_norm_rotate_arguments_are_checked_before_any_launch(L):
                 {"positions_type": -1}, {"first_pair": (1, 2, 4, 0, 0)}, {"first_pair": (0, 2, 2, 0, 0)}, {"first_pair": (0, 3, 1, 0, 0)}, {"first_pair": (0, 1, 5, 0, 0)},
                 {"rates": None}, {"positions": None}, {"position_batch": -1}, {"position_token": -1}, {"position_axis": -1}):
         assert _heads(L, bad, {}) == INVALID, bad
-    for bad in ({"x": None}, {"out": None}, {"heads": -1}, {"batch_stride": -1}, {"token_stride": -1}, {"head_stride": -1}, {"weight": 16, "weight_dtype": L.F16},
+    for bad in ({"x": None}, {"out": None}, {"heads": -1}, {"batch_stride": -1}, {"token_stride": -1}, {"head_stride": -1}, {"x": (1 << 22) + 1}, {"weight": 16, "weight_dtype": L.F16},
                 {"out": 1 << 22}, {"out": (1 << 22) + 94}, {"out": (1 << 22) - 94}):
         assert _heads(L, None, bad) == INVALID, bad
         assert _heads(L, None, {}, bad) == INVALID, bad
@@ -72,7 +72,7 @@ def test_attention_arguments_are_checked_before_any_launch(L):
     assert L.lib().i8f_attention(None, None) == INVALID
     for bad in (*({n: -1} for n in ("batch", "queries", "keys", "heads", "kv_heads", "width", "q_batch", "q_token", "q_head", "k_batch", "k_token", "k_head", "v_batch",
                                     "v_token", "v_head")),
-                {"width": 0}, {"dtype": 9}, {"kv_heads": 0}, {"kv_heads": 3}, {"scale": 0.0}, {"scale": -1.0}, {"scale": float("inf")}, {"scale": float("nan")},
+                {"width": 0}, {"dtype": 9}, {"kv_heads": 0}, {"kv_heads": 3}, {"scale": 0.0}, {"scale": -1.0}, {"scale": float("inf")}, {"scale": float("nan")}, {"scale": 2.0 ** 127}, {"q": (1 << 20) + 1}, {"v": (1 << 23) + 1},
                 {"q": None}, {"k": None}, {"v": None}, {"out": None}, {"key_lengths": 16, "lengths_type": 2}, {"key_mask": 16, "mask_type": 4}, {"key_mask": 16, "mask_type": -1},
                 {"key_mask": 16, "mask_batch": -1}, {"key_mask": 16, "mask_key": -1}, {"out": 1 << 20}, {"out": (1 << 22) + 16}, {"out": (1 << 23) - 16}):
         assert _attention(L, **bad) == INVALID, bad
@@ -103,6 +103,8 @@ def test_a_rotation_keeps_turns_to_a_unit(pkg):
 
 
 def test_rotations_refuse_what_is_none(pkg):
+    with pytest.raises(TypeError):
+        pkg.RotaryAxes((2.0, 4), device="cpu")
     for dims in ((), (2, 2, 2, 2, 2), (3,), (0,), (-2,)):
         with pytest.raises(ValueError, match="even numbers"):
             pkg.RotaryAxes(dims, device="cpu")
@@ -130,6 +132,10 @@ def test_arguments_that_do_not_go_together(pkg):
         pkg.norm_heads(x, positions=torch.zeros(2, 2))
     with pytest.raises(ValueError, match="its axes"):
         pkg.rotate_heads(x, None, torch.zeros(2, 2))
+    with pytest.raises(TypeError, match="RotaryAxes"):
+        pkg.rotate_heads(x, (4, 4), torch.zeros(2, 2))
+    with pytest.raises(TypeError, match="tensors"):
+        pkg.norm_heads([1.0])
     with pytest.raises(ValueError, match="weights"):
         pkg.norm_heads([x, x], [None])
     for bad in ({"q_weight": torch.ones(8)}, {"rotary": r}, {"positions": torch.zeros(2, 2)}, {"context_positions": torch.zeros(2, 2)}, {"gate": torch.ones(8)},

@@ -258,7 +258,7 @@ def test_refusals(pkg, dev):
     for bad in (lambda: call(q[0], k, v), lambda: call(q, k[0], v[0]), lambda: call(q, k, v[:, :4]), lambda: call(q, k[:1], v[:1]), lambda: call(q, k[..., :32], v[..., :32]),
                 lambda: call(q[:, :, :3], k, v), lambda: call(q, k[:, :, :0], v[:, :, :0]), lambda: call(q.half(), k, v), lambda: call(q, k, v.half()),
                 lambda: call(q.float(), k.float(), v.float()), lambda: call(q, k.cpu(), v), lambda: call(q, k, v, scale=0.0), lambda: call(q, k, v, scale=-1.0),
-                lambda: call(q, k, v, scale=math.inf), lambda: call(q, k, v, scale=math.nan), lambda: call(q, k, v, scale=1e39), lambda: call(q[..., :0], k[..., :0], v[..., :0]),
+                lambda: call(q, k, v, scale=math.inf), lambda: call(q, k, v, scale=math.nan), lambda: call(q, k, v, scale=1e39), lambda: call(q, k, v, scale=1e-60), lambda: call(q[..., :0], k[..., :0], v[..., :0]),
                 lambda: call(*(torch.zeros(1, 1, 1, 257, device="cuda", dtype=torch.bfloat16) for _ in range(3))),
                 lambda: call(q, k, v, key_lengths=torch.ones(3, dtype=torch.int32, device="cuda")), lambda: call(q, k, v, key_lengths=torch.ones(2, device="cuda")),
                 lambda: call(q, k, v, key_lengths=torch.ones(2, dtype=torch.int32)), lambda: call(q, k, v, key_mask=torch.ones(2, 4, dtype=torch.bool, device="cuda")),
