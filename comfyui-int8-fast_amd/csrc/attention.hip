@@ -10,12 +10,14 @@
 // What bounds it.  Long calls the card's power: 8192 x 8192, 40 heads of 128, 1270 us, 1.08 PFLOP/s, the matrix unit 53 % busy at 1.95 of 2.4 GHz
 // (eight waves; four: 55 % at 1.8 GHz, 1340 us); 1.58 PFLOP/s is what a large library product reaches.  A wave's 64 states are 32 matrix
 // instructions of 32 cycles and 124 vector instructions of arithmetic (32 exponentials among them, 8 cycles each), which share the issue with
-// them.  Calls over few states their start and end, in which nothing multiplies: 32760 x 512 420 us (0.82), over 64 states 181 us, 3.7 TB/s.  One
+// them.  Calls over few states have the traffic of their rows on top: 32760 x 512 420 us (0.82), over 64 states 171 to 181 us, 3.8 TB/s; the
+// clock is at 1.72 GHz there as well.  One
 // token memory: 65536 states of 8 heads 58 us with the join, 4.6 TB/s; small ones the latencies of a launch (5 us).
 // Measured and not kept: 64 rows to a wave, which halve the LDS reads but leave one wave to a SIMD and a third of the vector instructions
 // moving scores between register files (1450 us for 8192 x 8192); tiles of 32 states with three waves to a SIMD (405 against 419 us for 32768 x 512,
 // 1320 against 1290 for 8192 x 8192, 82 to 107 for 1024 x 4096 of 32 heads); LDS reads three products ahead of their use in a fixed order (no
-// faster); two steps unrolled so that addresses are constants (registers spilled).
+// faster); two steps unrolled so that addresses are constants (registers spilled); the rows of the workgroup to come requested into the L2
+// (408 for 415 us at 32760 x 512, 2 to 5 % more everywhere else).
 #include <initializer_list>
 #include <type_traits>
 #include <utility>
@@ -303,7 +305,7 @@ __global__ __launch_bounds__(WAVES * 64, (Shape<DT, DP, WAVES, APART, MASK>::PER
         }
         most = max_of_halves(most) * factor;
         // The reference of the exponentials follows the maximum only where that has grown by 2^8: the weights are below 2^8 then, which costs
-        // no bits, and the result is divided by their sum either way.
+        // no bits, and the result is divided by their sum either way.  (bf16's values times such weights stay finite up to 2^120 / states.)
         if (__any(most > top + 8.0f)) {
             const float to = fmaxf(top, most), fade = __builtin_amdgcn_exp2f(top - to);
             top = to;

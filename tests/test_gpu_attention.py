@@ -224,6 +224,22 @@ def test_values_that_are_not_finite_stay_in_their_rows(pkg, dev):
         assert torch.equal(got[same], want[same]) and not torch.isfinite(got[~same].float()).any()
 
 
+@pytest.mark.parametrize("queries, keys", [(200, 300), (3, 300), (1, 3000)])
+def test_scores_and_values_at_the_ends_of_binary32(pkg, dev, queries, keys):
+    q, k, v = inputs(2, queries, keys, 2, 2, 64, torch.bfloat16)
+    some = torch.arange(keys, device="cuda").expand(2, -1) % 3 > 0
+    for mask in (None, some, some.float() - 1.0):
+        got = pkg.cross_attention(torch.full_like(q, -2.0 ** 64), torch.full_like(k, 2.0 ** 64), v, key_mask=mask)
+        assert torch.equal(got, torch.zeros_like(got))   # (every score is -inf)
+        # scores that grow by just less than the running maximum lets them, values as large as the documentation has them: equal ones are their mean
+        grow = torch.linspace(0.0, 1.0, keys, device="cuda")[None, :, None, None] * 5.0
+        large = torch.full_like(v, 2.0 ** 119 / 2 ** math.ceil(math.log2(keys)))
+        got = pkg.cross_attention(torch.ones_like(q), (grow / 8).expand(2, -1, 2, 64).bfloat16(), large, key_mask=mask)
+        # sums and weights in binary32 cancel but for keys roundings of 2^-24 each in two sums, the result is rounded by 2^-8
+        off = ((got.double() / large[0, 0, 0, 0].double()) - 1.0).abs().max().item()
+        assert off <= 2.0 ** -8 + 2 * keys * 2.0 ** -24 + 2.0 ** -20, off
+
+
 def test_rows_of_nothing(pkg, dev):
     for shape in ((0, 3, 5, 2, 2, 64), (2, 0, 5, 2, 2, 64), (2, 3, 5, 0, 0, 64)):
         q, k, v = inputs(*shape, torch.bfloat16)
