@@ -43,6 +43,7 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 
 constexpr float LOWEST = -3.4028234663852886e38f, TO_LOG2 = 1.4426950408889634f;
+constexpr float NONE = -__builtin_inff();   // a maximum of no scores
 
 struct Launch {
     i8f_attention_args a;
@@ -83,6 +84,14 @@ __device__ __forceinline__ float sum_of_halves(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+
+// What a score is multiplied by in the exponential: its unit and log2 e, or nothing where addends were put on top of scaled scores.
+__device__ __forceinline__ float exponents_of(const i8f_attention_args &a) {
+    return a.key_mask && a.mask_type != I8F_MASK_BYTES ? 1.0f : a.scale * TO_LOG2;
+}
+
+// What weights under one maximum become under a larger or the same one (which may be that of no scores).
+__device__ __forceinline__ float fading(float from, float to, float unit) { return from == to ? 1.0f : __builtin_amdgcn_exp2f((from - to) * unit); }
 
 // A state's element of the mask as it is in memory, and whether it counts by it, with its addend in units of log 2.
 __device__ __forceinline__ uint32_t mask_bits(const i8f_attention_args &a, int64_t b, int64_t j) {
@@ -234,8 +243,20 @@ __global__ __launch_bounds__(WAVES * 64, (Shape<DT, DP, WAVES, APART, MASK>::PER
     v16f o[ND], s[KB];
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = v16f{};
-    float top = LOWEST, sum = 0.0f, most = LOWEST;
+    float top = NONE, sum = 0.0f, most = NONE;   // (the maxima in the scores' own unit)
     constexpr float RAISE = DT == I8F_F16 ? 6.0f : 0.0f;   // (binary16 weights lie between 2^6 and 2^14 for the largest: see below)
+    // A weight is 2^(unit x - unit top), one fused operation on x with unit top rounded beforehand.  That rounding is the same for all weights under
+    // one reference, but weights of other tiles were formed under others, and in the end it would leave the type's range: at 2^28 binary16's, at
+    // 2^33 bfloat16's.  Below 2^12 it is 2^-13 at the most, less than half of what binary16 rounds a weight by.  A row that is beyond has its
+    // maximum taken off the scores first, exactly where they are close to it, and scales them afterwards; the wave's other rows get what they
+    // would have had (a few more operations a score for all of them).  A row whose scores so far are all -inf or NaN has no reference.
+    constexpr float FAR = 4096.0f;
+    const float unit = MASK ? exponents_of(a) : to_log2;
+    const float allowed = 8.0f / unit;   // growth of the maximum that `top` need not follow, while its own steps are small beside that
+    auto beyond = [&]() { return fabsf(top) < __builtin_inff() && !(fabsf(top * unit) < FAR); };
+    auto off = [&]() { return top == NONE ? RAISE : __builtin_fmaf(-top, unit, RAISE); };
+    bool far = false;                                  // a row of the wave is beyond
+    float limit = NONE, factor = unit, from = RAISE;   // `top`'s; the exponents are factor x + from
 
     // where a lane reads: K row (lane & 31) of a block, V's four rows from 4 half on by 16 elements
     char *const tiles = lds + (APART ? wave * 4 * S::TILE : 0);
@@ -283,10 +304,9 @@ __global__ __launch_bounds__(WAVES * 64, (Shape<DT, DP, WAVES, APART, MASK>::PER
     int stage = 0;
     auto step = [&](auto more) __attribute__((always_inline)) {
         constexpr bool MORE = decltype(more)::value;
-        float factor = to_log2;   // scores are scaled in the exponential's argument, or here where addends come on top
         if constexpr (MASK) {
-            if (a.mask_type != I8F_MASK_BYTES) {
-                adds[lane] = now.add, factor = 1.0f;
+            if (a.mask_type != I8F_MASK_BYTES) {   // (scaled here, since addends come on top)
+                adds[lane] = now.add;
 #pragma unroll
                 for (int k = 0; k < KB; ++k)
 #pragma unroll
@@ -303,17 +323,27 @@ __global__ __launch_bounds__(WAVES * 64, (Shape<DT, DP, WAVES, APART, MASK>::PER
             }
             most = largest(s);
         }
-        most = max_of_halves(most) * factor;
+        most = max_of_halves(most);
         // The reference of the exponentials follows the maximum only where that has grown by 2^8: the weights are below 2^8 then, which costs
         // no bits, and the result is divided by their sum either way.  (bf16's values times such weights stay finite up to 2^120 / states.)
-        if (__any(most > top + 8.0f)) {
-            const float to = fmaxf(top, most), fade = __builtin_amdgcn_exp2f(top - to);
+        if (__any(most > limit)) {
+            const float to = most > limit ? most : top, fade = fading(top, to, unit);   // (a row's bits do not depend on the rows beside it)
             top = to;
+            const bool mine = beyond();
+            far = __any(mine);
+            limit = mine ? top : top + allowed, factor = far ? 1.0f : unit, from = !far ? off() : mine ? RAISE : 0.0f;
             sum *= fade;
 #pragma unroll
             for (int d = 0; d < ND; ++d) o[d] *= fade;
         }
-        const float from = RAISE - top;
+        if (far) {
+            const bool mine = beyond();
+            const float near = off();
+#pragma unroll
+            for (int k = 0; k < KB; ++k)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[k][i] = mine ? (s[k][i] - top) * unit : __builtin_fmaf(s[k][i], unit, near);
+        }
         all_here();   // the tile's V and the next one's K
         const Tile after = MORE ? tile_from(next.at + STEP, ahead) : next;
         if constexpr (MORE) request_k(after, stage), request_v(next, stage ^ 1), ahead = peek(after.at + STEP);
@@ -385,12 +415,12 @@ __global__ __launch_bounds__(WAVES * 64, (Shape<DT, DP, WAVES, APART, MASK>::PER
             const int r = at / QUADS, e = at % QUADS * 4;
             const unsigned own = row_tile * 32 + r;
             if (own >= p.rows) continue;
-            float best = LOWEST, total = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float best = NONE, total = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) best = fmaxf(best, heads[(w * 32 + r) * 2]);
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
-                const float f = __builtin_amdgcn_exp2f(heads[(w * 32 + r) * 2] - best);
+                const float f = fading(heads[(w * 32 + r) * 2], best, unit);
                 total = __builtin_fmaf(heads[(w * 32 + r) * 2 + 1], f, total);
                 const float4 x = *(const float4 *)(others + (w * 32 + r) * PITCH + e);
                 v[0] = __builtin_fmaf(x.x, f, v[0]), v[1] = __builtin_fmaf(x.y, f, v[1]), v[2] = __builtin_fmaf(x.z, f, v[2]), v[3] = __builtin_fmaf(x.w, f, v[3]);
@@ -466,13 +496,13 @@ __global__ __launch_bounds__(256) void join_kernel(const Launch p) {
     const unsigned row = blockIdx.x % p.rows;
     const int64_t bg = blockIdx.x / p.rows, b = bg / a.kv_heads, g = bg % a.kv_heads, first = bg * p.splits * p.rows + row;
     const bool mine = tid < splits;
-    const float2 own = mine ? *(const float2 *)(p.stats + 2 * (first + (int64_t)tid * p.rows)) : make_float2(LOWEST, 0.0f);
+    const float2 own = mine ? *(const float2 *)(p.stats + 2 * (first + (int64_t)tid * p.rows)) : make_float2(NONE, 0.0f);
     float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
     const float top = wave_max(own.x);
     if (lane == 0) red[wave] = top;
     __syncthreads();
     const float best = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float f = mine ? __builtin_amdgcn_exp2f(own.x - best) : 0.0f;
+    const float f = mine ? fading(own.x, best, exponents_of(a)) : 0.0f;
     weight[tid] = f;
     float total = own.y * f;
 #pragma unroll
