@@ -85,15 +85,16 @@ __device__ __forceinline__ float sum_of_halves(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// What a score is multiplied by in the exponential: its unit and log2 e, or nothing where addends were put on top of scaled scores.
+// What a score is multiplied by in the exponential: the scale and log2 e, or log2 e where addends were put on top of scaled scores (not in units
+// of log 2: addends reach to the ends of binary32).
 __device__ __forceinline__ float exponents_of(const i8f_attention_args &a) {
-    return a.key_mask && a.mask_type != I8F_MASK_BYTES ? 1.0f : a.scale * TO_LOG2;
+    return a.key_mask && a.mask_type != I8F_MASK_BYTES ? TO_LOG2 : a.scale * TO_LOG2;
 }
 
 // What weights under one maximum become under a larger or the same one (which may be that of no scores).
 __device__ __forceinline__ float fading(float from, float to, float unit) { return from == to ? 1.0f : __builtin_amdgcn_exp2f((from - to) * unit); }
 
-// A state's element of the mask as it is in memory, and whether it counts by it, with its addend in units of log 2.
+// A state's element of the mask as it is in memory, and whether it counts by it, with its addend.
 __device__ __forceinline__ uint32_t mask_bits(const i8f_attention_args &a, int64_t b, int64_t j) {
     const int64_t at = b * a.mask_batch + j * a.mask_key;
     switch (a.mask_type) {
@@ -108,7 +109,7 @@ __device__ __forceinline__ bool counts(int type, uint32_t bits, float &add) {
     const float m = type == I8F_MASK_BF16 ? bf16_bits_to_f32(bits) : type == I8F_MASK_F16 ? f16_bits_to_f32(bits) : __uint_as_float(bits);
     const float lowest = type == I8F_MASK_BF16 ? -3.3895313892515355e38f : type == I8F_MASK_F16 ? -65504.0f : LOWEST;
     if (m <= lowest) return false;
-    add = m * TO_LOG2 < LOWEST ? LOWEST : m * TO_LOG2;   // (a NaN stays one)
+    add = m;
     return true;
 }
 
@@ -160,7 +161,6 @@ __global__ __launch_bounds__(WAVES * 64, (Shape<DT, DP, WAVES, APART, MASK>::PER
     const int from_tile = (int)(split * p.tiles) + (APART ? wave : 0), all_tiles = (n - 1 + KT) / KT, to_tile = (int)((split + 1) * p.tiles);
     const int last_tile = all_tiles < to_tile ? all_tiles : to_tile;
     constexpr int STEP = APART ? WAVES : 1;   // (apart, every WAVES-th tile is a wave's)
-    const float to_log2 = a.scale * TO_LOG2;
 
     // where a lane's pieces of a tile come from: LDS is filled in order, 16 bytes a lane
     constexpr uint32_t NOWHERE = 0x80000000u;   // (behind the buffer's end: such a piece is zeros)
@@ -251,7 +251,7 @@ __global__ __launch_bounds__(WAVES * 64, (Shape<DT, DP, WAVES, APART, MASK>::PER
     // maximum taken off the scores first, exactly where they are close to it, and scales them afterwards; the wave's other rows get what they
     // would have had (a few more operations a score for all of them).  A row whose scores so far are all -inf or NaN has no reference.
     constexpr float FAR = 4096.0f;
-    const float unit = MASK ? exponents_of(a) : to_log2;
+    const float unit = exponents_of(a);
     const float allowed = 8.0f / unit;   // growth of the maximum that `top` need not follow, while its own steps are small beside that
     auto beyond = [&]() { return fabsf(top) < __builtin_inff() && !(fabsf(top * unit) < FAR); };
     auto off = [&]() { return top == NONE ? RAISE : __builtin_fmaf(-top, unit, RAISE); };
@@ -310,7 +310,7 @@ __global__ __launch_bounds__(WAVES * 64, (Shape<DT, DP, WAVES, APART, MASK>::PER
 #pragma unroll
                 for (int k = 0; k < KB; ++k)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) s[k][i] = __builtin_fmaf(s[k][i], to_log2, adds[k * 32 + 8 * (i / 4) + 4 * half + i % 4]);
+                    for (int i = 0; i < 16; ++i) s[k][i] = __builtin_fmaf(s[k][i], a.scale, adds[k * 32 + 8 * (i / 4) + 4 * half + i % 4]);
                 most = largest(s);
             }
         } else if (now.on != ALL) {   // (the last tile)

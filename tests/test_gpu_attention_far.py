@@ -180,3 +180,39 @@ def test_scores_without_a_maximum_beside_far_ones(pkg, dev):
             assert torch.equal(got[:, rest], want[:, rest]) and torch.isnan(got[:, ~rest]).all()
             bad[:, 1::5, :, 0] = 2.0 ** 64   # +inf: the formula has no value
             assert torch.isnan(pkg.cross_attention(bad, k, v)[:, ~rest]).all()
+
+
+@pytest.mark.parametrize("kind, large", [(torch.float32, 3.3e38), (torch.float32, 2.4e38), (torch.bfloat16, 3.3e38), (torch.bfloat16, 2.4e38), (torch.float16, 65504.0)])
+@pytest.mark.parametrize("size", [(2, 3, 300, 2, 2, 128), (1, 1, 3000, 4, 2, 72), (1, 700, 333, 8, 8, 128), (1, 300, 4000, 1, 1, 128)], ids=str)
+def test_addends_at_the_ends_of_their_type(pkg, dev, size, kind, large):
+    """A state whose finite addend is far above the others' is the result, bit for bit; below all of them it has no part; one for all states changes nothing but by
+    the roundings of sums of that size, which leave the result within the values."""
+    batch, keys = size[0], size[2]
+    for dtype in (torch.bfloat16, torch.float16):
+        q, k, v = inputs(*size, dtype)
+        picked = v[:, 77].repeat_interleave(size[3] // size[4], 1)[:, None]
+        near = torch.finfo(kind).max if kind == torch.float16 else large
+        m = torch.zeros(batch, keys, dtype=kind, device="cuda")
+        m[:, 77] = near
+        assert torch.equal(pkg.cross_attention(q, k, v, key_mask=m), picked.expand_as(q)), "above zeros"
+        m.fill_(-0.99 * near)
+        m[:, 77] = -0.9 * near
+        assert torch.equal(pkg.cross_attention(q, k, v, key_mask=m), picked.expand_as(q)), "above others as low"
+        m.fill_(0.9 * near)
+        m[:, 77] = near
+        assert torch.equal(pkg.cross_attention(q, k, v, key_mask=m), picked.expand_as(q)), "above others as high"
+        m.zero_()
+        m[:, 77] = -0.99 * near
+        off = torch.arange(keys, device="cuda") != 77
+        compared = pkg.cross_attention(q, k, v, key_mask=m)
+        assert torch.equal(compared, pkg.cross_attention(q, k, v, key_mask=torch.where(off, torch.zeros_like(m), -math.inf))), "below all"
+        u = torch.finfo(dtype).eps / 2
+        for every in (0.97 * near, -0.97 * near):
+            got = pkg.cross_attention(q, k, v, key_mask=torch.full_like(m, every)).double()
+            assert torch.isfinite(got).all()
+            wide = v.double().repeat_interleave(size[3] // size[4], 2)
+            slack = (2 * u + 2 * keys * V + 2.0 ** -17) * wide.abs().amax(1, keepdim=True)
+            assert (got >= wide.amin(1, keepdim=True) - slack).all() and (got <= wide.amax(1, keepdim=True) + slack).all()
+        m.fill_(-math.inf)
+        m[:, 5], m[:, 200] = math.inf, 0.0      # an infinite addend has no weight that is a number
+        assert torch.isnan(pkg.cross_attention(q, k, v, key_mask=m)).all()
