@@ -107,7 +107,7 @@ def cross_attention(q: Tensor, k: Tensor, v: Tensor, *, key_lengths: Tensor | No
 
     -> [batch, queries, heads, width], contiguous.  A query over which no state counts, or a finite one whose scores all are -inf, gets zeros, and what the states that do not count hold
     (NaN, infinities) reaches nothing.  Scores, maximum and sums are in binary32, the weights are rounded to q's type for the second product,
-    the result is rounded once; bfloat16 values up to 2^119 / keys cannot overflow its sums.  key_lengths and key_mask are read on the device: a captured graph follows what is written into them.  No gradients: under
+    the result is rounded once; bfloat16 values up to 2^127 / keys cannot overflow its sums.  key_lengths and key_mask are read on the device: a captured graph follows what is written into them.  No gradients: under
     grad mode an input that asks for one is refused, one with a tangent always."""
     compiling = torch.compiler.is_compiling()
     if type(q) is Tensor and q.is_cuda and not compiling:

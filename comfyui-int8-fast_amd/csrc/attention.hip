@@ -244,7 +244,9 @@ __global__ __launch_bounds__(WAVES * 64, (Shape<DT, DP, WAVES, APART, MASK>::PER
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = v16f{};
     float top = NONE, sum = 0.0f, most = NONE;   // (the maxima in the scores' own unit)
-    constexpr float RAISE = DT == I8F_F16 ? 6.0f : 0.0f;   // (binary16 weights lie between 2^6 and 2^14 for the largest: see below)
+    // The largest weight of a row lies between 2^RAISE and 2^(RAISE + 8) (see below).  Binary16's fixed step below 2^-14 asks for 2^14; bfloat16 has the
+    // exponents of binary32, and weights up to 1 leave the sums of their products with values the whole of its range.
+    constexpr float RAISE = DT == I8F_F16 ? 6.0f : -8.0f;
     // A weight is 2^(unit x - unit top), one fused operation on x with unit top rounded beforehand.  That rounding is the same for all weights under
     // one reference, but weights of other tiles were formed under others, and in the end it would leave the type's range: at 2^28 binary16's, at
     // 2^33 bfloat16's.  Below 2^12 it is 2^-13 at the most, less than half of what binary16 rounds a weight by.  A row that is beyond has its
@@ -324,8 +326,8 @@ __global__ __launch_bounds__(WAVES * 64, (Shape<DT, DP, WAVES, APART, MASK>::PER
             most = largest(s);
         }
         most = max_of_halves(most);
-        // The reference of the exponentials follows the maximum only where that has grown by 2^8: the weights are below 2^8 then, which costs
-        // no bits, and the result is divided by their sum either way.  (bf16's values times such weights stay finite up to 2^120 / states.)
+        // The reference of the exponentials follows the maximum only where that has grown by 2^8: the weights are below 2^8 times 2^RAISE then, which
+        // costs no bits, and the result is divided by their sum either way.
         if (__any(most > limit)) {
             const float to = most > limit ? most : top, fade = fading(top, to, unit);   // (a row's bits do not depend on the rows beside it)
             top = to;

@@ -10,7 +10,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_attention import V, counts_of, inputs
+from test_gpu_attention import V, check, counts_of, expected, inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -216,3 +216,19 @@ def test_addends_at_the_ends_of_their_type(pkg, dev, size, kind, large):
         m.fill_(-math.inf)
         m[:, 5], m[:, 200] = math.inf, 0.0      # an infinite addend has no weight that is a number
         assert torch.isnan(pkg.cross_attention(q, k, v, key_mask=m)).all()
+
+
+@pytest.mark.parametrize("queries, keys", [(200, 300), (3, 300), (1, 1), (1, 3000), (700, 333)])
+def test_values_at_the_ends_of_bfloat16(pkg, dev, queries, keys):
+    """Values of 2^127 / keys whose weights grow by just less than the running maximum lets them, equal ones (their mean is themselves, but for keys roundings of
+    2^-24 in two sums and 2^-8 at the end); and values around 2^-122, whose products with weights reach below binary32's normal numbers."""
+    q, k, v = inputs(2, queries, keys, 4, 2, 64, torch.bfloat16)
+    on = torch.arange(keys, device="cuda").expand(2, -1) % 3 != 1
+    for mask in (None, on, torch.where(on, 0.25, -math.inf)):
+        grow = torch.linspace(0.0, 1.0, keys, device="cuda")[None, :, None, None] * 5.0
+        large = torch.full_like(v, 2.0 ** 127 / 2 ** math.ceil(math.log2(keys)))
+        got = pkg.cross_attention(torch.ones_like(q), (grow / 8).expand(2, -1, 2, 64).bfloat16(), large, key_mask=mask)
+        off = ((got.double() / large[0, 0, 0, 0].double()) - 1.0).abs().max().item()
+        assert off <= 2.0 ** -8 + 2 * keys * V + 2.0 ** -20, off
+        tiny = (v.double() * 2.0 ** -122).bfloat16()
+        check(pkg.cross_attention(q, k, tiny, key_mask=mask), expected(q, k, tiny, key_mask=mask))
