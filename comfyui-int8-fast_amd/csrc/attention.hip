@@ -710,6 +710,19 @@ extern "C" int64_t i8f_attention_workspace_bytes(const i8f_attention_args *args)
     return plan_of(a.batch, a.queries, a.keys, a.heads, a.kv_heads, a.width).partial_bytes + bytes[0] + bytes[1] + bytes[2];
 }
 
+// How a call of these arguments is cut, for tests to know which form they reach: waves of a workgroup, whether they take the states apart, splits
+// of the states, the kernel's width.
+extern "C" int i8f_internal_attention_plan(const i8f_attention_args *args, int64_t *waves, int64_t *apart, int64_t *splits, int64_t *padded) {
+    using namespace i8f;
+    if (!args || !waves || !apart || !splits || !padded) return I8F_ERR_INVALID;
+    const i8f_attention_args &a = *args;
+    if (int rc = validate(a)) return rc;
+    if (!a.batch || !a.queries || !a.keys || !a.heads) return I8F_ERR_INVALID;   // (nothing is cut)
+    const Plan p = plan_of(a.batch, a.queries, a.keys, a.heads, a.kv_heads, a.width);
+    *waves = p.waves, *apart = p.apart, *splits = p.splits, *padded = p.padded;
+    return I8F_OK;
+}
+
 extern "C" int i8f_attention(const i8f_attention_args *args, void *stream) {
     using namespace i8f;
     if (!args) return I8F_ERR_INVALID;
