@@ -571,7 +571,8 @@ struct Plan {
     bool apart;               // the waves of a workgroup take the states in turn
     int waves;                // of a workgroup
     int64_t row_tiles, splits, tiles;
-    int64_t partial_bytes;    // of results and statistics of the splits
+    int64_t partials;         // floats of the splits' results, behind which two to a row are their statistics
+    int64_t partial_bytes;    // of both, whole pieces of 16 (the copies lie behind them)
 };
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
@@ -599,7 +600,8 @@ Plan plan_of(int64_t batch, int64_t queries, int64_t keys, int64_t heads, int64_
     p.tiles = round_up((all + p.splits - 1) / p.splits, p.apart ? p.waves : 1);
     if (p.tiles < 1) p.tiles = 1;
     p.splits = all ? (all + p.tiles - 1) / p.tiles : 1;
-    p.partial_bytes = p.splits > 1 ? sets * p.splits * rows * (p.padded + 2) * 4 : 0;
+    const int64_t results = p.splits > 1 ? sets * p.splits * rows : 0;
+    p.partials = results * p.padded, p.partial_bytes = round_up((p.partials + 2 * results) * 4, 16);
     return p;
 }
 
@@ -744,7 +746,7 @@ extern "C" int i8f_attention(const i8f_attention_args *args, void *stream) {
     p.wide_out = a.width % 8 == 0 && (uintptr_t)a.out % 16 == 0;
     p.by_share = Divisor(p.share), p.by_row_tiles = Divisor(p.row_tiles), p.by_splits = Divisor(p.splits), p.by_kv_heads = Divisor((uint32_t)a.kv_heads);
     p.partial = (float *)a.workspace;
-    p.stats = p.partial ? p.partial + plan.partial_bytes / 4 / (plan.padded + 2) * plan.padded : nullptr;
+    p.stats = p.partial ? p.partial + plan.partials : nullptr;
     int64_t bytes[3];
     const int which = to_pack(a, bytes);
     if (which) {

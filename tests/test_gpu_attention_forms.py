@@ -95,3 +95,14 @@ def test_calls_of_every_form_agree_bit_for_bit(pkg, L, dev, form, size):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, eager), n
+
+
+@pytest.mark.parametrize("size", [(1, 1, 1536, 1, 1, 37), (1, 1, 4097, 1, 1, 37), (1, 3, 5000, 1, 1, 33), (1, 5, 3000, 3, 1, 199)], ids=str)
+def test_copies_behind_an_odd_number_of_split_rows(pkg, dev, size):
+    for dtype in (torch.bfloat16, torch.float16):
+        q, k, v = inputs(*size, dtype)
+        got = pkg.cross_attention(q, k, v)
+        check(got, expected(q, k, v))
+        wide = -(-size[-1] // 8) * 8
+        whole = [torch.nn.functional.pad(t, (0, wide - size[-1])) for t in (q, k, v)]
+        assert torch.equal(pkg.cross_attention(*whole, scale=size[-1] ** -0.5)[..., :size[-1]], got)
