@@ -585,10 +585,13 @@ Plan plan_of(int64_t batch, int64_t queries, int64_t keys, int64_t heads, int64_
     // 4096 28 and 35; 256 heads of 64, 77 rows over 512 11.7 and 15.0.
     p.apart = rows <= 32 || (sets * ((rows + 31) / 32) <= 128 && keys <= 2048);
     p.waves = p.apart && p.padded > 128 ? 2 : 4;
-    // Eight waves read the states half as often, which is energy, and the card runs at its power limit in long calls; four start and end beside
-    // another workgroup.  us with four and eight for 40 heads of 128: 8192 x 8192 1338 and 1284, 32768 x 4096 2603 and 2546, 32768 x 2048 1333 and
-    // 1333, 32768 x 512 419 and 449, 4096 x 4096 336 and 356.
-    if (!p.apart && (p.padded == 64 || p.padded == 128) && keys >= 4096 && sets * ((rows + 255) / 256) >= 1024) p.waves = 8;
+    // Eight waves read the states half as often, which is energy, and the card runs at its power limit in long calls; but theirs is the CU's only
+    // workgroup, so that rows filled up to 256 and a last round of few workgroups cost more than that.  us with four and eight, heads of 128, (batch,
+    // head) pairs x rows x states: 8 x 32768 x 4096 517 and 503, 32 x 8192 x 8192 1022 and 1005, 40 x 8192 x 8192 1270 and 1258, 4096 x 200 x 4096 2509 and
+    // 2462; 40 x 32768 x 2048 1333 and 1333, 40 x 32768 x 512 419 and 449; with 5.5 rounds, 176 x 2048 x 4096, 739 and 757; with 16.03, 456 x 2300 x 4096,
+    // 2156 and 2210; filled up, 2048 x 300 x 4096 1757 and 2189, 1024 x 64 x 4096 401 and 571.  Heads of 64: 40 x 8192 x 8192 746 and 773.
+    const int64_t wide = sets * ((rows + 255) / 256);
+    if (!p.apart && p.padded == 128 && keys >= 4096 && wide >= 1024 && round_up(rows, 256) == round_up(rows, 128) && (round_up(wide, 256) - wide) * 32 <= wide) p.waves = 8;
     const int64_t to_group = p.apart ? 32 : 32 * p.waves;
     p.row_tiles = (rows + to_group - 1) / to_group;
     const int64_t tile = p.apart ? 32 : 64, all = (keys + tile - 1) / tile, groups = sets * p.row_tiles;
@@ -632,7 +635,7 @@ int launch_tiles(const Launch &p, int64_t groups, hipStream_t st) {
 template <int DT, int DP, bool MASK>
 int launch_masked(const Launch &p, const Plan &plan, int64_t groups, hipStream_t st) {
     if (plan.apart) return launch_tiles<DT, DP, DP <= 128 ? 4 : 2, true, MASK>(p, groups, st);
-    if constexpr (DP == 64 || DP == 128) {
+    if constexpr (DP == 128) {
         if (plan.waves == 8) return launch_tiles<DT, DP, 8, false, MASK>(p, groups, st);
     }
     return launch_tiles<DT, DP, 4, false, MASK>(p, groups, st);

@@ -8,7 +8,7 @@ SIZES = {
     "apart, split": [(2, 2, 3001, 4, 2, w) for w in WIDTHS],
     "together": [(3, 150, 203, 10, 5, w) for w in WIDTHS],
     "together, split": [(3, 150, 705, 10, 5, w) for w in WIDTHS],
-    "eight": [(2, 4200, 4113, 32, 32, w) for w in (64, 128, 120, 37)],
+    "eight": [(2, 4050, 4113, 32, 32, w) for w in (128, 120, 101)],
 }
 
 
