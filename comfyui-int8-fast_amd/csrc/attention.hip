@@ -24,6 +24,7 @@
 
 #include "divisor.hpp"
 #include "dma.hpp"
+#include "extents.hpp"
 #include "i8f_common.hpp"
 
 #include "../../include/i8f_attention.h"
@@ -664,20 +665,6 @@ int launch(const Launch &p, const Plan &plan, hipStream_t st) {
     }
 }
 
-// The elements that a strided tensor reaches to from its first one, 0 for one without elements, -1 past 2^62.
-int64_t extent(std::initializer_list<std::pair<int64_t, int64_t>> dims) {
-    __int128 last = 0;
-    for (auto [size, stride] : dims) {
-        if (size < 1) return 0;
-        last += (__int128)(size - 1) * stride;
-    }
-    return last >= ((__int128)1 << 62) ? -1 : (int64_t)last + 1;
-}
-
-bool overlap(const void *a, int64_t na, const void *b, int64_t nb) {
-    return na > 0 && nb > 0 && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
-}
-
 int validate(const i8f_attention_args &a) {
     if (a.batch < 0 || a.queries < 0 || a.keys < 0 || a.heads < 0 || a.kv_heads < 0 || a.width < 1) return I8F_ERR_INVALID;
     if (a.dtype != I8F_BF16 && a.dtype != I8F_F16) return valid_dtype(a.dtype) ? I8F_ERR_UNSUPPORTED : I8F_ERR_INVALID;
@@ -691,15 +678,18 @@ int validate(const i8f_attention_args &a) {
         if (n > 1 << 30) return I8F_ERR_UNSUPPORTED;
     const int64_t rows = a.batch * a.queries;
     if (rows && a.heads > 0x7fffffff / rows) return I8F_ERR_UNSUPPORTED;   // (rows are counted in 32 bits)
-    if (a.key_lengths && a.lengths_type != 0 && a.lengths_type != 1) return I8F_ERR_INVALID;
-    if (a.key_mask && (a.mask_type < I8F_MASK_BYTES || a.mask_type > I8F_MASK_F32 || a.mask_batch < 0 || a.mask_key < 0)) return I8F_ERR_INVALID;
+    const int length_size = a.lengths_type ? 8 : 4, mask_size = a.mask_type == I8F_MASK_BYTES ? 1 : a.mask_type == I8F_MASK_F32 ? 4 : 2;
+    if (a.key_lengths && ((a.lengths_type != 0 && a.lengths_type != 1) || (uintptr_t)a.key_lengths % length_size)) return I8F_ERR_INVALID;
+    if (a.key_mask && ((uintptr_t)a.key_mask % mask_size || a.mask_type < I8F_MASK_BYTES || a.mask_type > I8F_MASK_F32 || a.mask_batch < 0 || a.mask_key < 0)) return I8F_ERR_INVALID;
     const int64_t out = rows * a.heads * a.width, q = extent({{a.batch, a.q_batch}, {a.queries, a.q_token}, {a.heads, a.q_head}, {a.width, 1}});
     const int64_t k = extent({{a.batch, a.k_batch}, {a.keys, a.k_token}, {a.kv_heads, a.k_head}, {a.width, 1}});
     const int64_t v = extent({{a.batch, a.v_batch}, {a.keys, a.v_token}, {a.kv_heads, a.v_head}, {a.width, 1}});
-    if (q < 0 || k < 0 || v < 0) return I8F_ERR_UNSUPPORTED;
+    const int64_t mask = a.key_mask ? extent({{a.batch, a.mask_batch}, {a.keys, a.mask_key}}) : 0;
+    if (q < 0 || k < 0 || v < 0 || mask < 0) return I8F_ERR_UNSUPPORTED;
     if (!out) return I8F_OK;   // (nothing to write: the pointers may be NULL)
     if (!a.q || !a.out || (a.keys && (!a.k || !a.v))) return I8F_ERR_INVALID;
     if (overlap(a.out, 2 * out, a.q, 2 * q) || overlap(a.out, 2 * out, a.k, 2 * k) || overlap(a.out, 2 * out, a.v, 2 * v)) return I8F_ERR_INVALID;
+    if ((a.key_lengths && overlap(a.out, 2 * out, a.key_lengths, length_size * a.batch)) || overlap(a.out, 2 * out, a.key_mask, mask_size * mask)) return I8F_ERR_INVALID;
     return I8F_OK;
 }
 

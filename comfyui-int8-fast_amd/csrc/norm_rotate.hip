@@ -5,6 +5,7 @@
 #include <utility>
 
 #include "divisor.hpp"
+#include "extents.hpp"
 #include "i8f_common.hpp"
 
 #include "../../include/i8f_attention.h"
@@ -288,20 +289,6 @@ int launch(const i8f_norm_rotate_args &a, const Groups &groups, hipStream_t st) 
     return a.axes && a.apart ? launch_lanes<DT, true>(a, groups, st) : launch_lanes<DT, false>(a, groups, st);
 }
 
-// The elements that a strided tensor reaches to from its first one, -1 past 2^62.
-int64_t extent(std::initializer_list<std::pair<int64_t, int64_t>> dims) {
-    __int128 last = 0;
-    for (auto [size, stride] : dims) {
-        if (size < 1) return 0;
-        last += (__int128)(size - 1) * stride;
-    }
-    return last >= ((__int128)1 << 62) ? -1 : (int64_t)last + 1;
-}
-
-bool overlap(const void *a, int64_t na, const void *b, int64_t nb) {
-    return na > 0 && nb > 0 && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
-}
-
 int validate(const i8f_norm_rotate_args &a, const i8f_heads *groups, int n) {
     if (a.batch < 0 || a.tokens < 0 || a.width < 1 || !valid_dtype(a.dtype) || n < 0 || (n && !groups)) return I8F_ERR_INVALID;
     if (a.norm && !(a.eps >= 0.0f)) return I8F_ERR_INVALID;
@@ -309,6 +296,8 @@ int validate(const i8f_norm_rotate_args &a, const i8f_heads *groups, int n) {
     if (a.axes > I8F_MAX_AXES || n > I8F_MAX_HEAD_GROUPS || a.width > 256) return I8F_ERR_UNSUPPORTED;
     if (a.batch > 0x7fffffff || a.tokens > 0x7fffffff || (a.batch && a.tokens > 0x7fffffff / a.batch)) return I8F_ERR_UNSUPPORTED;
     const bool any = a.batch && a.tokens;
+    const int64_t position_size = a.positions_type == I8F_POSITION_I32 || a.positions_type == I8F_POSITION_F32 ? 4 : 8;
+    int64_t positions = 0, rates = 0;   // elements
     if (a.axes) {
         if (a.positions_type < I8F_POSITION_I32 || a.positions_type > I8F_POSITION_F64 || a.first_pair[0] != 0) return I8F_ERR_INVALID;
         for (int x = 0; x < a.axes; ++x)
@@ -316,6 +305,9 @@ int validate(const i8f_norm_rotate_args &a, const i8f_heads *groups, int n) {
         if (2 * (int64_t)a.first_pair[a.axes] > a.width) return I8F_ERR_INVALID;
         if (any && (!a.rates || !a.positions)) return I8F_ERR_INVALID;
         if (a.position_batch < 0 || a.position_token < 0 || a.position_axis < 0) return I8F_ERR_INVALID;
+        if ((uintptr_t)a.positions % position_size || (uintptr_t)a.rates % 8) return I8F_ERR_INVALID;
+        positions = extent({{a.batch, a.position_batch}, {a.tokens, a.position_token}, {a.axes, a.position_axis}}), rates = a.first_pair[a.axes];
+        if (positions < 0) return I8F_ERR_UNSUPPORTED;
     }
     const int64_t size = (int64_t)dtype_size(a.dtype);
     int64_t in[I8F_MAX_HEAD_GROUPS], out[I8F_MAX_HEAD_GROUPS];
@@ -328,12 +320,17 @@ int validate(const i8f_norm_rotate_args &a, const i8f_heads *groups, int n) {
         out[i] = extent({{a.batch, a.tokens * g.heads * a.width}, {a.tokens, g.heads * a.width}, {g.heads, a.width}, {a.width, 1}});
         if (in[i] < 0 || out[i] < 0) return I8F_ERR_UNSUPPORTED;
         if (in[i] && (!g.x || !g.out)) return I8F_ERR_INVALID;
-        if (((uintptr_t)g.x | (uintptr_t)g.out) % size) return I8F_ERR_INVALID;
+        if (((uintptr_t)g.x | (uintptr_t)g.out) % size || (g.weight && (uintptr_t)g.weight % dtype_size(g.weight_dtype))) return I8F_ERR_INVALID;
     }
-    for (int i = 0; i < n; ++i)
-        for (int j = 0; j < n; ++j)   // (a head is written while other waves read)
+    for (int i = 0; i < n; ++i) {     // (a head is written while other waves read)
+        if (overlap(groups[i].out, out[i] * size, a.positions, positions * position_size) || overlap(groups[i].out, out[i] * size, a.rates, rates * 8)) return I8F_ERR_INVALID;
+        for (int j = 0; j < n; ++j) {
+            const int64_t weight = groups[j].weight ? a.width * (int64_t)dtype_size(groups[j].weight_dtype) : 0;
+            if (overlap(groups[i].out, out[i] * size, groups[j].weight, weight)) return I8F_ERR_INVALID;
             if (overlap(groups[i].out, out[i] * size, groups[j].x, in[j] * size) || (i != j && overlap(groups[i].out, out[i] * size, groups[j].out, out[j] * size)))
                 return I8F_ERR_INVALID;
+        }
+    }
     return I8F_OK;
 }
 

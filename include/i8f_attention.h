@@ -1,7 +1,8 @@
 /*
  * What lies between the projections of an attention block, beside the layers of i8f.h and with its conventions (device pointers owned by
  * the caller, the caller's stream, negative i8f_status on errors, arguments checked on the host before anything is launched): the norm of
- * every head of queries and keys, the rotation by their positions, and the attention over an encoder's states.
+ * every head of queries and keys, the rotation by their positions, and the attention over an encoder's states.  Every pointer lies on an element of
+ * its type, and no result on an input.
  */
 #ifndef I8F_ATTENTION_H
 #define I8F_ATTENTION_H
