@@ -684,6 +684,8 @@ int validate(const i8f_attention_args &a) {
     const int64_t out = rows * a.heads * a.width, q = extent({{a.batch, a.q_batch}, {a.queries, a.q_token}, {a.heads, a.q_head}, {a.width, 1}});
     const int64_t k = extent({{a.batch, a.k_batch}, {a.keys, a.k_token}, {a.kv_heads, a.k_head}, {a.width, 1}});
     const int64_t v = extent({{a.batch, a.v_batch}, {a.keys, a.v_token}, {a.kv_heads, a.v_head}, {a.width, 1}});
+    // (expanded operands have few elements and states without end, whose copies are counted in 64 bits)
+    if ((__int128)a.batch * a.keys * a.kv_heads * 512 > (__int128)1 << 58) return I8F_ERR_UNSUPPORTED;
     const int64_t mask = a.key_mask ? extent({{a.batch, a.mask_batch}, {a.keys, a.mask_key}}) : 0;
     if (q < 0 || k < 0 || v < 0 || mask < 0) return I8F_ERR_UNSUPPORTED;
     if (!out) return I8F_OK;   // (nothing to write: the pointers may be NULL)

@@ -69,7 +69,7 @@ int i8f_norm_rotate(const i8f_norm_rotate_args *args, const i8f_heads *groups, i
  *   workspace    any contents, 16-byte aligned, i8f_attention_workspace_bytes() of these arguments (which looks at all but workspace and
  *                key_lengths' and key_mask's contents); less, or NULL, is refused where that is not 0.  It overlaps nothing else, and calls that overlap in
  *                time do not share it.
- * batch * queries * heads is below 2^31, keys at most 2^30; more workgroups than a launch has (2^24 of 128 rows, of 32 where there are fewer) are
+ * batch * queries * heads is below 2^31, keys at most 2^30, batch * keys * kv_heads at most 2^49; more workgroups than a launch has (2^24 of 128 rows, of 32 where there are fewer) are
  * I8F_ERR_UNSUPPORTED.
  */
 typedef enum i8f_key_mask { I8F_MASK_BYTES = 0, I8F_MASK_BF16 = 1, I8F_MASK_F16 = 2, I8F_MASK_F32 = 3 } i8f_key_mask;
