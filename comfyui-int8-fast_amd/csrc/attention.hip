@@ -535,11 +535,13 @@ __global__ __launch_bounds__(256) void join_kernel(const Launch p) {
         if (tid * 4 + i < a.width) store_from_f32<DT>(a.out, to + i, total == 0.0f ? 0.0f : o[i] / total);
 }
 
-// [batch, tokens, heads, width] of any strides and alignment as contiguous rows of whole 16-byte pieces, the rest of them zeros.
+// [batch, tokens, heads, width] of any strides and alignment as rows of whole 16-byte pieces, the rest of them zeros, in the same order; or with
+// a head's tokens side by side where a tile's rows would lie farther apart than the kernel's 32-bit offsets reach.
 struct Pack {
     const uint16_t *x;
     uint16_t *out;
     int64_t rows, tokens, heads, batch_stride, token_stride, head_stride;
+    int64_t out_token, out_head;
     int width, padded;
 };
 struct Packs {
@@ -557,7 +559,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const Packs packs) {
         for (int i = 0; i < 8; ++i) v[i] = e + i < p.width ? x[i] : (uint16_t)0;
         uint4 o;
         __builtin_memcpy(&o, v, 16);
-        *(uint4 *)(p.out + at * 8) = o;
+        *(uint4 *)(p.out + b * p.tokens * p.heads * p.padded + t * p.out_token + h * p.out_head + e) = o;
     }
 }
 
@@ -752,8 +754,10 @@ extern "C" int i8f_attention(const i8f_attention_args *args, void *stream) {
         auto pack = [&](int i, const void *&x, int64_t tokens, int64_t heads, int64_t &batch_stride, int64_t &token_stride, int64_t &head_stride) {
             if (!(which >> i & 1)) return;
             const int64_t padded = round_up(a.width, 8);
-            packs.p[count++] = {(const uint16_t *)x, (uint16_t *)at, a.batch * tokens * heads, tokens, heads, batch_stride, token_stride, head_stride, (int)a.width, (int)padded};
-            x = at, head_stride = padded, token_stride = heads * padded, batch_stride = tokens * heads * padded;
+            const bool apart = heads * padded > MOST_STRIDE;
+            const int64_t out_token = apart ? padded : heads * padded, out_head = apart ? tokens * padded : padded;
+            packs.p[count++] = {(const uint16_t *)x, (uint16_t *)at, a.batch * tokens * heads, tokens, heads, batch_stride, token_stride, head_stride, out_token, out_head, (int)a.width, (int)padded};
+            x = at, head_stride = out_head, token_stride = out_token, batch_stride = tokens * heads * padded;
             most = bytes[i] > most ? bytes[i] : most;
             at += bytes[i];
         };

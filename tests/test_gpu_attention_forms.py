@@ -106,3 +106,15 @@ def test_copies_behind_an_odd_number_of_split_rows(pkg, dev, size):
         wide = -(-size[-1] // 8) * 8
         whole = [torch.nn.functional.pad(t, (0, wide - size[-1])) for t in (q, k, v)]
         assert torch.equal(pkg.cross_attention(*whole, scale=size[-1] ** -0.5)[..., :size[-1]], got)
+
+
+def test_copies_of_more_heads_than_a_tile_reaches_over(pkg, L, dev):
+    """Odd widths of so many heads that 63 tokens of all of them are more than 2^31 bytes: tiles of 64 states reach over them by 32-bit offsets."""
+    size = (1, 33, 64, 67000, 67000, 255)
+    assert form_of(L, size)[0] == "together" and 63 * 67000 * 256 * 2 > 1 << 31
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v = (torch.empty(1, n, 67000, 255, dtype=torch.bfloat16, device="cuda").normal_(generator=g) for n in (33, 64, 64))
+    got = pkg.cross_attention(q, k, v)
+    for heads in (slice(0, 2), slice(40000, 40002), slice(66998, 67000)):
+        part = [t[:, :, heads] for t in (q, k, v)]
+        check(got[:, :, heads].contiguous(), expected(*part))
