@@ -29,14 +29,30 @@ __device__ __forceinline__ double position_at(const void *p, int type, int64_t i
 
 // Cosine and sine of pair j's angle at the token's positions.  The turns are a product in binary64 (rounded by half a unit of 2^-53 of its
 // size: a position of 2^31 leaves 2^-24 turns) and what is left of them behind the whole ones is at most a half, so that binary32 holds it to 2^-26.
-// The hardware's functions take turns: over all of -1/2 ... 1/2 in steps of 2^-25 they are within 1.26e-7 (2^-22.9) of sine and cosine.
+// The hardware's functions take turns: over all of -1/2 ... 1/2 in steps of 2^-25 they are within 1.26e-7 (2^-22.9) of sine and cosine.  That is
+// far below the steps of 16 bits.  For heads in binary32 quarters are taken off, so that what is left of the angle, at most pi/4, is off by 2^-25, and
+// the series of sine and cosine, to x^9 and x^10, are within 2^-23.4 together with it.
+template <int DT>
 __device__ __forceinline__ void turn(const i8f_norm_rotate_args &a, const double (&pos)[I8F_MAX_AXES], int j, float &c, float &s) {
     double p = pos[0];
 #pragma unroll
     for (int x = 1; x < I8F_MAX_AXES; ++x) p = x < a.axes && j >= a.first_pair[x] ? pos[x] : p;
     const double t = p * a.rates[j];
-    const float left = (float)(t - __builtin_rint(t));
-    c = __builtin_amdgcn_cosf(left), s = __builtin_amdgcn_sinf(left);
+    if constexpr (DT != I8F_F32) {
+        const float left = (float)(t - __builtin_rint(t));
+        c = __builtin_amdgcn_cosf(left), s = __builtin_amdgcn_sinf(left);
+    } else {
+        const double quarters = __builtin_rint(4.0 * t);
+        const float x = (float)(__builtin_fma(quarters, -0.25, t) * 6.283185307179586476925), z = x * x;
+        const float quarter = (float)(quarters - 4.0 * __builtin_rint(0.25 * quarters));   // -2 ... 2
+        float sine = __builtin_fmaf(z, 1.0f / 362880, -1.0f / 5040), cosine = __builtin_fmaf(z, -1.0f / 3628800, 1.0f / 40320);
+        sine = __builtin_fmaf(__builtin_fmaf(sine, z, 1.0f / 120), z, -1.0f / 6);
+        cosine = __builtin_fmaf(__builtin_fmaf(cosine, z, -1.0f / 720), z, 1.0f / 24);
+        sine = __builtin_fmaf(x * z, sine, x), cosine = __builtin_fmaf(z, __builtin_fmaf(z, cosine, -0.5f), 1.0f);
+        const bool odd = fabsf(quarter) == 1.0f, back = fabsf(quarter) == 2.0f;
+        c = odd ? sine : cosine, s = odd ? cosine : sine;
+        c = quarter == 1.0f || back ? -c : c, s = quarter == -1.0f || back ? -s : s;
+    }
 }
 
 __device__ __forceinline__ void token_positions(const i8f_norm_rotate_args &a, unsigned b, unsigned t, double (&pos)[I8F_MAX_AXES]) {
@@ -185,7 +201,7 @@ __global__ __launch_bounds__(256) void norm_rotate_kernel(const unsigned first, 
         token_positions(a, b, t, pos);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (pair + i < pairs) turn(a, pos, pair + i, c[i], s[i]);
+            if (pair + i < pairs) turn<DT>(a, pos, pair + i, c[i], s[i]);
     }
     int before = 0;
     for (int g = 0; g < groups.n; ++g) {
