@@ -54,7 +54,7 @@ def norm_heads(xs, weights=None, *, eps: float = 1e-6, rotary: RotaryAxes | None
     weights:   [width] of their type or float32, one for each of xs (None for none), or None for none at all.
     positions: [tokens, axes], or [batch, tokens, axes] (a batch of 1 for all), int32, int64, float32 or float64, on xs' device.
 
-    Everything is computed in binary32, the angles in binary64, and rounded once.  The results are contiguous.  No gradients: under grad
+    Everything is computed in binary32 (squares too, whose sum must stay within it), the angles in binary64, and rounded once.  The results are contiguous.  No gradients: under grad
     mode an input that asks for one is refused, one with a tangent always."""
     single = isinstance(xs, Tensor)
     xs = (xs,) if single else tuple(xs)
@@ -105,10 +105,12 @@ def cross_attention(q: Tensor, k: Tensor, v: Tensor, *, key_lengths: Tensor | No
                  or the lowest value of its type does not count.  With lengths both hold.
     scale:       positive, at most 2^126; width ** -0.5 by default.
 
-    -> [batch, queries, heads, width], contiguous.  A query over which no state counts, or a finite one whose scores all are -inf, gets zeros, and what the states that do not count hold
-    (NaN, infinities) reaches nothing.  Scores, maximum and sums are in binary32, the weights are rounded to q's type for the second product,
-    the result is rounded once; bfloat16 values up to 2^127 / keys cannot overflow its sums.  key_lengths and key_mask are read on the device: a captured graph follows what is written into them.  No gradients: under
-    grad mode an input that asks for one is refused, one with a tangent always."""
+    -> [batch, queries, heads, width], contiguous.  A query over which no state counts, or a finite one whose scores all are -inf, gets zeros, and what
+    the states that do not count hold (NaN, infinities) reaches nothing.  Scores (with their addends), maximum and sums are in binary32, and finite
+    scores of any size are the formula's; one that passes binary32 upwards gives NaN.  The weights are rounded to q's type for the second product, the
+    result is rounded once; bfloat16 values up to 2^127 / keys cannot overflow its sums.  A row's bits do not depend on the rows beside it.  key_lengths
+    and key_mask are read on the device: a captured graph follows what is written into them.  No gradients: under grad mode an input that asks for
+    one is refused, one with a tangent always."""
     compiling = torch.compiler.is_compiling()
     if type(q) is Tensor and q.is_cuda and not compiling:
         out = _lib.host().attention(q, k, v, key_lengths, key_mask, scale)
@@ -126,7 +128,8 @@ def forward_cross_attention(x: Tensor, context: Tensor | None, to_q, to_k, to_v,
                             key_mask: Tensor | None = None, scale: float | None = None, gate: Tensor | None = None, residual: Tensor | None = None) -> Tensor:
     """An attention block from its quantised projections to the residual stream: to_out(attention(to_q(x), to_k(context), to_v(context))).
 
-    x [batch, queries, features], context [batch, keys, features] or None for x itself; layers that read one tensor quantise it once
+    x [batch, queries, features], context [batch, keys, features] or None for x itself, in the types of the attention (bfloat16 or float16: float32 is
+    refused behind the projections); layers that read one tensor quantise it once
     (int8_quant.forward_fanout).  q_weight, k_weight [head width]: the norms of the heads (both or neither); rotary with `positions` of x's tokens
     and `context_positions` of the context's (None: its keys are not turned; without a context those of x).  gate and residual as
     Linear.forward takes them, applied behind to_out; without to_out the heads side by side are returned.  No gradients: under grad mode an

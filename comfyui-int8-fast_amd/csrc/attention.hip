@@ -7,12 +7,15 @@
 // O^T = V^T P^T, the contraction index being free to run in the order in which a lane happens to hold the states; the first operand comes
 // out of row-major V by LDS reads that transpose (ds_read_b64_tr_b16).
 //
-// What bounds it.  Long calls the card's power: 8192 x 8192, 40 heads of 128, 1270 us, 1.08 PFLOP/s, the matrix unit 53 % busy at 1.95 of 2.4 GHz
-// (eight waves; four: 55 % at 1.8 GHz, 1340 us); 1.58 PFLOP/s is what a large library product reaches.  A wave's 64 states are 32 matrix
-// instructions of 32 cycles and 124 vector instructions of arithmetic (32 exponentials among them, 8 cycles each), which share the issue with
-// them.  Calls over few states have the traffic of their rows on top: 32760 x 512 420 us (0.82), over 64 states 171 to 181 us, 3.8 TB/s; the
-// clock is at 1.72 GHz there as well.  One
-// token memory: 65536 states of 8 heads 58 us with the join, 4.6 TB/s; small ones the latencies of a launch (5 us).
+// What bounds it.  Long calls the matrix unit and the other vector instructions one after the other: for 8192 x 8192, 40 heads of 128, a wave's 64
+// states take 1930 cycles of its SIMD, 1024 of them 32 matrix instructions, 755 the other 156 vector instructions (32 exponentials among them),
+// which hardly run beside the products of the SIMD's other wave; the LDS is read in 27 % of them.  The clock is at 1.9 of 2.4 GHz besides.  1243 to
+// 1340 us over cards and runs, 1.03 to 1.11 PFLOP/s; 1.58 is what a large library product reaches.  Calls over few states have the traffic of their rows on
+// top, at the start and the end of a workgroup, when it multiplies nothing: 32760 x 512 408 to 446 us (0.77 to 0.84 PFLOP/s), over 64 states 171 to
+// 181 us, 3.8 TB/s.  One token memory: 65536 states of 8 heads 58 us with the join, 4.6 TB/s; small ones the latencies of a launch (5 us).  Widths
+// above 128 one workgroup of four waves to a CU: 4096 x 1024, 16 heads of 256, 92 to 97 us (0.71 to 0.75 PFLOP/s).  Widths that are no whole pieces
+// the copies in front on top: 4096 x 4096, 40 heads of 100, 378 us (0.71 PFLOP/s; heads of 128 in
+// binary16, whole pieces, 350 to 357: 0.97), one query over 257 states, 16 heads of 37, 10.4 us.
 // Measured and not kept: 64 rows to a wave, which halve the LDS reads but leave one wave to a SIMD and a third of the vector instructions
 // moving scores between register files (1450 us for 8192 x 8192); tiles of 32 states with three waves to a SIMD (405 against 419 us for 32768 x 512,
 // 1320 against 1290 for 8192 x 8192, 82 to 107 for 1024 x 4096 of 32 heads); LDS reads three products ahead of their use in a fixed order (no
@@ -63,7 +66,9 @@ __device__ __forceinline__ v16f mfma(v8s a, v8s b, v16f c) {
     if constexpr (DT == I8F_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
-// two weights rounded to the type, and their sum as they were rounded added to `sum`
+// Two weights rounded to the type, and their sum as they were rounded added to `sum`.  The matrix unit takes operands of 16 bits: with u half a step
+// each weight is off by u of itself at the most, either way, and what is divided by is the sum of what was multiplied, so that equal values stay what they are.
+// Weights in 32 bits would be a second product with the remainders: 16 more matrix instructions to a step's 32.
 template <int DT>
 __device__ __forceinline__ uint32_t round_weights(float lo, float hi, float &sum) {
     if constexpr (DT == I8F_BF16) {

@@ -163,8 +163,8 @@ __device__ __forceinline__ float sum_of_lanes(float v) {
 
 // Memory bounds it: a head is read once and written once, its elements stay in registers between, the sum goes over the lanes that hold them,
 // and what a token's heads share (positions, sine and cosine, the norm's weights) is made once for the passes of a wave.  32760 tokens of 40 + 40 heads
-// of 128 225 us, 5.95 TB/s (a copy of 2 GiB 4.97); 4096 of 30 + 30 23.6 us, 5.3; 8192 of 32 x 64 in
-// binary32 22.8 us, 5.9; 4071 of 16 heads of 72, pairs apart, 8 to 9 us, 2.2 (10 of 16 lanes hold elements); a few tokens 4 to 5 us, a launch and the
+// of 128 222 to 225 us, 6.0 TB/s (256 us when each launch starts on its own; a copy of 2 GiB 4.97 TB/s); 4096 of 30 + 30 23 us, 5.5; 8192 of 32 x 64 in
+// binary32 23.2 us, 5.8; 4071 of 16 heads of 72, pairs apart, 8 to 9 us, 2.2 (10 of 16 lanes hold elements); a few tokens 4 to 5 us, a launch and the
 // chain of position, angle and head.  Eight elements to a lane, so that a head of 128 in 16 bits is one
 // 16-byte access of 16 lanes.  Measured and not kept: everything that a wave reads requested before the first of it is used (4.1 us for 2 tokens as
 // now, 300 for the 32760).
@@ -268,8 +268,9 @@ int launch_passes(const i8f_norm_rotate_args &a, const Groups &groups, hipStream
     int64_t passes = 0;
     for (int i = 0; i < groups.n; ++i) passes += (groups.g[i].heads + 64 / LPH - 1) / (64 / LPH);
     if (passes > 0x7fffffff) return I8F_ERR_UNSUPPORTED;
-    // As many passes to a wave as it requests at a time: us for 4096 tokens of 30 + 30 heads of 128 and 32760 of 40 + 40, 1 pass 45 and 239, 4 or 5
-    // 24.1 and 238, 8 24.6 and 246, a whole token 24.8 and 248.  Fewer where the waves would be few.
+    // As many passes to a wave as it requests at a time: us for 4096 tokens of 30 + 30 heads of 128 and 32760 of 40 + 40, 1 pass 35.4 and 464, 2 24.0 and
+    // 281, 4 23.0 and 224, 8 23.6 and 233, a whole token 23.2 and 248.  Fewer where the waves would be few: 4071 tokens of 16 heads of 72 10.4 with one
+    // pass, 7.7 with four.
     const int64_t tokens = a.batch * a.tokens, total = tokens * passes;
     int64_t per = total / 2048;
     per = per < 1 ? 1 : per > DEEP ? DEEP : per;

@@ -58,7 +58,8 @@ int i8f_norm_rotate(const i8f_norm_rotate_args *args, const i8f_heads *groups, i
  * out[b, i, h] = sum_j e^s_ij v[b, j, g] / sum_j e^s_ij,   s_ij = scale q[b, i, h] . k[b, j, g] + m_bj,   g = h / (heads / kv_heads)
  * over the states j that count: j < key_lengths[b] where there are lengths, and of a mask those whose byte is not 0, or whose addend m is
  * above the lowest value of its type.  A row over which no state counts is zeros, and so is one of a finite query whose scores are all -inf;
- * what the states that do not count hold is not looked at.  Bfloat16 values up to 2^127 / keys cannot overflow the sums.
+ * what the states that do not count hold is not looked at.  Finite scores and addends of any size are the formula's; a score that passes binary32
+ * upwards gives NaN.  Bfloat16 values up to 2^127 / keys cannot overflow the sums.
  * Products of dtype, sums, maximum and exponentials in binary32, e^s rounded to dtype for the second product, one rounding at the end.
  *   q, k, v      [batch, queries or keys, heads or kv_heads, width] of dtype (I8F_BF16 or I8F_F16), last dimension contiguous, strides in
  *                elements, none negative; width up to 256, heads a multiple of kv_heads
