@@ -232,3 +232,13 @@ def test_values_at_the_ends_of_bfloat16(pkg, dev, queries, keys):
         assert off <= 2.0 ** -8 + 2 * keys * V + 2.0 ** -20, off
         tiny = (v.double() * 2.0 ** -122).bfloat16()
         check(pkg.cross_attention(q, k, tiny, key_mask=mask), expected(q, k, tiny, key_mask=mask))
+
+
+@pytest.mark.parametrize("size", [(1, 3, 300, 2, 2, 64), (1, 1, 3000, 2, 2, 64), (1, 700, 300, 8, 8, 128)], ids=str)
+def test_scales_at_the_ends_of_binary32(pkg, dev, size):
+    """The largest scale over heads whose products are small, the smallest over ones whose products are large, with scores of about one either way, and of nothing."""
+    for scale, std in ((2.0 ** 126, 2.0 ** -61), (2.0 ** 126, 2.0 ** -60), (2.0 ** -126, 2.0 ** 61), (2.0 ** -120, 2.0 ** 58), (2.0 ** -149, 1.0), (2.0 ** -140, 2.0 ** 10)):
+        q, k, v = inputs(*size, torch.float32, std=1.0)
+        q, k, v = (q * std).bfloat16(), (k * std).bfloat16(), v.bfloat16()
+        for mask in ({}, masked("bool", size[0], size[2]), {"key_mask": torch.linspace(-1, 1, size[2], device="cuda").expand(size[0], -1)}):
+            check(pkg.cross_attention(q, k, v, scale=scale, **mask), expected(q, k, v, scale=scale, **mask), (scale, std))
